@@ -50,6 +50,13 @@ _SIGS = {
     "arcb_mla_out": (i32, [vp, i32, i32, i32, vp, vp, i32, vp, vp, vp, vp]),
     "arcb_attn_mla": (i32, [vp, vp, vp, i32, vp, i32, i32, i32, i64, i32, i32, i32, vp, vp, vp]),
     "arcb_moe_route": (i32, [vp, i32, i32, i32, i32, i32, vp, vp]),
+    "arcb_attn_tree_ws": (i64, [i32, i32, i32, i32, i32, i32]),
+    "arcb_attn_tree": (i32, [vp, vp, vp, i32, vp, i64, i32, vp, vp, vp, i32, i32, i32, i32, i64, i32, i32, vp, vp, vp, vp,
+                             vp, vp]),
+    "arcb_draw_max_vocab": (i32, []),
+    "arcb_draw_tokens": (i32, [vp, i64, i32, i32, i32, i32, i32, i32, vp, vp, vp, vp, vp, vp, vp, vp]),
+    "arcb_verify_tree": (i32, [vp, i64, vp, i64, i32, i32, i32, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp]),
+    "arcb_kv_keep_path": (i32, [vp, i32, i32, i32, i32, vp, i64, i32, vp, vp, vp, i32, i32, vp, vp]),
     "arcb_set_pdl": (None, [i32]),
     "arcb_set_attn_paged": (None, [i32]),
     "arcb_wg_layernorm": (i32, [vp, i64, vp, i64, vp, i64, i32, vp]),

@@ -16,7 +16,8 @@ ints are wrapped explicitly with :func:`wrap`.  ``/`` truncates toward zero
 (:func:`tdiv`), ``>>`` is arithmetic.
 
 The MLA, MoE, Q4 group-32 and batching semantics that the reference lacks are
-defined at the end of this module (``mla_*``, ``moe_*``, ``q4g_*``).
+defined at the end of this module (``mla_*``, ``moe_*``, ``q4g_*``), with the
+tree-speculation operators (``tree_*``, ``draw_*``).
 """
 from __future__ import annotations
 
@@ -335,3 +336,99 @@ def tokens_hash(tokens) -> bytes:
     from arc_chain_b200.utils.hashing import blake3
 
     return blake3(np.asarray(list(tokens), dtype="<u4").tobytes())
+
+
+# ---------------------------------------------------------------------------
+# Tree speculation (extension): attention of drafted nodes, drawing tokens and
+# verifying drafts with given random numbers u in [0, 2^31)
+# ---------------------------------------------------------------------------
+LOGIT_CLAMP = 1 << 40
+MAX_INV_TEMP = 1 << 20
+
+
+def tree_attention(q: np.ndarray, K: np.ndarray, V: np.ndarray, base: int, n_tree: int, mask: int,
+                   attn_scale: int) -> np.ndarray:
+    """One query [dh] over the rows K, V [base + n_tree, dh]: the keys below
+    base and the nodes whose bit is set; zeros when there are none."""
+    keys = list(range(base)) + [base + j for j in range(n_tree) if mask >> j & 1]
+    if not keys:
+        return np.zeros_like(q)
+    dots = (K[keys] * q).sum(axis=1, dtype=np.int64)
+    w = softmax(((dots >> FRAC_BITS) * np.int64(attn_scale)) >> FRAC_BITS)
+    return ((w[:, None] * V[keys]) >> FRAC_BITS).sum(axis=0, dtype=np.int64)
+
+
+def tree_history(tokens, parent, hist, count: int, node: int) -> list:
+    """The newest 64 ids behind a node: its path up to the root (the root's
+    token is confirmed already), then the lane's ring, newest first."""
+    ids = []
+    while node > 0 and len(ids) < 64:
+        ids.append(int(tokens[node]))
+        p = int(parent[node])
+        node = p if 0 <= p < node else -1
+    for k in range(min(int(count), 64 - len(ids))):
+        ids.append(int(hist[(int(count) - 1 - k) & 63]))
+    return ids
+
+
+def draw_weights(logits: np.ndarray, ids, inv_temp: int) -> np.ndarray:
+    """Unnormalised Q16 weights of a logits row (csrc/kernels/draw_ops.cu)."""
+    x = np.clip(np.asarray(logits, dtype=np.int64), -LOGIT_CLAMP, LOGIT_CLAMP)
+    for t in ids:
+        if 0 <= t < len(x):
+            x[t] = max(-LOGIT_CLAMP, min(LOGIT_CLAMP, penalize(int(x[t]))))
+    if inv_temp <= 0:
+        e = np.zeros_like(x)
+        e[argmax(x)] = ONE
+        return e
+    z = (x * np.int64(min(inv_temp, MAX_INV_TEMP))) >> FRAC_BITS
+    return integer_exp_np(z - z.max())
+
+
+def draw_index(w: np.ndarray, u: int) -> int:
+    """The first index whose running sum of w exceeds floor(u * sum / 2^31); -1 for an empty row."""
+    total = int(w.sum(dtype=np.int64))
+    if total == 0:
+        return -1
+    return int(np.searchsorted(np.cumsum(w, dtype=np.int64), int(u) * total >> 31, side="right"))
+
+
+def draw_tokens(logits: np.ndarray, ids, inv_temp: int, us) -> list:
+    """len(us) tokens of one row, without replacement."""
+    e = draw_weights(logits, ids, inv_temp)
+    out = []
+    for u in us:
+        v = draw_index(e, u)
+        out.append(v)
+        if v >= 0:
+            e[v] = 0
+    return out
+
+
+def tree_verify(logits, dlogits, tokens, parent, n_tree: int, inv_temp: int, d_inv_temp: int, u, hist, count: int):
+    """(accepted path from the root, next token) of one lane's tree; logits
+    and dlogits [nodes, vocab], u [nodes, 2]."""
+    if n_tree <= 0:
+        return [], -1
+    path = [0]
+    while True:
+        node = path[-1]
+        ids = tree_history(tokens, parent, hist, count, node)
+        e = draw_weights(logits[node], ids, inv_temp)
+        p = (e << 31) // int(e.sum())
+        kids = [c for c in range(node + 1, n_tree) if int(parent[c]) == node]
+        eq = draw_weights(dlogits[node], ids, d_inv_temp) if kids else None
+        for c in kids:
+            d, s = int(tokens[c]), int(eq.sum())
+            if s == 0 or not 0 <= d < len(p):
+                continue
+            q = (eq << 31) // s
+            if int(u[c][0]) * int(q[d]) >> 31 < int(p[d]):
+                path.append(c)
+                break
+            rest = np.maximum(p - q, 0)
+            if rest.sum() > 0:
+                p = (rest << 31) // int(rest.sum())
+            eq[d] = 0
+        if path[-1] == node:
+            return path, draw_index(p, int(u[node][1]))

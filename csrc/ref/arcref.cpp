@@ -3,6 +3,8 @@
 // semantics; see arcref.h for the API.
 #include "arcref.h"
 
+#include "../common/tree.h"
+
 #include <fcntl.h>
 #include <stdio.h>
 #include <string.h>
@@ -882,3 +884,16 @@ extern "C" void arcref_merkle_root(const uint8_t* leaves, int64_t n, const char*
 // Installs a full-precision Q16 embedding table (borrowed; the caller keeps
 // it alive for the model's lifetime).
 extern "C" void arcref_set_embedding_q16(arcref_model* m, const int64_t* q16) { m->emb_q16 = q16; }
+
+// The drafted-tree bounds rules as the kernels compile them (csrc/common/tree.h).
+extern "C" int arcref_tree_lane_keys(int base, int n_tree, int t_lim, int width) {
+  return tree::lane_keys(base, n_tree, t_lim, width);
+}
+extern "C" int arcref_tree_page_ok(int page, int n_pages) { return tree::page_ok(page, n_pages); }
+extern "C" int arcref_tree_visible(int j, int base, int n_tree, uint64_t mask) {
+  return tree::visible(j, base, n_tree, mask);
+}
+extern "C" int arcref_tree_parent_of(const int* parent, int i) { return tree::parent_of(parent, i); }
+extern "C" int arcref_tree_path_ok(const int* path, int i, int n, int base, int width) {
+  return tree::path_ok(path, i, n, base, width);
+}
