@@ -117,9 +117,12 @@ def cmd_generate(a) -> dict:
     prompt = _prompt_ids(host, a.prompt, a.prompt_ids)
     text = a.prompt if a.prompt is not None else ",".join(map(str, prompt))
     t0 = time.perf_counter()
+    sampled = cfg.temperature > 0 or cfg.spec_tree
     if a.oracle:
         from arc_chain_b200.oracle import arcref
 
+        if sampled:
+            raise SystemExit("the CPU oracle decodes greedily: temperature must be 0 and spec_tree empty")
         m = arcref.Model(host)
         if cfg.quant == "q4-row":
             m.enable_q4()
@@ -134,7 +137,16 @@ def cmd_generate(a) -> dict:
         if cfg.quant == "q4-group":
             m = dense.to_q4(m, "group")
         eng = Engine(m, max_seq=cfg.max_seq or None)
-        toks, h = eng.generate(prompt, a.max_tokens, eos=cfg.eos, use_graph=cfg.use_graph)
+        if sampled:
+            from arc_chain_b200.config import build_tree_decoder
+
+            draft = None
+            if cfg.spec_tree:
+                dcfg = RunConfig(model=cfg.draft, seed=cfg.seed, max_seq=cfg.max_seq)
+                draft = Engine(dense.from_host(load_host_model(dcfg), "cuda"), max_seq=cfg.max_seq or None)
+            toks, h = build_tree_decoder(cfg, eng, draft).generate([prompt], a.max_tokens, eos=cfg.eos)[0]
+        else:
+            toks, h = eng.generate(prompt, a.max_tokens, eos=cfg.eos, use_graph=cfg.use_graph)
         engine = "arc_chain_b200 (B200)"
     ms = (time.perf_counter() - t0) * 1000
     out = attest.inference_result(host.cfg, text, prompt, toks, _decode(host, toks), ms, 0.0, engine)

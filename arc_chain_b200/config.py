@@ -35,6 +35,10 @@ class RunConfig:
     gen_cap: int = 0             # 0: max_seq
     draft: str = ""              # speculative decoding draft (preset or path); "" = off
     spec_k: int = 4
+    spec_tree: List[int] = field(default_factory=list)  # children per node of each drafted level; [] = no tree
+    temperature: float = 0.0     # 0: greedy (the reference's step); else sampled from the target's distribution
+    draft_temperature: float = 1.0
+    sample_seed: int = 0         # random streams of sampled decoding
     eos: List[int] = field(default_factory=list)
     use_graph: bool = True       # CUDA-graph the decode step
     pdl: bool = True             # programmatic dependent launch between kernels
@@ -49,6 +53,14 @@ class RunConfig:
             raise ValueError("comm must be 'fused' or 'nccl'")
         if self.tp < 1 or self.ep < 1 or (self.tp > 1 and self.ep > 1):
             raise ValueError("tp and ep are >= 1, and at most one of them is > 1")
+        if not self.temperature >= 0 or not self.draft_temperature >= 0:
+            raise ValueError("temperatures are >= 0")
+        if self.spec_tree:
+            from arc_chain_b200.runtime.tree_spec import tree_levels
+
+            tree_levels(self.spec_tree)
+            if not self.draft:
+                raise ValueError("spec_tree needs a draft model")
 
     # ------------------------------------------------------------ loading
     @classmethod
@@ -121,6 +133,8 @@ def _parse(v: str, typ: str, cur):
         return [int(x) for x in v.split(",") if x.strip()]
     if "int" in typ:
         return int(v)
+    if "float" in typ:
+        return float(v)
     return v
 
 
@@ -195,3 +209,12 @@ def build_engine(cfg: RunConfig, rank: int = 0, world: int = 1, comm=None):
     eng = Engine(m, max_seq=cfg.max_seq or None, comm=comm, n_pages=cfg.kv_pages or None)
     eng.gqa_block = bool(cfg.gqa_block)
     return eng
+
+
+def build_tree_decoder(cfg: RunConfig, target, draft=None, lanes: int = 1):
+    """The tree-speculation decoder of a run (cfg.spec_tree drafted by `draft`;
+    without a tree, plain sampled decoding) over the engine `target`."""
+    from arc_chain_b200.runtime.tree_spec import TreeSpecDecoder
+
+    return TreeSpecDecoder(target, draft, cfg.spec_tree, lanes, cfg.temperature, cfg.draft_temperature,
+                           cfg.sample_seed, cfg.use_graph)

@@ -124,7 +124,7 @@ class Epi(C.Structure):
                 ("grp_rows", C.c_int), ("grp_koff", C.c_int), ("route", C.c_void_p), ("route_ld", C.c_int),
                 ("max_ctas", C.c_int), ("b_box", C.c_int), ("route_gs", C.c_int), ("peer_h", C.c_void_p),
                 ("peer_sig", C.c_void_p), ("sched", C.c_int), ("rs_ag", C.c_int), ("rs_cnt_off", C.c_int),
-                ("ep_rows", C.c_int)]
+                ("ep_rows", C.c_int), ("kv_pos", C.c_void_p)]
 
 
 PARTIAL, STORE, RESID, QKV, SWIGLU, MOE_COMBINE, STORE_PEERS = 0, 1, 2, 3, 4, 5, 6

@@ -27,6 +27,7 @@ from arc_chain_b200.ops._lib import check, lib
 
 MAX_NODES = 64
 HIST = 64
+MAX_INV_TEMP = 1 << 20  # Q16: inverse temperatures are used up to 16
 PAGE = 16
 I32, I64, I8 = torch.int32, torch.int64, torch.int8
 

@@ -31,6 +31,7 @@ import torch
 
 from arc_chain_b200.models.dense import DenseModel
 from arc_chain_b200.ops import int_ops as ops
+from arc_chain_b200.ops import tree_ops
 from arc_chain_b200.runtime.kv_paged import PAGE, PagedKV
 from arc_chain_b200.utils.hashing import blake3
 import numpy as np
@@ -102,6 +103,21 @@ class StepBuffers:
         self.n_eos = 0
         # per-M-tile arrival counters of the fused GEMM (zero between uses)
         self.tiles = torch.zeros(ops.tile_counters(mmax, B), dtype=I32, device=dev)
+        # drafted trees (Engine.tree_buffers): cache rows of the slots, and what attn_tree reads
+        self.tree: Optional[TreeStep] = None
+        self.kv_pos: Optional[torch.Tensor] = None
+
+
+class TreeStep:
+    """What a forward over drafted-tree nodes needs besides StepBuffers: nq
+    slots per lane; base, n_tree [lanes] and mask [lanes * nq] as
+    tree_ops.attn_tree takes them."""
+
+    def __init__(self, lanes: int, nq: int, device):
+        self.lanes, self.nq = lanes, nq
+        self.base = torch.zeros(lanes, dtype=I32, device=device)
+        self.n_tree = torch.zeros(lanes, dtype=I32, device=device)
+        self.mask = torch.zeros(lanes * nq, dtype=I64, device=device)
 
 
 class Engine:
@@ -138,13 +154,26 @@ class Engine:
             self._bufs[key] = StepBuffers(self.m, B, self.max_pages, gen_cap)
         return self._bufs[key]
 
+    def tree_buffers(self, lanes: int, nq: int) -> StepBuffers:
+        """Buffers of a forward over nq drafted-tree nodes of each of `lanes`
+        requests (slot = lane * nq + node): besides tokens, pos (RoPE) and pt,
+        the caller sets kv_pos (cache rows) and the fields of `tree`."""
+        key = ("tree", lanes, nq)
+        if key not in self._bufs:
+            bb = StepBuffers(self.m, lanes * nq, self.max_pages)
+            bb.tree = TreeStep(lanes, nq, self.m.emb.device)
+            bb.kv_pos = torch.zeros(lanes * nq, dtype=I32, device=self.m.emb.device)
+            self._bufs[key] = bb
+        return self._bufs[key]
+
     # ------------------------------------------------------------------ forward
     def forward(self, bb: StepBuffers, B: int, with_logits: bool = True, span=None) -> None:
         """One forward over slots 0..B-1 of `bb` (tokens/pos/pt already set).
         span = (n, p0): slots [0, n) are positions p0.. of one sequence (page
         table row 0) and the rest padding; attention then runs as one
         chunk-attention launch that reads every K/V page once per 16
-        positions (the same exact values as the per-position kernel)."""
+        positions (the same exact values as the per-position kernel).
+        Buffers of tree_buffers run tree attention."""
         m, c, cm = self.m, self.m.cfg, self.comm
         d, dh = c.d_model, c.d_head
         nh, nkv = m.n_heads_local, m.n_kv_local
@@ -178,7 +207,12 @@ class Engine:
             ops.linear_gemm(Ly.qkv, bb.mXd, B, c0, bb.P, bb.tiles, e["qkv"])
             mark("qkv")
             T_all = self.max_pages * PAGE
-            if span is not None:
+            if bb.tree is not None:
+                t = bb.tree
+                tree_ops.attn_tree(bb.q, self.kv.K[l], self.kv.V[l], bb.pt[::t.nq], t.base, t.n_tree, t.mask, nh, nkv,
+                                   dh, m.attn_scale, t.lanes, t.nq, bb.Xo, c1, T_all, bb.err)
+                done = True
+            elif span is not None:
                 done = self.prefill_attn and ops.attn_prefill(bb.q, self.kv.K[l], self.kv.V[l], bb.pt[0], span[0],
                                                               span[1], nh, nkv, dh, m.attn_scale, B, bb.Xo, c1, T_all,
                                                               bb.err)
@@ -235,7 +269,8 @@ class Engine:
             out.append({
                 "qkv": ops.epi(ops.QKV, Ly.qkv.s, bb.err, n_heads=m.n_heads_local, n_kv=m.n_kv_local, dh=dh,
                                q_out=bb.q, Kc=self.kv.K[l], Vc=self.kv.V[l], pt=bb.pt, pt_stride=bb.pt.shape[1],
-                               pos=bb.pos, rcos=m.rope_cos, rsin=m.rope_sin, max_seq=self.max_seq),
+                               pos=bb.pos, kv_pos=bb.kv_pos, rcos=m.rope_cos, rsin=m.rope_sin,
+                               max_seq=self.max_seq),
                 "wo": ops.epi(ops.RESID, Ly.wo.s, bb.err, out=bb.h, ldo=d, ss_out=ss[2 * l + 1]),
                 "gu": ops.epi(ops.SWIGLU, Ly.gu.s, bb.err, X=bb.Xf, ldx=m.d_ff_local,
                               lmax_out=bb.cnt[4 * l + 3:4 * l + 4]),

@@ -44,6 +44,7 @@ class PagedKV:
         self.V = [torch.zeros(n_pages, n_kv, PAGE, d_head, dtype=torch.int64, device=device)
                   for _ in range(n_layers)] if with_v else self.K
         self.pool = PagePool(n_pages)
+        self._planes = None
         self.tables: Dict[int, List[int]] = {}
 
     @staticmethod
@@ -68,3 +69,12 @@ class PagedKV:
     def table_row(self, rid: int) -> List[int]:
         t = self.tables.get(rid, [])
         return t + [0] * (self.max_pages_per_seq - len(t))
+
+    def keep_path(self, pt, base, path, n_path, lanes: int, n: int, err) -> None:
+        """Moves the accepted path of each lane's drafted tree to consecutive
+        rows in every layer (tree_ops.kv_keep_path)."""
+        from arc_chain_b200.ops import tree_ops
+
+        if self._planes is None:
+            self._planes = tree_ops.KvPlanes(self.K, self.V)
+        tree_ops.kv_keep_path(self._planes, pt, base, path, n_path, lanes, n, err)

@@ -1,0 +1,309 @@
+"""Speculative decoding with a tree of drafted tokens, greedy or sampled.
+
+The reference decodes greedily only; with temperature 0 the output equals its
+greedy step's (crates/arc-inference/src/cached_integer_model.rs:1518-1557) token
+for token, like ``runtime.spec_decode``.  With a temperature the tokens follow
+the target's own distribution (softmax of its penalised logits over the
+temperature, in the exact integers of csrc/kernels/draw_ops.cu), whatever the
+draft proposes.  Random numbers come from the seeded SplitMix64 streams of
+``formats.gen``, one stream per request, so a run is a function of the
+model, the prompts and the seed: neither the other requests of the batch nor
+CUDA graphs change it.
+
+A round, per lane (request), with branches (b_1, ..., b_L):
+
+1. the draft runs the root (the last confirmed token) and draws b_1 children
+   from its distribution without replacement, then b_2 for each of those, and
+   so on: a level is one forward of the draft over its nodes, whose K/V rows
+   follow the confirmed prefix in the order of the nodes;
+2. the target runs all nodes in one forward (RoPE positions by depth, attention
+   over the prefix and each node's own path);
+3. the accepted path and the token behind it are decided on the device;
+4. the path's K/V rows move to their positions in both caches.
+
+With branches () there is no draft: plain sampled decoding.  The draft never
+runs the deepest level; where the path ends there, it is fed that token before
+the next round.  With tensor parallelism the draft, the drawing and the
+decision run on rank 0 and are broadcast; every rank runs the target's forward.
+"""
+from __future__ import annotations
+
+from dataclasses import dataclass, field
+from typing import List, Optional, Sequence, Tuple
+
+import numpy as np
+import torch
+
+from arc_chain_b200.formats import gen
+from arc_chain_b200.ops import tree_ops as ops
+from arc_chain_b200.runtime.engine import Engine, I32, I64
+from arc_chain_b200.utils.hashing import blake3
+
+ONE = 1 << 16
+STREAM = 0x54524545  # random streams of the requests: STREAM + request
+
+
+def tree_levels(branches: Sequence[int]) -> List[Tuple[int, int]]:
+    """[first, last) node of each level of a tree that is numbered level by
+    level, children of one node next to each other."""
+    levels = [(0, 1)]
+    for b in branches:
+        if b < 1:
+            raise ValueError(f"every level has at least one child per node, got {tuple(branches)}")
+        a, e = levels[-1]
+        levels.append((e, e + (e - a) * b))
+    if levels[-1][1] > ops.MAX_NODES:
+        raise ValueError(f"branches {tuple(branches)} make {levels[-1][1]} nodes; a tree has at most {ops.MAX_NODES}")
+    return levels
+
+
+def tree_parents(branches: Sequence[int]) -> List[int]:
+    par = [-1]
+    for (a, _), (s, e), b in zip(tree_levels(branches), tree_levels(branches)[1:], branches):
+        par += [a + i // b for i in range(e - s)]
+    return par
+
+
+def inverse_temperature(t: float) -> int:
+    """Q16 inverse temperature; 0 is greedy."""
+    if not t >= 0:
+        raise ValueError(f"a temperature is at least 0, got {t}")
+    return 0 if t == 0 else max(1, min(ops.MAX_INV_TEMP, int(round(ONE / t))))
+
+
+@dataclass
+class _Lane:
+    rid_t: int
+    rid_d: int
+    max_tokens: int
+    stream: int
+    gen: List[int] = field(default_factory=list)
+    last: int = 0
+    pos: int = 0
+    drawn: int = 0                                    # random numbers used
+    pending: List[int] = field(default_factory=list)  # tokens the draft has not consumed
+    done: bool = False
+
+
+class TreeSpecDecoder:
+    def __init__(self, target: Engine, draft: Optional[Engine] = None, branches: Sequence[int] = (3, 2, 1),
+                 lanes: int = 1, temperature: float = 0.0, draft_temperature: float = 1.0, seed: int = 0,
+                 use_graph: bool = True):
+        for e in (target, draft):
+            if e is not None and not hasattr(e, "tree_buffers"):
+                raise TypeError(f"tree speculation runs dense engines, got {type(e).__name__}")
+        if lanes < 1:
+            raise ValueError(f"lanes must be at least 1, got {lanes}")
+        self.branches = tuple(int(b) for b in branches)
+        self.t, self.d, self.n_lanes, self.seed, self.use_graph = target, draft, lanes, seed, use_graph
+        self.cm = target.comm
+        self.leads = self.cm.rank == 0
+        if self.branches and self.leads and draft is None:
+            raise ValueError("a tree of drafted tokens needs a draft engine")
+        if draft is not None and draft.m.cfg.vocab != target.m.cfg.vocab:
+            raise ValueError("target and draft must share a vocabulary")
+        self.levels = tree_levels(self.branches)
+        self.n = n = self.levels[-1][1]
+        dev = target.m.emb.device
+        par = tree_parents(self.branches)
+        depth, mask = [], []
+        for i, p in enumerate(par):
+            depth.append(0 if p < 0 else depth[p] + 1)
+            mask.append((0 if p < 0 else mask[p]) | 1 << i)
+        signed = [m - (1 << 64) if m >> 63 else m for m in mask]
+        self.parent = torch.tensor([par] * lanes, dtype=I32, device=dev)
+        self.depth = torch.tensor(depth, dtype=I32, device=dev)
+        self.node = torch.arange(n, dtype=I32, device=dev)
+        self.mask = torch.tensor(signed, dtype=I64, device=dev)
+        V = target.m.cfg.vocab
+        self.tb = target.tree_buffers(lanes, n)
+        self.db = [draft.tree_buffers(lanes, b - a) for a, b in self.levels[:-1]] if draft is not None else []
+        z = lambda *s, dt=I32: torch.zeros(*s, dtype=dt, device=dev)
+        self.pos, self.live, self.root = z(lanes), z(lanes), z(lanes)
+        self.tokens = z(lanes, n)
+        self.hist, self.count = z(lanes, 64), z(lanes)
+        self.inv = torch.full((lanes,), inverse_temperature(temperature), dtype=I64, device=dev)
+        self.dinv = torch.full((lanes,), inverse_temperature(draft_temperature), dtype=I64, device=dev)
+        self.dlogits = z(lanes * n, V, dt=I64) if self.branches and self.leads else None
+        # random numbers of a round: one per drafted node (its drawing), then two per node (its verification)
+        self.u_draw = [z(lanes * (b - a), k) for (a, b), k in zip(self.levels, self.branches)]
+        self.u_ver = z(lanes, n, 2)
+        self.path, self.n_path, self.nxt = z(lanes, n), z(lanes), z(lanes)
+        self._graph = None
+        self.rounds = self.proposed = self.accepted = 0
+
+    # ------------------------------------------------------------ device side
+    def _set(self, bb, a: int, b: int) -> None:
+        """Node range [a, b) of every lane into a forward's buffers."""
+        L, w = self.n_lanes, b - a
+        live = self.live[:, None]
+        bb.tokens.view(L, w).copy_(self.tokens[:, a:b].clamp(min=0))  # -1: nothing was left to draw
+        bb.pos.view(L, w).copy_(live * (self.pos[:, None] + self.depth[a:b]))
+        bb.kv_pos.view(L, w).copy_(live * (self.pos[:, None] + self.node[a:b]))
+        bb.tree.base.copy_(self.pos * self.live)
+        bb.tree.n_tree.copy_(self.live * b)
+        bb.tree.mask.view(L, w).copy_(self.mask[a:b].expand(L, w))
+
+    def _draft(self) -> None:
+        L, n, V = self.n_lanes, self.n, self.t.m.cfg.vocab
+        for (a, b), (s, e), k, bb, u in zip(self.levels, self.levels[1:], self.branches, self.db, self.u_draw):
+            self._set(bb, a, b)
+            self.d.forward(bb, bb.B, True)
+            self.dlogits.view(L, n, V)[:, a:b].copy_(bb.logits.view(L, b - a, V))
+            out = torch.empty(L * (b - a), k, dtype=I32, device=u.device)
+            ops.draw_tokens(bb.logits, V, L, b - a, a, k, self.dinv, u, self.hist, self.count, self.tokens,
+                            self.parent, out)
+            self.tokens[:, s:e].copy_(out.view(L, e - s))
+
+    def _decide(self) -> None:
+        d = self.dlogits if self.dlogits is not None else self.tb.logits
+        ops.verify_tree(self.tb.logits, d, self.t.m.cfg.vocab, self.n_lanes, self.n, self.tokens, self.parent,
+                        self.tb.tree.n_tree, self.inv, self.dinv, self.u_ver, self.hist, self.count, self.path,
+                        self.n_path, self.nxt)
+
+    def _keep(self, eng: Engine, bb) -> None:
+        eng.kv.keep_path(bb.pt[::bb.tree.nq], bb.tree.base, self.path, self.n_path, self.n_lanes, self.n, bb.err)
+
+    def _round(self) -> None:
+        if self.cm.size > 1:
+            import torch.distributed as dist
+
+        self.tokens[:, 0].copy_(self.root)
+        if self.branches and self.leads:
+            self._draft()
+        if self.cm.size > 1:
+            dist.broadcast(self.tokens, src=0)
+        self._set(self.tb, 0, self.n)
+        self.t.forward(self.tb, self.tb.B, True)
+        if self.leads:
+            self._decide()
+        if self.cm.size > 1:
+            for x in (self.path, self.n_path, self.nxt):
+                dist.broadcast(x, src=0)
+        if self.branches:
+            self._keep(self.t, self.tb)
+            if self.leads:
+                self._keep(self.d, self.db[0])
+
+    def _run(self) -> None:
+        if not self.use_graph or self.cm.size > 1:
+            self._round()
+            return
+        if self._graph is None:
+            # a first round with every lane idle: it sets the kernels'
+            # attributes and writes no request's rows
+            live = self.live.clone()
+            saved = [bb.pt.clone() for bb in (self.tb, *self.db)]
+            self.live.zero_()
+            for bb, e in ((self.tb, self.t), *((x, self.d) for x in self.db)):
+                bb.pt.copy_(torch.tensor(e.kv.table_row(e.scratch_rid), dtype=I32).expand_as(bb.pt))
+            self._round()
+            torch.cuda.synchronize()
+            for bb, s in zip((self.tb, *self.db), saved):
+                bb.pt.copy_(s)
+            self.live.copy_(live)
+            g = torch.cuda.CUDAGraph()
+            s = torch.cuda.Stream()
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                with torch.cuda.graph(g, stream=s):
+                    self._round()
+            torch.cuda.current_stream().wait_stream(s)
+            self._graph = g
+        self._graph.replay()
+
+    # ------------------------------------------------------------ host side
+    def _numbers(self, ln: _Lane, k: int) -> np.ndarray:
+        r = gen.rng_u64(self.seed, ln.stream, k, start=ln.drawn)
+        ln.drawn += k
+        return (r >> np.uint64(33)).astype(np.int32)
+
+    def _upload(self, lanes: List[_Lane]) -> None:
+        L, n = self.n_lanes, self.n
+        I = lambda x: torch.from_numpy(np.ascontiguousarray(x, dtype=np.int32))
+        self.pos.copy_(I([0 if ln.done else ln.pos for ln in lanes]))
+        self.live.copy_(I([0 if ln.done else 1 for ln in lanes]))
+        self.root.copy_(I([0 if ln.done else ln.last for ln in lanes]))
+        ring = np.zeros((L, 64), np.int32)
+        for i, ln in enumerate(lanes):
+            for k in range(max(0, len(ln.gen) - 64), len(ln.gen)):
+                ring[i, k & 63] = ln.gen[k]
+        self.hist.copy_(I(ring))
+        self.count.copy_(I([len(ln.gen) for ln in lanes]))
+        draws, ver = [[] for _ in self.u_draw], np.zeros((L, n, 2), np.int32)
+        for i, ln in enumerate(lanes):
+            u = np.zeros(3 * n - 1, np.int32) if ln.done else self._numbers(ln, 3 * n - 1)
+            for k, (s, e) in enumerate(self.levels[1:]):
+                draws[k].append(u[s - 1:e - 1])
+            ver[i] = u[n - 1:].reshape(n, 2)
+        for t, u in zip(self.u_draw, draws):
+            t.copy_(I(np.concatenate(u).reshape(t.shape)))
+        self.u_ver.copy_(torch.from_numpy(ver))
+        for bb, e, rid in ((self.tb, self.t, "rid_t"), *((x, self.d, "rid_d") for x in self.db)):
+            idle = e.kv.table_row(e.scratch_rid)
+            rows = [idle if ln.done else e.kv.table_row(getattr(ln, rid)) for ln in lanes]
+            bb.pt.copy_(I(np.repeat(rows, bb.tree.nq, 0)))
+
+    def _step(self, lanes: List[_Lane], eos: set) -> None:
+        if self.db:
+            for ln in lanes:
+                if not ln.done and ln.pending:
+                    self.d.prefill(ln.rid_d, ln.pending, start_pos=ln.pos - len(ln.pending))
+                    ln.pending = []
+        self._upload(lanes)
+        self._run()
+        path, n_path, nxt = self.path.cpu().numpy(), self.n_path.cpu().numpy(), self.nxt.cpu().numpy()
+        tokens = self.tokens.cpu().numpy()
+        self.rounds += 1
+        for i, ln in enumerate(lanes):
+            if ln.done:
+                continue
+            k = int(n_path[i])
+            if k < 1:
+                raise RuntimeError("the verification kernel returned no path (a kernel error bit is set)")
+            new = [int(tokens[i, j]) for j in path[i, 1:k]] + [int(nxt[i])]
+            self.proposed += len(self.branches)
+            self.accepted += k - 1
+            for tok in new:
+                ln.gen.append(tok)
+                if tok in eos or len(ln.gen) >= ln.max_tokens:
+                    ln.done = True
+                    break
+            if not ln.done:
+                # the draft has run every level but the deepest
+                ln.pending = [new[-2]] if self.branches and k == len(self.levels) else []
+                ln.last = new[-1]
+                ln.pos += k
+
+    def generate(self, prompts: Sequence[Sequence[int]], max_tokens: int, eos: Sequence[int] = ()) \
+            -> List[Tuple[List[int], bytes]]:
+        """Tokens and output hash of each prompt.  Request i of a call uses
+        random stream i of the decoder's seed."""
+        if len(prompts) != self.n_lanes:
+            raise ValueError(f"one prompt per lane: {self.n_lanes} lanes, {len(prompts)} prompts")
+        ends = set(int(e) for e in eos)
+        lanes: List[_Lane] = []
+        try:
+            for i, p in enumerate(prompts):
+                p = [int(x) for x in p]
+                need = 1 + len(p) + max_tokens + self.n
+                ln = _Lane(self.t.new_request(need), -1, max_tokens, STREAM + i, last=p[-1] if p else 0,
+                           pos=len(p) + 1, done=max_tokens <= 0)
+                lanes.append(ln)
+                self.t.prefill(ln.rid_t, [1] + p)
+                if self.db:
+                    ln.rid_d = self.d.new_request(need)
+                    self.d.prefill(ln.rid_d, [1] + p)
+            while not all(ln.done for ln in lanes):
+                self._step(lanes, ends)
+        finally:
+            for ln in lanes:
+                self.t.kv.release(ln.rid_t)
+                if ln.rid_d >= 0:
+                    self.d.kv.release(ln.rid_d)
+        return [(ln.gen, blake3(np.asarray(ln.gen, dtype="<u4").tobytes())) for ln in lanes]
+
+    @property
+    def acceptance(self) -> float:
+        """Accepted drafted tokens over the tree's depth, mean of the rounds."""
+        return self.accepted / max(1, self.proposed)

@@ -113,6 +113,10 @@ struct Epi {
   // b / ep_rows, at row b % ep_rows of that rank's combine buffer (each rank
   // owns ep_rows consecutive slots).  0 = add into every rank's buffer.
   int ep_rows;
+  // QKV: cache row of each slot's K/V where it is not its RoPE position (a
+  // drafted tree's nodes lie row after row, with the positions of their
+  // depths); null = pos.
+  const int* kv_pos;
 };
 
 // Ring depth for decode-sized tiles (BN <= 32).  A 5-stage ring (two CTAs
@@ -188,13 +192,13 @@ __device__ __forceinline__ void apply_row(const Epi& E, int M, int m, bool valid
       const int d = E.n_heads * E.dh, dkv = E.n_kv * E.dh, half = E.dh / 2;
       const int64_t partner = (int64_t)__shfl_xor_sync(0xffffffffu, (long long)v, 1);
       if (!valid) break;
-      const int p = E.pos[b];
-      if (p < 0 || p >= E.max_seq) {
+      const int p = E.pos[b], row = E.kv_pos ? E.kv_pos[b] : p;
+      if (p < 0 || p >= E.max_seq || row < 0 || row >= E.max_seq) {
         set_error(E.err, ARCB_ERR_SEQ_OVERFLOW);
         break;
       }
-      const int page = E.pt[(size_t)b * E.pt_stride + p / PAGE];
-      const int slot = p % PAGE;
+      const int page = E.pt[(size_t)b * E.pt_stride + row / PAGE];
+      const int slot = row % PAGE;
       if (m < d + dkv) {
         const bool is_q = m < d;
         const int r = is_q ? m : m - d;

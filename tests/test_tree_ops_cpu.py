@@ -184,3 +184,45 @@ def test_masked_and_extreme_logits():
     assert list(spec.draw_weights(np.full(3, lo), [], 65536)) == [65536] * 3
     assert spec.draw_index(np.zeros(4, np.int64), 5) == -1
     assert spec.draw_tokens(x, [], 0, [7, 7]) == [1, -1]
+
+
+# ------------------------------------------------------------ topology and configuration
+def test_tree_topology():
+    from arc_chain_b200.runtime import tree_spec as ts
+
+    assert ts.tree_levels((3, 2, 1)) == [(0, 1), (1, 4), (4, 10), (10, 16)]
+    assert ts.tree_parents((3, 2)) == [-1, 0, 0, 0, 1, 1, 2, 2, 3, 3]
+    assert ts.tree_levels(()) == [(0, 1)] and ts.tree_parents(()) == [-1]
+    assert ts.tree_levels((63,))[-1][1] == 64
+    for bad in ((64,), (2, 0), (4, 4, 4), (-1,)):
+        with pytest.raises(ValueError):
+            ts.tree_levels(bad)
+    assert [ts.inverse_temperature(t) for t in (0, 1, 0.5, 1e-9, 1e9)] == [0, 65536, 131072, 1 << 20, 1]
+    for bad in (-0.1, float("nan")):
+        with pytest.raises(ValueError):
+            ts.inverse_temperature(bad)
+
+
+def test_run_config_of_sampled_trees():
+    from arc_chain_b200.config import RunConfig
+
+    c = RunConfig().with_overrides(["draft=draft1b", "spec_tree=3,2,1", "temperature=0.7", "sample_seed=4"])
+    assert (c.spec_tree, c.temperature, c.sample_seed, c.draft_temperature) == ([3, 2, 1], 0.7, 4, 1.0)
+    assert RunConfig.from_dict(__import__("json").loads(c.to_json())) == c
+    for bad in (["spec_tree=3,2"], ["temperature=-1"], ["draft=tiny", "spec_tree=9,9"], ["draft_temperature=nan"]):
+        with pytest.raises(ValueError):
+            RunConfig().with_overrides(bad)
+
+
+def test_oracle_refuses_sampling():
+    from arc_chain_b200 import cli
+
+    with pytest.raises(SystemExit):
+        cli.main(["generate", "--prompt-ids", "5", "--oracle", "--set", "model=micro", "--set", "temperature=1"])
+
+
+def test_decoder_refuses():
+    from arc_chain_b200.runtime.tree_spec import TreeSpecDecoder
+
+    with pytest.raises(TypeError):
+        TreeSpecDecoder(object())
