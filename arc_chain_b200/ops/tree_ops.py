@@ -125,6 +125,8 @@ def attn_tree(q, Kc, Vc, pt, base, n_tree, mask, n_heads: int, n_kv: int, dh: in
     if o_out is not None:
         _need("o_out", o_out, I64, (B, d))
     dev = _place(q, Kc, Vc, pt, base, n_tree, mask, err, X, lmax, o_out)
+    if any(t is not None and t.data_ptr() % 16 for t in (q, Kc, Vc, X, o_out)):
+        raise ValueError("q, Kc, Vc, X and o_out must start on a 16-byte boundary")
     L = lib()
     ws = torch.empty(L.arcb_attn_tree_ws(lanes, nq, n_heads, n_kv, dh, t_lim), dtype=torch.uint8, device=dev)
     _call(dev, L.arcb_attn_tree, "attn_tree", _p(q), _p(Kc), _p(Vc), Kc.shape[0], _p(pt), ps, pt.shape[1], _p(base),

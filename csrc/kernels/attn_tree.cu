@@ -11,6 +11,30 @@
 // o = sum_j (w_j * v_j) >> 16, each term rounded down by itself.  A node's
 // output therefore equals a plain decode's along its path.  A query that sees
 // no key gets zeros.
+//
+// The queries of a KV head (nq nodes x G query heads: R rows) share its K and
+// V.  Exact weights need the global max and sum before the first value, so
+// there are three kernels:
+//
+//  1. k_scores, one CTA per 128 keys.  K's int64 elements become signed
+//     radix-256 digits (byte l of (x + 0x80..80) ^ 0x80..80, int8), one
+//     128-byte-swizzled plane of 128 keys x dh per digit, read once from DRAM;
+//     so do 32 query rows at a time.  q.k = sum over digit pairs (a, b) of
+//     D_{a+b} << 8(a+b) with D_s = sum_{a+b=s} K_a.Q_b^T: tcgen05 kind::i8
+//     products of M = 128 keys, N = 32 rows into one TMEM accumulator per s
+//     (exact in int32: at most 4 * 128 * 2^14).  3 digits (|x| < 2^23) are
+//     usual; up to 4 (|x| < 2^31) run this way, wider tiles take 64-bit
+//     products.  Scores are stored relative to their tile's max (differences
+//     below -2^30 clamped: their exp is 0 either way), which is stored beside.
+//  2. k_sums: each row's global max and sum of exps, split over key chunks.
+//  3. k_values: w.v for up to 64 rows and a range of keys.  The floor of each
+//     term rules out a matrix product, but one single-precision FMA rounding
+//     toward minus infinity is exact: acc <- rd(acc + w * (v / 2^16)) with acc
+//     an integer in [2^23, 2^24), where floats are the integers, adds
+//     floor(w * v / 2^16).  acc starts at 1.5 * 2^23 and moves by at most
+//     max|v| + (number of keys) < 2^22, since the weights sum to at most ONE.
+//     Chunks with wider values take 64-bit terms.
+//     Key ranges of one row group are summed by the last CTA to arrive.
 #include "../common/tree.h"
 #include "common.cuh"
 #include "lut.cuh"
@@ -19,106 +43,682 @@ using namespace q16;
 
 namespace at {
 
-constexpr int NT = 128;
 constexpr int PAGE = tree::PAGE;
+constexpr int TILE = 128;           // keys per score CTA
+constexpr int RQ = 32;              // query rows per MMA group
+constexpr int PLANES = 4;           // digits that take the tensor path
+constexpr int NT_S = 256;           // k_scores threads
+constexpr int NT_B = 256;           // k_sums threads
+constexpr int CK = 64;              // keys per k_values chunk
+constexpr int MAX_RG = 64;          // rows per k_values CTA
+constexpr int FAR = -(1 << 30);     // a score whose exp is 0
+constexpr int64_t NONE = -(int64_t(1) << 62);  // max of no keys
+constexpr int VMAX = (1 << 22) - (1 << 17);    // values of the single-precision form
+constexpr int MAX_RANGE = 1 << 16;             // keys per k_values CTA: VMAX + MAX_RANGE < 2^22
 
-// One CTA per (head, query): scores of every key to scratch, then the exact
-// max, sum and weights, then the values.
-__global__ void __launch_bounds__(NT) k_attn_tree(const int64_t* __restrict__ q, const int64_t* __restrict__ Kc,
-                                                  const int64_t* __restrict__ Vc, int n_pages,
-                                                  const int* __restrict__ pt, int64_t pt_stride, int width,
-                                                  const int* __restrict__ base, const int* __restrict__ n_tree,
-                                                  const int64_t* __restrict__ mask, int nq, int n_heads, int n_kv,
-                                                  int dh, int64_t attn_scale, int t_lim, int B,
-                                                  int64_t* __restrict__ scores, int8_t* __restrict__ X,
-                                                  int* __restrict__ lmax, int64_t* __restrict__ o_out,
-                                                  int* __restrict__ err) {
+struct Args {
+  const int64_t* q;
+  const int64_t* Kc;
+  const int64_t* Vc;
+  const int* pt;
+  const int* base;
+  const int* n_tree;
+  const int64_t* mask;
+  int64_t pt_stride, attn_scale;
+  int n_pages, width, nq, n_heads, n_kv, dh, t_lim, B, lane0;
+  int R, Rp, G, tiles, chunks, groups, RG, splits;
+  // workspace
+  int* S;              // [lanes][n_kv][tiles][TILE][Rp] scores relative to M
+  int64_t* M;          // [lanes][n_kv][tiles][Rp] max of the tile
+  int64_t* gmax;       // [lanes][n_kv][Rp]
+  uint64_t* sums;      // [lanes][n_kv][chunks][Rp]
+  int64_t* part;       // [lanes][n_kv][groups][splits][RG][dh]
+  int* arrived;        // [lanes][n_kv][groups]
+  int8_t* X;
+  int* lmax;
+  int64_t* o_out;
+  int* err;
+};
+
+// exp table as (value, step to the next): e = value + (step * frac >> 11)
+__device__ __forceinline__ void load_lut(int2* lut, int nt) {
+  for (int i = threadIdx.x; i < EXP_LUT_N; i += nt) {
+    const int lo = (int)g_exp_lut.v[i];
+    lut[i] = make_int2(lo, i < EXP_LUT_N - 1 ? (int)g_exp_lut.v[i + 1] - lo : 0);
+  }
+}
+// integer_exp of x <= 0 in 32 bits.
+__device__ __forceinline__ int exp32(int x, const int2* lut) {
+  const int off = max(x + (int)EXP_RANGE, 0);
+  const int2 t = lut[off >> 11];
+  return off > 0 ? t.x + ((t.y * (off & 2047)) >> 11) : 0;
+}
+// What a tile's relative scores need added to be relative to the row's max.
+__device__ __forceinline__ int rebase(int64_t tile_max, int64_t row_max) {
+  const int64_t d = tile_max - row_max;
+  return d < FAR ? FAR : (int)d;
+}
+
+// Four int64 -> digit words: plane l's word in p[l]; the low and high digit
+// words are or-ed into lo / hi.
+__device__ __forceinline__ void digits4(const int64_t* x, uint32_t* p, uint32_t& lo, uint32_t& hi) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint64_t y = ((uint64_t)x[i] + 0x8080808080808080ull) ^ 0x8080808080808080ull;
+    w[i] = (uint32_t)y;
+    lo |= w[i];
+    hi |= (uint32_t)(y >> 32);
+  }
+  const uint32_t t0 = __byte_perm(w[0], w[1], 0x5140), t1 = __byte_perm(w[2], w[3], 0x5140);
+  const uint32_t t2 = __byte_perm(w[0], w[1], 0x7362), t3 = __byte_perm(w[2], w[3], 0x7362);
+  p[0] = __byte_perm(t0, t1, 0x5410);
+  p[1] = __byte_perm(t0, t1, 0x7632);
+  p[2] = __byte_perm(t2, t3, 0x5410);
+  p[3] = __byte_perm(t2, t3, 0x7632);
+}
+// Digit planes that an or of low digit words needs.
+__device__ __forceinline__ int planes_of(uint32_t lo) { return lo >> 24 ? 4 : lo >> 16 ? 3 : lo >> 8 ? 2 : 1; }
+
+__device__ __forceinline__ void load4(int64_t* x, const int64_t* src) {
+  const longlong2 a = __ldg((const longlong2*)src), b = __ldg((const longlong2*)src + 1);
+  x[0] = a.x, x[1] = a.y, x[2] = b.x, x[3] = b.y;
+}
+
+// ------------------------------------------------------------------ 1. scores
+// DHP: row pitch class of the planes (64 or 128 >= dh).
+template <int DHP>
+__global__ void __launch_bounds__(NT_S, 2) k_scores(const Args A) {
+  constexpr int KP = TILE * 128, QP = RQ * 128;  // bytes per plane
+  constexpr int TPR = DHP / 4;                   // threads per row
+  constexpr int TMEM_COLS = 256;                 // (2 * PLANES - 1) * RQ = 224 used
+  extern __shared__ __align__(1024) uint8_t dsm[];
+  __shared__ int64_t wmax[4][RQ];
+  __shared__ uint64_t qmask[RQ];
+  __shared__ int pages[TILE / PAGE];
+  __shared__ uint32_t or_k[2], or_q[2][2];  // digit words or-ed: keys; queries of even / odd groups
+  __shared__ uint32_t tslot;
+  __shared__ __align__(8) uint64_t done;
+  __shared__ int s_abort;
+  const int tid = threadIdx.x, ln = tid & 31, w = tid >> 5;
+  const int tile = blockIdx.x, kvh = blockIdx.y, lane = A.lane0 + blockIdx.z;
+  const size_t lk = (size_t)blockIdx.z * A.n_kv + kvh;
+  const uint32_t kbase = (smem_u32(dsm) + 1023u) & ~1023u, qbase = kbase + PLANES * KP;
+  uint8_t* kp = dsm + (kbase - smem_u32(dsm));
+  uint8_t* qp = kp + PLANES * KP;
+  if (w == 0) {
+    tmem_alloc(smem_u32(&tslot), TMEM_COLS);
+    tmem_relinquish();
+  }
+  if (tid == 0) {
+    mbar_init(smem_u32(&done), 1);
+    fence_barrier_init();
+    s_abort = 0;
+  }
+  if (tid < 2) or_k[tid] = or_q[0][tid] = 0;
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tslot;
+  // the dependents start only after every CTA of this grid holds its TMEM
   pdl_wait_dep();
   pdl_allow_next();
-  __shared__ int64_t lut[EXP_LUT_N];
-  __shared__ int64_t red[NT / 32];
-  const int tid = threadIdx.x, ln = tid & 31, w = tid >> 5;
-  const int slot = blockIdx.y, head = blockIdx.x, lane = slot / nq, kvh = head / (n_heads / n_kv);
-  for (int i = tid; i < EXP_LUT_N; i += NT) lut[i] = g_exp_lut.v[i];
-  const int b = base[lane], nt = n_tree[lane];
-  int T = tree::lane_keys(b, nt, t_lim, width);
-  pt += lane * pt_stride;
-  bool bad = T < 0;
-  for (int i = tid; !bad && i < (T + PAGE - 1) / PAGE; i += NT) bad |= !tree::page_ok(pt[i], n_pages);
-  bad = __syncthreads_or(bad);
-  if (bad) {
-    if (tid == 0) set_error(err, T < 0 ? ARCB_ERR_SEQ_OVERFLOW : ARCB_ERR_BOUNDS);
-    T = 0;
+  const int base = A.base[lane], nt = A.n_tree[lane];
+  const int T = tree::lane_keys(base, nt, A.t_lim, A.width);
+  if (tile == 0)
+    for (int i = tid; i < A.groups; i += NT_S) A.arrived[lk * A.groups + i] = 0;
+  const int j0 = tile * TILE;
+  const bool live = j0 < T;
+  if (live && tid < TILE / PAGE) {
+    const int j = j0 + tid * PAGE;
+    const int p = j < T ? A.pt[lane * A.pt_stride + j / PAGE] : -1;
+    pages[tid] = tree::page_ok(p, A.n_pages) ? p : -1;
   }
-  const uint64_t m = (uint64_t)mask[slot];
-  const int64_t* qr = q + ((size_t)slot * n_heads + head) * dh;
-  int64_t* sc = scores + ((size_t)slot * n_heads + head) * t_lim;
-  auto row = [&](const int64_t* c, int j) {
-    return c + (((size_t)pt[j / PAGE] * n_kv + kvh) * PAGE + j % PAGE) * dh;
-  };
-  int64_t mx = INT64_MIN;
-  for (int j = w; j < T; j += NT / 32) {
-    if (!tree::visible(j, b, nt, m)) continue;
-    const int64_t* kr = row(Kc, j);
-    uint64_t d = 0;
-    for (int e = ln; e < dh; e += 32) d += (uint64_t)wmul(qr[e], kr[e]);
+  __syncthreads();
+  if (live) {
+    // ---- K digit planes: a warp reads 32 / TPR whole rows at a time
+    constexpr int RPW = 32 / TPR, STEPS = TILE / (8 * RPW), UN = 8;
+    const int col = (ln % TPR) * 4;
+    uint32_t lo = 0, hi = 0;
+#pragma unroll 1
+    for (int s0 = 0; s0 < STEPS; s0 += UN) {
+      int64_t x[UN][4];
 #pragma unroll
-    for (int s = 16; s >= 1; s >>= 1) d += (uint64_t)shfl_xor_i64((int64_t)d, s);
-    const int64_t x = attn_score((int64_t)d, attn_scale);
-    if (ln == 0) sc[j] = x;
-    mx = x > mx ? x : mx;
-  }
-  if (ln == 0) red[w] = mx;
-  __syncthreads();
-  for (int i = 0; i < NT / 32; ++i) mx = red[i] > mx ? red[i] : mx;
-  __syncthreads();
-  int64_t su = 0;
-  for (int j = tid; j < T; j += NT) {
-    const int64_t e = tree::visible(j, b, nt, m) ? integer_exp(wsub(sc[j], mx), lut) : 0;
-    sc[j] = e;
-    su += e;
-  }
+      for (int u = 0; u < UN; ++u) {
+        const int r = ((s0 + u) * 8 + w) * RPW + ln / TPR, p = pages[r / PAGE];
+        if (col < A.dh && p >= 0 && j0 + r < T)
+          load4(x[u], A.Kc + (((size_t)p * A.n_kv + kvh) * PAGE + r % PAGE) * A.dh + col);
+        else
+          x[u][0] = x[u][1] = x[u][2] = x[u][3] = 0;
+      }
 #pragma unroll
-  for (int s = 16; s >= 1; s >>= 1) su += shfl_xor_i64(su, s);
-  if (ln == 0) red[w] = su;
-  __syncthreads();
-  su = 0;
-  for (int i = 0; i < NT / 32; ++i) su += red[i];
-  int need = 0;
-  for (int e = tid; e < dh; e += NT) {
-    uint64_t o = 0;
-    for (int j = 0; j < T; ++j)
-      if (sc[j] != 0) o += (uint64_t)mulshr(udiv_small(sc[j] * ONE, su), row(Vc, j)[e]);
-    const size_t col = (size_t)head * dh + e;
-    if (o_out) o_out[(size_t)slot * n_heads * dh + col] = (int64_t)o;
-    if (X) {
-      int8_t dg[8];
-      const int nl = limb_split8((int64_t)o, dg);
-      need = nl > need ? nl : need;
-      for (int l = 0; l < 8; ++l) X[limb_row(l, slot, B) * n_heads * dh + col] = dg[l];
+      for (int u = 0; u < UN; ++u) {
+        const int r = ((s0 + u) * 8 + w) * RPW + ln / TPR;
+        uint32_t d[4];
+        digits4(x[u], d, lo, hi);
+        const uint32_t at = r * 128 + (((col >> 4) ^ (r & 7)) << 4) + (col & 15);
+#pragma unroll
+        for (int l = 0; l < PLANES; ++l) *(uint32_t*)(kp + l * KP + at) = d[l];
+      }
+    }
+    lo = __reduce_or_sync(0xffffffffu, lo);
+    hi = __reduce_or_sync(0xffffffffu, hi);
+    if (ln == 0) {
+      atomicOr(&or_k[0], lo);
+      atomicOr(&or_k[1], hi);
+    }
+    const int j = j0 + (w & 3) * 32 + ln;  // this thread's key in the epilogue
+    int* Srow = A.S + ((lk * A.tiles + tile) * TILE + (w & 3) * 32 + ln) * A.Rp;
+    const int kend = (A.dh + 31) / 32;
+    uint32_t parity = 0;
+    for (int r0 = 0, g = 0; r0 < A.R; r0 += RQ, g ^= 1) {
+      const int rows = min(RQ, A.R - r0), nmma = rows > 16 ? 32 : 16;
+      __syncthreads();  // the last group's epilogue and the planes' readers are done
+      // ---- query digit planes and masks of rows [r0, r0 + 32)
+      lo = hi = 0;
+      for (int r = tid / TPR; r < nmma; r += NT_S / TPR) {
+        int64_t x[4] = {0, 0, 0, 0};
+        const int rr = r0 + r;
+        if (r < rows && col < A.dh)
+          load4(x, A.q + ((size_t)(lane * A.nq + rr / A.G) * A.n_heads + kvh * A.G + rr % A.G) * A.dh + col);
+        uint32_t d[4];
+        digits4(x, d, lo, hi);
+        const uint32_t at = r * 128 + (((col >> 4) ^ (r & 7)) << 4) + (col & 15);
+#pragma unroll
+        for (int l = 0; l < PLANES; ++l) *(uint32_t*)(qp + l * QP + at) = d[l];
+      }
+      if (tid < rows) qmask[tid] = (uint64_t)A.mask[(size_t)lane * A.nq + (r0 + tid) / A.G];
+      if (tid >= rows && tid < RQ) qmask[tid] = 0;
+      lo = __reduce_or_sync(0xffffffffu, lo);
+      hi = __reduce_or_sync(0xffffffffu, hi);
+      if (ln == 0) {
+        atomicOr(&or_q[g][0], lo);
+        atomicOr(&or_q[g][1], hi);
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      tc_fence_before();
+      __syncthreads();
+      tc_fence_after();
+      const int lk_n = planes_of(or_k[0]), lq_n = planes_of(or_q[g][0]);
+      const bool wide = (or_k[1] | or_q[g][1]) != 0;
+      if (tid < 2) or_q[g ^ 1][tid] = 0;  // its readers passed two barriers ago
+      if (!wide) {
+        if (tid == 0) {
+          const uint32_t idesc = idesc_i8(TILE, nmma);
+          for (int a = 0; a < lk_n; ++a)
+            for (int b = 0; b < lq_n; ++b)
+              for (int k = 0; k < kend; ++k)
+                // the first pair of a sum a + b (a = 0, or b = lq_n - 1) overwrites its accumulator
+                mma_i8(tmem + (a + b) * RQ, sw128_kmajor_desc(kbase + a * KP + k * 32),
+                       sw128_kmajor_desc(qbase + b * QP + k * 32), idesc,
+                       (k > 0 || (a > 0 && b < lq_n - 1)) ? 1u : 0u);
+          mma_commit(smem_u32(&done));
+        }
+        if (!mbar_wait(smem_u32(&done), parity)) s_abort = 1;
+        parity ^= 1;
+        tc_fence_after();
+      }
+      // ---- scores of 16 rows per warp: rows c0 .. c0 + 15 of the group
+      const int c0 = (w >> 2) * 16;
+      int64_t sc[16];
+      if (c0 < rows) {
+        if (!wide) {
+          const int ns = lk_n + lq_n - 1;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) sc[i] = 0;
+          for (int s = 0; s < ns; ++s) {
+            uint32_t r[16];
+            tmem_ld16(tmem + ((uint32_t)(w & 3) << 21) + s * RQ + c0, r);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 16; ++i) sc[i] += (int64_t)((uint64_t)(int64_t)(int)r[i] << (8 * s));
+          }
+        } else {
+          const int p = pages[(j - j0) / PAGE];
+          const int64_t* kr = A.Kc + (((size_t)(p < 0 ? 0 : p) * A.n_kv + kvh) * PAGE + j % PAGE) * A.dh;
+          for (int i = 0; i < 16; ++i) {
+            uint64_t d = 0;
+            const int rr = r0 + c0 + i;
+            if (p >= 0 && j < T && c0 + i < rows) {
+              const int64_t* qr = A.q + ((size_t)(lane * A.nq + rr / A.G) * A.n_heads + kvh * A.G + rr % A.G) * A.dh;
+              for (int e = 0; e < A.dh; ++e) d += (uint64_t)wmul(qr[e], kr[e]);
+            }
+#pragma unroll
+            for (int m = 0; m < 16; ++m)
+              if (m == i) sc[m] = (int64_t)d;
+          }
+        }
+        bool fits = true;
+        uint32_t seen = 0;  // bit i: row c0 + i sees this key
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          sc[i] = attn_score(sc[i], A.attn_scale);
+          fits &= sc[i] == (int64_t)(int)sc[i];
+          if (tree::visible(j, base, nt, qmask[c0 + i]) && c0 + i < rows) seen |= 1u << i;
+        }
+        fits = __all_sync(0xffffffffu, fits);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const bool see = seen >> i & 1;
+          int64_t m;
+          if (fits) {
+            m = __reduce_max_sync(0xffffffffu, see ? (int)sc[i] : INT32_MIN);
+            if (!__any_sync(0xffffffffu, see)) m = NONE;
+          } else {
+            m = see ? sc[i] : NONE;
+#pragma unroll
+            for (int b = 16; b >= 1; b >>= 1) {
+              const int64_t o = shfl_xor_i64(m, b);
+              m = o > m ? o : m;
+            }
+          }
+          if (ln == 0) wmax[w & 3][c0 + i] = m;
+        }
+        tc_fence_before();
+        // the four warps of these 16 rows
+        asm volatile("bar.sync %0, 128;" ::"r"(1 + (w >> 2)) : "memory");
+        int out[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          int64_t m = wmax[0][c0 + i];
+#pragma unroll
+          for (int k = 1; k < 4; ++k) m = wmax[k][c0 + i] > m ? wmax[k][c0 + i] : m;
+          const int64_t d = sc[i] - m;
+          out[i] = (seen >> i & 1) && d > FAR ? (int)d : FAR;
+          if ((w & 3) == 0 && ln == i && c0 + i < rows) A.M[(lk * A.tiles + tile) * A.Rp + r0 + c0 + i] = m;
+        }
+#pragma unroll
+        for (int i = 0; i < 16; i += 4)
+          if (c0 + i < rows) *(int4*)(Srow + r0 + c0 + i) = make_int4(out[i], out[i + 1], out[i + 2], out[i + 3]);
+      }
     }
   }
-  if (need && lmax) atomicMax(lmax, need);
+  tc_fence_before();
+  __syncthreads();
+  if (tid == 0 && s_abort) set_error(A.err, ARCB_ERR_TIMEOUT_DONE);
+  if (w == 0) {
+    tc_fence_after();
+    tmem_dealloc(tmem, TMEM_COLS);
+  }
+}
+
+// -------------------------------------------------------------------- 2. sums
+// grid (chunks, n_kv * row blocks of 32, lanes): lane = row, warps over keys.
+__global__ void __launch_bounds__(NT_B) k_sums(const Args A) {
+  __shared__ int2 lut[EXP_LUT_N];
+  __shared__ int64_t red[NT_B / 32][32];
+  load_lut(lut, NT_B);
+  pdl_wait_dep();
+  pdl_allow_next();
+  const int ln = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const int rb = (A.R + 31) / 32, kvh = blockIdx.y / rb, r = (blockIdx.y % rb) * 32 + ln;
+  const int lane = A.lane0 + blockIdx.z, T = tree::lane_keys(A.base[lane], A.n_tree[lane], A.t_lim, A.width);
+  if (T <= 0) return;
+  const size_t lk = (size_t)blockIdx.z * A.n_kv + kvh;
+  const int nt = (T + TILE - 1) / TILE;
+  const int t0 = (int)((int64_t)blockIdx.x * nt / A.chunks), t1 = (int)((int64_t)(blockIdx.x + 1) * nt / A.chunks);
+  const bool row = r < A.R;
+  const int64_t* M = A.M + lk * A.tiles * A.Rp + r;
+  int64_t m = NONE;
+  if (row)
+    for (int t = w; t < nt; t += NT_B / 32) m = max(m, M[(size_t)t * A.Rp]);
+  red[w][ln] = m;
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < NT_B / 32; ++k) m = max(m, red[k][ln]);
+  __syncthreads();
+  uint64_t s = 0;
+  if (row) {
+    if (blockIdx.x == 0 && w == 0) A.gmax[lk * A.Rp + r] = m;
+    for (int t = t0; t < t1; ++t) {
+      const int off = rebase(M[(size_t)t * A.Rp], m);
+      const int* S = A.S + ((lk * A.tiles + t) * TILE) * A.Rp + r;
+#pragma unroll 4
+      for (int k = w; k < TILE; k += NT_B / 32) s += (uint64_t)exp32(S[(size_t)k * A.Rp] + off, lut);
+    }
+  }
+  red[w][ln] = (int64_t)s;
+  __syncthreads();
+  if (w == 0 && row) {
+#pragma unroll
+    for (int k = 1; k < NT_B / 32; ++k) s += (uint64_t)red[k][ln];
+    A.sums[(lk * A.chunks + blockIdx.x) * A.Rp + r] = s;
+  }
+}
+
+// ------------------------------------------------------------------ 3. values
+__device__ __forceinline__ uint64_t fma2_rd(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rm.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t dup2(float x) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %1};" : "=l"(d) : "f"(x));
+  return d;
+}
+
+// 8 consecutive digits planes of four int64 outputs, and their limb count.
+__device__ __forceinline__ int store_limbs4(int8_t* X, int slot, int B, size_t ldx, size_t col, const int64_t* o) {
+  int need = 0;
+  uint32_t lo[4], hi[4], l4 = 0, h4 = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint64_t y = ((uint64_t)o[i] + 0x8080808080808080ull) ^ 0x8080808080808080ull;
+    lo[i] = (uint32_t)y;
+    hi[i] = (uint32_t)(y >> 32);
+    l4 |= lo[i];
+    h4 |= hi[i];
+  }
+  need = h4 ? 4 + planes_of(h4) : (l4 ? planes_of(l4) : 0);
+#pragma unroll
+  for (int l = 0; l < 8; ++l) {
+    const uint32_t* v = l < 4 ? lo : hi;
+    const int s = 8 * (l & 3);
+    const uint32_t word = (v[0] >> s & 255u) | (v[1] >> s & 255u) << 8 | (v[2] >> s & 255u) << 16 | (v[3] >> s & 255u) << 24;
+    *(uint32_t*)(X + limb_row(l, slot, B) * ldx + col) = word;
+  }
+  return need;
+}
+
+// grid (splits, n_kv * groups, lanes).  A warp takes 8 rows (unit) x all dims,
+// lane = DPL consecutive dims; KPART warps per unit take every KPART-th key.
+template <int DPL>
+__global__ void __launch_bounds__(256) k_values(const Args A) {
+  extern __shared__ __align__(1024) uint8_t dsm[];
+  constexpr int DHP = 32 * DPL;
+  __shared__ int2 lut[EXP_LUT_N];
+  __shared__ int64_t rmax[MAX_RG];
+  __shared__ uint64_t rsum[MAX_RG];
+  __shared__ float rrcp[MAX_RG];
+  __shared__ int roff[MAX_RG];
+  __shared__ int s_last, s_need;
+  const int NT = blockDim.x, tid = threadIdx.x, ln = tid & 31, w = tid >> 5;
+  const int RG = A.RG, units = RG / 8, unit = w % units, kpart = w / units, kparts = NT / 32 / units;
+  float* vs = (float*)dsm;                                   // [CK][DHP] v / 2^16
+  float* ws = vs + CK * DHP;                                 // [CK][RG] weights
+  int* osum = (int*)dsm;                                     // [RG][DHP] at the end
+  load_lut(lut, NT);
+  if (tid == 0) s_need = 0;
+  pdl_wait_dep();
+  pdl_allow_next();
+  const int kvh = blockIdx.y / A.groups, grp = blockIdx.y % A.groups, r0 = grp * RG, rows = min(RG, A.R - r0);
+  const int lane = A.lane0 + blockIdx.z;
+  const size_t lk = (size_t)blockIdx.z * A.n_kv + kvh, lkg = lk * A.groups + grp;
+  const int base = A.base[lane], ntree = A.n_tree[lane];
+  int T = tree::lane_keys(base, ntree, A.t_lim, A.width);
+  const int* pt = A.pt + lane * A.pt_stride;
+  bool bad = T < 0;
+  for (int i = tid; !bad && i < (T + PAGE - 1) / PAGE; i += NT) bad |= !tree::page_ok(pt[i], A.n_pages);
+  bad = __syncthreads_or(bad);
+  if (bad && tid == 0) set_error(A.err, T < 0 ? ARCB_ERR_SEQ_OVERFLOW : ARCB_ERR_BOUNDS);
+  if (bad) T = 0;
+  if (T == 0 && blockIdx.x > 0) return;
+  const int nt = (T + TILE - 1) / TILE;
+  const int t0 = (int)((int64_t)blockIdx.x * nt / A.splits), t1 = (int)((int64_t)(blockIdx.x + 1) * nt / A.splits);
+  if (T > 0 && tid < RG) {
+    const bool row = tid < rows;
+    uint64_t s = 0;
+    if (row)
+      for (int c = 0; c < A.chunks; ++c) s += A.sums[(lk * A.chunks + c) * A.Rp + r0 + tid];
+    rmax[tid] = row ? A.gmax[lk * A.Rp + r0 + tid] : NONE;
+    rsum[tid] = s ? s : 1;  // a row without keys: every exp is 0
+    rrcp[tid] = __frcp_rn((float)(int64_t)rsum[tid]);
+  }
+  uint64_t acc[DPL][4];  // pairs of rows
+#pragma unroll
+  for (int d = 0; d < DPL; ++d)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[d][i] = dup2(12582912.0f);
+  int64_t* part = A.part + (lkg * A.splits + blockIdx.x) * (size_t)RG * A.dh;
+  bool any_wide = false;
+  for (int j0 = t0 * TILE; j0 < min(t1 * TILE, T); j0 += CK) {
+    const int t = j0 / TILE, keys = min(CK, T - j0);
+    __syncthreads();  // rsum / the last chunk's readers
+    if (j0 % TILE == 0 && tid < RG)
+      roff[tid] = tid < rows ? rebase(A.M[(lk * A.tiles + t) * A.Rp + r0 + tid], rmax[tid]) : FAR;
+    // values: v / 2^16 in single precision, 0 past the last key and dim
+    bool fit = true;
+    for (int i = tid; i < CK * (DHP / 4); i += NT) {
+      const int k = i / (DHP / 4), col = i % (DHP / 4) * 4;
+      float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (k < keys && col < A.dh) {
+        const int j = j0 + k;
+        int64_t x[4];
+        load4(x, A.Vc + (((size_t)pt[j / PAGE] * A.n_kv + kvh) * PAGE + j % PAGE) * A.dh + col);
+        float* p = &f.x;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          fit &= x[c] >= -VMAX && x[c] <= VMAX;
+          // 1.5 * 2^23 + x as a float, then exact: (that - 1.5 * 2^23) / 2^16
+          p[c] = __fmaf_rn(__int_as_float(0x4B400000 + (int)x[c]), 1.0f / 65536.0f, -192.0f);
+        }
+      }
+      *(float4*)(vs + k * DHP + col) = f;
+    }
+    fit = __syncthreads_and(fit);
+    // weights: w = (e * ONE) / sum, at most ONE
+    for (int i = tid; i < CK * (RG / 4); i += NT) {
+      const int k = i / (RG / 4), r = i % (RG / 4) * 4;
+      float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (k < keys && r < rows) {
+        const int4 x = *(const int4*)(A.S + ((lk * A.tiles + t) * TILE + (j0 % TILE) + k) * (size_t)A.Rp + r0 + r);
+        const int xs[4] = {x.x, x.y, x.z, x.w};
+        float* p = &f.x;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          if (r + c >= rows) continue;
+          const uint32_t e = (uint32_t)exp32(xs[c] + roff[r + c], lut);
+          if (e) {
+            const uint64_t num = (uint64_t)e << 16;
+            const uint64_t den = rsum[r + c];
+            uint64_t q = (uint64_t)(uint32_t)__float2uint_rz((float)e * 65536.0f * rrcp[r + c]);
+            const int64_t rem = (int64_t)(num - q * den);
+            if (rem < 0) --q;
+            else if ((uint64_t)rem >= den) ++q;
+            p[c] = (float)(uint32_t)q;
+          }
+        }
+      }
+      *(float4*)(ws + k * RG + r) = f;
+    }
+    __syncthreads();
+    if (fit) {
+#pragma unroll 2
+      for (int k = kpart; k < CK; k += kparts) {
+        const ulonglong2 wa = *(const ulonglong2*)(ws + k * RG + unit * 8);
+        const ulonglong2 wb = *(const ulonglong2*)(ws + k * RG + unit * 8 + 4);
+        float v[DPL];
+        if constexpr (DPL == 4) *(float4*)v = *(const float4*)(vs + k * DHP + ln * 4);
+        else *(float2*)v = *(const float2*)(vs + k * DHP + ln * 2);
+#pragma unroll
+        for (int d = 0; d < DPL; ++d) {
+          const uint64_t vv = dup2(v[d]);
+          acc[d][0] = fma2_rd(wa.x, vv, acc[d][0]);
+          acc[d][1] = fma2_rd(wa.y, vv, acc[d][1]);
+          acc[d][2] = fma2_rd(wb.x, vv, acc[d][2]);
+          acc[d][3] = fma2_rd(wb.y, vv, acc[d][3]);
+        }
+      }
+    } else {  // 64-bit terms into this CTA's partial sums
+      for (int i = tid; i < RG * A.dh; i += NT) {
+        const int r = i / A.dh, e = i - r * A.dh;
+        uint64_t o = any_wide ? (uint64_t)part[i] : 0;
+        for (int k = 0; k < keys; ++k) {
+          const int j = j0 + k;
+          const int64_t wt = (int64_t)ws[k * RG + r];
+          if (wt) o += (uint64_t)mulshr(wt, A.Vc[(((size_t)pt[j / PAGE] * A.n_kv + kvh) * PAGE + j % PAGE) * A.dh + e]);
+        }
+        part[i] = (int64_t)o;
+      }
+      any_wide = true;
+    }
+  }
+  __syncthreads();
+  for (int i = tid; i < RG * DHP; i += NT) osum[i] = 0;
+  __syncthreads();
+  if (T > 0)
+#pragma unroll
+    for (int d = 0; d < DPL; ++d)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        int* o = osum + (unit * 8 + 2 * i) * DHP + ln * DPL + d;
+        const int a = (int)(uint32_t)acc[d][i] - 0x4B400000, b = (int)(uint32_t)(acc[d][i] >> 32) - 0x4B400000;
+        if (kparts == 1) o[0] = a, o[DHP] = b;
+        else atomicAdd(o, a), atomicAdd(o + DHP, b);
+      }
+  __syncthreads();
+  const int quads = A.dh / 4;
+  if (A.splits > 1 && T > 0) {
+    for (int i = tid; i < rows * quads; i += NT) {
+      const int r = i / quads, e = i % quads * 4;
+      const int4 x = *(const int4*)(osum + r * DHP + e);
+      longlong2* p = (longlong2*)(part + r * A.dh + e);
+      longlong2 a = make_longlong2(x.x, x.y), b = make_longlong2(x.z, x.w);
+      if (any_wide) {
+        const longlong2 c = p[0], d = p[1];
+        a.x = wadd(a.x, c.x), a.y = wadd(a.y, c.y), b.x = wadd(b.x, d.x), b.y = wadd(b.y, d.y);
+      }
+      __stcg(p, a);
+      __stcg(p + 1, b);
+    }
+    __threadfence();
+    __syncthreads();
+    if (tid == 0) s_last = atomicAdd(A.arrived + lkg, 1) == A.splits - 1;
+    __syncthreads();
+    if (!s_last) return;
+    __threadfence();
+  }
+  const size_t d = (size_t)A.n_heads * A.dh;
+  int need = 0;
+  for (int i = tid; i < rows * quads; i += NT) {
+    const int r = i / quads, e = i % quads * 4, rr = r0 + r;
+    int64_t o[4] = {0, 0, 0, 0};
+    if (T > 0 && A.splits > 1) {
+      const int64_t* p = A.part + lkg * A.splits * (size_t)RG * A.dh + r * A.dh + e;
+      for (int s = 0; s < A.splits; ++s, p += (size_t)RG * A.dh) {
+        const longlong2 a = __ldcg((const longlong2*)p), b = __ldcg((const longlong2*)p + 1);
+        o[0] = wadd(o[0], a.x), o[1] = wadd(o[1], a.y), o[2] = wadd(o[2], b.x), o[3] = wadd(o[3], b.y);
+      }
+    } else if (T > 0) {
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        o[c] = wadd(osum[r * DHP + e + c], any_wide ? part[r * A.dh + e + c] : 0);
+    }
+    const int slot = lane * A.nq + rr / A.G;
+    const size_t col = (size_t)(kvh * A.G + rr % A.G) * A.dh + e;
+    if (A.o_out) {
+      longlong2* p = (longlong2*)(A.o_out + slot * d + col);
+      p[0] = make_longlong2(o[0], o[1]);
+      p[1] = make_longlong2(o[2], o[3]);
+    }
+    if (A.X) need = max(need, store_limbs4(A.X, slot, A.B, d, col, o));
+  }
+  if (A.X && A.lmax) {
+    need = __reduce_max_sync(0xffffffffu, need);
+    if (ln == 0 && need) atomicMax(&s_need, need);
+    __syncthreads();
+    if (tid == 0 && s_need) atomicMax(A.lmax, s_need);
+  }
+}
+
+// Sizes that follow from the shapes; `lanes` of them per launch.
+struct Plan {
+  int lanes, R, Rp, G, tiles, chunks, groups, RG, splits, threads;
+  size_t oS, oM, oG, oSum, oP, oA, bytes;
+};
+
+constexpr size_t WS_TARGET = size_t(1) << 30;  // lanes are batched to about this much workspace
+
+static Plan plan(int lanes, int nq, int n_heads, int n_kv, int dh, int t_lim) {
+  Plan p;
+  p.G = n_heads / n_kv;
+  p.R = nq * p.G;
+  p.groups = (p.R + MAX_RG - 1) / MAX_RG;
+  p.RG = ((p.R + p.groups - 1) / p.groups + 7) / 8 * 8;
+  p.Rp = p.groups * p.RG;
+  p.tiles = (t_lim + TILE - 1) / TILE;
+  p.chunks = p.tiles < 16 ? p.tiles : 16;
+  const size_t per_s = (size_t)n_kv * p.tiles * TILE * p.Rp * 4;
+  p.lanes = (int)(WS_TARGET / per_s);
+  p.lanes = p.lanes < 1 ? 1 : (p.lanes > lanes ? lanes : p.lanes);
+  // enough CTAs for three per SM, at least a tile of keys each
+  const int have = p.lanes * n_kv * p.groups;
+  p.splits = (3 * 148 + have - 1) / have;
+  if (p.splits > p.tiles) p.splits = p.tiles;
+  const int least = (int)(((int64_t)p.tiles * TILE + MAX_RANGE - TILE - 1) / (MAX_RANGE - TILE));
+  if (p.splits < least) p.splits = least;
+  const int units = p.RG / 8;
+  p.threads = 32 * units * (units >= 5 ? 1 : (units >= 3 ? 2 : (units == 2 ? 4 : 8)));
+  size_t o = 0;
+  auto take = [&](size_t n) {
+    const size_t at = o;
+    o += (n + 255) / 256 * 256;
+    return at;
+  };
+  const size_t lk = (size_t)p.lanes * n_kv;
+  p.oS = take((size_t)p.lanes * per_s);
+  p.oM = take(lk * p.tiles * p.Rp * 8);
+  p.oG = take(lk * p.Rp * 8);
+  p.oSum = take(lk * p.chunks * p.Rp * 8);
+  p.oP = take(lk * p.groups * p.splits * p.RG * dh * 8);
+  p.oA = take(lk * p.groups * 4);
+  p.bytes = o;
+  return p;
+}
+
+template <int DHP>
+static int run(Args A, const Plan& p, int lanes, cudaStream_t st) {
+  constexpr int smem_s = 1024 + PLANES * (TILE + RQ) * 128;
+  const int vals = CK * (DHP + p.RG) * 4, sums = p.RG * DHP * 4, smem_v = vals > sums ? vals : sums;
+  cudaError_t e = cudaFuncSetAttribute(k_scores<DHP>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_s);
+  if (e == cudaSuccess)
+    e = cudaFuncSetAttribute(k_values<DHP / 32>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             CK * (DHP + MAX_RG) * 4);
+  if (e != cudaSuccess) return (int)e;
+  for (int l0 = 0; l0 < lanes; l0 += p.lanes) {
+    const int n = lanes - l0 < p.lanes ? lanes - l0 : p.lanes;
+    A.lane0 = l0;
+    int rc = launch_k(k_scores<DHP>, dim3(p.tiles, A.n_kv, n), dim3(NT_S), smem_s, st, A);
+    if (!rc) rc = launch_k(k_sums, dim3(p.chunks, A.n_kv * ((p.R + 31) / 32), n), dim3(NT_B), 0, st, A);
+    if (!rc) rc = launch_k(k_values<DHP / 32>, dim3(p.splits, A.n_kv * p.groups, n), dim3(p.threads), smem_v, st, A);
+    if (rc) return rc;
+  }
+  return 0;
 }
 
 }  // namespace at
 
 extern "C" {
 
+// Workspace bytes of arcb_attn_tree.
 int64_t arcb_attn_tree_ws(int lanes, int nq, int n_heads, int n_kv, int dh, int t_lim) {
-  (void)n_kv;
-  (void)dh;
-  return (int64_t)lanes * nq * n_heads * t_lim * 8;
+  return (int64_t)at::plan(lanes, nq, n_heads, n_kv, dh, t_lim).bytes;
 }
 
 int arcb_attn_tree(const int64_t* q, const int64_t* Kc, const int64_t* Vc, int n_pages, const int* pt,
                    int64_t pt_stride, int width, const int* base, const int* n_tree, const int64_t* mask, int nq,
                    int n_heads, int n_kv, int dh, int64_t attn_scale, int t_lim, int lanes, void* ws, int8_t* X,
                    int* lmax, int64_t* o_out, int* err, void* stream) {
-  if (lanes < 1 || nq < 1 || n_kv < 1 || n_heads < 1 || n_heads % n_kv || dh < 1 || t_lim < 1) return -2;
-  return launch_k(at::k_attn_tree, dim3(n_heads, lanes * nq), dim3(at::NT), 0, (cudaStream_t)stream, q, Kc, Vc,
-                  n_pages, pt, pt_stride, width, base, n_tree, mask, nq, n_heads, n_kv, dh, attn_scale, t_lim,
-                  lanes * nq, (int64_t*)ws, X, lmax, o_out, err);
+  if (lanes < 1 || nq < 1 || n_kv < 1 || n_heads < 1 || n_heads % n_kv || dh < 8 || dh > 128 || dh % 8 || t_lim < 1)
+    return -2;
+  const at::Plan p = at::plan(lanes, nq, n_heads, n_kv, dh, t_lim);
+  if (p.tiles > 65535 * 16 || (int64_t)n_kv * p.groups > 65535 || (int64_t)n_kv * ((p.R + 31) / 32) > 65535 ||
+      p.lanes > 65535)
+    return -2;
+  uint8_t* b = (uint8_t*)ws;
+  at::Args A = {};
+  A.q = q, A.Kc = Kc, A.Vc = Vc, A.pt = pt, A.base = base, A.n_tree = n_tree, A.mask = mask;
+  A.pt_stride = pt_stride, A.attn_scale = attn_scale;
+  A.n_pages = n_pages, A.width = width, A.nq = nq, A.n_heads = n_heads, A.n_kv = n_kv, A.dh = dh, A.t_lim = t_lim;
+  A.B = lanes * nq;
+  A.R = p.R, A.Rp = p.Rp, A.G = p.G, A.tiles = p.tiles, A.chunks = p.chunks, A.groups = p.groups, A.RG = p.RG;
+  A.splits = p.splits;
+  A.S = (int*)(b + p.oS), A.M = (int64_t*)(b + p.oM), A.gmax = (int64_t*)(b + p.oG);
+  A.sums = (uint64_t*)(b + p.oSum), A.part = (int64_t*)(b + p.oP), A.arrived = (int*)(b + p.oA);
+  A.X = X, A.lmax = lmax, A.o_out = o_out, A.err = err;
+  cudaStream_t st = (cudaStream_t)stream;
+  return dh <= 64 ? at::run<64>(A, p, lanes, st) : at::run<128>(A, p, lanes, st);
 }
 
 }  // extern "C"
