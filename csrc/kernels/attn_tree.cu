@@ -49,8 +49,11 @@ constexpr int RQ = 32;              // query rows per MMA group
 constexpr int PLANES = 4;           // digits that take the tensor path
 constexpr int NT_S = 256;           // k_scores threads
 constexpr int NT_B = 256;           // k_sums threads
+constexpr int RB = 64;              // rows per k_sums CTA
+constexpr int NT_V = 256;           // k_values threads, at most
 constexpr int CK = 64;              // keys per k_values chunk
-constexpr int MAX_RG = 64;          // rows per k_values CTA
+constexpr int MAX_RG = 128;         // rows per k_values CTA
+constexpr int SMALL = 1 << 29;      // bound of scores stored as they are
 constexpr int FAR = -(1 << 30);     // a score whose exp is 0
 constexpr int64_t NONE = -(int64_t(1) << 62);  // max of no keys
 constexpr int VMAX = (1 << 22) - (1 << 17);    // values of the single-precision form
@@ -66,10 +69,11 @@ struct Args {
   const int64_t* mask;
   int64_t pt_stride, attn_scale;
   int n_pages, width, nq, n_heads, n_kv, dh, t_lim, B, lane0;
-  int R, Rp, G, tiles, chunks, groups, RG, splits;
+  int R, Rp, G, tiles, chunks, groups, RG, splits, rows_s;
   // workspace
-  int* S;              // [lanes][n_kv][tiles][TILE][Rp] scores relative to M
+  int* S;              // [lanes][n_kv][tiles][TILE][Rp] scores less ref
   int64_t* M;          // [lanes][n_kv][tiles][Rp] max of the tile
+  int64_t* ref;        // [lanes][n_kv][tiles][Rp]: 0, or M where scores are not small
   int64_t* gmax;       // [lanes][n_kv][Rp]
   uint64_t* sums;      // [lanes][n_kv][chunks][Rp]
   int64_t* part;       // [lanes][n_kv][groups][splits][RG][dh]
@@ -87,16 +91,18 @@ __device__ __forceinline__ void load_lut(int2* lut, int nt) {
     lut[i] = make_int2(lo, i < EXP_LUT_N - 1 ? (int)g_exp_lut.v[i + 1] - lo : 0);
   }
 }
-// integer_exp of x <= 0 in 32 bits.
+// integer_exp in 32 bits, x > 0 as 0 (rows behind the last are computed too).
 __device__ __forceinline__ int exp32(int x, const int2* lut) {
-  const int off = max(x + (int)EXP_RANGE, 0);
+  const int off = min(max(x + (int)EXP_RANGE, 0), (int)EXP_RANGE);
   const int2 t = lut[off >> 11];
   return off > 0 ? t.x + ((t.y * (off & 2047)) >> 11) : 0;
 }
-// What a tile's relative scores need added to be relative to the row's max.
-__device__ __forceinline__ int rebase(int64_t tile_max, int64_t row_max) {
-  const int64_t d = tile_max - row_max;
-  return d < FAR ? FAR : (int)d;
+// What a tile's stored scores need added to be relative to the row's max.  A
+// score that is not seen is stored as FAR; both clamps leave its exp 0 and
+// the sum within int32.
+__device__ __forceinline__ int rebase(int64_t ref, int64_t row_max) {
+  const int64_t d = ref - row_max;
+  return d < FAR ? FAR : (d > SMALL ? SMALL : (int)d);
 }
 
 // Four int64 -> digit words: plane l's word in p[l]; the low and high digit
@@ -117,6 +123,13 @@ __device__ __forceinline__ void digits4(const int64_t* x, uint32_t* p, uint32_t&
   p[2] = __byte_perm(t2, t3, 0x5410);
   p[3] = __byte_perm(t2, t3, 0x7632);
 }
+// The largest |x| of four values that fit in 32 bits (one less for a negative x).
+__device__ __forceinline__ uint32_t magnitude4(const int64_t* x) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) m = max(m, (uint32_t)(x[i] ^ (x[i] >> 63)));
+  return m;
+}
 // Digit planes that an or of low digit words needs.
 __device__ __forceinline__ int planes_of(uint32_t lo) { return lo >> 24 ? 4 : lo >> 16 ? 3 : lo >> 8 ? 2 : 1; }
 
@@ -126,22 +139,27 @@ __device__ __forceinline__ void load4(int64_t* x, const int64_t* src) {
 }
 
 // ------------------------------------------------------------------ 1. scores
+// grid (tiles, n_kv * row blocks of rows_s, lanes).
 // DHP: row pitch class of the planes (64 or 128 >= dh).
 template <int DHP>
 __global__ void __launch_bounds__(NT_S, 2) k_scores(const Args A) {
   constexpr int KP = TILE * 128, QP = RQ * 128;  // bytes per plane
   constexpr int TPR = DHP / 4;                   // threads per row
+  constexpr int QN = RQ * TPR / NT_S;            // query quads per thread
   constexpr int TMEM_COLS = 256;                 // (2 * PLANES - 1) * RQ = 224 used
   extern __shared__ __align__(1024) uint8_t dsm[];
   __shared__ int64_t wmax[4][RQ];
-  __shared__ uint64_t qmask[RQ];
+  __shared__ uint64_t qmask[2][RQ];
   __shared__ int pages[TILE / PAGE];
-  __shared__ uint32_t or_k[2], or_q[2][2];  // digit words or-ed: keys; queries of even / odd groups
+  // ors of low and high digit words, largest magnitude: keys; queries of even / odd groups
+  __shared__ uint32_t or_k[3], or_q[2][3];
   __shared__ uint32_t tslot;
   __shared__ __align__(8) uint64_t done;
   __shared__ int s_abort;
   const int tid = threadIdx.x, ln = tid & 31, w = tid >> 5;
-  const int tile = blockIdx.x, kvh = blockIdx.y, lane = A.lane0 + blockIdx.z;
+  const int rbs = (A.R + A.rows_s - 1) / A.rows_s;
+  const int tile = blockIdx.x, kvh = blockIdx.y / rbs, lane = A.lane0 + blockIdx.z;
+  const int r_lo = (blockIdx.y % rbs) * A.rows_s, r_hi = min(A.R, r_lo + A.rows_s);
   const size_t lk = (size_t)blockIdx.z * A.n_kv + kvh;
   const uint32_t kbase = (smem_u32(dsm) + 1023u) & ~1023u, qbase = kbase + PLANES * KP;
   uint8_t* kp = dsm + (kbase - smem_u32(dsm));
@@ -155,7 +173,7 @@ __global__ void __launch_bounds__(NT_S, 2) k_scores(const Args A) {
     fence_barrier_init();
     s_abort = 0;
   }
-  if (tid < 2) or_k[tid] = or_q[0][tid] = 0;
+  if (tid < 3) or_k[tid] = or_q[0][tid] = 0;
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -165,7 +183,7 @@ __global__ void __launch_bounds__(NT_S, 2) k_scores(const Args A) {
   pdl_allow_next();
   const int base = A.base[lane], nt = A.n_tree[lane];
   const int T = tree::lane_keys(base, nt, A.t_lim, A.width);
-  if (tile == 0)
+  if (tile == 0 && r_lo == 0)
     for (int i = tid; i < A.groups; i += NT_S) A.arrived[lk * A.groups + i] = 0;
   const int j0 = tile * TILE;
   const bool live = j0 < T;
@@ -176,10 +194,23 @@ __global__ void __launch_bounds__(NT_S, 2) k_scores(const Args A) {
   }
   __syncthreads();
   if (live) {
-    // ---- K digit planes: a warp reads 32 / TPR whole rows at a time
-    constexpr int RPW = 32 / TPR, STEPS = TILE / (8 * RPW), UN = 8;
     const int col = (ln % TPR) * 4;
-    uint32_t lo = 0, hi = 0;
+    // ---- the first query rows' loads in flight beside the keys'
+    int64_t xq[QN][4];
+    auto load_q = [&](int r0) {
+#pragma unroll
+      for (int i = 0; i < QN; ++i) {
+        const int rr = r0 + tid / TPR + i * (NT_S / TPR);
+        if (rr < r_hi && col < A.dh)
+          load4(xq[i], A.q + ((size_t)(lane * A.nq + rr / A.G) * A.n_heads + kvh * A.G + rr % A.G) * A.dh + col);
+        else
+          xq[i][0] = xq[i][1] = xq[i][2] = xq[i][3] = 0;
+      }
+    };
+    load_q(r_lo);
+    // ---- K digit planes: a warp reads 32 / TPR whole rows at a time
+    constexpr int RPW = 32 / TPR, STEPS = TILE / (8 * RPW), UN = STEPS < 8 ? STEPS : 8;
+    uint32_t lo = 0, hi = 0, mag = 0;
 #pragma unroll 1
     for (int s0 = 0; s0 < STEPS; s0 += UN) {
       int64_t x[UN][4];
@@ -196,6 +227,7 @@ __global__ void __launch_bounds__(NT_S, 2) k_scores(const Args A) {
         const int r = ((s0 + u) * 8 + w) * RPW + ln / TPR;
         uint32_t d[4];
         digits4(x[u], d, lo, hi);
+        mag = max(mag, magnitude4(x[u]));
         const uint32_t at = r * 128 + (((col >> 4) ^ (r & 7)) << 4) + (col & 15);
 #pragma unroll
         for (int l = 0; l < PLANES; ++l) *(uint32_t*)(kp + l * KP + at) = d[l];
@@ -203,37 +235,41 @@ __global__ void __launch_bounds__(NT_S, 2) k_scores(const Args A) {
     }
     lo = __reduce_or_sync(0xffffffffu, lo);
     hi = __reduce_or_sync(0xffffffffu, hi);
+    mag = __reduce_max_sync(0xffffffffu, mag);
     if (ln == 0) {
       atomicOr(&or_k[0], lo);
       atomicOr(&or_k[1], hi);
+      atomicMax(&or_k[2], mag);
     }
     const int j = j0 + (w & 3) * 32 + ln;  // this thread's key in the epilogue
     int* Srow = A.S + ((lk * A.tiles + tile) * TILE + (w & 3) * 32 + ln) * A.Rp;
     const int kend = (A.dh + 31) / 32;
+    const bool all_seen = j0 + TILE <= base;  // every key of the tile is below the tree
     uint32_t parity = 0;
-    for (int r0 = 0, g = 0; r0 < A.R; r0 += RQ, g ^= 1) {
-      const int rows = min(RQ, A.R - r0), nmma = rows > 16 ? 32 : 16;
-      __syncthreads();  // the last group's epilogue and the planes' readers are done
-      // ---- query digit planes and masks of rows [r0, r0 + 32)
-      lo = hi = 0;
-      for (int r = tid / TPR; r < nmma; r += NT_S / TPR) {
-        int64_t x[4] = {0, 0, 0, 0};
-        const int rr = r0 + r;
-        if (r < rows && col < A.dh)
-          load4(x, A.q + ((size_t)(lane * A.nq + rr / A.G) * A.n_heads + kvh * A.G + rr % A.G) * A.dh + col);
+    for (int r0 = r_lo, g = 0; r0 < r_hi; r0 += RQ, g ^= 1) {
+      const int rows = min(RQ, r_hi - r0), nmma = rows > 16 ? 32 : 16;
+      // ---- query digit planes and masks of rows [r0, r0 + 32); the last
+      // group's products are done, so its planes are free
+      lo = hi = mag = 0;
+#pragma unroll
+      for (int i = 0; i < QN; ++i) {
+        const int r = tid / TPR + i * (NT_S / TPR);
         uint32_t d[4];
-        digits4(x, d, lo, hi);
+        digits4(xq[i], d, lo, hi);
+        mag = max(mag, magnitude4(xq[i]));
         const uint32_t at = r * 128 + (((col >> 4) ^ (r & 7)) << 4) + (col & 15);
 #pragma unroll
         for (int l = 0; l < PLANES; ++l) *(uint32_t*)(qp + l * QP + at) = d[l];
       }
-      if (tid < rows) qmask[tid] = (uint64_t)A.mask[(size_t)lane * A.nq + (r0 + tid) / A.G];
-      if (tid >= rows && tid < RQ) qmask[tid] = 0;
+      if (!all_seen && tid < RQ)
+        qmask[g][tid] = tid < rows ? (uint64_t)A.mask[(size_t)lane * A.nq + (r0 + tid) / A.G] : 0;
       lo = __reduce_or_sync(0xffffffffu, lo);
       hi = __reduce_or_sync(0xffffffffu, hi);
+      mag = __reduce_max_sync(0xffffffffu, mag);
       if (ln == 0) {
         atomicOr(&or_q[g][0], lo);
         atomicOr(&or_q[g][1], hi);
+        atomicMax(&or_q[g][2], mag);
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       tc_fence_before();
@@ -241,7 +277,10 @@ __global__ void __launch_bounds__(NT_S, 2) k_scores(const Args A) {
       tc_fence_after();
       const int lk_n = planes_of(or_k[0]), lq_n = planes_of(or_q[g][0]);
       const bool wide = (or_k[1] | or_q[g][1]) != 0;
-      if (tid < 2) or_q[g ^ 1][tid] = 0;  // its readers passed two barriers ago
+      // |q.k| <= dh * max|k| * max|q| < 2^47 and scale <= ONE / 4: 32 bits hold
+      // every step below, and |score| <= 2^29
+      const bool small = !wide && A.attn_scale >= 0 && A.attn_scale <= ONE / 4 &&
+                         ((uint64_t)or_k[2] + 1) * ((uint64_t)or_q[g][2] + 1) < (uint64_t(1) << 47) / A.dh;
       if (!wide) {
         if (tid == 0) {
           const uint32_t idesc = idesc_i8(TILE, nmma);
@@ -254,83 +293,126 @@ __global__ void __launch_bounds__(NT_S, 2) k_scores(const Args A) {
                        (k > 0 || (a > 0 && b < lq_n - 1)) ? 1u : 0u);
           mma_commit(smem_u32(&done));
         }
+        if (r0 + RQ < r_hi) load_q(r0 + RQ);  // in flight beside the products and the epilogue
         if (!mbar_wait(smem_u32(&done), parity)) s_abort = 1;
         parity ^= 1;
         tc_fence_after();
+      } else if (r0 + RQ < r_hi) {
+        load_q(r0 + RQ);
       }
       // ---- scores of 16 rows per warp: rows c0 .. c0 + 15 of the group
-      const int c0 = (w >> 2) * 16;
-      int64_t sc[16];
+      const int c0 = (w >> 2) * 16, ns = lk_n + lq_n - 1;
+      const uint32_t tcol = tmem + ((uint32_t)(w & 3) << 21) + c0;
       if (c0 < rows) {
-        if (!wide) {
-          const int ns = lk_n + lq_n - 1;
+        uint32_t seen = 0xffff;  // bit i: row c0 + i sees this key
+        if (!all_seen) {
+          seen = 0;
 #pragma unroll
-          for (int i = 0; i < 16; ++i) sc[i] = 0;
-          for (int s = 0; s < ns; ++s) {
-            uint32_t r[16];
-            tmem_ld16(tmem + ((uint32_t)(w & 3) << 21) + s * RQ + c0, r);
+          for (int i = 0; i < 16; ++i)
+            if (tree::visible(j, base, nt, qmask[g][c0 + i])) seen |= 1u << i;
+        }
+        int out[16];
+        int64_t m64 = NONE;  // lane i: max of row c0 + i over the warp's keys
+        if (small) {
+          // dot >> 16 = D_2 + (D_3 << 8) + (D_4 << 16) + .. + ((D_0 + (D_1 << 8)) >> 16): modulo 2^32
+          uint32_t r[16], t[16];
+          tmem_ld16(tcol, t);
+          if (ns > 1) {
+            tmem_ld16(tcol + RQ, r);
             tmem_ld_wait();
 #pragma unroll
-            for (int i = 0; i < 16; ++i) sc[i] += (int64_t)((uint64_t)(int64_t)(int)r[i] << (8 * s));
+            for (int i = 0; i < 16; ++i) t[i] += r[i] << 8;
+          } else {
+            tmem_ld_wait();
+          }
+#pragma unroll
+          for (int i = 0; i < 16; ++i) t[i] = (uint32_t)((int)t[i] >> 16);
+#pragma unroll 1
+          for (int s = 2; s < ns; ++s) {
+            tmem_ld16(tcol + s * RQ, r);
+            tmem_ld_wait();
+            const int sh = 8 * s - 16;  // up to 32: a shift of 32 gives 0, right modulo 2^32
+#pragma unroll
+            for (int i = 0; i < 16; ++i) t[i] += __funnelshift_lc(0u, r[i], sh);
+          }
+          const int sc = (int)A.attn_scale << 16;  // (x * scale) >> 16 = the high word of x * (scale << 16)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            out[i] = seen >> i & 1 ? __mulhi((int)t[i], sc) : FAR;
+            const int m = __reduce_max_sync(0xffffffffu, out[i]);
+            if (ln == i) m64 = m == FAR ? NONE : m;
           }
         } else {
-          const int p = pages[(j - j0) / PAGE];
-          const int64_t* kr = A.Kc + (((size_t)(p < 0 ? 0 : p) * A.n_kv + kvh) * PAGE + j % PAGE) * A.dh;
-          for (int i = 0; i < 16; ++i) {
-            uint64_t d = 0;
-            const int rr = r0 + c0 + i;
-            if (p >= 0 && j < T && c0 + i < rows) {
-              const int64_t* qr = A.q + ((size_t)(lane * A.nq + rr / A.G) * A.n_heads + kvh * A.G + rr % A.G) * A.dh;
-              for (int e = 0; e < A.dh; ++e) d += (uint64_t)wmul(qr[e], kr[e]);
+          int64_t sc[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) sc[i] = 0;
+          if (!wide) {
+#pragma unroll 1
+            for (int s = 0; s < ns; ++s) {
+              uint32_t r[16];
+              tmem_ld16(tcol + s * RQ, r);
+              tmem_ld_wait();
+#pragma unroll
+              for (int i = 0; i < 16; ++i) sc[i] += (int64_t)((uint64_t)(int64_t)(int)r[i] << (8 * s));
             }
-#pragma unroll
-            for (int m = 0; m < 16; ++m)
-              if (m == i) sc[m] = (int64_t)d;
-          }
-        }
-        bool fits = true;
-        uint32_t seen = 0;  // bit i: row c0 + i sees this key
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          sc[i] = attn_score(sc[i], A.attn_scale);
-          fits &= sc[i] == (int64_t)(int)sc[i];
-          if (tree::visible(j, base, nt, qmask[c0 + i]) && c0 + i < rows) seen |= 1u << i;
-        }
-        fits = __all_sync(0xffffffffu, fits);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const bool see = seen >> i & 1;
-          int64_t m;
-          if (fits) {
-            m = __reduce_max_sync(0xffffffffu, see ? (int)sc[i] : INT32_MIN);
-            if (!__any_sync(0xffffffffu, see)) m = NONE;
           } else {
-            m = see ? sc[i] : NONE;
+            const int p = pages[(j - j0) / PAGE];
+            const int64_t* kr = A.Kc + (((size_t)(p < 0 ? 0 : p) * A.n_kv + kvh) * PAGE + j % PAGE) * A.dh;
+#pragma unroll 1
+            for (int i = 0; i < 16; ++i) {
+              uint64_t d = 0;
+              const int rr = r0 + c0 + i;
+              if (p >= 0 && j < T && c0 + i < rows) {
+                const int64_t* qr =
+                    A.q + ((size_t)(lane * A.nq + rr / A.G) * A.n_heads + kvh * A.G + rr % A.G) * A.dh;
+                for (int e = 0; e < A.dh; ++e) d += (uint64_t)wmul(qr[e], kr[e]);
+              }
+#pragma unroll
+              for (int m = 0; m < 16; ++m)
+                if (m == i) sc[m] = (int64_t)d;
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            sc[i] = attn_score(sc[i], A.attn_scale);
+            int64_t m = seen >> i & 1 ? sc[i] : NONE;
 #pragma unroll
             for (int b = 16; b >= 1; b >>= 1) {
               const int64_t o = shfl_xor_i64(m, b);
               m = o > m ? o : m;
             }
+            if (ln == i) m64 = m;
           }
-          if (ln == 0) wmax[w & 3][c0 + i] = m;
-        }
-        tc_fence_before();
-        // the four warps of these 16 rows
-        asm volatile("bar.sync %0, 128;" ::"r"(1 + (w >> 2)) : "memory");
-        int out[16];
+          if (ln < 16) wmax[w & 3][c0 + ln] = m64;
+          asm volatile("bar.sync %0, 128;" ::"r"(1 + (w >> 2)) : "memory");  // the four warps of these rows
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          int64_t m = wmax[0][c0 + i];
+          for (int i = 0; i < 16; ++i) {
+            int64_t m = wmax[0][c0 + i];
 #pragma unroll
-          for (int k = 1; k < 4; ++k) m = wmax[k][c0 + i] > m ? wmax[k][c0 + i] : m;
-          const int64_t d = sc[i] - m;
-          out[i] = (seen >> i & 1) && d > FAR ? (int)d : FAR;
-          if ((w & 3) == 0 && ln == i && c0 + i < rows) A.M[(lk * A.tiles + tile) * A.Rp + r0 + c0 + i] = m;
+            for (int k = 1; k < 4; ++k) m = wmax[k][c0 + i] > m ? wmax[k][c0 + i] : m;
+            const int64_t d = sc[i] - m;
+            out[i] = (seen >> i & 1) && d > FAR ? (int)d : FAR;
+          }
+          asm volatile("bar.sync %0, 128;" ::"r"(1 + (w >> 2)) : "memory");
         }
+        if (ln < 16) wmax[w & 3][c0 + ln] = m64;
 #pragma unroll
         for (int i = 0; i < 16; i += 4)
           if (c0 + i < rows) *(int4*)(Srow + r0 + c0 + i) = make_int4(out[i], out[i + 1], out[i + 2], out[i + 3]);
       }
+      tc_fence_before();
+      __syncthreads();  // wmax; this group's accumulators and query planes are read
+      tc_fence_after();
+      if (tid < rows) {
+        int64_t m = wmax[0][tid];
+#pragma unroll
+        for (int k = 1; k < 4; ++k) m = wmax[k][tid] > m ? wmax[k][tid] : m;
+        const size_t at = (lk * A.tiles + tile) * A.Rp + r0 + tid;
+        A.M[at] = m;
+        A.ref[at] = small ? 0 : m;
+      }
+      if (tid < 3) or_q[g ^ 1][tid] = 0;  // read before the last group's end, next or-ed after this one's writes
+      __syncthreads();
     }
   }
   tc_fence_before();
@@ -343,46 +425,69 @@ __global__ void __launch_bounds__(NT_S, 2) k_scores(const Args A) {
 }
 
 // -------------------------------------------------------------------- 2. sums
-// grid (chunks, n_kv * row blocks of 32, lanes): lane = row, warps over keys.
+// grid (chunks, n_kv * row blocks of RB, lanes): a thread takes four rows of
+// every sixteenth key.
 __global__ void __launch_bounds__(NT_B) k_sums(const Args A) {
+  constexpr int Q = RB / 4, KL = NT_B / Q;
   __shared__ int2 lut[EXP_LUT_N];
-  __shared__ int64_t red[NT_B / 32][32];
+  __shared__ int64_t red[KL][RB];
+  __shared__ int64_t rmax[RB];
   load_lut(lut, NT_B);
   pdl_wait_dep();
   pdl_allow_next();
-  const int ln = threadIdx.x & 31, w = threadIdx.x >> 5;
-  const int rb = (A.R + 31) / 32, kvh = blockIdx.y / rb, r = (blockIdx.y % rb) * 32 + ln;
+  const int tid = threadIdx.x, rb = (A.R + RB - 1) / RB, kvh = blockIdx.y / rb, r0 = (blockIdx.y % rb) * RB;
   const int lane = A.lane0 + blockIdx.z, T = tree::lane_keys(A.base[lane], A.n_tree[lane], A.t_lim, A.width);
   if (T <= 0) return;
   const size_t lk = (size_t)blockIdx.z * A.n_kv + kvh;
   const int nt = (T + TILE - 1) / TILE;
   const int t0 = (int)((int64_t)blockIdx.x * nt / A.chunks), t1 = (int)((int64_t)(blockIdx.x + 1) * nt / A.chunks);
-  const bool row = r < A.R;
-  const int64_t* M = A.M + lk * A.tiles * A.Rp + r;
-  int64_t m = NONE;
-  if (row)
-    for (int t = w; t < nt; t += NT_B / 32) m = max(m, M[(size_t)t * A.Rp]);
-  red[w][ln] = m;
-  __syncthreads();
-#pragma unroll
-  for (int k = 0; k < NT_B / 32; ++k) m = max(m, red[k][ln]);
-  __syncthreads();
-  uint64_t s = 0;
-  if (row) {
-    if (blockIdx.x == 0 && w == 0) A.gmax[lk * A.Rp + r] = m;
-    for (int t = t0; t < t1; ++t) {
-      const int off = rebase(M[(size_t)t * A.Rp], m);
-      const int* S = A.S + ((lk * A.tiles + t) * TILE) * A.Rp + r;
+  const int64_t* M = A.M + lk * A.tiles * A.Rp + r0;
+  const int64_t* ref = A.ref + lk * A.tiles * A.Rp + r0;
+  {
+    const int r = tid % RB;
+    int64_t m = NONE;
+    if (r0 + r < A.R)
 #pragma unroll 4
-      for (int k = w; k < TILE; k += NT_B / 32) s += (uint64_t)exp32(S[(size_t)k * A.Rp] + off, lut);
-    }
+      for (int t = tid / RB; t < nt; t += NT_B / RB) m = max(m, M[(size_t)t * A.Rp + r]);
+    red[tid / RB][r] = m;
   }
-  red[w][ln] = (int64_t)s;
   __syncthreads();
-  if (w == 0 && row) {
+  if (tid < RB) {
+    int64_t m = red[0][tid];
 #pragma unroll
-    for (int k = 1; k < NT_B / 32; ++k) s += (uint64_t)red[k][ln];
-    A.sums[(lk * A.chunks + blockIdx.x) * A.Rp + r] = s;
+    for (int k = 1; k < NT_B / RB; ++k) m = max(m, red[k][tid]);
+    rmax[tid] = m;
+    if (blockIdx.x == 0 && r0 + tid < A.R) A.gmax[lk * A.Rp + r0 + tid] = m;
+  }
+  __syncthreads();
+  const int q = tid % Q * 4, k0 = tid / Q;
+  uint64_t s[4] = {0, 0, 0, 0};
+  if (r0 + q < A.R)
+    for (int t = t0; t < t1; ++t) {
+      int off[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) off[c] = r0 + q + c < A.R ? rebase(ref[(size_t)t * A.Rp + q + c], rmax[q + c]) : FAR;
+      const int* S = A.S + ((lk * A.tiles + t) * TILE + k0) * (size_t)A.Rp + r0 + q;
+      uint32_t p[4] = {0, 0, 0, 0};  // of TILE / KL exps
+#pragma unroll
+      for (int k = 0; k < TILE / KL; ++k) {
+        const int4 x = *(const int4*)(S + (size_t)k * KL * A.Rp);
+        p[0] += exp32(x.x + off[0], lut);
+        p[1] += exp32(x.y + off[1], lut);
+        p[2] += exp32(x.z + off[2], lut);
+        p[3] += exp32(x.w + off[3], lut);
+      }
+#pragma unroll
+      for (int c = 0; c < 4; ++c) s[c] += p[c];
+    }
+#pragma unroll
+  for (int c = 0; c < 4; ++c) red[k0][q + c] = (int64_t)s[c];
+  __syncthreads();
+  if (tid < RB && r0 + tid < A.R) {
+    uint64_t x = 0;
+#pragma unroll
+    for (int k = 0; k < KL; ++k) x += (uint64_t)red[k][tid];
+    A.sums[(lk * A.chunks + blockIdx.x) * A.Rp + r0 + tid] = x;
   }
 }
 
@@ -421,25 +526,25 @@ __device__ __forceinline__ int store_limbs4(int8_t* X, int slot, int B, size_t l
   return need;
 }
 
-// grid (splits, n_kv * groups, lanes).  A warp takes 8 rows (unit) x all dims,
-// lane = DPL consecutive dims; KPART warps per unit take every KPART-th key.
-template <int DPL>
-__global__ void __launch_bounds__(256) k_values(const Args A) {
+// grid (splits, n_kv * groups, lanes).  A warp takes UR rows (unit) x all dims,
+// lane = DPL consecutive dims; kparts warps per unit take every kparts-th key.
+template <int DPL, int UR>
+__global__ void __launch_bounds__(NT_V, 2) k_values(const Args A) {
   extern __shared__ __align__(1024) uint8_t dsm[];
-  constexpr int DHP = 32 * DPL;
+  constexpr int DHP = 32 * DPL, UP = UR / 2;
   __shared__ int2 lut[EXP_LUT_N];
   __shared__ int64_t rmax[MAX_RG];
   __shared__ uint64_t rsum[MAX_RG];
-  __shared__ float rrcp[MAX_RG];
+  __shared__ float rrcp[MAX_RG];   // ONE / sum
   __shared__ int roff[MAX_RG];
-  __shared__ int s_last, s_need;
+  __shared__ int s_last, s_need, s_long;
   const int NT = blockDim.x, tid = threadIdx.x, ln = tid & 31, w = tid >> 5;
-  const int RG = A.RG, units = RG / 8, unit = w % units, kpart = w / units, kparts = NT / 32 / units;
+  const int RG = A.RG, units = RG / UR, unit = w % units, kpart = w / units, kparts = NT / 32 / units;
   float* vs = (float*)dsm;                                   // [CK][DHP] v / 2^16
   float* ws = vs + CK * DHP;                                 // [CK][RG] weights
   int* osum = (int*)dsm;                                     // [RG][DHP] at the end
   load_lut(lut, NT);
-  if (tid == 0) s_need = 0;
+  if (tid == 0) s_need = s_long = 0;
   pdl_wait_dep();
   pdl_allow_next();
   const int kvh = blockIdx.y / A.groups, grp = blockIdx.y % A.groups, r0 = grp * RG, rows = min(RG, A.R - r0);
@@ -460,25 +565,29 @@ __global__ void __launch_bounds__(256) k_values(const Args A) {
     const bool row = tid < rows;
     uint64_t s = 0;
     if (row)
+#pragma unroll 4
       for (int c = 0; c < A.chunks; ++c) s += A.sums[(lk * A.chunks + c) * A.Rp + r0 + tid];
     rmax[tid] = row ? A.gmax[lk * A.Rp + r0 + tid] : NONE;
     rsum[tid] = s ? s : 1;  // a row without keys: every exp is 0
-    rrcp[tid] = __frcp_rn((float)(int64_t)rsum[tid]);
+    rrcp[tid] = 65536.0f * __frcp_rn((float)(int64_t)rsum[tid]);
+    if (s >> 30) s_long = 1;
   }
-  uint64_t acc[DPL][4];  // pairs of rows
+  uint64_t acc[DPL][UP];  // pairs of rows
 #pragma unroll
   for (int d = 0; d < DPL; ++d)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) acc[d][i] = dup2(12582912.0f);
+    for (int i = 0; i < UP; ++i) acc[d][i] = dup2(12582912.0f);
   int64_t* part = A.part + (lkg * A.splits + blockIdx.x) * (size_t)RG * A.dh;
   bool any_wide = false;
   for (int j0 = t0 * TILE; j0 < min(t1 * TILE, T); j0 += CK) {
     const int t = j0 / TILE, keys = min(CK, T - j0);
     __syncthreads();  // rsum / the last chunk's readers
     if (j0 % TILE == 0 && tid < RG)
-      roff[tid] = tid < rows ? rebase(A.M[(lk * A.tiles + t) * A.Rp + r0 + tid], rmax[tid]) : FAR;
-    // values: v / 2^16 in single precision, 0 past the last key and dim
-    bool fit = true;
+      roff[tid] = tid < rows ? rebase(A.ref[(lk * A.tiles + t) * A.Rp + r0 + tid], rmax[tid]) : FAR;
+    // values: v / 2^16 in single precision, 0 past the last key and dim.  y = v + VMAX
+    // in [0, 2 VMAX] as the low bits of 2^23 + y, then exact: (that - 2^23 - VMAX) / 2^16
+    uint32_t high = 0, most = 0;
+#pragma unroll 4
     for (int i = tid; i < CK * (DHP / 4); i += NT) {
       const int k = i / (DHP / 4), col = i % (DHP / 4) * 4;
       float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -489,15 +598,20 @@ __global__ void __launch_bounds__(256) k_values(const Args A) {
         float* p = &f.x;
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          fit &= x[c] >= -VMAX && x[c] <= VMAX;
-          // 1.5 * 2^23 + x as a float, then exact: (that - 1.5 * 2^23) / 2^16
-          p[c] = __fmaf_rn(__int_as_float(0x4B400000 + (int)x[c]), 1.0f / 65536.0f, -192.0f);
+          const uint64_t y = (uint64_t)x[c] + VMAX;
+          high |= (uint32_t)(y >> 32);
+          most = max(most, (uint32_t)y);
+          p[c] = __fmaf_rn(__uint_as_float(0x4B000000u + (uint32_t)y), 1.0f / 65536.0f,
+                           -(float)(8388608 + VMAX) / 65536.0f);
         }
       }
       *(float4*)(vs + k * DHP + col) = f;
     }
-    fit = __syncthreads_and(fit);
-    // weights: w = (e * ONE) / sum, at most ONE
+    const bool fit = __syncthreads_and(high == 0 && most <= 2 * VMAX);
+    // weights floor(e * ONE / sum), at most ONE: the estimate e * (ONE / sum) in single
+    // precision is within 1, the remainder decides (32 bits hold it for sums below 2^30)
+    const bool lng = s_long != 0;
+#pragma unroll 2
     for (int i = tid; i < CK * (RG / 4); i += NT) {
       const int k = i / (RG / 4), r = i % (RG / 4) * 4;
       float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -507,17 +621,20 @@ __global__ void __launch_bounds__(256) k_values(const Args A) {
         float* p = &f.x;
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          if (r + c >= rows) continue;
-          const uint32_t e = (uint32_t)exp32(xs[c] + roff[r + c], lut);
-          if (e) {
-            const uint64_t num = (uint64_t)e << 16;
-            const uint64_t den = rsum[r + c];
-            uint64_t q = (uint64_t)(uint32_t)__float2uint_rz((float)e * 65536.0f * rrcp[r + c]);
-            const int64_t rem = (int64_t)(num - q * den);
-            if (rem < 0) --q;
-            else if ((uint64_t)rem >= den) ++q;
-            p[c] = (float)(uint32_t)q;
+          const uint32_t e = r + c < rows ? (uint32_t)exp32(xs[c] + roff[r + c], lut) : 0u;
+          const float ef = __uint_as_float(0x4B000000u + e) - 8388608.0f;
+          const float qf = __fmaf_rd(ef, rrcp[r + c], 8388608.0f);
+          const uint32_t q = __float_as_uint(qf) - 0x4B000000u;
+          float wt = qf - 8388608.0f;
+          if (!lng) {
+            const uint32_t den = (uint32_t)rsum[r + c];
+            const int rem = (int)((e << 16) - q * den);
+            wt += rem < 0 ? -1.0f : (rem >= (int)den ? 1.0f : 0.0f);
+          } else {
+            const int64_t rem = (int64_t)(((uint64_t)e << 16) - (uint64_t)q * rsum[r + c]);
+            wt += rem < 0 ? -1.0f : (rem >= (int64_t)rsum[r + c] ? 1.0f : 0.0f);
           }
+          p[c] = wt;
         }
       }
       *(float4*)(ws + k * RG + r) = f;
@@ -526,18 +643,20 @@ __global__ void __launch_bounds__(256) k_values(const Args A) {
     if (fit) {
 #pragma unroll 2
       for (int k = kpart; k < CK; k += kparts) {
-        const ulonglong2 wa = *(const ulonglong2*)(ws + k * RG + unit * 8);
-        const ulonglong2 wb = *(const ulonglong2*)(ws + k * RG + unit * 8 + 4);
+        uint64_t wp[UP];
+#pragma unroll
+        for (int i = 0; i < UP; i += 2) {
+          const ulonglong2 x = *(const ulonglong2*)(ws + k * RG + unit * UR + 2 * i);
+          wp[i] = x.x, wp[i + 1] = x.y;
+        }
         float v[DPL];
         if constexpr (DPL == 4) *(float4*)v = *(const float4*)(vs + k * DHP + ln * 4);
         else *(float2*)v = *(const float2*)(vs + k * DHP + ln * 2);
 #pragma unroll
         for (int d = 0; d < DPL; ++d) {
           const uint64_t vv = dup2(v[d]);
-          acc[d][0] = fma2_rd(wa.x, vv, acc[d][0]);
-          acc[d][1] = fma2_rd(wa.y, vv, acc[d][1]);
-          acc[d][2] = fma2_rd(wb.x, vv, acc[d][2]);
-          acc[d][3] = fma2_rd(wb.y, vv, acc[d][3]);
+#pragma unroll
+          for (int i = 0; i < UP; ++i) acc[d][i] = fma2_rd(wp[i], vv, acc[d][i]);
         }
       }
     } else {  // 64-bit terms into this CTA's partial sums
@@ -561,8 +680,8 @@ __global__ void __launch_bounds__(256) k_values(const Args A) {
 #pragma unroll
     for (int d = 0; d < DPL; ++d)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        int* o = osum + (unit * 8 + 2 * i) * DHP + ln * DPL + d;
+      for (int i = 0; i < UP; ++i) {
+        int* o = osum + (unit * UR + 2 * i) * DHP + ln * DPL + d;
         const int a = (int)(uint32_t)acc[d][i] - 0x4B400000, b = (int)(uint32_t)(acc[d][i] >> 32) - 0x4B400000;
         if (kparts == 1) o[0] = a, o[DHP] = b;
         else atomicAdd(o, a), atomicAdd(o + DHP, b);
@@ -624,8 +743,8 @@ __global__ void __launch_bounds__(256) k_values(const Args A) {
 
 // Sizes that follow from the shapes; `lanes` of them per launch.
 struct Plan {
-  int lanes, R, Rp, G, tiles, chunks, groups, RG, splits, threads;
-  size_t oS, oM, oG, oSum, oP, oA, bytes;
+  int lanes, R, Rp, G, tiles, chunks, groups, RG, splits, threads, unit, rows_s;
+  size_t oS, oM, oR, oG, oSum, oP, oA, bytes;
 };
 
 constexpr size_t WS_TARGET = size_t(1) << 30;  // lanes are batched to about this much workspace
@@ -635,21 +754,25 @@ static Plan plan(int lanes, int nq, int n_heads, int n_kv, int dh, int t_lim) {
   p.G = n_heads / n_kv;
   p.R = nq * p.G;
   p.groups = (p.R + MAX_RG - 1) / MAX_RG;
-  p.RG = ((p.R + p.groups - 1) / p.groups + 7) / 8 * 8;
+  p.unit = p.R <= 8 ? 8 : 16;
+  p.RG = ((p.R + p.groups - 1) / p.groups + p.unit - 1) / p.unit * p.unit;
   p.Rp = p.groups * p.RG;
   p.tiles = (t_lim + TILE - 1) / TILE;
   p.chunks = p.tiles < 16 ? p.tiles : 16;
   const size_t per_s = (size_t)n_kv * p.tiles * TILE * p.Rp * 4;
   p.lanes = (int)(WS_TARGET / per_s);
   p.lanes = p.lanes < 1 ? 1 : (p.lanes > lanes ? lanes : p.lanes);
-  // enough CTAs for three per SM, at least a tile of keys each
+  // enough CTAs for two rounds of two per SM, at least a tile of keys each
   const int have = p.lanes * n_kv * p.groups;
-  p.splits = (3 * 148 + have - 1) / have;
+  p.splits = (4 * 148 + have - 1) / have;
   if (p.splits > p.tiles) p.splits = p.tiles;
   const int least = (int)(((int64_t)p.tiles * TILE + MAX_RANGE - TILE - 1) / (MAX_RANGE - TILE));
   if (p.splits < least) p.splits = least;
-  const int units = p.RG / 8;
+  const int units = p.RG / p.unit;
   p.threads = 32 * units * (units >= 5 ? 1 : (units >= 3 ? 2 : (units == 2 ? 4 : 8)));
+  // score CTAs take all rows of their tile unless that leaves SMs idle (two CTAs each)
+  const int blocks = p.tiles * n_kv * p.lanes, want = (4 * 148 + blocks - 1) / blocks, most = (p.R + 63) / 64;
+  p.rows_s = ((p.R + (want < most ? want : most) - 1) / (want < most ? want : most) + RQ - 1) / RQ * RQ;
   size_t o = 0;
   auto take = [&](size_t n) {
     const size_t at = o;
@@ -659,6 +782,7 @@ static Plan plan(int lanes, int nq, int n_heads, int n_kv, int dh, int t_lim) {
   const size_t lk = (size_t)p.lanes * n_kv;
   p.oS = take((size_t)p.lanes * per_s);
   p.oM = take(lk * p.tiles * p.Rp * 8);
+  p.oR = take(lk * p.tiles * p.Rp * 8);
   p.oG = take(lk * p.Rp * 8);
   p.oSum = take(lk * p.chunks * p.Rp * 8);
   p.oP = take(lk * p.groups * p.splits * p.RG * dh * 8);
@@ -667,21 +791,21 @@ static Plan plan(int lanes, int nq, int n_heads, int n_kv, int dh, int t_lim) {
   return p;
 }
 
-template <int DHP>
+template <int DHP, int UR>
 static int run(Args A, const Plan& p, int lanes, cudaStream_t st) {
   constexpr int smem_s = 1024 + PLANES * (TILE + RQ) * 128;
   const int vals = CK * (DHP + p.RG) * 4, sums = p.RG * DHP * 4, smem_v = vals > sums ? vals : sums;
+  const auto kv = k_values<DHP / 32, UR>;
   cudaError_t e = cudaFuncSetAttribute(k_scores<DHP>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_s);
-  if (e == cudaSuccess)
-    e = cudaFuncSetAttribute(k_values<DHP / 32>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             CK * (DHP + MAX_RG) * 4);
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(kv, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_v);
   if (e != cudaSuccess) return (int)e;
   for (int l0 = 0; l0 < lanes; l0 += p.lanes) {
     const int n = lanes - l0 < p.lanes ? lanes - l0 : p.lanes;
     A.lane0 = l0;
-    int rc = launch_k(k_scores<DHP>, dim3(p.tiles, A.n_kv, n), dim3(NT_S), smem_s, st, A);
-    if (!rc) rc = launch_k(k_sums, dim3(p.chunks, A.n_kv * ((p.R + 31) / 32), n), dim3(NT_B), 0, st, A);
-    if (!rc) rc = launch_k(k_values<DHP / 32>, dim3(p.splits, A.n_kv * p.groups, n), dim3(p.threads), smem_v, st, A);
+    int rc = launch_k(k_scores<DHP>, dim3(p.tiles, A.n_kv * ((p.R + p.rows_s - 1) / p.rows_s), n), dim3(NT_S), smem_s,
+                      st, A);
+    if (!rc) rc = launch_k(k_sums, dim3(p.chunks, A.n_kv * ((p.R + RB - 1) / RB), n), dim3(NT_B), 0, st, A);
+    if (!rc) rc = launch_k(kv, dim3(p.splits, A.n_kv * p.groups, n), dim3(p.threads), smem_v, st, A);
     if (rc) return rc;
   }
   return 0;
@@ -703,7 +827,7 @@ int arcb_attn_tree(const int64_t* q, const int64_t* Kc, const int64_t* Vc, int n
   if (lanes < 1 || nq < 1 || n_kv < 1 || n_heads < 1 || n_heads % n_kv || dh < 8 || dh > 128 || dh % 8 || t_lim < 1)
     return -2;
   const at::Plan p = at::plan(lanes, nq, n_heads, n_kv, dh, t_lim);
-  if (p.tiles > 65535 * 16 || (int64_t)n_kv * p.groups > 65535 || (int64_t)n_kv * ((p.R + 31) / 32) > 65535 ||
+  if (p.tiles > 65535 * 16 || (int64_t)n_kv * p.groups > 65535 || (int64_t)n_kv * ((p.R + at::RQ - 1) / at::RQ) > 65535 ||
       p.lanes > 65535)
     return -2;
   uint8_t* b = (uint8_t*)ws;
@@ -713,12 +837,13 @@ int arcb_attn_tree(const int64_t* q, const int64_t* Kc, const int64_t* Vc, int n
   A.n_pages = n_pages, A.width = width, A.nq = nq, A.n_heads = n_heads, A.n_kv = n_kv, A.dh = dh, A.t_lim = t_lim;
   A.B = lanes * nq;
   A.R = p.R, A.Rp = p.Rp, A.G = p.G, A.tiles = p.tiles, A.chunks = p.chunks, A.groups = p.groups, A.RG = p.RG;
-  A.splits = p.splits;
-  A.S = (int*)(b + p.oS), A.M = (int64_t*)(b + p.oM), A.gmax = (int64_t*)(b + p.oG);
+  A.splits = p.splits, A.rows_s = p.rows_s;
+  A.S = (int*)(b + p.oS), A.M = (int64_t*)(b + p.oM), A.ref = (int64_t*)(b + p.oR), A.gmax = (int64_t*)(b + p.oG);
   A.sums = (uint64_t*)(b + p.oSum), A.part = (int64_t*)(b + p.oP), A.arrived = (int*)(b + p.oA);
   A.X = X, A.lmax = lmax, A.o_out = o_out, A.err = err;
   cudaStream_t st = (cudaStream_t)stream;
-  return dh <= 64 ? at::run<64>(A, p, lanes, st) : at::run<128>(A, p, lanes, st);
+  if (p.unit == 8) return dh <= 64 ? at::run<64, 8>(A, p, lanes, st) : at::run<128, 8>(A, p, lanes, st);
+  return dh <= 64 ? at::run<64, 16>(A, p, lanes, st) : at::run<128, 16>(A, p, lanes, st);
 }
 
 }  // extern "C"
