@@ -27,14 +27,14 @@
 //     products.  Scores are stored relative to their tile's max (differences
 //     below -2^30 clamped: their exp is 0 either way), which is stored beside.
 //  2. k_sums: each row's global max and sum of exps, split over key chunks.
-//  3. k_values: w.v for up to 64 rows and a range of keys.  The floor of each
+//  3. k_values: w.v for up to 128 rows and a range of keys.  The floor of each
 //     term rules out a matrix product, but one single-precision FMA rounding
 //     toward minus infinity is exact: acc <- rd(acc + w * (v / 2^16)) with acc
 //     an integer in [2^23, 2^24), where floats are the integers, adds
 //     floor(w * v / 2^16).  acc starts at 1.5 * 2^23 and moves by at most
 //     max|v| + (number of keys) < 2^22, since the weights sum to at most ONE.
 //     Chunks with wider values take 64-bit terms.
-//     Key ranges of one row group are summed by the last CTA to arrive.
+//     CTAs that share a lane leave partial sums; the last to arrive adds them.
 #include "../common/tree.h"
 #include "common.cuh"
 #include "lut.cuh"
@@ -51,7 +51,7 @@ constexpr int NT_S = 256;           // k_scores threads
 constexpr int NT_B = 256;           // k_sums threads
 constexpr int RB = 64;              // rows per k_sums CTA
 constexpr int NT_V = 256;           // k_values threads, at most
-constexpr int CK = 64;              // keys per k_values chunk
+constexpr int CK = 32;              // keys per k_values chunk: two pages
 constexpr int MAX_RG = 128;         // rows per k_values CTA
 constexpr int SMALL = 1 << 29;      // bound of scores stored as they are
 constexpr int FAR = -(1 << 30);     // a score whose exp is 0
@@ -68,15 +68,15 @@ struct Args {
   const int* n_tree;
   const int64_t* mask;
   int64_t pt_stride, attn_scale;
-  int n_pages, width, nq, n_heads, n_kv, dh, t_lim, B, lane0;
+  int n_pages, width, nq, n_heads, n_kv, dh, t_lim, B, lane0, lanes;
   int R, Rp, G, tiles, chunks, groups, RG, splits, rows_s;
   // workspace
-  int* S;              // [lanes][n_kv][tiles][TILE][Rp] scores less ref
+  int* S;              // [lanes][n_kv][tiles][groups][TILE][RG] scores less ref
   int64_t* M;          // [lanes][n_kv][tiles][Rp] max of the tile
   int64_t* ref;        // [lanes][n_kv][tiles][Rp]: 0, or M where scores are not small
   int64_t* gmax;       // [lanes][n_kv][Rp]
   uint64_t* sums;      // [lanes][n_kv][chunks][Rp]
-  int64_t* part;       // [lanes][n_kv][groups][splits][RG][dh]
+  int64_t* part;       // [n_kv][groups][splits + lanes][RG][dh]
   int* arrived;        // [lanes][n_kv][groups]
   int8_t* X;
   int* lmax;
@@ -242,7 +242,8 @@ __global__ void __launch_bounds__(NT_S, 2) k_scores(const Args A) {
       atomicMax(&or_k[2], mag);
     }
     const int j = j0 + (w & 3) * 32 + ln;  // this thread's key in the epilogue
-    int* Srow = A.S + ((lk * A.tiles + tile) * TILE + (w & 3) * 32 + ln) * A.Rp;
+    const size_t group_elems = (size_t)TILE * A.RG;
+    int* Srow = A.S + (lk * A.tiles + tile) * A.groups * group_elems + (size_t)((w & 3) * 32 + ln) * A.RG;
     const int kend = (A.dh + 31) / 32;
     const bool all_seen = j0 + TILE <= base;  // every key of the tile is below the tree
     uint32_t parity = 0;
@@ -396,9 +397,11 @@ __global__ void __launch_bounds__(NT_S, 2) k_scores(const Args A) {
           asm volatile("bar.sync %0, 128;" ::"r"(1 + (w >> 2)) : "memory");
         }
         if (ln < 16) wmax[w & 3][c0 + ln] = m64;
+        // 16 rows lie in one group: RG is a multiple of 16, or the only group's 8
+        int* dst = Srow + (r0 + c0) / A.RG * group_elems + (r0 + c0) % A.RG;
 #pragma unroll
         for (int i = 0; i < 16; i += 4)
-          if (c0 + i < rows) *(int4*)(Srow + r0 + c0 + i) = make_int4(out[i], out[i + 1], out[i + 2], out[i + 3]);
+          if (c0 + i < rows) *(int4*)(dst + i) = make_int4(out[i], out[i + 1], out[i + 2], out[i + 3]);
       }
       tc_fence_before();
       __syncthreads();  // wmax; this group's accumulators and query planes are read
@@ -467,11 +470,12 @@ __global__ void __launch_bounds__(NT_B) k_sums(const Args A) {
       int off[4];
 #pragma unroll
       for (int c = 0; c < 4; ++c) off[c] = r0 + q + c < A.R ? rebase(ref[(size_t)t * A.Rp + q + c], rmax[q + c]) : FAR;
-      const int* S = A.S + ((lk * A.tiles + t) * TILE + k0) * (size_t)A.Rp + r0 + q;
+      const int* S = A.S + ((lk * A.tiles + t) * A.groups + (r0 + q) / A.RG) * (size_t)TILE * A.RG +
+                     (size_t)k0 * A.RG + (r0 + q) % A.RG;
       uint32_t p[4] = {0, 0, 0, 0};  // of TILE / KL exps
 #pragma unroll
       for (int k = 0; k < TILE / KL; ++k) {
-        const int4 x = *(const int4*)(S + (size_t)k * KL * A.Rp);
+        const int4 x = *(const int4*)(S + (size_t)k * KL * A.RG);
         p[0] += exp32(x.x + off[0], lut);
         p[1] += exp32(x.y + off[1], lut);
         p[2] += exp32(x.z + off[2], lut);
@@ -492,17 +496,6 @@ __global__ void __launch_bounds__(NT_B) k_sums(const Args A) {
 }
 
 // ------------------------------------------------------------------ 3. values
-__device__ __forceinline__ uint64_t fma2_rd(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t d;
-  asm("fma.rm.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-  return d;
-}
-__device__ __forceinline__ uint64_t dup2(float x) {
-  uint64_t d;
-  asm("mov.b64 %0, {%1, %1};" : "=l"(d) : "f"(x));
-  return d;
-}
-
 // 8 consecutive digits planes of four int64 outputs, and their limb count.
 __device__ __forceinline__ int store_limbs4(int8_t* X, int slot, int B, size_t ldx, size_t col, const int64_t* o) {
   int need = 0;
@@ -526,212 +519,269 @@ __device__ __forceinline__ int store_limbs4(int8_t* X, int slot, int B, size_t l
   return need;
 }
 
-// grid (splits, n_kv * groups, lanes).  A warp takes UR rows (unit) x all dims,
-// lane = DPL consecutive dims; kparts warps per unit take every kparts-th key.
+__device__ __forceinline__ void bulk_g2s(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+               "l"(src), "r"(bytes), "r"(bar)
+               : "memory");
+}
+
+// grid (splits, n_kv * groups).  The lanes' chunks of CK keys, one after
+// another, are divided evenly over the splits; a CTA works through its part
+// of each lane that it touches (a segment).  V pages and scores come by bulk
+// copies, one chunk ahead.  A warp takes UR rows (unit) x all dims, a lane
+// the dims 2 ln, 2 ln + 1 (and 64 + those); kparts warps per unit take every
+// kparts-th key.
 template <int DPL, int UR>
 __global__ void __launch_bounds__(NT_V, 2) k_values(const Args A) {
   extern __shared__ __align__(1024) uint8_t dsm[];
-  constexpr int DHP = 32 * DPL, UP = UR / 2;
+  constexpr int DHP = 32 * DPL;
   __shared__ int2 lut[EXP_LUT_N];
   __shared__ int64_t rmax[MAX_RG];
   __shared__ uint64_t rsum[MAX_RG];
-  __shared__ float rrcp[MAX_RG];   // ONE / sum
-  __shared__ int roff[MAX_RG];
+  __shared__ __align__(8) uint64_t full[2];
   __shared__ int s_last, s_need, s_long;
   const int NT = blockDim.x, tid = threadIdx.x, ln = tid & 31, w = tid >> 5;
   const int RG = A.RG, units = RG / UR, unit = w % units, kpart = w / units, kparts = NT / 32 / units;
-  float* vs = (float*)dsm;                                   // [CK][DHP] v / 2^16
-  float* ws = vs + CK * DHP;                                 // [CK][RG] weights
-  int* osum = (int*)dsm;                                     // [RG][DHP] at the end
+  const int vbytes = CK * A.dh * 8, sbytes = CK * RG * 4;
+  uint8_t* vbuf = dsm;                                 // 2 x [CK][dh] int64
+  float* wbuf = (float*)(dsm + 2 * vbytes);            // 2 x [CK][RG] scores, then weights in place
+  int* osum = (int*)dsm;                               // [RG][DHP] at a segment's end
   load_lut(lut, NT);
-  if (tid == 0) s_need = s_long = 0;
+  if (tid == 0) {
+    s_need = 0;
+    mbar_init(smem_u32(&full[0]), 1);
+    mbar_init(smem_u32(&full[1]), 1);
+    fence_barrier_init();
+  }
   pdl_wait_dep();
   pdl_allow_next();
   const int kvh = blockIdx.y / A.groups, grp = blockIdx.y % A.groups, r0 = grp * RG, rows = min(RG, A.R - r0);
-  const int lane = A.lane0 + blockIdx.z;
-  const size_t lk = (size_t)blockIdx.z * A.n_kv + kvh, lkg = lk * A.groups + grp;
-  const int base = A.base[lane], ntree = A.n_tree[lane];
-  int T = tree::lane_keys(base, ntree, A.t_lim, A.width);
-  const int* pt = A.pt + lane * A.pt_stride;
-  bool bad = T < 0;
-  for (int i = tid; !bad && i < (T + PAGE - 1) / PAGE; i += NT) bad |= !tree::page_ok(pt[i], A.n_pages);
-  bad = __syncthreads_or(bad);
-  if (bad && tid == 0) set_error(A.err, T < 0 ? ARCB_ERR_SEQ_OVERFLOW : ARCB_ERR_BOUNDS);
-  if (bad) T = 0;
-  if (T == 0 && blockIdx.x > 0) return;
-  const int nt = (T + TILE - 1) / TILE;
-  const int t0 = (int)((int64_t)blockIdx.x * nt / A.splits), t1 = (int)((int64_t)(blockIdx.x + 1) * nt / A.splits);
-  if (T > 0 && tid < RG) {
-    const bool row = tid < rows;
-    uint64_t s = 0;
-    if (row)
+  auto chunks_of = [&](int T) { return T > 0 ? (T + CK - 1) / CK : 1; };  // a lane without keys: one, for its zeros
+  int64_t N = 0;
+  for (int b = 0; b < A.lanes; ++b)
+    N += chunks_of(tree::lane_keys(A.base[A.lane0 + b], A.n_tree[A.lane0 + b], A.t_lim, A.width));
+  const int64_t x = blockIdx.x, X = N < (int64_t)gridDim.x ? N : (int64_t)gridDim.x;
+  if (x >= X) return;
+  const int64_t c_lo = x * N / X, c_hi = (x + 1) * N / X;
+  // the softmax rows of this thread's quad in the weight stage: NT is a multiple of RG / 4
+  const int rq = tid % (RG / 4) * 4, kq = tid / (RG / 4), kq_step = NT / (RG / 4);
+  uint32_t issued = 0, used = 0;  // chunks
+  int need = 0;
+  int64_t off = 0;
+  for (int bz = 0; bz < A.lanes && off < c_hi; ++bz) {
+    const int lane = A.lane0 + bz;
+    int T = tree::lane_keys(A.base[lane], A.n_tree[lane], A.t_lim, A.width);
+    const int n = chunks_of(T);
+    const int64_t first = off;
+    off += n;
+    if (off <= c_lo) continue;
+    const int a0 = (int)(c_lo > first ? c_lo - first : 0), a1 = (int)(c_hi < off ? c_hi - first : n);
+    // CTAs that share the lane
+    const int64_t xf = ((first + 1) * X - 1) / N, xl = (off * X - 1) / N;
+    const size_t lk = (size_t)bz * A.n_kv + kvh, lkg = lk * A.groups + grp;
+    const int* pt = A.pt + lane * A.pt_stride;
+    int64_t* part0 = A.part + (size_t)blockIdx.y * (gridDim.x + A.lanes) * RG * A.dh;
+    int64_t* part = part0 + (size_t)(x + bz) * RG * A.dh;
+    bool bad = T < 0;
+    for (int i = tid; !bad && i < (T + PAGE - 1) / PAGE; i += NT) bad |= !tree::page_ok(pt[i], A.n_pages);
+    if (tid == 0) s_long = 0;
+    bad = __syncthreads_or(bad);
+    if (bad && tid == 0) set_error(A.err, T < 0 ? ARCB_ERR_SEQ_OVERFLOW : ARCB_ERR_BOUNDS);
+    const bool live = T > 0 && !bad;
+    if (live && tid < RG) {
+      const bool row = tid < rows;
+      uint64_t s = 0;
+      if (row)
 #pragma unroll 4
-      for (int c = 0; c < A.chunks; ++c) s += A.sums[(lk * A.chunks + c) * A.Rp + r0 + tid];
-    rmax[tid] = row ? A.gmax[lk * A.Rp + r0 + tid] : NONE;
-    rsum[tid] = s ? s : 1;  // a row without keys: every exp is 0
-    rrcp[tid] = 65536.0f * __frcp_rn((float)(int64_t)rsum[tid]);
-    if (s >> 30) s_long = 1;
-  }
-  uint64_t acc[DPL][UP];  // pairs of rows
-#pragma unroll
-  for (int d = 0; d < DPL; ++d)
-#pragma unroll
-    for (int i = 0; i < UP; ++i) acc[d][i] = dup2(12582912.0f);
-  int64_t* part = A.part + (lkg * A.splits + blockIdx.x) * (size_t)RG * A.dh;
-  bool any_wide = false;
-  for (int j0 = t0 * TILE; j0 < min(t1 * TILE, T); j0 += CK) {
-    const int t = j0 / TILE, keys = min(CK, T - j0);
-    __syncthreads();  // rsum / the last chunk's readers
-    if (j0 % TILE == 0 && tid < RG)
-      roff[tid] = tid < rows ? rebase(A.ref[(lk * A.tiles + t) * A.Rp + r0 + tid], rmax[tid]) : FAR;
-    // values: v / 2^16 in single precision, 0 past the last key and dim.  y = v + VMAX
-    // in [0, 2 VMAX] as the low bits of 2^23 + y, then exact: (that - 2^23 - VMAX) / 2^16
-    uint32_t high = 0, most = 0;
-#pragma unroll 4
-    for (int i = tid; i < CK * (DHP / 4); i += NT) {
-      const int k = i / (DHP / 4), col = i % (DHP / 4) * 4;
-      float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (k < keys && col < A.dh) {
-        const int j = j0 + k;
-        int64_t x[4];
-        load4(x, A.Vc + (((size_t)pt[j / PAGE] * A.n_kv + kvh) * PAGE + j % PAGE) * A.dh + col);
-        float* p = &f.x;
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const uint64_t y = (uint64_t)x[c] + VMAX;
-          high |= (uint32_t)(y >> 32);
-          most = max(most, (uint32_t)y);
-          p[c] = __fmaf_rn(__uint_as_float(0x4B000000u + (uint32_t)y), 1.0f / 65536.0f,
-                           -(float)(8388608 + VMAX) / 65536.0f);
-        }
-      }
-      *(float4*)(vs + k * DHP + col) = f;
+        for (int c = 0; c < A.chunks; ++c) s += A.sums[(lk * A.chunks + c) * A.Rp + r0 + tid];
+      rmax[tid] = row ? A.gmax[lk * A.Rp + r0 + tid] : NONE;
+      rsum[tid] = s ? s : 1;  // a row without keys: every exp is 0
+      if (s >> 30) s_long = 1;
     }
-    const bool fit = __syncthreads_and(high == 0 && most <= 2 * VMAX);
-    // weights floor(e * ONE / sum), at most ONE: the estimate e * (ONE / sum) in single
-    // precision is within 1, the remainder decides (32 bits hold it for sums below 2^30)
-    const bool lng = s_long != 0;
-#pragma unroll 2
-    for (int i = tid; i < CK * (RG / 4); i += NT) {
-      const int k = i / (RG / 4), r = i % (RG / 4) * 4;
-      float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (k < keys && r < rows) {
-        const int4 x = *(const int4*)(A.S + ((lk * A.tiles + t) * TILE + (j0 % TILE) + k) * (size_t)A.Rp + r0 + r);
-        const int xs[4] = {x.x, x.y, x.z, x.w};
-        float* p = &f.x;
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const uint32_t e = r + c < rows ? (uint32_t)exp32(xs[c] + roff[r + c], lut) : 0u;
-          const float ef = __uint_as_float(0x4B000000u + e) - 8388608.0f;
-          const float qf = __fmaf_rd(ef, rrcp[r + c], 8388608.0f);
-          const uint32_t q = __float_as_uint(qf) - 0x4B000000u;
-          float wt = qf - 8388608.0f;
-          if (!lng) {
-            const uint32_t den = (uint32_t)rsum[r + c];
-            const int rem = (int)((e << 16) - q * den);
-            wt += rem < 0 ? -1.0f : (rem >= (int)den ? 1.0f : 0.0f);
-          } else {
-            const int64_t rem = (int64_t)(((uint64_t)e << 16) - (uint64_t)q * rsum[r + c]);
-            wt += rem < 0 ? -1.0f : (rem >= (int64_t)rsum[r + c] ? 1.0f : 0.0f);
-          }
-          p[c] = wt;
-        }
-      }
-      *(float4*)(ws + k * RG + r) = f;
-    }
-    __syncthreads();
-    if (fit) {
-#pragma unroll 2
-      for (int k = kpart; k < CK; k += kparts) {
-        uint64_t wp[UP];
-#pragma unroll
-        for (int i = 0; i < UP; i += 2) {
-          const ulonglong2 x = *(const ulonglong2*)(ws + k * RG + unit * UR + 2 * i);
-          wp[i] = x.x, wp[i + 1] = x.y;
-        }
-        float v[DPL];
-        if constexpr (DPL == 4) *(float4*)v = *(const float4*)(vs + k * DHP + ln * 4);
-        else *(float2*)v = *(const float2*)(vs + k * DHP + ln * 2);
-#pragma unroll
-        for (int d = 0; d < DPL; ++d) {
-          const uint64_t vv = dup2(v[d]);
-#pragma unroll
-          for (int i = 0; i < UP; ++i) acc[d][i] = fma2_rd(wp[i], vv, acc[d][i]);
-        }
-      }
-    } else {  // 64-bit terms into this CTA's partial sums
-      for (int i = tid; i < RG * A.dh; i += NT) {
-        const int r = i / A.dh, e = i - r * A.dh;
-        uint64_t o = any_wide ? (uint64_t)part[i] : 0;
-        for (int k = 0; k < keys; ++k) {
-          const int j = j0 + k;
-          const int64_t wt = (int64_t)ws[k * RG + r];
-          if (wt) o += (uint64_t)mulshr(wt, A.Vc[(((size_t)pt[j / PAGE] * A.n_kv + kvh) * PAGE + j % PAGE) * A.dh + e]);
-        }
-        part[i] = (int64_t)o;
-      }
-      any_wide = true;
-    }
-  }
-  __syncthreads();
-  for (int i = tid; i < RG * DHP; i += NT) osum[i] = 0;
-  __syncthreads();
-  if (T > 0)
+    float acc[DPL][UR];
 #pragma unroll
     for (int d = 0; d < DPL; ++d)
 #pragma unroll
-      for (int i = 0; i < UP; ++i) {
-        int* o = osum + (unit * UR + 2 * i) * DHP + ln * DPL + d;
-        const int a = (int)(uint32_t)acc[d][i] - 0x4B400000, b = (int)(uint32_t)(acc[d][i] >> 32) - 0x4B400000;
-        if (kparts == 1) o[0] = a, o[DHP] = b;
-        else atomicAdd(o, a), atomicAdd(o + DHP, b);
-      }
-  __syncthreads();
-  const int quads = A.dh / 4;
-  if (A.splits > 1 && T > 0) {
-    for (int i = tid; i < rows * quads; i += NT) {
-      const int r = i / quads, e = i % quads * 4;
-      const int4 x = *(const int4*)(osum + r * DHP + e);
-      longlong2* p = (longlong2*)(part + r * A.dh + e);
-      longlong2 a = make_longlong2(x.x, x.y), b = make_longlong2(x.z, x.w);
-      if (any_wide) {
-        const longlong2 c = p[0], d = p[1];
-        a.x = wadd(a.x, c.x), a.y = wadd(a.y, c.y), b.x = wadd(b.x, d.x), b.y = wadd(b.y, d.y);
-      }
-      __stcg(p, a);
-      __stcg(p + 1, b);
-    }
-    __threadfence();
+      for (int i = 0; i < UR; ++i) acc[d][i] = 12582912.0f;
     __syncthreads();
-    if (tid == 0) s_last = atomicAdd(A.arrived + lkg, 1) == A.splits - 1;
-    __syncthreads();
-    if (!s_last) return;
-    __threadfence();
-  }
-  const size_t d = (size_t)A.n_heads * A.dh;
-  int need = 0;
-  for (int i = tid; i < rows * quads; i += NT) {
-    const int r = i / quads, e = i % quads * 4, rr = r0 + r;
-    int64_t o[4] = {0, 0, 0, 0};
-    if (T > 0 && A.splits > 1) {
-      const int64_t* p = A.part + lkg * A.splits * (size_t)RG * A.dh + r * A.dh + e;
-      for (int s = 0; s < A.splits; ++s, p += (size_t)RG * A.dh) {
-        const longlong2 a = __ldcg((const longlong2*)p), b = __ldcg((const longlong2*)p + 1);
-        o[0] = wadd(o[0], a.x), o[1] = wadd(o[1], a.y), o[2] = wadd(o[2], b.x), o[3] = wadd(o[3], b.y);
-      }
-    } else if (T > 0) {
+    bool any_wide = false;
+    if (live) {
+      const bool lng = s_long != 0;
+      float rcp[4];    // ONE / sum
+      uint32_t den[4];
+      int ro[4];
 #pragma unroll
-      for (int c = 0; c < 4; ++c)
-        o[c] = wadd(osum[r * DHP + e + c], any_wide ? part[r * A.dh + e + c] : 0);
+      for (int c = 0; c < 4; ++c) {
+        den[c] = (uint32_t)rsum[rq + c];
+        rcp[c] = 65536.0f * __frcp_rn((float)(int64_t)rsum[rq + c]);
+        ro[c] = FAR;
+      }
+      auto issue = [&](int c) {  // one thread
+        const uint32_t bar = smem_u32(&full[issued & 1]), buf = issued & 1;
+        const int pages = min(CK / PAGE, (T + PAGE - 1) / PAGE - c * (CK / PAGE));
+        const uint32_t pbytes = PAGE * A.dh * 8;
+        mbar_arrive_expect_tx(bar, pages * pbytes + sbytes);
+        for (int i = 0; i < pages; ++i)
+          bulk_g2s(smem_u32(vbuf) + buf * vbytes + i * pbytes,
+                   A.Vc + ((size_t)pt[c * (CK / PAGE) + i] * A.n_kv + kvh) * PAGE * A.dh, pbytes, bar);
+        const int t = c / (TILE / CK);
+        bulk_g2s(smem_u32(wbuf) + buf * sbytes,
+                 A.S + (((lk * A.tiles + t) * A.groups + grp) * TILE + (c % (TILE / CK)) * CK) * (size_t)RG, sbytes, bar);
+      };
+      if (tid == 0) {
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // after the last segment's accesses
+        issue(a0);
+      }
+      ++issued;
+      for (int c = a0; c < a1; ++c) {
+        const int j0 = c * CK, t = j0 / TILE, keys = min(CK, T - j0);
+        if (c + 1 < a1) {
+          if (tid == 0) issue(c + 1);
+          ++issued;
+        }
+        if (c == a0 || j0 % TILE == 0) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            ro[k] = rq + k < rows ? rebase(A.ref[(lk * A.tiles + t) * A.Rp + r0 + rq + k], rmax[rq + k]) : FAR;
+        }
+        if (!mbar_wait(smem_u32(&full[used & 1]), (used >> 1) & 1)) set_error(A.err, ARCB_ERR_TIMEOUT_FULL);
+        int64_t* vb = (int64_t*)(vbuf + (used & 1) * vbytes);
+        float* wb = wbuf + (used & 1) * CK * RG;
+        ++used;
+        // values to single precision, v / 2^16 over each low word.  Where they fit, y = v + VMAX is in
+        // [0, 2 VMAX]: the low bits of the float 2^23 + y, then exact: (that - 2^23 - VMAX) / 2^16
+        uint32_t high = 0, most = 0;
+#pragma unroll 4
+        for (int i = tid; i < keys * A.dh / 2; i += NT) {
+          longlong2* cell = (longlong2*)(vb + 2 * i);
+          const longlong2 v = *cell;
+          const uint64_t y0 = (uint64_t)v.x + VMAX, y1 = (uint64_t)v.y + VMAX;
+          high |= (uint32_t)(y0 >> 32) | (uint32_t)(y1 >> 32);
+          most = max(most, max((uint32_t)y0, (uint32_t)y1));
+          const float c = -(float)(8388608 + VMAX) / 65536.0f;
+          *(float4*)cell = make_float4(__fmaf_rn(__uint_as_float(0x4B000000u + (uint32_t)y0), 1.0f / 65536.0f, c), 0.f,
+                                       __fmaf_rn(__uint_as_float(0x4B000000u + (uint32_t)y1), 1.0f / 65536.0f, c), 0.f);
+        }
+        // weights floor(e * ONE / sum), at most ONE, in place: the estimate e * (ONE / sum)
+        // in single precision is within 1, the remainder decides (in 32 bits for sums below 2^30)
+#pragma unroll 4
+        for (int k = kq; k < CK; k += kq_step) {
+          float4* cell = (float4*)(wb + k * RG + rq);
+          const int4 sc = *(const int4*)cell;
+          const int xs[4] = {sc.x, sc.y, sc.z, sc.w};
+          float o[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t e = (uint32_t)exp32(xs[i] + ro[i], lut);
+            const float ef = __uint_as_float(0x4B000000u + e) - 8388608.0f;
+            const float qf = __fmaf_rd(ef, rcp[i], 8388608.0f);
+            const uint32_t q = __float_as_uint(qf) - 0x4B000000u;
+            int rem = (int)((e << 16) - q * den[i]);
+            bool up = rem >= (int)den[i];
+            if (lng) {
+              const int64_t r64 = (int64_t)(((uint64_t)e << 16) - (uint64_t)q * rsum[rq + i]);
+              rem = r64 < 0 ? -1 : 0;
+              up = r64 >= (int64_t)rsum[rq + i];
+            }
+            o[i] = qf - (rem < 0 ? 8388609.0f : (up ? 8388607.0f : 8388608.0f));
+          }
+          *cell = make_float4(o[0], o[1], o[2], o[3]);
+        }
+        const bool fit = __syncthreads_and(high == 0 && most <= 2 * VMAX);
+        if (fit) {
+          const int64_t* vrow = vb + min(2 * ln, A.dh - 2);
+          const int second = min(64, A.dh - 2 - min(2 * ln, A.dh - 2));  // dims of the second pair, inside the row
+#pragma unroll 2
+          for (int k = kpart; k < keys; k += kparts) {  // rows behind may hold anything
+            float wt[UR], v[DPL];
+#pragma unroll
+            for (int i = 0; i < UR; i += 4) *(float4*)(wt + i) = *(const float4*)(wb + k * RG + unit * UR + i);
+#pragma unroll
+            for (int d = 0; d < DPL; d += 2) {
+              const float4 p = *(const float4*)(vrow + k * A.dh + (d ? second : 0));
+              v[d] = p.x, v[d + 1] = p.z;
+            }
+#pragma unroll
+            for (int d = 0; d < DPL; ++d)
+#pragma unroll
+              for (int i = 0; i < UR; ++i) acc[d][i] = __fmaf_rd(wt[i], v[d], acc[d][i]);
+          }
+        } else {  // 64-bit terms into this CTA's partial sums
+          for (int i = tid; i < RG * A.dh; i += NT) {
+            const int r = i / A.dh, e = i - r * A.dh;
+            uint64_t o = any_wide ? (uint64_t)part[i] : 0;
+            for (int k = 0; k < keys; ++k) {
+              const int64_t wt = (int64_t)wb[k * RG + r];
+              const int64_t* v = A.Vc + (((size_t)pt[(j0 + k) / PAGE] * A.n_kv + kvh) * PAGE + (j0 + k) % PAGE) * A.dh;
+              if (wt) o += (uint64_t)mulshr(wt, v[e]);
+            }
+            part[i] = (int64_t)o;
+          }
+          any_wide = true;
+        }
+        __syncthreads();
+        if (tid == 0) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // before the next copies
+      }
+      for (int i = tid; i < RG * DHP; i += NT) osum[i] = 0;
+      __syncthreads();
+#pragma unroll
+      for (int d = 0; d < DPL; ++d)
+#pragma unroll
+        for (int i = 0; i < UR; ++i) {
+          int* o = osum + (unit * UR + i) * DHP + 2 * ln + (d & 1) + (d >> 1) * 64;
+          const int a = __float_as_int(acc[d][i]) - 0x4B400000;
+          if (kparts == 1) *o = a;
+          else atomicAdd(o, a);
+        }
+      __syncthreads();
     }
-    const int slot = lane * A.nq + rr / A.G;
-    const size_t col = (size_t)(kvh * A.G + rr % A.G) * A.dh + e;
-    if (A.o_out) {
-      longlong2* p = (longlong2*)(A.o_out + slot * d + col);
-      p[0] = make_longlong2(o[0], o[1]);
-      p[1] = make_longlong2(o[2], o[3]);
+    const int quads = A.dh / 4;
+    if (xl > xf) {
+      for (int i = tid; i < rows * quads; i += NT) {
+        const int r = i / quads, e = i % quads * 4;
+        longlong2* p = (longlong2*)(part + r * A.dh + e);
+        longlong2 a = make_longlong2(0, 0), b = make_longlong2(0, 0);
+        if (live) {
+          const int4 v = *(const int4*)(osum + r * DHP + e);
+          a = make_longlong2(v.x, v.y), b = make_longlong2(v.z, v.w);
+        }
+        if (any_wide) {
+          const longlong2 c = p[0], d = p[1];
+          a.x = wadd(a.x, c.x), a.y = wadd(a.y, c.y), b.x = wadd(b.x, d.x), b.y = wadd(b.y, d.y);
+        }
+        __stcg(p, a);
+        __stcg(p + 1, b);
+      }
+      __threadfence();
+      __syncthreads();
+      if (tid == 0) s_last = atomicAdd(A.arrived + lkg, 1) == (int)(xl - xf);
+      __syncthreads();
+      if (!s_last) continue;
+      __threadfence();
     }
-    if (A.X) need = max(need, store_limbs4(A.X, slot, A.B, d, col, o));
+    const size_t d = (size_t)A.n_heads * A.dh;
+    for (int i = tid; i < rows * quads; i += NT) {
+      const int r = i / quads, e = i % quads * 4, rr = r0 + r;
+      int64_t o[4] = {0, 0, 0, 0};
+      if (xl > xf) {
+        const int64_t* p = part0 + (size_t)(xf + bz) * RG * A.dh + r * A.dh + e;
+        for (int64_t s = xf; s <= xl; ++s, p += (size_t)RG * A.dh) {
+          const longlong2 a = __ldcg((const longlong2*)p), b = __ldcg((const longlong2*)p + 1);
+          o[0] = wadd(o[0], a.x), o[1] = wadd(o[1], a.y), o[2] = wadd(o[2], b.x), o[3] = wadd(o[3], b.y);
+        }
+      } else if (live) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) o[c] = wadd(osum[r * DHP + e + c], any_wide ? part[r * A.dh + e + c] : 0);
+      }
+      const int slot = lane * A.nq + rr / A.G;
+      const size_t col = (size_t)(kvh * A.G + rr % A.G) * A.dh + e;
+      if (A.o_out) {
+        longlong2* p = (longlong2*)(A.o_out + slot * d + col);
+        p[0] = make_longlong2(o[0], o[1]);
+        p[1] = make_longlong2(o[2], o[3]);
+      }
+      if (A.X) need = max(need, store_limbs4(A.X, slot, A.B, d, col, o));
+    }
   }
   if (A.X && A.lmax) {
     need = __reduce_max_sync(0xffffffffu, need);
@@ -762,12 +812,12 @@ static Plan plan(int lanes, int nq, int n_heads, int n_kv, int dh, int t_lim) {
   const size_t per_s = (size_t)n_kv * p.tiles * TILE * p.Rp * 4;
   p.lanes = (int)(WS_TARGET / per_s);
   p.lanes = p.lanes < 1 ? 1 : (p.lanes > lanes ? lanes : p.lanes);
-  // enough CTAs for two rounds of two per SM, at least a tile of keys each
-  const int have = p.lanes * n_kv * p.groups;
-  p.splits = (4 * 148 + have - 1) / have;
-  if (p.splits > p.tiles) p.splits = p.tiles;
-  const int least = (int)(((int64_t)p.tiles * TILE + MAX_RANGE - TILE - 1) / (MAX_RANGE - TILE));
-  if (p.splits < least) p.splits = least;
+  // the lanes' keys are divided evenly over two CTAs per SM in all; a CTA's
+  // part of a lane stays below MAX_RANGE keys
+  p.splits = 2 * 148 / (n_kv * p.groups);
+  if (p.splits < 1) p.splits = 1;
+  const int64_t least = ((int64_t)p.lanes * p.tiles * TILE + MAX_RANGE - 1) / (MAX_RANGE - CK);
+  if (p.splits < least) p.splits = (int)least;
   const int units = p.RG / p.unit;
   p.threads = 32 * units * (units >= 5 ? 1 : (units >= 3 ? 2 : (units == 2 ? 4 : 8)));
   // score CTAs take all rows of their tile unless that leaves SMs idle (two CTAs each)
@@ -785,7 +835,7 @@ static Plan plan(int lanes, int nq, int n_heads, int n_kv, int dh, int t_lim) {
   p.oR = take(lk * p.tiles * p.Rp * 8);
   p.oG = take(lk * p.Rp * 8);
   p.oSum = take(lk * p.chunks * p.Rp * 8);
-  p.oP = take(lk * p.groups * p.splits * p.RG * dh * 8);
+  p.oP = take((size_t)n_kv * p.groups * (p.splits + p.lanes) * p.RG * dh * 8);
   p.oA = take(lk * p.groups * 4);
   p.bytes = o;
   return p;
@@ -794,18 +844,18 @@ static Plan plan(int lanes, int nq, int n_heads, int n_kv, int dh, int t_lim) {
 template <int DHP, int UR>
 static int run(Args A, const Plan& p, int lanes, cudaStream_t st) {
   constexpr int smem_s = 1024 + PLANES * (TILE + RQ) * 128;
-  const int vals = CK * (DHP + p.RG) * 4, sums = p.RG * DHP * 4, smem_v = vals > sums ? vals : sums;
+  const int vals = 2 * CK * (A.dh * 8 + p.RG * 4), sums = p.RG * DHP * 4, smem_v = vals > sums ? vals : sums;
   const auto kv = k_values<DHP / 32, UR>;
   cudaError_t e = cudaFuncSetAttribute(k_scores<DHP>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_s);
   if (e == cudaSuccess) e = cudaFuncSetAttribute(kv, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_v);
   if (e != cudaSuccess) return (int)e;
   for (int l0 = 0; l0 < lanes; l0 += p.lanes) {
     const int n = lanes - l0 < p.lanes ? lanes - l0 : p.lanes;
-    A.lane0 = l0;
+    A.lane0 = l0, A.lanes = n;
     int rc = launch_k(k_scores<DHP>, dim3(p.tiles, A.n_kv * ((p.R + p.rows_s - 1) / p.rows_s), n), dim3(NT_S), smem_s,
                       st, A);
     if (!rc) rc = launch_k(k_sums, dim3(p.chunks, A.n_kv * ((p.R + RB - 1) / RB), n), dim3(NT_B), 0, st, A);
-    if (!rc) rc = launch_k(kv, dim3(p.splits, A.n_kv * p.groups, n), dim3(p.threads), smem_v, st, A);
+    if (!rc) rc = launch_k(kv, dim3(p.splits, A.n_kv * p.groups), dim3(p.threads), smem_v, st, A);
     if (rc) return rc;
   }
   return 0;
