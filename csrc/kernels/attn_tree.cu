@@ -34,7 +34,8 @@
 //     floor(w * v / 2^16).  acc starts at 1.5 * 2^23 and moves by at most
 //     max|v| + (number of keys) < 2^22, since the weights sum to at most ONE.
 //     Chunks with wider values take 64-bit terms.
-//     CTAs that share a lane leave partial sums; the last to arrive adds them.
+//     CTAs that share a lane add their sums with atomics (integers: any order
+//     gives the same), two int32 in one 64-bit word; the last to arrive writes.
 #include "../common/tree.h"
 #include "common.cuh"
 #include "lut.cuh"
@@ -48,9 +49,7 @@ constexpr int TILE = 128;           // keys per score CTA
 constexpr int RQ = 32;              // query rows per MMA group
 constexpr int PLANES = 4;           // digits that take the tensor path
 constexpr int NT_S = 256;           // k_scores threads
-constexpr int NT_B = 256;           // k_sums threads
-constexpr int RB = 64;              // rows per k_sums CTA
-constexpr int NT_V = 256;           // k_values threads, at most
+constexpr int NT_V = 256;           // k_sums and k_values threads, at most
 constexpr int CK = 32;              // keys per k_values chunk: two pages
 constexpr int MAX_RG = 128;         // rows per k_values CTA
 constexpr int SMALL = 1 << 29;      // bound of scores stored as they are
@@ -75,9 +74,13 @@ struct Args {
   int64_t* M;          // [lanes][n_kv][tiles][Rp] max of the tile
   int64_t* ref;        // [lanes][n_kv][tiles][Rp]: 0, or M where scores are not small
   int64_t* gmax;       // [lanes][n_kv][Rp]
-  uint64_t* sums;      // [lanes][n_kv][chunks][Rp]
-  int64_t* part;       // [n_kv][groups][splits + lanes][RG][dh]
+  int64_t* wide;       // [n_kv][groups][splits + lanes][RG][dh]: 64-bit terms of a segment
+  // zeroed by k_scores:
+  uint64_t* sums;      // [lanes][n_kv][Rp] of exps
+  uint64_t* acc;       // [lanes][n_kv][groups][RG][dh / 2]: two int32 sums each
   int* arrived;        // [lanes][n_kv][groups]
+  int* bad;            // [lanes]
+  int* is_wide;        // [n_kv][groups][splits + lanes]
   int8_t* X;
   int* lmax;
   int64_t* o_out;
@@ -183,8 +186,20 @@ __global__ void __launch_bounds__(NT_S, 2) k_scores(const Args A) {
   pdl_allow_next();
   const int base = A.base[lane], nt = A.n_tree[lane];
   const int T = tree::lane_keys(base, nt, A.t_lim, A.width);
-  if (tile == 0 && r_lo == 0)
-    for (int i = tid; i < A.groups; i += NT_S) A.arrived[lk * A.groups + i] = 0;
+  // what the next kernels add into, zeroed by the CTAs of each lane and KV head
+  {
+    const int cta = tile * rbs + blockIdx.y % rbs, ctas = gridDim.x * rbs;
+    ulonglong2* z = (ulonglong2*)(A.acc + lk * A.groups * A.RG * (A.dh / 2));
+    for (int i = cta * NT_S + tid; i < A.groups * A.RG * (A.dh / 4); i += ctas * NT_S) z[i] = make_ulonglong2(0, 0);
+    if (cta == 0) {
+      for (int i = tid; i < A.Rp; i += NT_S) A.sums[lk * A.Rp + i] = 0;
+      for (int i = tid; i < A.groups; i += NT_S) A.arrived[lk * A.groups + i] = 0;
+      if (kvh == 0 && tid == 0) A.bad[blockIdx.z] = 0;
+      if (blockIdx.z == 0)
+        for (int i = tid; i < A.groups * (A.splits + A.lanes); i += NT_S)
+          A.is_wide[(size_t)kvh * A.groups * (A.splits + A.lanes) + i] = 0;
+    }
+  }
   const int j0 = tile * TILE;
   const bool live = j0 < T;
   if (live && tid < TILE / PAGE) {
@@ -428,71 +443,65 @@ __global__ void __launch_bounds__(NT_S, 2) k_scores(const Args A) {
 }
 
 // -------------------------------------------------------------------- 2. sums
-// grid (chunks, n_kv * row blocks of RB, lanes): a thread takes four rows of
-// every sixteenth key.
-__global__ void __launch_bounds__(NT_B) k_sums(const Args A) {
-  constexpr int Q = RB / 4, KL = NT_B / Q;
+// grid (chunks, n_kv * groups, lanes): a thread takes four rows of every
+// (threads / (RG / 4))-th key.
+__global__ void __launch_bounds__(NT_V) k_sums(const Args A) {
   __shared__ int2 lut[EXP_LUT_N];
-  __shared__ int64_t red[KL][RB];
-  __shared__ int64_t rmax[RB];
-  load_lut(lut, NT_B);
+  __shared__ int64_t rmax[MAX_RG];
+  __shared__ unsigned long long rsum[MAX_RG];
+  const int NT = blockDim.x, tid = threadIdx.x, RG = A.RG;
+  load_lut(lut, NT);
   pdl_wait_dep();
   pdl_allow_next();
-  const int tid = threadIdx.x, rb = (A.R + RB - 1) / RB, kvh = blockIdx.y / rb, r0 = (blockIdx.y % rb) * RB;
+  const int kvh = blockIdx.y / A.groups, grp = blockIdx.y % A.groups, r0 = grp * RG, rows = min(RG, A.R - r0);
   const int lane = A.lane0 + blockIdx.z, T = tree::lane_keys(A.base[lane], A.n_tree[lane], A.t_lim, A.width);
   if (T <= 0) return;
   const size_t lk = (size_t)blockIdx.z * A.n_kv + kvh;
-  const int nt = (T + TILE - 1) / TILE;
-  const int t0 = (int)((int64_t)blockIdx.x * nt / A.chunks), t1 = (int)((int64_t)(blockIdx.x + 1) * nt / A.chunks);
+  const int nt = (T + TILE - 1) / TILE, X = min((int)gridDim.x, nt);
+  if ((int)blockIdx.x >= X) return;
+  const int t0 = (int)((int64_t)blockIdx.x * nt / X), t1 = (int)((int64_t)(blockIdx.x + 1) * nt / X);
   const int64_t* M = A.M + lk * A.tiles * A.Rp + r0;
   const int64_t* ref = A.ref + lk * A.tiles * A.Rp + r0;
+  if (tid < RG) rmax[tid] = NONE, rsum[tid] = 0;
+  __syncthreads();
+  const int q = tid % (RG / 4) * 4, k0 = tid / (RG / 4), kl = NT / (RG / 4);
   {
-    const int r = tid % RB;
-    int64_t m = NONE;
-    if (r0 + r < A.R)
+    int64_t m[4] = {NONE, NONE, NONE, NONE};
 #pragma unroll 4
-      for (int t = tid / RB; t < nt; t += NT_B / RB) m = max(m, M[(size_t)t * A.Rp + r]);
-    red[tid / RB][r] = m;
-  }
-  __syncthreads();
-  if (tid < RB) {
-    int64_t m = red[0][tid];
-#pragma unroll
-    for (int k = 1; k < NT_B / RB; ++k) m = max(m, red[k][tid]);
-    rmax[tid] = m;
-    if (blockIdx.x == 0 && r0 + tid < A.R) A.gmax[lk * A.Rp + r0 + tid] = m;
-  }
-  __syncthreads();
-  const int q = tid % Q * 4, k0 = tid / Q;
-  uint64_t s[4] = {0, 0, 0, 0};
-  if (r0 + q < A.R)
-    for (int t = t0; t < t1; ++t) {
-      int off[4];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) off[c] = r0 + q + c < A.R ? rebase(ref[(size_t)t * A.Rp + q + c], rmax[q + c]) : FAR;
-      const int* S = A.S + ((lk * A.tiles + t) * A.groups + (r0 + q) / A.RG) * (size_t)TILE * A.RG +
-                     (size_t)k0 * A.RG + (r0 + q) % A.RG;
-      uint32_t p[4] = {0, 0, 0, 0};  // of TILE / KL exps
-#pragma unroll
-      for (int k = 0; k < TILE / KL; ++k) {
-        const int4 x = *(const int4*)(S + (size_t)k * KL * A.RG);
-        p[0] += exp32(x.x + off[0], lut);
-        p[1] += exp32(x.y + off[1], lut);
-        p[2] += exp32(x.z + off[2], lut);
-        p[3] += exp32(x.w + off[3], lut);
-      }
-#pragma unroll
-      for (int c = 0; c < 4; ++c) s[c] += p[c];
+    for (int t = k0; t < nt; t += kl) {
+      const longlong2 a = *(const longlong2*)(M + (size_t)t * A.Rp + q), b = *(const longlong2*)(M + (size_t)t * A.Rp + q + 2);
+      m[0] = max(m[0], (int64_t)a.x), m[1] = max(m[1], (int64_t)a.y);
+      m[2] = max(m[2], (int64_t)b.x), m[3] = max(m[3], (int64_t)b.y);
     }
 #pragma unroll
-  for (int c = 0; c < 4; ++c) red[k0][q + c] = (int64_t)s[c];
-  __syncthreads();
-  if (tid < RB && r0 + tid < A.R) {
-    uint64_t x = 0;
-#pragma unroll
-    for (int k = 0; k < KL; ++k) x += (uint64_t)red[k][tid];
-    A.sums[(lk * A.chunks + blockIdx.x) * A.Rp + r0 + tid] = x;
+    for (int c = 0; c < 4; ++c)
+      if (q + c < rows) atomicMax((long long*)&rmax[q + c], (long long)m[c]);
   }
+  __syncthreads();
+  if (blockIdx.x == 0 && tid < rows) A.gmax[lk * A.Rp + r0 + tid] = rmax[tid];
+  uint64_t s[4] = {0, 0, 0, 0};
+  for (int t = t0; t < t1; ++t) {
+    int off[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) off[c] = q + c < rows ? rebase(ref[(size_t)t * A.Rp + q + c], rmax[q + c]) : FAR;
+    const int* S = A.S + ((lk * A.tiles + t) * A.groups + grp) * (size_t)TILE * RG + q;
+    uint32_t p[4] = {0, 0, 0, 0};  // at most TILE exps
+#pragma unroll 8
+    for (int k = k0; k < TILE; k += kl) {
+      const int4 x = *(const int4*)(S + k * RG);
+      p[0] += exp32(x.x + off[0], lut);
+      p[1] += exp32(x.y + off[1], lut);
+      p[2] += exp32(x.z + off[2], lut);
+      p[3] += exp32(x.w + off[3], lut);
+    }
+#pragma unroll
+    for (int c = 0; c < 4; ++c) s[c] += p[c];
+  }
+#pragma unroll
+  for (int c = 0; c < 4; ++c)
+    if (q + c < rows) atomicAdd(&rsum[q + c], (unsigned long long)s[c]);
+  __syncthreads();
+  if (tid < rows) atomicAdd((unsigned long long*)A.sums + lk * A.Rp + r0 + tid, rsum[tid]);
 }
 
 // ------------------------------------------------------------------ 3. values
@@ -545,6 +554,7 @@ __global__ void __launch_bounds__(NT_V, 2) k_values(const Args A) {
   const int vbytes = CK * A.dh * 8, sbytes = CK * RG * 4;
   uint8_t* vbuf = dsm;                                 // 2 x [CK][dh] int64
   float* wbuf = (float*)(dsm + 2 * vbytes);            // 2 x [CK][RG] scores, then weights in place
+  int64_t* rbuf = (int64_t*)(dsm + 2 * (vbytes + sbytes));  // 2 x [RG] what the scores are relative to
   int* osum = (int*)dsm;                               // [RG][DHP] at a segment's end
   load_lut(lut, NT);
   if (tid == 0) {
@@ -580,20 +590,22 @@ __global__ void __launch_bounds__(NT_V, 2) k_values(const Args A) {
     const int64_t xf = ((first + 1) * X - 1) / N, xl = (off * X - 1) / N;
     const size_t lk = (size_t)bz * A.n_kv + kvh, lkg = lk * A.groups + grp;
     const int* pt = A.pt + lane * A.pt_stride;
-    int64_t* part0 = A.part + (size_t)blockIdx.y * (gridDim.x + A.lanes) * RG * A.dh;
-    int64_t* part = part0 + (size_t)(x + bz) * RG * A.dh;
+    // the segment's slot for 64-bit terms: x + bz differs from any other's
+    const size_t slot0 = (size_t)blockIdx.y * (gridDim.x + A.lanes) + bz;
+    int64_t* part = A.wide + (slot0 + x) * RG * A.dh;
     bool bad = T < 0;
-    for (int i = tid; !bad && i < (T + PAGE - 1) / PAGE; i += NT) bad |= !tree::page_ok(pt[i], A.n_pages);
+    for (int i = a0 * (CK / PAGE) + tid; !bad && i < min(a1 * (CK / PAGE), (T + PAGE - 1) / PAGE); i += NT)
+      bad |= !tree::page_ok(pt[i], A.n_pages);
     if (tid == 0) s_long = 0;
     bad = __syncthreads_or(bad);
-    if (bad && tid == 0) set_error(A.err, T < 0 ? ARCB_ERR_SEQ_OVERFLOW : ARCB_ERR_BOUNDS);
+    if (bad && tid == 0) {
+      set_error(A.err, T < 0 ? ARCB_ERR_SEQ_OVERFLOW : ARCB_ERR_BOUNDS);
+      atomicOr(A.bad + bz, 1);
+    }
     const bool live = T > 0 && !bad;
     if (live && tid < RG) {
       const bool row = tid < rows;
-      uint64_t s = 0;
-      if (row)
-#pragma unroll 4
-        for (int c = 0; c < A.chunks; ++c) s += A.sums[(lk * A.chunks + c) * A.Rp + r0 + tid];
+      const uint64_t s = row ? A.sums[lk * A.Rp + r0 + tid] : 0;
       rmax[tid] = row ? A.gmax[lk * A.Rp + r0 + tid] : NONE;
       rsum[tid] = s ? s : 1;  // a row without keys: every exp is 0
       if (s >> 30) s_long = 1;
@@ -616,37 +628,52 @@ __global__ void __launch_bounds__(NT_V, 2) k_values(const Args A) {
         rcp[c] = 65536.0f * __frcp_rn((float)(int64_t)rsum[rq + c]);
         ro[c] = FAR;
       }
-      auto issue = [&](int c) {  // one thread
+      int pg[CK / PAGE];  // thread 0: page ids of the chunk to issue next
+      auto fetch = [&](int c) {
+#pragma unroll
+        for (int i = 0; i < CK / PAGE; ++i) {
+          const int at = c * (CK / PAGE) + i;
+          pg[i] = at < (T + PAGE - 1) / PAGE ? pt[at] : -1;
+        }
+      };
+      auto issue = [&](int c) {  // thread 0
         const uint32_t bar = smem_u32(&full[issued & 1]), buf = issued & 1;
-        const int pages = min(CK / PAGE, (T + PAGE - 1) / PAGE - c * (CK / PAGE));
         const uint32_t pbytes = PAGE * A.dh * 8;
-        mbar_arrive_expect_tx(bar, pages * pbytes + sbytes);
-        for (int i = 0; i < pages; ++i)
-          bulk_g2s(smem_u32(vbuf) + buf * vbytes + i * pbytes,
-                   A.Vc + ((size_t)pt[c * (CK / PAGE) + i] * A.n_kv + kvh) * PAGE * A.dh, pbytes, bar);
+        uint32_t bytes = sbytes + RG * 8;
+#pragma unroll
+        for (int i = 0; i < CK / PAGE; ++i) bytes += pg[i] >= 0 ? pbytes : 0;
+        mbar_arrive_expect_tx(bar, bytes);
+#pragma unroll
+        for (int i = 0; i < CK / PAGE; ++i)
+          if (pg[i] >= 0)
+            bulk_g2s(smem_u32(vbuf) + buf * vbytes + i * pbytes,
+                     A.Vc + ((size_t)pg[i] * A.n_kv + kvh) * PAGE * A.dh, pbytes, bar);
         const int t = c / (TILE / CK);
+        bulk_g2s(smem_u32(rbuf + buf * RG), A.ref + (lk * A.tiles + t) * A.Rp + r0, RG * 8, bar);
         bulk_g2s(smem_u32(wbuf) + buf * sbytes,
                  A.S + (((lk * A.tiles + t) * A.groups + grp) * TILE + (c % (TILE / CK)) * CK) * (size_t)RG, sbytes, bar);
       };
       if (tid == 0) {
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // after the last segment's accesses
+        fetch(a0);
         issue(a0);
+        fetch(a0 + 1);
       }
       ++issued;
       for (int c = a0; c < a1; ++c) {
-        const int j0 = c * CK, t = j0 / TILE, keys = min(CK, T - j0);
+        const int j0 = c * CK, keys = min(CK, T - j0);
         if (c + 1 < a1) {
-          if (tid == 0) issue(c + 1);
+          if (tid == 0) {
+            issue(c + 1);
+            fetch(c + 2);
+          }
           ++issued;
-        }
-        if (c == a0 || j0 % TILE == 0) {
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            ro[k] = rq + k < rows ? rebase(A.ref[(lk * A.tiles + t) * A.Rp + r0 + rq + k], rmax[rq + k]) : FAR;
         }
         if (!mbar_wait(smem_u32(&full[used & 1]), (used >> 1) & 1)) set_error(A.err, ARCB_ERR_TIMEOUT_FULL);
         int64_t* vb = (int64_t*)(vbuf + (used & 1) * vbytes);
         float* wb = wbuf + (used & 1) * CK * RG;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) ro[k] = rq + k < rows ? rebase(rbuf[(used & 1) * RG + rq + k], rmax[rq + k]) : FAR;
         ++used;
         // values to single precision, v / 2^16 over each low word.  Where they fit, y = v + VMAX is in
         // [0, 2 VMAX]: the low bits of the float 2^23 + y, then exact: (that - 2^23 - VMAX) / 2^16
@@ -736,40 +763,40 @@ __global__ void __launch_bounds__(NT_V, 2) k_values(const Args A) {
       __syncthreads();
     }
     const int quads = A.dh / 4;
+    bool lost = !live, wides = false;  // the lane gives zeros; some segment has 64-bit terms
+    unsigned long long* acc2 = (unsigned long long*)A.acc + lkg * RG * (A.dh / 2);
     if (xl > xf) {
-      for (int i = tid; i < rows * quads; i += NT) {
-        const int r = i / quads, e = i % quads * 4;
-        longlong2* p = (longlong2*)(part + r * A.dh + e);
-        longlong2 a = make_longlong2(0, 0), b = make_longlong2(0, 0);
-        if (live) {
-          const int4 v = *(const int4*)(osum + r * DHP + e);
-          a = make_longlong2(v.x, v.y), b = make_longlong2(v.z, v.w);
+      if (live)
+        for (int i = tid; i < rows * (A.dh / 2); i += NT) {
+          const int r = i / (A.dh / 2), e = i % (A.dh / 2) * 2;
+          const int2 v = *(const int2*)(osum + r * DHP + e);
+          // both sums and their totals over the lane fit in int32
+          atomicAdd(acc2 + i, (unsigned long long)(((int64_t)v.y << 32) + v.x));
         }
-        if (any_wide) {
-          const longlong2 c = p[0], d = p[1];
-          a.x = wadd(a.x, c.x), a.y = wadd(a.y, c.y), b.x = wadd(b.x, d.x), b.y = wadd(b.y, d.y);
-        }
-        __stcg(p, a);
-        __stcg(p + 1, b);
-      }
+      if (any_wide && tid == 0) A.is_wide[slot0 + x] = 1;
       __threadfence();
       __syncthreads();
       if (tid == 0) s_last = atomicAdd(A.arrived + lkg, 1) == (int)(xl - xf);
       __syncthreads();
       if (!s_last) continue;
       __threadfence();
+      lost |= __ldcg(A.bad + bz) != 0;
+      for (int64_t s = xf + tid; s <= xl; s += NT) wides |= __ldcg(A.is_wide + slot0 + s) != 0;
+      wides = __syncthreads_or(wides);
     }
     const size_t d = (size_t)A.n_heads * A.dh;
     for (int i = tid; i < rows * quads; i += NT) {
       const int r = i / quads, e = i % quads * 4, rr = r0 + r;
       int64_t o[4] = {0, 0, 0, 0};
-      if (xl > xf) {
-        const int64_t* p = part0 + (size_t)(xf + bz) * RG * A.dh + r * A.dh + e;
-        for (int64_t s = xf; s <= xl; ++s, p += (size_t)RG * A.dh) {
-          const longlong2 a = __ldcg((const longlong2*)p), b = __ldcg((const longlong2*)p + 1);
-          o[0] = wadd(o[0], a.x), o[1] = wadd(o[1], a.y), o[2] = wadd(o[2], b.x), o[3] = wadd(o[3], b.y);
-        }
-      } else if (live) {
+      if (!lost && xl > xf) {
+        const ulonglong2 v = __ldcg((const ulonglong2*)(acc2 + r * (A.dh / 2) + e / 2));
+        o[0] = (int)(uint32_t)v.x, o[1] = ((int64_t)v.x - o[0]) >> 32;
+        o[2] = (int)(uint32_t)v.y, o[3] = ((int64_t)v.y - o[2]) >> 32;
+        for (int64_t s = xf; wides && s <= xl; ++s)
+          if (__ldcg(A.is_wide + slot0 + s))
+#pragma unroll
+            for (int c = 0; c < 4; ++c) o[c] = wadd(o[c], __ldcg(A.wide + (slot0 + s) * RG * A.dh + r * A.dh + e + c));
+      } else if (!lost) {
 #pragma unroll
         for (int c = 0; c < 4; ++c) o[c] = wadd(osum[r * DHP + e + c], any_wide ? part[r * A.dh + e + c] : 0);
       }
@@ -794,7 +821,7 @@ __global__ void __launch_bounds__(NT_V, 2) k_values(const Args A) {
 // Sizes that follow from the shapes; `lanes` of them per launch.
 struct Plan {
   int lanes, R, Rp, G, tiles, chunks, groups, RG, splits, threads, unit, rows_s;
-  size_t oS, oM, oR, oG, oSum, oP, oA, bytes;
+  size_t oS, oM, oR, oG, oSum, oW, oAcc, oA, oB, oF, bytes;
 };
 
 constexpr size_t WS_TARGET = size_t(1) << 30;  // lanes are batched to about this much workspace
@@ -808,7 +835,7 @@ static Plan plan(int lanes, int nq, int n_heads, int n_kv, int dh, int t_lim) {
   p.RG = ((p.R + p.groups - 1) / p.groups + p.unit - 1) / p.unit * p.unit;
   p.Rp = p.groups * p.RG;
   p.tiles = (t_lim + TILE - 1) / TILE;
-  p.chunks = p.tiles < 16 ? p.tiles : 16;
+  p.chunks = p.tiles < 32 ? p.tiles : 32;
   const size_t per_s = (size_t)n_kv * p.tiles * TILE * p.Rp * 4;
   p.lanes = (int)(WS_TARGET / per_s);
   p.lanes = p.lanes < 1 ? 1 : (p.lanes > lanes ? lanes : p.lanes);
@@ -834,9 +861,13 @@ static Plan plan(int lanes, int nq, int n_heads, int n_kv, int dh, int t_lim) {
   p.oM = take(lk * p.tiles * p.Rp * 8);
   p.oR = take(lk * p.tiles * p.Rp * 8);
   p.oG = take(lk * p.Rp * 8);
-  p.oSum = take(lk * p.chunks * p.Rp * 8);
-  p.oP = take((size_t)n_kv * p.groups * (p.splits + p.lanes) * p.RG * dh * 8);
+  p.oSum = take(lk * p.Rp * 8);
+  const size_t slots = (size_t)n_kv * p.groups * (p.splits + p.lanes);
+  p.oW = take(slots * p.RG * dh * 8);
+  p.oAcc = take(lk * p.groups * p.RG * dh * 4);
   p.oA = take(lk * p.groups * 4);
+  p.oB = take(p.lanes * 4);
+  p.oF = take(slots * 4);
   p.bytes = o;
   return p;
 }
@@ -844,7 +875,7 @@ static Plan plan(int lanes, int nq, int n_heads, int n_kv, int dh, int t_lim) {
 template <int DHP, int UR>
 static int run(Args A, const Plan& p, int lanes, cudaStream_t st) {
   constexpr int smem_s = 1024 + PLANES * (TILE + RQ) * 128;
-  const int vals = 2 * CK * (A.dh * 8 + p.RG * 4), sums = p.RG * DHP * 4, smem_v = vals > sums ? vals : sums;
+  const int vals = 2 * (CK * (A.dh * 8 + p.RG * 4) + p.RG * 8), sums = p.RG * DHP * 4, smem_v = vals > sums ? vals : sums;
   const auto kv = k_values<DHP / 32, UR>;
   cudaError_t e = cudaFuncSetAttribute(k_scores<DHP>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_s);
   if (e == cudaSuccess) e = cudaFuncSetAttribute(kv, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_v);
@@ -854,7 +885,7 @@ static int run(Args A, const Plan& p, int lanes, cudaStream_t st) {
     A.lane0 = l0, A.lanes = n;
     int rc = launch_k(k_scores<DHP>, dim3(p.tiles, A.n_kv * ((p.R + p.rows_s - 1) / p.rows_s), n), dim3(NT_S), smem_s,
                       st, A);
-    if (!rc) rc = launch_k(k_sums, dim3(p.chunks, A.n_kv * ((p.R + RB - 1) / RB), n), dim3(NT_B), 0, st, A);
+    if (!rc) rc = launch_k(k_sums, dim3(p.chunks, A.n_kv * p.groups, n), dim3(p.threads), 0, st, A);
     if (!rc) rc = launch_k(kv, dim3(p.splits, A.n_kv * p.groups), dim3(p.threads), smem_v, st, A);
     if (rc) return rc;
   }
@@ -889,7 +920,8 @@ int arcb_attn_tree(const int64_t* q, const int64_t* Kc, const int64_t* Vc, int n
   A.R = p.R, A.Rp = p.Rp, A.G = p.G, A.tiles = p.tiles, A.chunks = p.chunks, A.groups = p.groups, A.RG = p.RG;
   A.splits = p.splits, A.rows_s = p.rows_s;
   A.S = (int*)(b + p.oS), A.M = (int64_t*)(b + p.oM), A.ref = (int64_t*)(b + p.oR), A.gmax = (int64_t*)(b + p.oG);
-  A.sums = (uint64_t*)(b + p.oSum), A.part = (int64_t*)(b + p.oP), A.arrived = (int*)(b + p.oA);
+  A.sums = (uint64_t*)(b + p.oSum), A.wide = (int64_t*)(b + p.oW), A.acc = (uint64_t*)(b + p.oAcc);
+  A.arrived = (int*)(b + p.oA), A.bad = (int*)(b + p.oB), A.is_wide = (int*)(b + p.oF);
   A.X = X, A.lmax = lmax, A.o_out = o_out, A.err = err;
   cudaStream_t st = (cudaStream_t)stream;
   if (p.unit == 8) return dh <= 64 ? at::run<64, 8>(A, p, lanes, st) : at::run<128, 8>(A, p, lanes, st);
