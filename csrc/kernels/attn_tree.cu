@@ -14,19 +14,21 @@
 //
 // The queries of a KV head (nq nodes x G query heads: R rows) share its K and
 // V.  Exact weights need the global max and sum before the first value, so
-// there are three kernels:
+// there are four kernels:
 //
+//  0. k_queries: the query rows' digits (see 1) in groups of 32 rows.
 //  1. k_scores, one CTA per 128 keys.  K's int64 elements become signed
 //     radix-256 digits (byte l of (x + 0x80..80) ^ 0x80..80, int8), one
 //     128-byte-swizzled plane of 128 keys x dh per digit, read once from DRAM;
-//     so do 32 query rows at a time.  q.k = sum over digit pairs (a, b) of
+//     the query rows' planes come by bulk copies, 32 rows at a time.  q.k = sum over digit pairs (a, b) of
 //     D_{a+b} << 8(a+b) with D_s = sum_{a+b=s} K_a.Q_b^T: tcgen05 kind::i8
 //     products of M = 128 keys, N = 32 rows into one TMEM accumulator per s
 //     (exact in int32: at most 4 * 128 * 2^14).  3 digits (|x| < 2^23) are
 //     usual; up to 4 (|x| < 2^31) run this way, wider tiles take 64-bit
 //     products.  Scores are stored relative to their tile's max (differences
-//     below -2^30 clamped: their exp is 0 either way), which is stored beside.
-//  2. k_sums: each row's global max and sum of exps, split over key chunks.
+//     below -2^30 clamped: their exp is 0 either way) or, where 32 bits hold
+//     them, as they are; the rows' maxima join by atomics.
+//  2. k_sums: each row's sum of exps, split over key chunks.
 //  3. k_values: w.v for up to 128 rows and a range of keys.  The floor of each
 //     term rules out a matrix product, but one single-precision FMA rounding
 //     toward minus infinity is exact: acc <- rd(acc + w * (v / 2^16)) with acc
@@ -68,14 +70,15 @@ struct Args {
   const int64_t* mask;
   int64_t pt_stride, attn_scale;
   int n_pages, width, nq, n_heads, n_kv, dh, t_lim, B, lane0, lanes;
-  int R, Rp, G, tiles, chunks, groups, RG, splits, rows_s;
+  int R, Rp, G, tiles, chunks, groups, RG, splits, rows_s, qgroups;
   // workspace
   int* S;              // [lanes][n_kv][tiles][groups][TILE][RG] scores less ref
-  int64_t* M;          // [lanes][n_kv][tiles][Rp] max of the tile
-  int64_t* ref;        // [lanes][n_kv][tiles][Rp]: 0, or M where scores are not small
-  int64_t* gmax;       // [lanes][n_kv][Rp]
+  int64_t* ref;        // [lanes][n_kv][tiles][Rp]: 0, or the tile's max where scores are not small
+  uint8_t* planes;     // [lanes][n_kv][qgroups][PLANES][RQ][128] query digits, swizzled
+  uint4* qinfo;        // [lanes][n_kv][qgroups] ors of low and high digit words, largest magnitude
   int64_t* wide;       // [n_kv][groups][splits + lanes][RG][dh]: 64-bit terms of a segment
-  // zeroed by k_scores:
+  // set to NONE and to zero by k_queries:
+  int64_t* gmax;       // [lanes][n_kv][Rp] rows' largest scores
   uint64_t* sums;      // [lanes][n_kv][Rp] of exps
   uint64_t* acc;       // [lanes][n_kv][groups][RG][dh / 2]: two int32 sums each
   int* arrived;        // [lanes][n_kv][groups]
@@ -141,23 +144,90 @@ __device__ __forceinline__ void load4(int64_t* x, const int64_t* src) {
   x[0] = a.x, x[1] = a.y, x[2] = b.x, x[3] = b.y;
 }
 
+// ----------------------------------------------------------------- 0. queries
+// grid (qgroups, n_kv, lanes): the digit planes of RQ query rows in the layout
+// that k_scores copies, and the start values of what the next kernels add to.
+template <int DHP>
+__global__ void __launch_bounds__(NT_S) k_queries(const Args A) {
+  constexpr int TPR = DHP / 4, QN = RQ * TPR / NT_S;
+  __shared__ uint32_t info[3];
+  const int tid = threadIdx.x, ln = tid & 31;
+  const int g = blockIdx.x, kvh = blockIdx.y, lane = A.lane0 + blockIdx.z;
+  const size_t lk = (size_t)blockIdx.z * A.n_kv + kvh;
+  if (tid < 3) info[tid] = 0;
+  __syncthreads();
+  pdl_wait_dep();
+  pdl_allow_next();
+  const int col = (tid % TPR) * 4;
+  int64_t x[QN][4];
+#pragma unroll
+  for (int i = 0; i < QN; ++i) {
+    const int rr = g * RQ + tid / TPR + i * (NT_S / TPR);
+    if (rr < A.R && col < A.dh)
+      load4(x[i], A.q + ((size_t)(lane * A.nq + rr / A.G) * A.n_heads + kvh * A.G + rr % A.G) * A.dh + col);
+    else
+      x[i][0] = x[i][1] = x[i][2] = x[i][3] = 0;
+  }
+  {
+    ulonglong2* z = (ulonglong2*)(A.acc + lk * A.groups * A.RG * (A.dh / 2));
+    for (int i = g * NT_S + tid; i < A.groups * A.RG * (A.dh / 4); i += A.qgroups * NT_S) z[i] = make_ulonglong2(0, 0);
+    for (int i = g * NT_S + tid; i < A.Rp; i += A.qgroups * NT_S) {
+      A.sums[lk * A.Rp + i] = 0;
+      A.gmax[lk * A.Rp + i] = NONE;
+    }
+    if (g == 0) {
+      for (int i = tid; i < A.groups; i += NT_S) A.arrived[lk * A.groups + i] = 0;
+      if (kvh == 0 && tid == 0) A.bad[blockIdx.z] = 0;
+      if (blockIdx.z == 0)
+        for (int i = tid; i < A.groups * (A.splits + A.lanes); i += NT_S)
+          A.is_wide[(size_t)kvh * A.groups * (A.splits + A.lanes) + i] = 0;
+    }
+  }
+  uint8_t* out = A.planes + (lk * A.qgroups + g) * (PLANES * RQ * 128);
+  uint32_t lo = 0, hi = 0, mag = 0;
+#pragma unroll
+  for (int i = 0; i < QN; ++i) {
+    const int r = tid / TPR + i * (NT_S / TPR);
+    uint32_t d[4];
+    digits4(x[i], d, lo, hi);
+    mag = max(mag, magnitude4(x[i]));
+    const uint32_t at = r * 128 + (((col >> 4) ^ (r & 7)) << 4) + (col & 15);
+#pragma unroll
+    for (int l = 0; l < PLANES; ++l) *(uint32_t*)(out + l * (RQ * 128) + at) = d[l];
+  }
+  lo = __reduce_or_sync(0xffffffffu, lo);
+  hi = __reduce_or_sync(0xffffffffu, hi);
+  mag = __reduce_max_sync(0xffffffffu, mag);
+  if (ln == 0) {
+    atomicOr(&info[0], lo);
+    atomicOr(&info[1], hi);
+    atomicMax(&info[2], mag);
+  }
+  __syncthreads();
+  if (tid == 0) A.qinfo[lk * A.qgroups + g] = make_uint4(info[0], info[1], info[2], 0);
+}
+
 // ------------------------------------------------------------------ 1. scores
+__device__ __forceinline__ void bulk_g2s(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+               "l"(src), "r"(bytes), "r"(bar)
+               : "memory");
+}
+
 // grid (tiles, n_kv * row blocks of rows_s, lanes).
 // DHP: row pitch class of the planes (64 or 128 >= dh).
 template <int DHP>
 __global__ void __launch_bounds__(NT_S, 2) k_scores(const Args A) {
   constexpr int KP = TILE * 128, QP = RQ * 128;  // bytes per plane
   constexpr int TPR = DHP / 4;                   // threads per row
-  constexpr int QN = RQ * TPR / NT_S;            // query quads per thread
   constexpr int TMEM_COLS = 256;                 // (2 * PLANES - 1) * RQ = 224 used
   extern __shared__ __align__(1024) uint8_t dsm[];
-  __shared__ int64_t wmax[4][RQ];
+  __shared__ int64_t wmax[2][4][RQ];
   __shared__ uint64_t qmask[2][RQ];
   __shared__ int pages[TILE / PAGE];
-  // ors of low and high digit words, largest magnitude: keys; queries of even / odd groups
-  __shared__ uint32_t or_k[3], or_q[2][3];
+  __shared__ uint32_t or_k[3];  // ors of the keys' low and high digit words, largest magnitude
   __shared__ uint32_t tslot;
-  __shared__ __align__(8) uint64_t done;
+  __shared__ __align__(8) uint64_t done, qfull[2];
   __shared__ int s_abort;
   const int tid = threadIdx.x, ln = tid & 31, w = tid >> 5;
   const int rbs = (A.R + A.rows_s - 1) / A.rows_s;
@@ -166,17 +236,18 @@ __global__ void __launch_bounds__(NT_S, 2) k_scores(const Args A) {
   const size_t lk = (size_t)blockIdx.z * A.n_kv + kvh;
   const uint32_t kbase = (smem_u32(dsm) + 1023u) & ~1023u, qbase = kbase + PLANES * KP;
   uint8_t* kp = dsm + (kbase - smem_u32(dsm));
-  uint8_t* qp = kp + PLANES * KP;
   if (w == 0) {
     tmem_alloc(smem_u32(&tslot), TMEM_COLS);
     tmem_relinquish();
   }
   if (tid == 0) {
     mbar_init(smem_u32(&done), 1);
+    mbar_init(smem_u32(&qfull[0]), 1);
+    mbar_init(smem_u32(&qfull[1]), 1);
     fence_barrier_init();
     s_abort = 0;
   }
-  if (tid < 3) or_k[tid] = or_q[0][tid] = 0;
+  if (tid < 3) or_k[tid] = 0;
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -186,20 +257,6 @@ __global__ void __launch_bounds__(NT_S, 2) k_scores(const Args A) {
   pdl_allow_next();
   const int base = A.base[lane], nt = A.n_tree[lane];
   const int T = tree::lane_keys(base, nt, A.t_lim, A.width);
-  // what the next kernels add into, zeroed by the CTAs of each lane and KV head
-  {
-    const int cta = tile * rbs + blockIdx.y % rbs, ctas = gridDim.x * rbs;
-    ulonglong2* z = (ulonglong2*)(A.acc + lk * A.groups * A.RG * (A.dh / 2));
-    for (int i = cta * NT_S + tid; i < A.groups * A.RG * (A.dh / 4); i += ctas * NT_S) z[i] = make_ulonglong2(0, 0);
-    if (cta == 0) {
-      for (int i = tid; i < A.Rp; i += NT_S) A.sums[lk * A.Rp + i] = 0;
-      for (int i = tid; i < A.groups; i += NT_S) A.arrived[lk * A.groups + i] = 0;
-      if (kvh == 0 && tid == 0) A.bad[blockIdx.z] = 0;
-      if (blockIdx.z == 0)
-        for (int i = tid; i < A.groups * (A.splits + A.lanes); i += NT_S)
-          A.is_wide[(size_t)kvh * A.groups * (A.splits + A.lanes) + i] = 0;
-    }
-  }
   const int j0 = tile * TILE;
   const bool live = j0 < T;
   if (live && tid < TILE / PAGE) {
@@ -207,22 +264,15 @@ __global__ void __launch_bounds__(NT_S, 2) k_scores(const Args A) {
     const int p = j < T ? A.pt[lane * A.pt_stride + j / PAGE] : -1;
     pages[tid] = tree::page_ok(p, A.n_pages) ? p : -1;
   }
+  auto load_q = [&](int r0, int b) {  // one thread: the planes of rows r0 .. r0 + RQ - 1 into buffer b
+    const uint32_t bar = smem_u32(&qfull[b]);
+    mbar_arrive_expect_tx(bar, PLANES * QP);
+    bulk_g2s(qbase + b * PLANES * QP, A.planes + (lk * A.qgroups + r0 / RQ) * (PLANES * QP), PLANES * QP, bar);
+  };
+  if (live && tid == 0) load_q(r_lo, 0);
   __syncthreads();
   if (live) {
     const int col = (ln % TPR) * 4;
-    // ---- the first query rows' loads in flight beside the keys'
-    int64_t xq[QN][4];
-    auto load_q = [&](int r0) {
-#pragma unroll
-      for (int i = 0; i < QN; ++i) {
-        const int rr = r0 + tid / TPR + i * (NT_S / TPR);
-        if (rr < r_hi && col < A.dh)
-          load4(xq[i], A.q + ((size_t)(lane * A.nq + rr / A.G) * A.n_heads + kvh * A.G + rr % A.G) * A.dh + col);
-        else
-          xq[i][0] = xq[i][1] = xq[i][2] = xq[i][3] = 0;
-      }
-    };
-    load_q(r_lo);
     // ---- K digit planes: a warp reads 32 / TPR whole rows at a time
     constexpr int RPW = 32 / TPR, STEPS = TILE / (8 * RPW), UN = STEPS < 8 ? STEPS : 8;
     uint32_t lo = 0, hi = 0, mag = 0;
@@ -261,60 +311,47 @@ __global__ void __launch_bounds__(NT_S, 2) k_scores(const Args A) {
     int* Srow = A.S + (lk * A.tiles + tile) * A.groups * group_elems + (size_t)((w & 3) * 32 + ln) * A.RG;
     const int kend = (A.dh + 31) / 32;
     const bool all_seen = j0 + TILE <= base;  // every key of the tile is below the tree
-    uint32_t parity = 0;
-    for (int r0 = r_lo, g = 0; r0 < r_hi; r0 += RQ, g ^= 1) {
-      const int rows = min(RQ, r_hi - r0), nmma = rows > 16 ? 32 : 16;
-      // ---- query digit planes and masks of rows [r0, r0 + 32); the last
-      // group's products are done, so its planes are free
-      lo = hi = mag = 0;
-#pragma unroll
-      for (int i = 0; i < QN; ++i) {
-        const int r = tid / TPR + i * (NT_S / TPR);
-        uint32_t d[4];
-        digits4(xq[i], d, lo, hi);
-        mag = max(mag, magnitude4(xq[i]));
-        const uint32_t at = r * 128 + (((col >> 4) ^ (r & 7)) << 4) + (col & 15);
-#pragma unroll
-        for (int l = 0; l < PLANES; ++l) *(uint32_t*)(qp + l * QP + at) = d[l];
-      }
-      if (!all_seen && tid < RQ)
-        qmask[g][tid] = tid < rows ? (uint64_t)A.mask[(size_t)lane * A.nq + (r0 + tid) / A.G] : 0;
-      lo = __reduce_or_sync(0xffffffffu, lo);
-      hi = __reduce_or_sync(0xffffffffu, hi);
-      mag = __reduce_max_sync(0xffffffffu, mag);
-      if (ln == 0) {
-        atomicOr(&or_q[g][0], lo);
-        atomicOr(&or_q[g][1], hi);
-        atomicMax(&or_q[g][2], mag);
-      }
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      tc_fence_before();
-      __syncthreads();
-      tc_fence_after();
-      const int lk_n = planes_of(or_k[0]), lq_n = planes_of(or_q[g][0]);
-      const bool wide = (or_k[1] | or_q[g][1]) != 0;
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncthreads();
+    const int lk_n = planes_of(or_k[0]);
+    uint32_t products = 0;  // groups that took the tensor path
+    for (int r0 = r_lo, n = 0; r0 < r_hi; r0 += RQ, ++n) {
+      const int rows = min(RQ, r_hi - r0), b = n & 1;
+      const uint4 qi = __ldg(A.qinfo + lk * A.qgroups + r0 / RQ);
+      const int lq_n = planes_of(qi.x);
+      const bool wide = (or_k[1] | qi.y) != 0;
       // |q.k| <= dh * max|k| * max|q| < 2^47 and scale <= ONE / 4: 32 bits hold
       // every step below, and |score| <= 2^29
       const bool small = !wide && A.attn_scale >= 0 && A.attn_scale <= ONE / 4 &&
-                         ((uint64_t)or_k[2] + 1) * ((uint64_t)or_q[g][2] + 1) < (uint64_t(1) << 47) / A.dh;
-      if (!wide) {
-        if (tid == 0) {
-          const uint32_t idesc = idesc_i8(TILE, nmma);
+                         ((uint64_t)or_k[2] + 1) * ((uint64_t)qi.z + 1) < (uint64_t(1) << 47) / A.dh;
+      if (!all_seen && tid < RQ)
+        qmask[b][tid] = tid < rows ? (uint64_t)A.mask[(size_t)lane * A.nq + (r0 + tid) / A.G] : 0;
+      if (tid == 0) {
+        // the other buffer's products are done (waited for by all before the last barrier)
+        if (r0 + RQ < r_hi) load_q(r0 + RQ, b ^ 1);
+        if (!mbar_wait(smem_u32(&qfull[b]), (n >> 1) & 1)) s_abort = 1;
+        if (!wide) {
+          // K_a times the stacked planes Q_0 | Q_1 | ..: plane b lands in accumulator a + b.
+          // At k = 0 the accumulator that a reaches first is overwritten, by a product of its own.
+          const uint32_t qb = qbase + b * PLANES * QP;
           for (int a = 0; a < lk_n; ++a)
-            for (int b = 0; b < lq_n; ++b)
-              for (int k = 0; k < kend; ++k)
-                // the first pair of a sum a + b (a = 0, or b = lq_n - 1) overwrites its accumulator
-                mma_i8(tmem + (a + b) * RQ, sw128_kmajor_desc(kbase + a * KP + k * 32),
-                       sw128_kmajor_desc(qbase + b * QP + k * 32), idesc,
-                       (k > 0 || (a > 0 && b < lq_n - 1)) ? 1u : 0u);
+            for (int k = 0; k < kend; ++k) {
+              const uint64_t ka = sw128_kmajor_desc(kbase + a * KP + k * 32);
+              const bool split = a > 0 && k == 0;
+              const int nb = split ? lq_n - 1 : lq_n;
+              if (nb > 0)
+                mma_i8(tmem + a * RQ, ka, sw128_kmajor_desc(qb + k * 32), idesc_i8(TILE, nb * RQ), a > 0 || k > 0);
+              if (split)
+                mma_i8(tmem + (a + nb) * RQ, ka, sw128_kmajor_desc(qb + nb * QP + k * 32), idesc_i8(TILE, RQ), 0u);
+            }
           mma_commit(smem_u32(&done));
         }
-        if (r0 + RQ < r_hi) load_q(r0 + RQ);  // in flight beside the products and the epilogue
-        if (!mbar_wait(smem_u32(&done), parity)) s_abort = 1;
-        parity ^= 1;
+      }
+      if (!all_seen) __syncthreads();  // qmask
+      if (!wide) {
+        if (!mbar_wait(smem_u32(&done), products & 1)) s_abort = 1;
+        ++products;
         tc_fence_after();
-      } else if (r0 + RQ < r_hi) {
-        load_q(r0 + RQ);
       }
       // ---- scores of 16 rows per warp: rows c0 .. c0 + 15 of the group
       const int c0 = (w >> 2) * 16, ns = lk_n + lq_n - 1;
@@ -325,7 +362,7 @@ __global__ void __launch_bounds__(NT_S, 2) k_scores(const Args A) {
           seen = 0;
 #pragma unroll
           for (int i = 0; i < 16; ++i)
-            if (tree::visible(j, base, nt, qmask[g][c0 + i])) seen |= 1u << i;
+            if (tree::visible(j, base, nt, qmask[b][c0 + i])) seen |= 1u << i;
         }
         int out[16];
         int64_t m64 = NONE;  // lane i: max of row c0 + i over the warp's keys
@@ -343,21 +380,24 @@ __global__ void __launch_bounds__(NT_S, 2) k_scores(const Args A) {
           }
 #pragma unroll
           for (int i = 0; i < 16; ++i) t[i] = (uint32_t)((int)t[i] >> 16);
-#pragma unroll 1
-          for (int s = 2; s < ns; ++s) {
-            tmem_ld16(tcol + s * RQ, r);
-            tmem_ld_wait();
-            const int sh = 8 * s - 16;  // up to 32: a shift of 32 gives 0, right modulo 2^32
 #pragma unroll
-            for (int i = 0; i < 16; ++i) t[i] += __funnelshift_lc(0u, r[i], sh);
-          }
+          for (int s = 2; s < 2 * PLANES - 2; ++s)  // D_6 << 32 is 0
+            if (s < ns) {
+              tmem_ld16(tcol + s * RQ, r);
+              tmem_ld_wait();
+#pragma unroll
+              for (int i = 0; i < 16; ++i) t[i] += r[i] << (8 * s - 16);
+            }
           const int sc = (int)A.attn_scale << 16;  // (x * scale) >> 16 = the high word of x * (scale << 16)
+          int m32 = FAR;
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
-            out[i] = seen >> i & 1 ? __mulhi((int)t[i], sc) : FAR;
+            out[i] = __mulhi((int)t[i], sc);
+            if (!all_seen && !(seen >> i & 1)) out[i] = FAR;
             const int m = __reduce_max_sync(0xffffffffu, out[i]);
-            if (ln == i) m64 = m == FAR ? NONE : m;
+            if (ln == i) m32 = m;
           }
+          m64 = m32 == FAR ? NONE : m32;
         } else {
           int64_t sc[16];
 #pragma unroll
@@ -393,25 +433,24 @@ __global__ void __launch_bounds__(NT_S, 2) k_scores(const Args A) {
             sc[i] = attn_score(sc[i], A.attn_scale);
             int64_t m = seen >> i & 1 ? sc[i] : NONE;
 #pragma unroll
-            for (int b = 16; b >= 1; b >>= 1) {
-              const int64_t o = shfl_xor_i64(m, b);
+            for (int x = 16; x >= 1; x >>= 1) {
+              const int64_t o = shfl_xor_i64(m, x);
               m = o > m ? o : m;
             }
             if (ln == i) m64 = m;
           }
-          if (ln < 16) wmax[w & 3][c0 + ln] = m64;
+          if (ln < 16) wmax[b][w & 3][c0 + ln] = m64;
           asm volatile("bar.sync %0, 128;" ::"r"(1 + (w >> 2)) : "memory");  // the four warps of these rows
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
-            int64_t m = wmax[0][c0 + i];
+            int64_t m = wmax[b][0][c0 + i];
 #pragma unroll
-            for (int k = 1; k < 4; ++k) m = wmax[k][c0 + i] > m ? wmax[k][c0 + i] : m;
+            for (int k = 1; k < 4; ++k) m = wmax[b][k][c0 + i] > m ? wmax[b][k][c0 + i] : m;
             const int64_t d = sc[i] - m;
             out[i] = (seen >> i & 1) && d > FAR ? (int)d : FAR;
           }
-          asm volatile("bar.sync %0, 128;" ::"r"(1 + (w >> 2)) : "memory");
         }
-        if (ln < 16) wmax[w & 3][c0 + ln] = m64;
+        if (ln < 16) wmax[b][w & 3][c0 + ln] = m64;
         // 16 rows lie in one group: RG is a multiple of 16, or the only group's 8
         int* dst = Srow + (r0 + c0) / A.RG * group_elems + (r0 + c0) % A.RG;
 #pragma unroll
@@ -422,15 +461,12 @@ __global__ void __launch_bounds__(NT_S, 2) k_scores(const Args A) {
       __syncthreads();  // wmax; this group's accumulators and query planes are read
       tc_fence_after();
       if (tid < rows) {
-        int64_t m = wmax[0][tid];
+        int64_t m = wmax[b][0][tid];
 #pragma unroll
-        for (int k = 1; k < 4; ++k) m = wmax[k][tid] > m ? wmax[k][tid] : m;
-        const size_t at = (lk * A.tiles + tile) * A.Rp + r0 + tid;
-        A.M[at] = m;
-        A.ref[at] = small ? 0 : m;
+        for (int k = 1; k < 4; ++k) m = wmax[b][k][tid] > m ? wmax[b][k][tid] : m;
+        A.ref[(lk * A.tiles + tile) * A.Rp + r0 + tid] = small ? 0 : m;
+        if (m != NONE) atomicMax((long long*)A.gmax + lk * A.Rp + r0 + tid, (long long)m);
       }
-      if (tid < 3) or_q[g ^ 1][tid] = 0;  // read before the last group's end, next or-ed after this one's writes
-      __syncthreads();
     }
   }
   tc_fence_before();
@@ -460,25 +496,10 @@ __global__ void __launch_bounds__(NT_V) k_sums(const Args A) {
   const int nt = (T + TILE - 1) / TILE, X = min((int)gridDim.x, nt);
   if ((int)blockIdx.x >= X) return;
   const int t0 = (int)((int64_t)blockIdx.x * nt / X), t1 = (int)((int64_t)(blockIdx.x + 1) * nt / X);
-  const int64_t* M = A.M + lk * A.tiles * A.Rp + r0;
   const int64_t* ref = A.ref + lk * A.tiles * A.Rp + r0;
-  if (tid < RG) rmax[tid] = NONE, rsum[tid] = 0;
+  if (tid < RG) rmax[tid] = tid < rows ? A.gmax[lk * A.Rp + r0 + tid] : NONE, rsum[tid] = 0;
   __syncthreads();
   const int q = tid % (RG / 4) * 4, k0 = tid / (RG / 4), kl = NT / (RG / 4);
-  {
-    int64_t m[4] = {NONE, NONE, NONE, NONE};
-#pragma unroll 4
-    for (int t = k0; t < nt; t += kl) {
-      const longlong2 a = *(const longlong2*)(M + (size_t)t * A.Rp + q), b = *(const longlong2*)(M + (size_t)t * A.Rp + q + 2);
-      m[0] = max(m[0], (int64_t)a.x), m[1] = max(m[1], (int64_t)a.y);
-      m[2] = max(m[2], (int64_t)b.x), m[3] = max(m[3], (int64_t)b.y);
-    }
-#pragma unroll
-    for (int c = 0; c < 4; ++c)
-      if (q + c < rows) atomicMax((long long*)&rmax[q + c], (long long)m[c]);
-  }
-  __syncthreads();
-  if (blockIdx.x == 0 && tid < rows) A.gmax[lk * A.Rp + r0 + tid] = rmax[tid];
   uint64_t s[4] = {0, 0, 0, 0};
   for (int t = t0; t < t1; ++t) {
     int off[4];
@@ -526,12 +547,6 @@ __device__ __forceinline__ int store_limbs4(int8_t* X, int slot, int B, size_t l
     *(uint32_t*)(X + limb_row(l, slot, B) * ldx + col) = word;
   }
   return need;
-}
-
-__device__ __forceinline__ void bulk_g2s(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
-               "l"(src), "r"(bytes), "r"(bar)
-               : "memory");
 }
 
 // grid (splits, n_kv * groups).  The lanes' chunks of CK keys, one after
@@ -820,8 +835,8 @@ __global__ void __launch_bounds__(NT_V, 2) k_values(const Args A) {
 
 // Sizes that follow from the shapes; `lanes` of them per launch.
 struct Plan {
-  int lanes, R, Rp, G, tiles, chunks, groups, RG, splits, threads, unit, rows_s;
-  size_t oS, oM, oR, oG, oSum, oW, oAcc, oA, oB, oF, bytes;
+  int lanes, R, Rp, G, tiles, chunks, groups, RG, splits, threads, unit, rows_s, qgroups;
+  size_t oS, oQ, oI, oR, oG, oSum, oW, oAcc, oA, oB, oF, bytes;
 };
 
 constexpr size_t WS_TARGET = size_t(1) << 30;  // lanes are batched to about this much workspace
@@ -835,16 +850,18 @@ static Plan plan(int lanes, int nq, int n_heads, int n_kv, int dh, int t_lim) {
   p.RG = ((p.R + p.groups - 1) / p.groups + p.unit - 1) / p.unit * p.unit;
   p.Rp = p.groups * p.RG;
   p.tiles = (t_lim + TILE - 1) / TILE;
-  p.chunks = p.tiles < 32 ? p.tiles : 32;
   const size_t per_s = (size_t)n_kv * p.tiles * TILE * p.Rp * 4;
   p.lanes = (int)(WS_TARGET / per_s);
   p.lanes = p.lanes < 1 ? 1 : (p.lanes > lanes ? lanes : p.lanes);
+  const int have = p.lanes * n_kv * p.groups;
   // the lanes' keys are divided evenly over two CTAs per SM in all; a CTA's
   // part of a lane stays below MAX_RANGE keys
   p.splits = 2 * 148 / (n_kv * p.groups);
   if (p.splits < 1) p.splits = 1;
   const int64_t least = ((int64_t)p.lanes * p.tiles * TILE + MAX_RANGE - 1) / (MAX_RANGE - CK);
   if (p.splits < least) p.splits = (int)least;
+  p.chunks = (4 * 148 + have - 1) / have;
+  if (p.chunks > p.tiles) p.chunks = p.tiles;
   const int units = p.RG / p.unit;
   p.threads = 32 * units * (units >= 5 ? 1 : (units >= 3 ? 2 : (units == 2 ? 4 : 8)));
   // score CTAs take all rows of their tile unless that leaves SMs idle (two CTAs each)
@@ -858,7 +875,9 @@ static Plan plan(int lanes, int nq, int n_heads, int n_kv, int dh, int t_lim) {
   };
   const size_t lk = (size_t)p.lanes * n_kv;
   p.oS = take((size_t)p.lanes * per_s);
-  p.oM = take(lk * p.tiles * p.Rp * 8);
+  p.qgroups = (p.R + RQ - 1) / RQ;
+  p.oQ = take(lk * p.qgroups * PLANES * RQ * 128);
+  p.oI = take(lk * p.qgroups * sizeof(uint4));
   p.oR = take(lk * p.tiles * p.Rp * 8);
   p.oG = take(lk * p.Rp * 8);
   p.oSum = take(lk * p.Rp * 8);
@@ -874,7 +893,7 @@ static Plan plan(int lanes, int nq, int n_heads, int n_kv, int dh, int t_lim) {
 
 template <int DHP, int UR>
 static int run(Args A, const Plan& p, int lanes, cudaStream_t st) {
-  constexpr int smem_s = 1024 + PLANES * (TILE + RQ) * 128;
+  constexpr int smem_s = 1024 + PLANES * (TILE + 2 * RQ) * 128;
   const int vals = 2 * (CK * (A.dh * 8 + p.RG * 4) + p.RG * 8), sums = p.RG * DHP * 4, smem_v = vals > sums ? vals : sums;
   const auto kv = k_values<DHP / 32, UR>;
   cudaError_t e = cudaFuncSetAttribute(k_scores<DHP>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_s);
@@ -883,7 +902,9 @@ static int run(Args A, const Plan& p, int lanes, cudaStream_t st) {
   for (int l0 = 0; l0 < lanes; l0 += p.lanes) {
     const int n = lanes - l0 < p.lanes ? lanes - l0 : p.lanes;
     A.lane0 = l0, A.lanes = n;
-    int rc = launch_k(k_scores<DHP>, dim3(p.tiles, A.n_kv * ((p.R + p.rows_s - 1) / p.rows_s), n), dim3(NT_S), smem_s,
+    int rc = launch_k(k_queries<DHP>, dim3(p.qgroups, A.n_kv, n), dim3(NT_S), 0, st, A);
+    if (!rc)
+      rc = launch_k(k_scores<DHP>, dim3(p.tiles, A.n_kv * ((p.R + p.rows_s - 1) / p.rows_s), n), dim3(NT_S), smem_s,
                       st, A);
     if (!rc) rc = launch_k(k_sums, dim3(p.chunks, A.n_kv * p.groups, n), dim3(p.threads), 0, st, A);
     if (!rc) rc = launch_k(kv, dim3(p.splits, A.n_kv * p.groups), dim3(p.threads), smem_v, st, A);
@@ -918,8 +939,8 @@ int arcb_attn_tree(const int64_t* q, const int64_t* Kc, const int64_t* Vc, int n
   A.n_pages = n_pages, A.width = width, A.nq = nq, A.n_heads = n_heads, A.n_kv = n_kv, A.dh = dh, A.t_lim = t_lim;
   A.B = lanes * nq;
   A.R = p.R, A.Rp = p.Rp, A.G = p.G, A.tiles = p.tiles, A.chunks = p.chunks, A.groups = p.groups, A.RG = p.RG;
-  A.splits = p.splits, A.rows_s = p.rows_s;
-  A.S = (int*)(b + p.oS), A.M = (int64_t*)(b + p.oM), A.ref = (int64_t*)(b + p.oR), A.gmax = (int64_t*)(b + p.oG);
+  A.splits = p.splits, A.rows_s = p.rows_s, A.qgroups = p.qgroups;
+  A.S = (int*)(b + p.oS), A.planes = b + p.oQ, A.qinfo = (uint4*)(b + p.oI), A.ref = (int64_t*)(b + p.oR), A.gmax = (int64_t*)(b + p.oG);
   A.sums = (uint64_t*)(b + p.oSum), A.wide = (int64_t*)(b + p.oW), A.acc = (uint64_t*)(b + p.oAcc);
   A.arrived = (int*)(b + p.oA), A.bad = (int*)(b + p.oB), A.is_wide = (int*)(b + p.oF);
   A.X = X, A.lmax = lmax, A.o_out = o_out, A.err = err;
