@@ -40,7 +40,7 @@
 //     gives the same), two int32 in one 64-bit word; the last to arrive writes.
 #include "../common/tree.h"
 #include "common.cuh"
-#include "lut.cuh"
+#include "exp32.cuh"
 
 using namespace q16;
 
@@ -90,19 +90,6 @@ struct Args {
   int* err;
 };
 
-// exp table as (value, step to the next): e = value + (step * frac >> 11)
-__device__ __forceinline__ void load_lut(int2* lut, int nt) {
-  for (int i = threadIdx.x; i < EXP_LUT_N; i += nt) {
-    const int lo = (int)g_exp_lut.v[i];
-    lut[i] = make_int2(lo, i < EXP_LUT_N - 1 ? (int)g_exp_lut.v[i + 1] - lo : 0);
-  }
-}
-// integer_exp in 32 bits, x > 0 as 0 (rows behind the last are computed too).
-__device__ __forceinline__ int exp32(int x, const int2* lut) {
-  const int off = min(max(x + (int)EXP_RANGE, 0), (int)EXP_RANGE);
-  const int2 t = lut[off >> 11];
-  return off > 0 ? t.x + ((t.y * (off & 2047)) >> 11) : 0;
-}
 // What a tile's stored scores need added to be relative to the row's max.  A
 // score that is not seen is stored as FAR; both clamps leave its exp 0 and
 // the sum within int32.

@@ -23,17 +23,22 @@
 //    the next child is asked.  Where no child is accepted the following token
 //    is drawn from P as it then stands.
 //
-// One cluster serves one row (draw) or one node (verify): each CTA holds a
-// contiguous part of the vocabulary in shared memory, and the sums and the
-// single elements that all of them need cross through distributed shared
-// memory.  Every node of every tree is decided at once, whether or not the
-// accepted path reaches it; a second small kernel follows the decisions from
-// the root.
+// A cluster serves one row (draw) or one node at a time (verify): each CTA
+// holds the weights of a contiguous part of the vocabulary in shared memory
+// (4 bytes an element; P and Q: 8), reads its logits twice (for the maximum,
+// then from the caches for the weights), and the sums and the single elements
+// that all of them need cross through distributed shared memory.
+//
+// Verification has two schedules.  Where a cluster per node fills no more than
+// the GPU, every node is decided at once, whether or not the accepted path
+// reaches it, and a second small kernel follows the decisions from the root:
+// one node's latency.  Larger trees and batches take one cluster per lane,
+// which walks from the root and reads only the rows that it meets.
 #include <climits>
 
 #include "../common/tree.h"
 #include "common.cuh"
-#include "lut.cuh"
+#include "exp32.cuh"
 
 using namespace q16;
 
@@ -87,102 +92,165 @@ __device__ __forceinline__ uint32_t div31(uint64_t num, uint64_t den, double rcp
   return (uint32_t)q;
 }
 
-// What the CTAs of a cluster exchange.
+// What the CTAs of a cluster exchange, and scratch.
 struct Shared {
-  int64_t lut[EXP_LUT_N];
-  int64_t redv[NW];
-  int redi[NW];
+  int2 lut[EXP_LUT_N];
+  int64_t redv[2][NW];
+  int redi[2][NW];
   uint64_t wsum[NW];
-  int64_t xmax;      // this CTA's largest value and its first index
-  int xidx;
+  int64_t xmax[2];   // this CTA's largest values (target, draft) and their first indexes
+  int xidx[2];
   uint64_t xsum[2];  // this CTA's sum, two phases
-  int ids[HIST];     // newest first; -1: none
-  int n_ids;
+  int ids[HIST];     // newest first
+  int met[HIST];     // times that an id is penalised; 0: not its first entry, or not an id
+  int n_ids, n_path;
 };
 
-// The newest 64 ids behind `node`: its path up to (not including) the root,
-// then the lane's ring.  The whole CTA calls it.
-__device__ void gather_ids(Shared& sh, const int* hist, int count, const int* tokens, const int* parent, int node) {
-  __shared__ int n_path;
-  if (threadIdx.x == 0) {
+// The newest 64 ids behind `node` (its path up to, not including, the root,
+// then the lane's ring), and `skip`: a bit for each of them in this CTA's part
+// [v0, v0 + len) of the vocabulary.  The whole CTA calls it.
+__device__ void gather_ids(Shared& sh, uint32_t* skip, const int* hist, int count, const int* tokens,
+                           const int* parent, int node, int V, int v0, int len) {
+  const int tid = threadIdx.x;
+  for (int i = tid; i < (len + 31) / 32; i += NT) skip[i] = 0;
+  if (tid == 0) {
     int k = 0;
     for (int i = node; i > 0 && k < HIST; i = tree::parent_of(parent, i)) sh.ids[k++] = tokens[i];
-    n_path = k;
+    sh.n_path = k;
   }
   __syncthreads();
-  const int np = n_path, c = count < 0 ? 0 : count;
-  const int n = np + (c < HIST - np ? c : HIST - np);
-  if (threadIdx.x >= np && threadIdx.x < n)
-    sh.ids[threadIdx.x] = hist[(unsigned)(c - 1 - ((int)threadIdx.x - np)) & (HIST - 1)];
-  if (threadIdx.x == 0) sh.n_ids = n;
+  const int np = sh.n_path, c = count < 0 ? 0 : count;
+  const int n = np + min(c, HIST - np);
+  if (tid >= np && tid < n) sh.ids[tid] = hist[(unsigned)(c - 1 - (tid - np)) & (HIST - 1)];
+  if (tid == 0) sh.n_ids = n;
+  __syncthreads();
+  if (tid < n) {
+    const int t = sh.ids[tid];
+    int m = 0;
+    bool first = t >= 0 && t < V;
+    for (int j = 0; j < n; ++j) {
+      m += sh.ids[j] == t;
+      first &= !(j < tid && sh.ids[j] == t);
+    }
+    sh.met[tid] = first ? m : 0;
+    if (first && t >= v0 && t < v0 + len) atomicOr(&skip[(t - v0) >> 5], 1u << ((t - v0) & 31));
+  }
   __syncthreads();
 }
 
-// Loads this CTA's part [v0, v0 + len) of a row into z (int64, temperature
-// applied) and agrees on the cluster's largest value; then e of each element
-// into the low words of z and the cluster's sum.  inv <= 0: the one-hot row.
-// `ph` is the phase of the exchange cells (the caller alternates it).
-__device__ uint64_t row_weights(Shared& sh, const int64_t* __restrict__ row, int v0, int len, int V, int64_t inv,
-                                int64_t* z, uint32_t cs) {
-  const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
-  inv = inv > MAX_INV_T ? MAX_INV_T : inv;
-  const bool greedy = inv <= 0;
-  for (int i = tid; i < len; i += NT) z[i] = clamp40(__ldcg((const long long*)row + v0 + i));
-  __syncthreads();
-  if (tid < sh.n_ids) {  // the first entry of an id applies its penalties
-    const int t = sh.ids[tid] - v0;
-    bool first = sh.ids[tid] >= 0 && sh.ids[tid] < V && t >= 0 && t < len;
-    int c = 0;
-    for (int j = 0; j < sh.n_ids; ++j) {
-      c += sh.ids[j] == sh.ids[tid];
-      first &= !(j < tid && sh.ids[j] == sh.ids[tid]);
+// f(i, x) for this thread's elements i of the part, x the logit; the skipped
+// ones too.  16-byte loads, four in flight, where the row allows them.
+template <class F>
+__device__ __forceinline__ void each(const int64_t* __restrict__ part, int len, F f) {
+  if (((uintptr_t)part & 15) == 0) {
+    const longlong2* p = (const longlong2*)part;
+    const int n2 = len / 2;
+    int i = threadIdx.x;
+    for (; i + 3 * NT < n2; i += 4 * NT) {
+      longlong2 x[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) x[k] = __ldg(p + i + k * NT);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        f(2 * (i + k * NT), (int64_t)x[k].x);
+        f(2 * (i + k * NT) + 1, (int64_t)x[k].y);
+      }
     }
-    if (first) {
-      int64_t v = z[t];
-      for (int r = 0; r < c; ++r) v = clamp40(penalize(v));
-      z[t] = v;
+    for (; i < n2; i += NT) {
+      const longlong2 x = __ldg(p + i);
+      f(2 * i, (int64_t)x.x);
+      f(2 * i + 1, (int64_t)x.y);
     }
+    if ((len & 1) && threadIdx.x == 0) f(len - 1, (int64_t)__ldg((const long long*)part + len - 1));
+  } else {
+#pragma unroll 4
+    for (int i = threadIdx.x; i < len; i += NT) f(i, (int64_t)__ldg((const long long*)part + i));
   }
-  __syncthreads();
+}
+
+// A row's part as it is used: clamped, and scaled unless greedy.
+struct Row {
+  const int64_t* part;
+  int64_t inv;
+  __device__ Row(const int64_t* row, int v0, int64_t inv_temp)
+      : part(row + v0), inv(inv_temp > MAX_INV_T ? MAX_INV_T : inv_temp) {}
+  __device__ bool greedy() const { return inv <= 0; }
+  __device__ int64_t scaled(int64_t x) const { return greedy() ? x : (x * inv) >> FRAC_BITS; }
+  __device__ int64_t value(int64_t x) const { return scaled(clamp40(x)); }
+  __device__ int64_t penalised(int64_t x, int times) const {
+    x = clamp40(x);
+    for (int r = 0; r < times; ++r) x = clamp40(penalize(x));
+    return scaled(x);
+  }
+};
+
+// Which of this thread's ids lies in the part: its index there, or -1.
+__device__ __forceinline__ int own_id(const Shared& sh, int v0, int len) {
+  if (threadIdx.x >= sh.n_ids || !sh.met[threadIdx.x]) return -1;
+  const int t = sh.ids[threadIdx.x] - v0;
+  return t >= 0 && t < len ? t : -1;
+}
+
+__device__ __forceinline__ void better(int64_t& v, int& i, int64_t ov, int oi) {
+  if (ov > v || (ov == v && oi < i)) v = ov, i = oi;
+}
+
+// Largest value and its first index over the CTA's part of row r, into the
+// cell k of redv / redi (per warp).
+__device__ void warp_max(Shared& sh, const uint32_t* skip, const Row& r, int v0, int len, int k) {
   int64_t bv = INT64_MIN;
   int bi = INT_MAX;
-  for (int i = tid; i < len; i += NT) {
-    int64_t x = z[i];
-    if (!greedy) {
-      x = (x * inv) >> FRAC_BITS;
-      z[i] = x;
-    }
-    if (x > bv) bv = x, bi = v0 + i;
-  }
+  each(r.part, len, [&](int i, int64_t x) {
+    const int64_t z = r.value(x);
+    if (z > bv && !(skip[i >> 5] >> (i & 31) & 1)) bv = z, bi = v0 + i;  // a thread meets rising indexes
+  });
+  const int t = own_id(sh, v0, len);
+  if (t >= 0) better(bv, bi, r.penalised(r.part[t], sh.met[threadIdx.x]), v0 + t);
 #pragma unroll
-  for (int m = 16; m >= 1; m >>= 1) {
-    const int64_t ov = shfl_xor_i64(bv, m);
-    const int oi = __shfl_xor_sync(0xffffffffu, bi, m);
-    if (ov > bv || (ov == bv && oi < bi)) bv = ov, bi = oi;
-  }
-  if (lane == 0) sh.redv[w] = bv, sh.redi[w] = bi;
+  for (int m = 16; m >= 1; m >>= 1) better(bv, bi, shfl_xor_i64(bv, m), __shfl_xor_sync(0xffffffffu, bi, m));
+  if ((threadIdx.x & 31) == 0) sh.redv[k][threadIdx.x >> 5] = bv, sh.redi[k][threadIdx.x >> 5] = bi;
+}
+
+// The cluster's largest value and first index of cells 0 .. n - 1.
+__device__ void cluster_max(Shared& sh, int n, uint32_t cs, int64_t* v, int* i) {
   __syncthreads();
-  if (tid == 0) {
-    for (int k = 1; k < NW; ++k)
-      if (sh.redv[k] > bv || (sh.redv[k] == bv && sh.redi[k] < bi)) bv = sh.redv[k], bi = sh.redi[k];
-    sh.xmax = bv;
-    sh.xidx = bi;
+  if (threadIdx.x < n) {
+    int64_t bv = INT64_MIN;
+    int bi = INT_MAX;
+    for (int k = 0; k < NW; ++k) better(bv, bi, sh.redv[threadIdx.x][k], sh.redi[threadIdx.x][k]);
+    sh.xmax[threadIdx.x] = bv;
+    sh.xidx[threadIdx.x] = bi;
   }
   cluster_sync();
-  bv = INT64_MIN;
-  bi = INT_MAX;
-  for (uint32_t r = 0; r < cs; ++r) {
-    const int64_t ov = (int64_t)peer_u64(&sh.xmax, r);
-    const int oi = (int)peer_u32(&sh.xidx, r);
-    if (ov > bv || (ov == bv && oi < bi)) bv = ov, bi = oi;
+  for (int k = 0; k < n; ++k) {
+    v[k] = INT64_MIN;
+    i[k] = INT_MAX;
+    for (uint32_t r = 0; r < cs; ++r) better(v[k], i[k], (int64_t)peer_u64(&sh.xmax[k], r), (int)peer_u32(&sh.xidx[k], r));
   }
+}
+
+// Weights of the CTA's part into e; this thread's part of their sum.
+__device__ uint64_t weights(Shared& sh, const Row& r, int v0, int len, int64_t top, int first, uint32_t* e) {
   uint64_t s = 0;
-  for (int i = tid; i < len; i += NT) {
-    const uint32_t e = greedy ? (v0 + i == bi ? (uint32_t)ONE : 0u) : (uint32_t)integer_exp(z[i] - bv, sh.lut);
-    ((uint32_t*)z)[2 * i] = e;
-    s += e;
+  auto weight = [&](int i, int64_t z) -> uint32_t {
+    if (r.greedy()) return v0 + i == first ? (uint32_t)ONE : 0u;
+    const int64_t d = z - top;
+    return (uint32_t)exp32(d < -(1 << 30) ? -(1 << 30) : (int)d, sh.lut);
+  };
+  each(r.part, len, [&](int i, int64_t x) {
+    const uint32_t w = weight(i, r.value(x));
+    e[i] = w;
+    s += w;
+  });
+  __syncthreads();
+  const int t = own_id(sh, v0, len);
+  if (t >= 0) {
+    s -= e[t];  // what the logit would have weighed, and what it does
+    const uint32_t w = weight(t, r.penalised(r.part[t], sh.met[threadIdx.x]));
+    e[t] = w;
+    s += w;
   }
-  return s;  // this thread's part
+  return s;
 }
 
 // Sum over the CTA; every thread gets it.
@@ -259,19 +327,24 @@ __global__ void __launch_bounds__(NT) k_draw(const int64_t* __restrict__ logits,
                                              const int* __restrict__ u, const int* __restrict__ hist,
                                              const int* __restrict__ count, const int* __restrict__ tokens,
                                              const int* __restrict__ parent, int seg, int* __restrict__ out) {
-  pdl_wait_dep();
-  pdl_allow_next();
   extern __shared__ __align__(16) uint8_t dsm[];
   __shared__ Shared sh;
   const uint32_t rank = cluster_rank(), cs = cluster_size();
   const int lane = blockIdx.z, row = lane * nr + blockIdx.y;
   const int v0 = min(V, (int)rank * seg), len = min(V - v0, seg);
-  int64_t* z = (int64_t*)dsm;
-  uint32_t* e = (uint32_t*)dsm;  // element i at e[2 * i]
-  for (int i = threadIdx.x; i < EXP_LUT_N; i += NT) sh.lut[i] = g_exp_lut.v[i];
-  gather_ids(sh, hist + lane * HIST, count[lane], tokens + (size_t)lane * n, parent + (size_t)lane * n,
-             node0 + blockIdx.y);
-  uint64_t mine = block_sum(sh, row_weights(sh, logits + (size_t)row * ldl, v0, len, V, inv_temp[lane], z, cs));
+  uint32_t* e = (uint32_t*)dsm;
+  uint32_t* skip = e + seg;
+  load_lut(sh.lut, NT);
+  pdl_wait_dep();
+  pdl_allow_next();
+  gather_ids(sh, skip, hist + lane * HIST, count[lane], tokens + (size_t)lane * n, parent + (size_t)lane * n,
+             node0 + blockIdx.y, V, v0, len);
+  const Row r(logits + (size_t)row * ldl, v0, inv_temp[lane]);
+  int64_t top;
+  int first;
+  warp_max(sh, skip, r, v0, len, 0);
+  cluster_max(sh, 1, cs, &top, &first);
+  uint64_t mine = block_sum(sh, weights(sh, r, v0, len, top, first, e));
   for (int k = 0; k < m; ++k) {
     uint64_t before;
     const uint64_t total = cluster_sum(sh, mine, k & 1, rank, cs, before);
@@ -279,11 +352,11 @@ __global__ void __launch_bounds__(NT) k_draw(const int64_t* __restrict__ logits,
     if (total == 0) {
       if (rank == 0 && threadIdx.x == 0) out[(size_t)row * m + k] = -1;
     } else if (before <= t && t < before + mine) {
-      const int i = find(sh, len, t - before, [&](int j) { return (uint64_t)e[2 * j]; });
-      mine -= e[2 * i];
+      const int i = find(sh, len, t - before, [&](int j) { return (uint64_t)e[j]; });
+      mine -= e[i];
       __syncthreads();
       if (threadIdx.x == 0) {
-        e[2 * i] = 0;
+        e[i] = 0;
         out[(size_t)row * m + k] = v0 + i;
       }
       __syncthreads();
@@ -292,88 +365,124 @@ __global__ void __launch_bounds__(NT) k_draw(const int64_t* __restrict__ logits,
   cluster_sync();  // no CTA may exit while a peer still reads its shared memory
 }
 
-// One node of one tree: choice = the accepted child or -1, drawn = the token
-// that follows the node when no child is accepted.
-__global__ void __launch_bounds__(NT) k_verify_node(const int64_t* __restrict__ logits, int64_t ldl,
-                                                    const int64_t* __restrict__ dlogits, int64_t ldd, int V, int n,
-                                                    const int* __restrict__ tokens, const int* __restrict__ parent,
-                                                    const int* __restrict__ n_tree,
-                                                    const int64_t* __restrict__ inv_temp,
-                                                    const int64_t* __restrict__ d_inv_temp, const int* __restrict__ u,
-                                                    const int* __restrict__ hist, const int* __restrict__ count,
-                                                    int seg, int* __restrict__ choice, int* __restrict__ drawn) {
-  pdl_wait_dep();
-  pdl_allow_next();
+// grid (cluster, nodes, lanes): every node's decision into choice (the
+// accepted child or -1) and drawn (the token that follows the node when no
+// child is accepted).  WALK, grid (cluster, 1, lanes): the lane's path.
+template <bool WALK>
+__global__ void __launch_bounds__(NT) k_verify(const int64_t* __restrict__ logits, int64_t ldl,
+                                               const int64_t* __restrict__ dlogits, int64_t ldd, int V, int n,
+                                               const int* __restrict__ tokens, const int* __restrict__ parent,
+                                               const int* __restrict__ n_tree, const int64_t* __restrict__ inv_temp,
+                                               const int64_t* __restrict__ d_inv_temp, const int* __restrict__ u,
+                                               const int* __restrict__ hist, const int* __restrict__ count, int seg,
+                                               int* __restrict__ choice, int* __restrict__ drawn,
+                                               int* __restrict__ path, int* __restrict__ n_path,
+                                               int* __restrict__ next) {
   extern __shared__ __align__(16) uint8_t dsm[];
   __shared__ Shared sh;
   const uint32_t rank = cluster_rank(), cs = cluster_size();
-  const int lane = blockIdx.z, node = blockIdx.y, tid = threadIdx.x;
-  const int live = min(n_tree[lane], n);
-  if (node >= live) return;  // the whole cluster
-  const size_t row = (size_t)lane * n + node;
-  tokens += (size_t)lane * n;
-  parent += (size_t)lane * n;
-  u += (size_t)lane * n * 2;
+  const int lane = blockIdx.z, tid = threadIdx.x;
   const int v0 = min(V, (int)rank * seg), len = min(V - v0, seg);
-  int64_t* z = (int64_t*)dsm;              // a row's values; then the draft's weights (low) and max(P - Q, 0) (high)
-  uint32_t* eq = (uint32_t*)dsm;
-  uint32_t* P = (uint32_t*)(z + seg);
-  for (int i = tid; i < EXP_LUT_N; i += NT) sh.lut[i] = g_exp_lut.v[i];
-  gather_ids(sh, hist + lane * HIST, count[lane], tokens, parent, node);
-  int ph = 0;
-  uint64_t before;
-  uint64_t mine = block_sum(sh, row_weights(sh, logits + row * ldl, v0, len, V, inv_temp[lane], z, cs));
-  uint64_t S = cluster_sum(sh, mine, ph ^= 1, rank, cs, before);
-  double rcp = 1.0 / (double)S;
-  for (int i = tid; i < len; i += NT) P[i] = div31((uint64_t)eq[2 * i] << 31, S, rcp);
-  int first = node + 1;
-  while (first < live && tree::parent_of(parent, first) != node) ++first;
-  int taken = -1;
-  if (first < live) {
-    __syncthreads();
-    mine = block_sum(sh, row_weights(sh, dlogits + row * ldd, v0, len, V, d_inv_temp[lane], z, cs));
-    uint64_t sq = cluster_sum(sh, mine, ph ^= 1, rank, cs, before);
-    for (int c = first; c < live; ++c) {
-      if (tree::parent_of(parent, c) != node) continue;
-      const int d = tokens[c];
-      if (d < 0 || d >= V || sq == 0) continue;
-      const uint32_t owner = (uint32_t)(d / seg);
-      const int at = d - (int)owner * seg;
-      const uint32_t pd = peer_u32(&P[at], owner), ed = peer_u32(&eq[2 * at], owner);
-      rcp = 1.0 / (double)sq;
-      if (scale31((uint32_t)u[2 * c], div31((uint64_t)ed << 31, sq, rcp)) < pd) {
-        taken = c;
-        break;
+  uint32_t* P = (uint32_t*)dsm;
+  uint32_t* eq = P + seg;
+  uint32_t* skip = eq + seg;
+  load_lut(sh.lut, NT);
+  pdl_wait_dep();
+  pdl_allow_next();
+  const int live = min(n_tree[lane], n);
+  int node = WALK ? 0 : blockIdx.y;
+  const size_t lane0 = (size_t)lane * n;
+  if (node >= live) {  // the whole cluster
+    if (WALK && rank == 0) {
+      for (int i = tid; i < n; i += NT) path[lane0 + i] = -1;
+      if (tid == 0) n_path[lane] = 0, next[lane] = -1;
+    }
+    return;
+  }
+  tokens += lane0;
+  parent += lane0;
+  u += lane0 * 2;
+  int ph = 0, length = 0;
+  for (;;) {
+    const size_t row = lane0 + node;
+    gather_ids(sh, skip, hist + lane * HIST, count[lane], tokens, parent, node, V, v0, len);
+    int c = node + 1;
+    while (c < live && tree::parent_of(parent, c) != node) ++c;
+    const bool inner = c < live;
+    const Row rt(logits + row * ldl, v0, inv_temp[lane]), rd(dlogits + row * ldd, v0, d_inv_temp[lane]);
+    int64_t top[2];
+    int first[2];
+    warp_max(sh, skip, rt, v0, len, 0);
+    if (inner) warp_max(sh, skip, rd, v0, len, 1);
+    cluster_max(sh, inner ? 2 : 1, cs, top, first);
+    uint64_t before, mine = block_sum(sh, weights(sh, rt, v0, len, top[0], first[0], P));
+    uint64_t S = cluster_sum(sh, mine, ph ^= 1, rank, cs, before);
+    double rcp = 1.0 / (double)S;
+    for (int i = tid; i < len; i += NT) P[i] = div31((uint64_t)P[i] << 31, S, rcp);
+    int taken = -1;
+    if (inner) {
+      mine = block_sum(sh, weights(sh, rd, v0, len, top[1], first[1], eq));
+      uint64_t sq = cluster_sum(sh, mine, ph ^= 1, rank, cs, before);  // and P and eq are complete
+      for (; c < live; ++c) {
+        if (tree::parent_of(parent, c) != node) continue;
+        const int d = tokens[c];
+        if (d < 0 || d >= V || sq == 0) continue;
+        const uint32_t owner = (uint32_t)(d / seg);
+        const int at = d - (int)owner * seg;
+        const uint32_t pd = peer_u32(&P[at], owner), ed = peer_u32(&eq[at], owner);
+        const double rq = 1.0 / (double)sq;
+        if (scale31((uint32_t)u[2 * c], div31((uint64_t)ed << 31, sq, rq)) < pd) {
+          taken = c;
+          break;
+        }
+        auto rest = [&](int i) -> uint32_t {
+          const uint32_t p = P[i], e = eq[i];
+          const uint32_t q = e ? div31((uint64_t)e << 31, sq, rq) : 0;
+          return p > q ? p - q : 0;
+        };
+        uint64_t s = 0;
+        for (int i = tid; i < len; i += NT) s += rest(i);
+        S = cluster_sum(sh, block_sum(sh, s), ph ^= 1, rank, cs, before);  // and the peers have read pd and ed
+        if (S > 0) {
+          rcp = 1.0 / (double)S;
+          for (int i = tid; i < len; i += NT) {
+            const uint32_t r = rest(i);
+            P[i] = r ? div31((uint64_t)r << 31, S, rcp) : 0;
+          }
+        }
+        __syncthreads();
+        if (rank == owner && tid == 0) eq[at] = 0;
+        sq -= ed;
+        cluster_sync();  // the new P and eq before the next child's reads
       }
+    }
+    if (taken < 0) {
       uint64_t s = 0;
-      for (int i = tid; i < len; i += NT) {
-        const uint32_t p = P[i], q = div31((uint64_t)eq[2 * i] << 31, sq, rcp);
-        const uint32_t r = p > q ? p - q : 0;
-        eq[2 * i + 1] = r;
-        s += r;
+      for (int i = tid; i < len; i += NT) s += P[i];
+      mine = block_sum(sh, s);
+      S = cluster_sum(sh, mine, ph ^= 1, rank, cs, before);
+      const uint64_t t = scale31((uint32_t)u[2 * node + 1], S);
+      if (before <= t && t < before + mine) {
+        const int i = find(sh, len, t - before, [&](int j) { return (uint64_t)P[j]; });
+        if (tid == 0) (WALK ? next[lane] : drawn[row]) = v0 + i;
       }
-      S = cluster_sum(sh, block_sum(sh, s), ph ^= 1, rank, cs, before);
-      if (S > 0) {
-        rcp = 1.0 / (double)S;
-        for (int i = tid; i < len; i += NT) P[i] = div31((uint64_t)eq[2 * i + 1] << 31, S, rcp);
+    }
+    if (!WALK) {
+      if (rank == 0 && tid == 0) choice[row] = taken;
+      break;
+    }
+    if (rank == 0 && tid == 0) path[lane0 + length] = node;
+    ++length;
+    if (taken < 0) {
+      if (rank == 0) {
+        for (int i = length + tid; i < n; i += NT) path[lane0 + i] = -1;
+        if (tid == 0) n_path[lane] = length;
       }
-      if (rank == owner && tid == 0) eq[2 * at] = 0;
-      sq -= ed;
-      cluster_sync();  // the new P and eq before the next child's reads
+      break;
     }
+    node = taken;  // a later node: the walk ends
+    cluster_sync();  // the peers have read this node's P and eq
   }
-  if (taken < 0) {
-    uint64_t s = 0;
-    for (int i = tid; i < len; i += NT) s += P[i];
-    mine = block_sum(sh, s);
-    S = cluster_sum(sh, mine, ph ^= 1, rank, cs, before);
-    const uint64_t t = scale31((uint32_t)u[2 * node + 1], S);
-    if (before <= t && t < before + mine) {
-      const int i = find(sh, len, t - before, [&](int j) { return (uint64_t)P[j]; });
-      if (tid == 0) drawn[row] = v0 + i;
-    }
-  }
-  if (rank == 0 && tid == 0) choice[row] = taken;
   cluster_sync();  // no CTA may exit while a peer still reads its shared memory
 }
 
@@ -402,14 +511,17 @@ __global__ void k_verify_path(int lanes, int n, const int* __restrict__ n_tree, 
   for (; k < n; ++k) path[r0 + k] = -1;
 }
 
-// CTAs per row: enough of them that a part of the vocabulary fits in shared
-// memory (`per` bytes an element).
-static int cluster_for(int V, int per, int& seg) {
-  for (int cs = 8; cs <= MAX_CS; cs *= 2) {
-    seg = ((V + cs - 1) / cs + 31) / 32 * 32;
-    if ((size_t)seg * per <= SMEM_MAX) return cs;
-  }
-  return 0;
+// Part of the vocabulary per CTA of a cluster of cs, and its shared memory
+// (`per` bytes an element and a bit for the penalised ids).
+static size_t part_of(int V, int cs, int per, int& seg) {
+  seg = ((V + cs - 1) / cs + 31) / 32 * 32;
+  return (size_t)seg * per + seg / 8;
+}
+
+// CTAs that the GPU holds at once.
+static int64_t capacity(size_t smem) {
+  const int by_smem = (int)((224 * 1024) / (smem + sizeof(Shared) + 1024)), by_threads = 2048 / NT;
+  return 148 * (int64_t)(by_smem < by_threads ? by_smem : by_threads);
 }
 
 template <typename... KArgs, typename... Args>
@@ -441,20 +553,26 @@ static int launch_cluster(void (*k)(KArgs...), int cs, dim3 grid, size_t smem, c
 extern "C" {
 
 // Largest vocabulary the two entry points below take.
-int arcb_draw_max_vocab() { return (int)(dr::SMEM_MAX / 12) / 32 * 32 * dr::MAX_CS; }
+int arcb_draw_max_vocab() { return (int)(dr::SMEM_MAX * 8 / 65) / 32 * 32 * dr::MAX_CS; }
 
 // m tokens of each row lane * nr + i (node node0 + i of the lane's tree) into
 // out [lanes * nr, m].
 int arcb_draw_tokens(const int64_t* logits, int64_t ldl, int V, int lanes, int nr, int n, int node0, int m,
                      const int64_t* inv_temp, const int* u, const int* hist, const int* count, const int* tokens,
                      const int* parent, int* out, void* stream) {
-  if (V < 1 || lanes < 1 || nr < 1 || m < 1 || node0 < 0 || node0 + nr > n || n > tree::MAX_NODES || lanes > 65535)
+  if (V < 1 || V > arcb_draw_max_vocab() || lanes < 1 || nr < 1 || m < 1 || node0 < 0 || node0 + nr > n ||
+      n > tree::MAX_NODES || lanes > 65535)
     return -2;
-  int seg = 0;
-  const int cs = dr::cluster_for(V, 8, seg);
-  if (!cs) return -2;
-  return dr::launch_cluster(dr::k_draw, cs, dim3(cs, nr, lanes), (size_t)seg * 8, (cudaStream_t)stream, logits,
-                            ldl, V, nr, n, node0, m, inv_temp, u, hist, count, tokens, parent, seg, out);
+  // 16 CTAs a row while they all run at once, else 8
+  int seg = 0, cs = 16;
+  size_t smem = dr::part_of(V, cs, 4, seg);
+  if ((int64_t)lanes * nr * cs > dr::capacity(smem)) {
+    int seg8 = 0;
+    const size_t smem8 = dr::part_of(V, 8, 4, seg8);
+    if (smem8 <= dr::SMEM_MAX) cs = 8, seg = seg8, smem = smem8;
+  }
+  return dr::launch_cluster(dr::k_draw, cs, dim3(cs, nr, lanes), smem, (cudaStream_t)stream, logits, ldl, V, nr, n,
+                            node0, m, inv_temp, u, hist, count, tokens, parent, seg, out);
 }
 
 // scratch: 2 * lanes * n ints.
@@ -462,17 +580,21 @@ int arcb_verify_tree(const int64_t* logits, int64_t ldl, const int64_t* dlogits,
                      const int* tokens, const int* parent, const int* n_tree, const int64_t* inv_temp,
                      const int64_t* d_inv_temp, const int* u, const int* hist, const int* count, int* scratch,
                      int* path, int* n_path, int* next, void* stream) {
-  if (V < 1 || lanes < 1 || n < 1 || n > tree::MAX_NODES || lanes > 65535) return -2;
-  int seg = 0;
-  const int cs = dr::cluster_for(V, 12, seg);
-  if (!cs) return -2;
+  if (V < 1 || V > arcb_draw_max_vocab() || lanes < 1 || n < 1 || n > tree::MAX_NODES || lanes > 65535) return -2;
+  cudaStream_t st = (cudaStream_t)stream;
   int* drawn = scratch + (size_t)lanes * n;
-  const int rc = dr::launch_cluster(dr::k_verify_node, cs, dim3(cs, n, lanes), (size_t)seg * 12,
-                                    (cudaStream_t)stream, logits, ldl, dlogits, ldd, V, n, tokens, parent, n_tree,
-                                    inv_temp, d_inv_temp, u, hist, count, seg, scratch, drawn);
+  int seg = 0;
+  size_t smem = dr::part_of(V, 16, 8, seg);
+  if ((int64_t)lanes * n * 16 > dr::capacity(smem))  // a cluster per node does not fit the GPU: one per lane
+    return dr::launch_cluster(dr::k_verify<true>, 16, dim3(16, 1, lanes), smem, st, logits, ldl, dlogits, ldd, V, n,
+                              tokens, parent, n_tree, inv_temp, d_inv_temp, u, hist, count, seg, scratch, drawn, path,
+                              n_path, next);
+  const int rc = dr::launch_cluster(dr::k_verify<false>, 16, dim3(16, n, lanes), smem, st, logits, ldl, dlogits, ldd, V,
+                                    n, tokens, parent, n_tree, inv_temp, d_inv_temp, u, hist, count, seg, scratch,
+                                    drawn, path, n_path, next);
   if (rc) return rc;
-  return launch_k(dr::k_verify_path, dim3((lanes + 63) / 64), dim3(64), 0, (cudaStream_t)stream, lanes, n, n_tree,
-                  scratch, drawn, path, n_path, next);
+  return launch_k(dr::k_verify_path, dim3((lanes + 63) / 64), dim3(64), 0, st, lanes, n, n_tree, scratch, drawn, path,
+                  n_path, next);
 }
 
 }  // extern "C"
