@@ -69,15 +69,11 @@ __device__ __forceinline__ uint32_t peer_addr(const void* local, uint32_t rank) 
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(ra) : "r"(smem_u32(local)), "r"(rank));
   return ra;
 }
-__device__ __forceinline__ uint64_t peer_u64(const void* local, uint32_t rank) {
-  uint64_t v;
-  asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(peer_addr(local, rank)) : "memory");
-  return v;
+__device__ __forceinline__ void push_u64(void* local, uint32_t rank, uint64_t v) {
+  asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(peer_addr(local, rank)), "l"(v) : "memory");
 }
-__device__ __forceinline__ uint32_t peer_u32(const void* local, uint32_t rank) {
-  uint32_t v;
-  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(peer_addr(local, rank)) : "memory");
-  return v;
+__device__ __forceinline__ void push_u32(void* local, uint32_t rank, uint32_t v) {
+  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(peer_addr(local, rank)), "r"(v) : "memory");
 }
 
 __device__ __forceinline__ int64_t clamp40(int64_t x) { return x > CLAMP ? CLAMP : (x < -CLAMP ? -CLAMP : x); }
@@ -92,30 +88,43 @@ __device__ __forceinline__ uint32_t div31(uint64_t num, uint64_t den, double rcp
   return (uint32_t)q;
 }
 
-// What the CTAs of a cluster exchange, and scratch.
+// Scratch, and what the CTAs of a cluster exchange: every CTA stores its value
+// into all of them before a cluster barrier and reads its own copies after
+// (reading sixteen peers one after another cost 2 us an exchange).  Sums come
+// in two phases, so that the next exchange may start while a peer still reads.
 struct Shared {
   int2 lut[EXP_LUT_N];
   int64_t redv[2][NW];
   int redi[2][NW];
-  uint64_t wsum[NW];
-  int64_t xmax[2];   // this CTA's largest values (target, draft) and their first indexes
-  int xidx[2];
-  uint64_t xsum[2];  // this CTA's sum, two phases
-  int ids[HIST];     // newest first
-  int met[HIST];     // times that an id is penalised; 0: not its first entry, or not an id
+  uint64_t wsum[2][NW];
+  int64_t xmax[2][MAX_CS];      // largest values (target, draft) and their first indexes
+  int xidx[2][MAX_CS];
+  uint64_t xsum[2][2][MAX_CS];  // [phase][target, draft]
+  uint32_t xchild[2][3];        // [phase] at a child's token: P or its weight, max(P - Q, 0), draft weight
+  int ids[HIST];                // newest first
+  int met[HIST];                // times that an id is penalised; 0: not its first entry, or not an id
+  int parent[tree::MAX_NODES], token[tree::MAX_NODES];
   int n_ids, n_path;
 };
+
+// The tree: each node's token and parent (-1 where that is no earlier node).
+__device__ __forceinline__ void load_tree(Shared& sh, const int* tokens, const int* parent, int n) {
+  for (int i = threadIdx.x; i < n; i += NT) {
+    sh.token[i] = tokens[i];
+    sh.parent[i] = tree::parent_of(parent, i);
+  }
+  __syncthreads();
+}
 
 // The newest 64 ids behind `node` (its path up to, not including, the root,
 // then the lane's ring), and `skip`: a bit for each of them in this CTA's part
 // [v0, v0 + len) of the vocabulary.  The whole CTA calls it.
-__device__ void gather_ids(Shared& sh, uint32_t* skip, const int* hist, int count, const int* tokens,
-                           const int* parent, int node, int V, int v0, int len) {
+__device__ void gather_ids(Shared& sh, uint32_t* skip, const int* hist, int count, int node, int V, int v0, int len) {
   const int tid = threadIdx.x;
   for (int i = tid; i < (len + 31) / 32; i += NT) skip[i] = 0;
   if (tid == 0) {
     int k = 0;
-    for (int i = node; i > 0 && k < HIST; i = tree::parent_of(parent, i)) sh.ids[k++] = tokens[i];
+    for (int i = node; i > 0 && k < HIST; i = sh.parent[i]) sh.ids[k++] = sh.token[i];
     sh.n_path = k;
   }
   __syncthreads();
@@ -128,9 +137,11 @@ __device__ void gather_ids(Shared& sh, uint32_t* skip, const int* hist, int coun
     const int t = sh.ids[tid];
     int m = 0;
     bool first = t >= 0 && t < V;
+#pragma unroll 8
     for (int j = 0; j < n; ++j) {
-      m += sh.ids[j] == t;
-      first &= !(j < tid && sh.ids[j] == t);
+      const bool same = sh.ids[j] == t;
+      m += same;
+      first &= !(same && j < tid);
     }
     sh.met[tid] = first ? m : 0;
     if (first && t >= v0 && t < v0 + len) atomicOr(&skip[(t - v0) >> 5], 1u << ((t - v0) & 31));
@@ -211,21 +222,26 @@ __device__ void warp_max(Shared& sh, const uint32_t* skip, const Row& r, int v0,
   if ((threadIdx.x & 31) == 0) sh.redv[k][threadIdx.x >> 5] = bv, sh.redi[k][threadIdx.x >> 5] = bi;
 }
 
-// The cluster's largest value and first index of cells 0 .. n - 1.
-__device__ void cluster_max(Shared& sh, int n, uint32_t cs, int64_t* v, int* i) {
+// The cluster's largest value and first index of cells 0 .. n - 1 (n <= 2).
+__device__ void cluster_max(Shared& sh, int n, uint32_t rank, uint32_t cs, int64_t* v, int* i) {
   __syncthreads();
-  if (threadIdx.x < n) {
-    int64_t bv = INT64_MIN;
-    int bi = INT_MAX;
-    for (int k = 0; k < NW; ++k) better(bv, bi, sh.redv[threadIdx.x][k], sh.redi[threadIdx.x][k]);
-    sh.xmax[threadIdx.x] = bv;
-    sh.xidx[threadIdx.x] = bi;
+  const int k = threadIdx.x >> 5, l = threadIdx.x & 31;
+  if (k < n) {  // warp k: cell k
+    int64_t bv = l < NW ? sh.redv[k][l] : INT64_MIN;
+    int bi = l < NW ? sh.redi[k][l] : INT_MAX;
+#pragma unroll
+    for (int m = 16; m >= 1; m >>= 1) better(bv, bi, shfl_xor_i64(bv, m), __shfl_xor_sync(0xffffffffu, bi, m));
+    if (l < (int)cs) {
+      push_u64(&sh.xmax[k][rank], l, (uint64_t)bv);
+      push_u32(&sh.xidx[k][rank], l, (uint32_t)bi);
+    }
   }
   cluster_sync();
-  for (int k = 0; k < n; ++k) {
-    v[k] = INT64_MIN;
-    i[k] = INT_MAX;
-    for (uint32_t r = 0; r < cs; ++r) better(v[k], i[k], (int64_t)peer_u64(&sh.xmax[k], r), (int)peer_u32(&sh.xidx[k], r));
+  for (int c = 0; c < n; ++c) {
+    v[c] = sh.xmax[c][0];
+    i[c] = sh.xidx[c][0];
+#pragma unroll 4
+    for (uint32_t r = 1; r < cs; ++r) better(v[c], i[c], sh.xmax[c][r], sh.xidx[c][r]);
   }
 }
 
@@ -253,31 +269,45 @@ __device__ uint64_t weights(Shared& sh, const Row& r, int v0, int len, int64_t t
   return s;
 }
 
-// Sum over the CTA; every thread gets it.
-__device__ uint64_t block_sum(Shared& sh, uint64_t s) {
+// Sums over the CTA; every thread gets them.
+template <int N>
+__device__ __forceinline__ void block_sum(Shared& sh, uint64_t* s) {
 #pragma unroll
-  for (int m = 16; m >= 1; m >>= 1) s += (uint64_t)shfl_xor_i64((int64_t)s, m);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) sh.wsum[threadIdx.x >> 5] = s;
-  __syncthreads();
-  s = 0;
+  for (int k = 0; k < N; ++k)
 #pragma unroll
-  for (int k = 0; k < NW; ++k) s += sh.wsum[k];
-  return s;
+    for (int m = 16; m >= 1; m >>= 1) s[k] += (uint64_t)shfl_xor_i64((int64_t)s[k], m);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0)
+#pragma unroll
+    for (int k = 0; k < N; ++k) sh.wsum[k][threadIdx.x >> 5] = s[k];
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    s[k] = 0;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) s[k] += sh.wsum[k][w];
+  }
 }
 
-// Sum over the cluster, and the sum of the CTAs before this one.
-__device__ uint64_t cluster_sum(Shared& sh, uint64_t cta, int ph, uint32_t rank, uint32_t cs, uint64_t& before) {
-  if (threadIdx.x == 0) sh.xsum[ph] = cta;
+// Exchange of the CTAs' sums mine[0 .. N); total over the cluster, and the
+// first one's sum over the CTAs before this one.
+template <int N>
+__device__ __forceinline__ uint64_t cluster_sum(Shared& sh, const uint64_t* mine, int ph, uint32_t rank, uint32_t cs,
+                                                uint64_t* total) {
+  if (threadIdx.x < cs)
+#pragma unroll
+    for (int k = 0; k < N; ++k) push_u64(&sh.xsum[ph][k][rank], threadIdx.x, mine[k]);
   cluster_sync();
-  uint64_t total = 0;
-  before = 0;
+  uint64_t before = 0;
+#pragma unroll
+  for (int k = 0; k < N; ++k) total[k] = 0;
+#pragma unroll 4
   for (uint32_t r = 0; r < cs; ++r) {
-    const uint64_t x = peer_u64(&sh.xsum[ph], r);
-    if (r < rank) before += x;
-    total += x;
+    if (r < rank) before += sh.xsum[ph][0][r];
+#pragma unroll
+    for (int k = 0; k < N; ++k) total[k] += sh.xsum[ph][k][r];
   }
-  return total;
+  return before;
 }
 
 // The first element of this CTA's part whose running sum exceeds t (which is
@@ -293,10 +323,10 @@ __device__ int find(Shared& sh, int len, uint64_t t, F val) {
 #pragma unroll
   for (int m = 16; m >= 1; m >>= 1) s += (uint64_t)shfl_xor_i64((int64_t)s, m);
   __syncthreads();
-  if (lane == 0) sh.wsum[w] = s;
+  if (lane == 0) sh.wsum[0][w] = s;
   __syncthreads();
   uint64_t before = 0;
-  for (int k = 0; k < w; ++k) before += sh.wsum[k];
+  for (int k = 0; k < w; ++k) before += sh.wsum[0][k];
   if (before <= t && t < before + s) {  // this warp's elements hold it
     for (int i0 = a; i0 < b; i0 += 32) {
       const int i = i0 + lane;
@@ -335,19 +365,21 @@ __global__ void __launch_bounds__(NT) k_draw(const int64_t* __restrict__ logits,
   uint32_t* e = (uint32_t*)dsm;
   uint32_t* skip = e + seg;
   load_lut(sh.lut, NT);
+  cluster_sync();  // every peer runs: its shared memory may be stored to
   pdl_wait_dep();
   pdl_allow_next();
-  gather_ids(sh, skip, hist + lane * HIST, count[lane], tokens + (size_t)lane * n, parent + (size_t)lane * n,
-             node0 + blockIdx.y, V, v0, len);
+  load_tree(sh, tokens + (size_t)lane * n, parent + (size_t)lane * n, n);
+  gather_ids(sh, skip, hist + lane * HIST, count[lane], node0 + blockIdx.y, V, v0, len);
   const Row r(logits + (size_t)row * ldl, v0, inv_temp[lane]);
   int64_t top;
   int first;
   warp_max(sh, skip, r, v0, len, 0);
-  cluster_max(sh, 1, cs, &top, &first);
-  uint64_t mine = block_sum(sh, weights(sh, r, v0, len, top, first, e));
+  cluster_max(sh, 1, rank, cs, &top, &first);
+  uint64_t mine = weights(sh, r, v0, len, top, first, e);
+  block_sum<1>(sh, &mine);
   for (int k = 0; k < m; ++k) {
-    uint64_t before;
-    const uint64_t total = cluster_sum(sh, mine, k & 1, rank, cs, before);
+    uint64_t total;
+    const uint64_t before = cluster_sum<1>(sh, &mine, k & 1, rank, cs, &total);
     const uint64_t t = scale31((uint32_t)u[(size_t)row * m + k], total);
     if (total == 0) {
       if (rank == 0 && threadIdx.x == 0) out[(size_t)row * m + k] = -1;
@@ -387,6 +419,7 @@ __global__ void __launch_bounds__(NT) k_verify(const int64_t* __restrict__ logit
   uint32_t* eq = P + seg;
   uint32_t* skip = eq + seg;
   load_lut(sh.lut, NT);
+  cluster_sync();  // every peer runs: its shared memory may be stored to
   pdl_wait_dep();
   pdl_allow_next();
   const int live = min(n_tree[lane], n);
@@ -399,70 +432,104 @@ __global__ void __launch_bounds__(NT) k_verify(const int64_t* __restrict__ logit
     }
     return;
   }
-  tokens += lane0;
-  parent += lane0;
+  load_tree(sh, tokens + lane0, parent + lane0, n);
   u += lane0 * 2;
   int ph = 0, length = 0;
+  auto next_child = [&](int c) {  // of the node, from c on, whose token is one
+    while (c < live && !(sh.parent[c] == node && sh.token[c] >= 0 && sh.token[c] < V)) ++c;
+    return c;
+  };
   for (;;) {
     const size_t row = lane0 + node;
-    gather_ids(sh, skip, hist + lane * HIST, count[lane], tokens, parent, node, V, v0, len);
-    int c = node + 1;
-    while (c < live && tree::parent_of(parent, c) != node) ++c;
+    gather_ids(sh, skip, hist + lane * HIST, count[lane], node, V, v0, len);
+    int c = next_child(node + 1);
     const bool inner = c < live;
     const Row rt(logits + row * ldl, v0, inv_temp[lane]), rd(dlogits + row * ldd, v0, d_inv_temp[lane]);
     int64_t top[2];
     int first[2];
     warp_max(sh, skip, rt, v0, len, 0);
     if (inner) warp_max(sh, skip, rd, v0, len, 1);
-    cluster_max(sh, inner ? 2 : 1, cs, top, first);
-    uint64_t before, mine = block_sum(sh, weights(sh, rt, v0, len, top[0], first[0], P));
-    uint64_t S = cluster_sum(sh, mine, ph ^= 1, rank, cs, before);
-    double rcp = 1.0 / (double)S;
-    for (int i = tid; i < len; i += NT) P[i] = div31((uint64_t)P[i] << 31, S, rcp);
-    int taken = -1;
-    if (inner) {
-      mine = block_sum(sh, weights(sh, rd, v0, len, top[1], first[1], eq));
-      uint64_t sq = cluster_sum(sh, mine, ph ^= 1, rank, cs, before);  // and P and eq are complete
-      for (; c < live; ++c) {
-        if (tree::parent_of(parent, c) != node) continue;
-        const int d = tokens[c];
-        if (d < 0 || d >= V || sq == 0) continue;
-        const uint32_t owner = (uint32_t)(d / seg);
-        const int at = d - (int)owner * seg;
-        const uint32_t pd = peer_u32(&P[at], owner), ed = peer_u32(&eq[at], owner);
-        const double rq = 1.0 / (double)sq;
-        if (scale31((uint32_t)u[2 * c], div31((uint64_t)ed << 31, sq, rq)) < pd) {
-          taken = c;
-          break;
-        }
-        auto rest = [&](int i) -> uint32_t {
-          const uint32_t p = P[i], e = eq[i];
-          const uint32_t q = e ? div31((uint64_t)e << 31, sq, rq) : 0;
-          return p > q ? p - q : 0;
-        };
-        uint64_t s = 0;
-        for (int i = tid; i < len; i += NT) s += rest(i);
-        S = cluster_sum(sh, block_sum(sh, s), ph ^= 1, rank, cs, before);  // and the peers have read pd and ed
-        if (S > 0) {
-          rcp = 1.0 / (double)S;
-          for (int i = tid; i < len; i += NT) {
-            const uint32_t r = rest(i);
-            P[i] = r ? div31((uint64_t)r << 31, S, rcp) : 0;
-          }
-        }
-        __syncthreads();
-        if (rank == owner && tid == 0) eq[at] = 0;
-        sq -= ed;
-        cluster_sync();  // the new P and eq before the next child's reads
+    cluster_max(sh, inner ? 2 : 1, rank, cs, top, first);
+    // one CTA stores what child c's test needs into all of them, with the sums of phase ph
+    auto push_child = [&](uint32_t a, uint32_t b, uint32_t e) {
+      if (tid < cs) {
+        push_u32(&sh.xchild[ph][0], tid, a);
+        push_u32(&sh.xchild[ph][1], tid, b);
+        push_u32(&sh.xchild[ph][2], tid, e);
       }
+    };
+    uint64_t mine[2], S[2], before;
+    mine[0] = weights(sh, rt, v0, len, top[0], first[0], P);
+    mine[1] = inner ? weights(sh, rd, v0, len, top[1], first[1], eq) : 0;
+    block_sum<2>(sh, mine);
+    ph ^= 1;
+    if (inner && sh.token[c] / seg == (int)rank) push_child(P[sh.token[c] - v0], 0, eq[sh.token[c] - v0]);
+    before = cluster_sum<2>(sh, mine, ph, rank, cs, S);
+    // P = floor(e * 2^31 / S), made of the weights in place once it is needed as a whole
+    const double rp = 1.0 / (double)S[0];
+    auto normalise = [&]() {
+      for (int i = tid; i < len; i += NT) {
+        const uint32_t e = P[i];
+        P[i] = e ? div31((uint64_t)e << 31, S[0], rp) : 0;
+      }
+    };
+    int taken = -1;
+    bool whole = false;
+    uint32_t pd = inner ? div31((uint64_t)sh.xchild[ph][0] << 31, S[0], rp) : 0, ed = sh.xchild[ph][2];
+    uint64_t sq = S[1];
+    while (c < live && sq > 0) {
+      const int d = sh.token[c];
+      const double rq = 1.0 / (double)sq;
+      if (scale31((uint32_t)u[2 * c], div31((uint64_t)ed << 31, sq, rq)) < pd) {
+        taken = c;
+        break;
+      }
+      if (!whole) {
+        normalise();
+        __syncthreads();
+        whole = true;
+      }
+      auto rest = [&](int i) -> uint32_t {
+        const uint32_t p = P[i], e = eq[i];
+        const uint32_t q = e ? div31((uint64_t)e << 31, sq, rq) : 0;
+        return p > q ? p - q : 0;
+      };
+      uint64_t s = 0, left;
+      for (int i = tid; i < len; i += NT) s += rest(i);
+      block_sum<1>(sh, &s);
+      const int c2 = next_child(c + 1), d2 = c2 < live ? sh.token[c2] : 0;
+      ph ^= 1;
+      if (c2 < live && d2 / seg == (int)rank) push_child(P[d2 - v0], rest(d2 - v0), d2 == d ? 0 : eq[d2 - v0]);
+      cluster_sum<1>(sh, &s, ph, rank, cs, &left);
+      if (left > 0) {
+        const double rl = 1.0 / (double)left;
+        for (int i = tid; i < len; i += NT) {
+          const uint32_t r = rest(i);
+          P[i] = r ? div31((uint64_t)r << 31, left, rl) : 0;
+        }
+        pd = div31((uint64_t)sh.xchild[ph][1] << 31, left, rl);
+      } else {
+        pd = sh.xchild[ph][0];
+      }
+      __syncthreads();
+      if (d / seg == (int)rank && tid == 0) eq[d - v0] = 0;
+      __syncthreads();
+      sq -= ed;
+      ed = sh.xchild[ph][2];
+      c = c2;
     }
     if (taken < 0) {
-      uint64_t s = 0;
+      if (!whole) {
+        normalise();
+        __syncthreads();
+      }
+      uint64_t s = 0, all;
       for (int i = tid; i < len; i += NT) s += P[i];
-      mine = block_sum(sh, s);
-      S = cluster_sum(sh, mine, ph ^= 1, rank, cs, before);
-      const uint64_t t = scale31((uint32_t)u[2 * node + 1], S);
-      if (before <= t && t < before + mine) {
+      block_sum<1>(sh, &s);
+      ph ^= 1;
+      before = cluster_sum<1>(sh, &s, ph, rank, cs, &all);
+      const uint64_t t = scale31((uint32_t)u[2 * node + 1], all);
+      if (before <= t && t < before + s) {
         const int i = find(sh, len, t - before, [&](int j) { return (uint64_t)P[j]; });
         if (tid == 0) (WALK ? next[lane] : drawn[row]) = v0 + i;
       }
@@ -481,7 +548,6 @@ __global__ void __launch_bounds__(NT) k_verify(const int64_t* __restrict__ logit
       break;
     }
     node = taken;  // a later node: the walk ends
-    cluster_sync();  // the peers have read this node's P and eq
   }
   cluster_sync();  // no CTA may exit while a peer still reads its shared memory
 }
