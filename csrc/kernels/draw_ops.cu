@@ -103,23 +103,28 @@ struct Shared {
   uint32_t xchild[2][3];        // [phase] at a child's token: P or its weight, max(P - Q, 0), draft weight
   int ids[HIST];                // newest first
   int met[HIST];                // times that an id is penalised; 0: not its first entry, or not an id
-  int parent[tree::MAX_NODES], token[tree::MAX_NODES];
-  int n_ids, n_path;
+  int parent[tree::MAX_NODES], token[tree::MAX_NODES], hist[HIST];
+  int count, n_ids, n_path;
 };
 
-// The tree: each node's token and parent (-1 where that is no earlier node).
-__device__ __forceinline__ void load_tree(Shared& sh, const int* tokens, const int* parent, int n) {
-  for (int i = threadIdx.x; i < n; i += NT) {
-    sh.token[i] = tokens[i];
-    sh.parent[i] = tree::parent_of(parent, i);
+// The lane's tree (each node's token and parent, -1 where that is no earlier
+// node) and ring.
+__device__ __forceinline__ void load_lane(Shared& sh, const int* tokens, const int* parent, int n, const int* hist,
+                                          const int* count) {
+  const int tid = threadIdx.x;
+  if (tid < n) {
+    sh.token[tid] = tokens[tid];
+    sh.parent[tid] = tree::parent_of(parent, tid);
   }
+  if (tid >= 64 && tid < 64 + HIST) sh.hist[tid - 64] = hist[tid - 64];
+  if (tid == 128) sh.count = max(*count, 0);
   __syncthreads();
 }
 
 // The newest 64 ids behind `node` (its path up to, not including, the root,
 // then the lane's ring), and `skip`: a bit for each of them in this CTA's part
 // [v0, v0 + len) of the vocabulary.  The whole CTA calls it.
-__device__ void gather_ids(Shared& sh, uint32_t* skip, const int* hist, int count, int node, int V, int v0, int len) {
+__device__ void gather_ids(Shared& sh, uint32_t* skip, int node, int V, int v0, int len) {
   const int tid = threadIdx.x;
   for (int i = tid; i < (len + 31) / 32; i += NT) skip[i] = 0;
   if (tid == 0) {
@@ -128,9 +133,8 @@ __device__ void gather_ids(Shared& sh, uint32_t* skip, const int* hist, int coun
     sh.n_path = k;
   }
   __syncthreads();
-  const int np = sh.n_path, c = count < 0 ? 0 : count;
-  const int n = np + min(c, HIST - np);
-  if (tid >= np && tid < n) sh.ids[tid] = hist[(unsigned)(c - 1 - (tid - np)) & (HIST - 1)];
+  const int np = sh.n_path, c = sh.count, n = np + min(c, HIST - np);
+  if (tid >= np && tid < n) sh.ids[tid] = sh.hist[(unsigned)(c - 1 - (tid - np)) & (HIST - 1)];
   if (tid == 0) sh.n_ids = n;
   __syncthreads();
   if (tid < n) {
@@ -150,27 +154,23 @@ __device__ void gather_ids(Shared& sh, uint32_t* skip, const int* hist, int coun
 }
 
 // f(i, x) for this thread's elements i of the part, x the logit; the skipped
-// ones too.  16-byte loads, four in flight, where the row allows them.
+// ones too.  16-byte loads, several in flight, where the row allows them.
 template <class F>
 __device__ __forceinline__ void each(const int64_t* __restrict__ part, int len, F f) {
   if (((uintptr_t)part & 15) == 0) {
     const longlong2* p = (const longlong2*)part;
     const int n2 = len / 2;
     int i = threadIdx.x;
-    for (; i + 3 * NT < n2; i += 4 * NT) {
+    for (; i < n2; i += 4 * NT) {
       longlong2 x[4];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) x[k] = __ldg(p + i + k * NT);
+      for (int k = 0; k < 4; ++k) x[k] = i + k * NT < n2 ? __ldg(p + i + k * NT) : make_longlong2(0, 0);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        f(2 * (i + k * NT), (int64_t)x[k].x);
-        f(2 * (i + k * NT) + 1, (int64_t)x[k].y);
-      }
-    }
-    for (; i < n2; i += NT) {
-      const longlong2 x = __ldg(p + i);
-      f(2 * i, (int64_t)x.x);
-      f(2 * i + 1, (int64_t)x.y);
+      for (int k = 0; k < 4; ++k)
+        if (i + k * NT < n2) {
+          f(2 * (i + k * NT), (int64_t)x[k].x);
+          f(2 * (i + k * NT) + 1, (int64_t)x[k].y);
+        }
     }
     if ((len & 1) && threadIdx.x == 0) f(len - 1, (int64_t)__ldg((const long long*)part + len - 1));
   } else {
@@ -179,19 +179,28 @@ __device__ __forceinline__ void each(const int64_t* __restrict__ part, int len, 
   }
 }
 
-// A row's part as it is used: clamped, and scaled unless greedy.
+// The part into the cache, ahead of its first use.
+__device__ __forceinline__ void fetch(const int64_t* part, int len) {
+  for (int i = threadIdx.x * 16; i < len; i += NT * 16)
+    asm volatile("prefetch.global.L2 [%0];" ::"l"(part + i));
+}
+
+// A row's part as it is used.  Clamping and scaling keep the order, so the
+// maximum is found before them.
 struct Row {
   const int64_t* part;
   int64_t inv;
   __device__ Row(const int64_t* row, int v0, int64_t inv_temp)
       : part(row + v0), inv(inv_temp > MAX_INV_T ? MAX_INV_T : inv_temp) {}
   __device__ bool greedy() const { return inv <= 0; }
-  __device__ int64_t scaled(int64_t x) const { return greedy() ? x : (x * inv) >> FRAC_BITS; }
-  __device__ int64_t value(int64_t x) const { return scaled(clamp40(x)); }
-  __device__ int64_t penalised(int64_t x, int times) const {
+  // the weighted value of a logit; 32-bit logits need no clamp and one product
+  __device__ int64_t value(int64_t x) const {
+    return x == (int64_t)(int)x ? ((int64_t)(int)x * (int)inv) >> FRAC_BITS : (clamp40(x) * inv) >> FRAC_BITS;
+  }
+  __device__ int64_t penalised(int64_t x, int times) const {  // not scaled
     x = clamp40(x);
     for (int r = 0; r < times; ++r) x = clamp40(penalize(x));
-    return scaled(x);
+    return x;
   }
 };
 
@@ -206,15 +215,16 @@ __device__ __forceinline__ void better(int64_t& v, int& i, int64_t ov, int oi) {
   if (ov > v || (ov == v && oi < i)) v = ov, i = oi;
 }
 
-// Largest value and its first index over the CTA's part of row r, into the
-// cell k of redv / redi (per warp).
+// Largest clamped logit and its first index over the CTA's part of row r, into
+// the cell k of redv / redi (per warp).  The index matters to greedy rows only.
 __device__ void warp_max(Shared& sh, const uint32_t* skip, const Row& r, int v0, int len, int k) {
   int64_t bv = INT64_MIN;
   int bi = INT_MAX;
   each(r.part, len, [&](int i, int64_t x) {
-    const int64_t z = r.value(x);
-    if (z > bv && !(skip[i >> 5] >> (i & 31) & 1)) bv = z, bi = v0 + i;  // a thread meets rising indexes
+    x = r.greedy() ? clamp40(x) : x;
+    if (x > bv && !(skip[i >> 5] >> (i & 31) & 1)) bv = x, bi = v0 + i;  // a thread meets rising indexes
   });
+  if (bi != INT_MAX) bv = clamp40(bv);
   const int t = own_id(sh, v0, len);
   if (t >= 0) better(bv, bi, r.penalised(r.part[t], sh.met[threadIdx.x]), v0 + t);
 #pragma unroll
@@ -245,12 +255,14 @@ __device__ void cluster_max(Shared& sh, int n, uint32_t rank, uint32_t cs, int64
   }
 }
 
-// Weights of the CTA's part into e; this thread's part of their sum.
+// Weights of the CTA's part into e; this thread's part of their sum.  `top` is
+// the row's largest clamped logit.
 __device__ uint64_t weights(Shared& sh, const Row& r, int v0, int len, int64_t top, int first, uint32_t* e) {
+  const int64_t zt = (clamp40(top) * r.inv) >> FRAC_BITS;  // a row of the type's lowest value has no larger one
   uint64_t s = 0;
-  auto weight = [&](int i, int64_t z) -> uint32_t {
+  auto weight = [&](int i, int64_t z) -> uint32_t {  // z the scaled value
     if (r.greedy()) return v0 + i == first ? (uint32_t)ONE : 0u;
-    const int64_t d = z - top;
+    const int64_t d = z - zt;
     return (uint32_t)exp32(d < -(1 << 30) ? -(1 << 30) : (int)d, sh.lut);
   };
   each(r.part, len, [&](int i, int64_t x) {
@@ -262,7 +274,7 @@ __device__ uint64_t weights(Shared& sh, const Row& r, int v0, int len, int64_t t
   const int t = own_id(sh, v0, len);
   if (t >= 0) {
     s -= e[t];  // what the logit would have weighed, and what it does
-    const uint32_t w = weight(t, r.penalised(r.part[t], sh.met[threadIdx.x]));
+    const uint32_t w = weight(t, (r.penalised(r.part[t], sh.met[threadIdx.x]) * r.inv) >> FRAC_BITS);
     e[t] = w;
     s += w;
   }
@@ -311,38 +323,31 @@ __device__ __forceinline__ uint64_t cluster_sum(Shared& sh, const uint64_t* mine
 }
 
 // The first element of this CTA's part whose running sum exceeds t (which is
-// below the part's sum); val(i) is element i.  The whole CTA calls it.
+// below the part's sum); val(i) is element i.  Every thread sums its own
+// stretch (an odd number of elements: no bank conflicts), the one whose
+// stretch holds t walks through it.  The whole CTA calls it.
 template <class F>
 __device__ int find(Shared& sh, int len, uint64_t t, F val) {
   __shared__ int found;
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
-  const int per = (len + NW * 32 - 1) / (NW * 32) * 32;  // elements per warp
-  const int a = w * per, b = min(len, a + per);
+  const int per = (len + NT - 1) / NT | 1, a = min(len, tid * per), b = min(len, a + per);
   uint64_t s = 0;
-  for (int i = a + lane; i < b; i += 32) s += val(i);
+  for (int i = a; i < b; ++i) s += val(i);
+  uint64_t incl = s;
 #pragma unroll
-  for (int m = 16; m >= 1; m >>= 1) s += (uint64_t)shfl_xor_i64((int64_t)s, m);
+  for (int m = 1; m < 32; m <<= 1) {
+    const uint64_t y = (uint64_t)__shfl_up_sync(0xffffffffu, (unsigned long long)incl, m);
+    if (lane >= m) incl += y;
+  }
   __syncthreads();
-  if (lane == 0) sh.wsum[0][w] = s;
+  if (lane == 31) sh.wsum[0][w] = incl;
   __syncthreads();
-  uint64_t before = 0;
+  uint64_t before = incl - s;
   for (int k = 0; k < w; ++k) before += sh.wsum[0][k];
-  if (before <= t && t < before + s) {  // this warp's elements hold it
-    for (int i0 = a; i0 < b; i0 += 32) {
-      const int i = i0 + lane;
-      uint64_t x = i < b ? val(i) : 0;
-#pragma unroll
-      for (int m = 1; m < 32; m <<= 1) {
-        const uint64_t y = (uint64_t)__shfl_up_sync(0xffffffffu, (unsigned long long)x, m);
-        if (lane >= m) x += y;
-      }
-      const unsigned hit = __ballot_sync(0xffffffffu, before + x > t);
-      if (hit) {
-        if (lane == 0) found = i0 + __ffs(hit) - 1;
-        break;
-      }
-      before += (uint64_t)__shfl_sync(0xffffffffu, (unsigned long long)x, 31);
-    }
+  if (before <= t && t < before + s) {
+    int i = a;
+    for (before += val(i); before <= t; before += val(i)) ++i;
+    found = i;
   }
   __syncthreads();
   return found;
@@ -352,7 +357,7 @@ __device__ __forceinline__ uint64_t scale31(uint32_t u, uint64_t s) {  // floor(
   return __umul64hi((uint64_t)(u & 0x7fffffffu) << 33, s);
 }
 
-__global__ void __launch_bounds__(NT) k_draw(const int64_t* __restrict__ logits, int64_t ldl, int V, int nr, int n,
+__global__ void __launch_bounds__(NT, 3) k_draw(const int64_t* __restrict__ logits, int64_t ldl, int V, int nr, int n,
                                              int node0, int m, const int64_t* __restrict__ inv_temp,
                                              const int* __restrict__ u, const int* __restrict__ hist,
                                              const int* __restrict__ count, const int* __restrict__ tokens,
@@ -368,9 +373,10 @@ __global__ void __launch_bounds__(NT) k_draw(const int64_t* __restrict__ logits,
   cluster_sync();  // every peer runs: its shared memory may be stored to
   pdl_wait_dep();
   pdl_allow_next();
-  load_tree(sh, tokens + (size_t)lane * n, parent + (size_t)lane * n, n);
-  gather_ids(sh, skip, hist + lane * HIST, count[lane], node0 + blockIdx.y, V, v0, len);
   const Row r(logits + (size_t)row * ldl, v0, inv_temp[lane]);
+  fetch(r.part, len);
+  load_lane(sh, tokens + (size_t)lane * n, parent + (size_t)lane * n, n, hist + lane * HIST, count + lane);
+  gather_ids(sh, skip, node0 + blockIdx.y, V, v0, len);
   int64_t top;
   int first;
   warp_max(sh, skip, r, v0, len, 0);
@@ -401,7 +407,7 @@ __global__ void __launch_bounds__(NT) k_draw(const int64_t* __restrict__ logits,
 // accepted child or -1) and drawn (the token that follows the node when no
 // child is accepted).  WALK, grid (cluster, 1, lanes): the lane's path.
 template <bool WALK>
-__global__ void __launch_bounds__(NT) k_verify(const int64_t* __restrict__ logits, int64_t ldl,
+__global__ void __launch_bounds__(NT, 2) k_verify(const int64_t* __restrict__ logits, int64_t ldl,
                                                const int64_t* __restrict__ dlogits, int64_t ldd, int V, int n,
                                                const int* __restrict__ tokens, const int* __restrict__ parent,
                                                const int* __restrict__ n_tree, const int64_t* __restrict__ inv_temp,
@@ -432,7 +438,7 @@ __global__ void __launch_bounds__(NT) k_verify(const int64_t* __restrict__ logit
     }
     return;
   }
-  load_tree(sh, tokens + lane0, parent + lane0, n);
+  load_lane(sh, tokens + lane0, parent + lane0, n, hist + lane * HIST, count + lane);
   u += lane0 * 2;
   int ph = 0, length = 0;
   auto next_child = [&](int c) {  // of the node, from c on, whose token is one
@@ -441,10 +447,12 @@ __global__ void __launch_bounds__(NT) k_verify(const int64_t* __restrict__ logit
   };
   for (;;) {
     const size_t row = lane0 + node;
-    gather_ids(sh, skip, hist + lane * HIST, count[lane], node, V, v0, len);
     int c = next_child(node + 1);
     const bool inner = c < live;
     const Row rt(logits + row * ldl, v0, inv_temp[lane]), rd(dlogits + row * ldd, v0, d_inv_temp[lane]);
+    fetch(rt.part, len);
+    if (inner) fetch(rd.part, len);
+    gather_ids(sh, skip, node, V, v0, len);
     int64_t top[2];
     int first[2];
     warp_max(sh, skip, rt, v0, len, 0);
@@ -584,10 +592,10 @@ static size_t part_of(int V, int cs, int per, int& seg) {
   return (size_t)seg * per + seg / 8;
 }
 
-// CTAs that the GPU holds at once.
-static int64_t capacity(size_t smem) {
-  const int by_smem = (int)((224 * 1024) / (smem + sizeof(Shared) + 1024)), by_threads = 2048 / NT;
-  return 148 * (int64_t)(by_smem < by_threads ? by_smem : by_threads);
+// CTAs that the GPU holds at once, `most` per SM by their registers.
+static int64_t capacity(size_t smem, int most) {
+  const int by_smem = (int)((224 * 1024) / (smem + sizeof(Shared) + 1024));
+  return 148 * (int64_t)(by_smem < most ? by_smem : most);
 }
 
 template <typename... KArgs, typename... Args>
@@ -632,7 +640,7 @@ int arcb_draw_tokens(const int64_t* logits, int64_t ldl, int V, int lanes, int n
   // 16 CTAs a row while they all run at once, else 8
   int seg = 0, cs = 16;
   size_t smem = dr::part_of(V, cs, 4, seg);
-  if ((int64_t)lanes * nr * cs > dr::capacity(smem)) {
+  if ((int64_t)lanes * nr * cs > dr::capacity(smem, 3)) {
     int seg8 = 0;
     const size_t smem8 = dr::part_of(V, 8, 4, seg8);
     if (smem8 <= dr::SMEM_MAX) cs = 8, seg = seg8, smem = smem8;
@@ -651,7 +659,7 @@ int arcb_verify_tree(const int64_t* logits, int64_t ldl, const int64_t* dlogits,
   int* drawn = scratch + (size_t)lanes * n;
   int seg = 0;
   size_t smem = dr::part_of(V, 16, 8, seg);
-  if ((int64_t)lanes * n * 16 > dr::capacity(smem))  // a cluster per node does not fit the GPU: one per lane
+  if ((int64_t)lanes * n * 16 > dr::capacity(smem, 2))  // a cluster per node does not fit the GPU: one per lane
     return dr::launch_cluster(dr::k_verify<true>, 16, dim3(16, 1, lanes), smem, st, logits, ldl, dlogits, ldd, V, n,
                               tokens, parent, n_tree, inv_temp, d_inv_temp, u, hist, count, seg, scratch, drawn, path,
                               n_path, next);
