@@ -18,6 +18,7 @@ the kernels, which skip the lane and set a bit of ``err``.
 """
 from __future__ import annotations
 
+import functools
 from typing import Optional, Sequence
 
 import torch
@@ -32,48 +33,61 @@ PAGE = 16
 I32, I64, I8 = torch.int32, torch.int64, torch.int8
 
 
-def _need(what: str, t, dtype, shape) -> None:
-    """t is a contiguous tensor of the given type and shape (None: any size)."""
+def _refuse(what: str, t, dtype, shape, dev) -> None:
+    """Raises what is wrong with a tensor that _check did not pass."""
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{what} must be a tensor, got {type(t).__name__}")
     if t.dtype is not dtype:
         raise TypeError(f"{what} must be {dtype}, got {t.dtype}")
-    s = t.shape
-    if len(s) != len(shape) or any(w is not None and g != w for g, w in zip(s, shape)):
-        raise ValueError(f"{what} must have shape {tuple('any' if w is None else w for w in shape)}, got {tuple(s)}")
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{what} must have shape {tuple(shape)}, got {tuple(t.shape)}")
     if not t.is_contiguous():
         raise ValueError(f"{what} must be contiguous")
+    raise ValueError(f"{what} is on {t.device}, other tensors on {dev}")
 
 
-def _rows(what: str, t, dtype, rows: int, cols: int) -> int:
-    """t is [>= rows, >= cols] with contiguous rows; returns the row stride."""
+def _check(dev, *specs) -> None:
+    """Every (name, tensor, type, shape) is a contiguous tensor on dev."""
+    for what, t, dtype, shape in specs:
+        if not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.shape != shape or not t.is_contiguous() \
+                or t.device != dev:
+            _refuse(what, t, dtype, shape, dev)
+
+
+def _rows(dev, what: str, t, dtype, rows: int, cols: int) -> int:
+    """t is [>= rows, >= cols] on dev with contiguous rows; returns the row stride."""
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{what} must be a tensor, got {type(t).__name__}")
     if t.dtype is not dtype:
         raise TypeError(f"{what} must be {dtype}, got {t.dtype}")
     if t.dim() != 2 or t.shape[0] < rows or t.shape[1] < cols:
         raise ValueError(f"{what} must be at least [{rows}, {cols}], got {tuple(t.shape)}")
-    if t.stride(1) != 1 or (rows > 1 and t.stride(0) < cols):
+    step, one = t.stride()
+    if one != 1 or (rows > 1 and step < cols):
         raise ValueError(f"{what} must have contiguous rows that do not overlap")
-    return t.stride(0)
+    if t.device != dev:
+        raise ValueError(f"{what} is on {t.device}, other tensors on {dev}")
+    return step
 
 
-def _place(*ts) -> torch.device:
-    dev = ts[0].device
-    for t in ts:
-        if t is not None and t.device != dev:
-            raise ValueError(f"all tensors must be on one device, got {dev} and {t.device}")
-    if dev.type != "cuda":
-        raise ValueError(f"tensors must be on a CUDA device, got {dev}")
-    return dev
+def _device(what: str, t, dims: int) -> torch.device:
+    """The device that the first tensor of a call is on."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{what} must be a tensor, got {type(t).__name__}")
+    if t.dim() != dims:
+        raise ValueError(f"{what} must have {dims} dimensions, got {tuple(t.shape)}")
+    return t.device
 
 
 def _call(dev: torch.device, f, what: str, *args) -> None:
+    """Launches on dev's current stream."""
+    if dev.type != "cuda":
+        raise ValueError(f"tensors must be on a CUDA device, got {dev}")
     if dev.index == torch.cuda.current_device():
-        rc = f(*args, torch.cuda.current_stream().cuda_stream)
+        rc = f(*args, torch._C._cuda_getCurrentRawStream(dev.index))
     else:
         with torch.cuda.device(dev):
-            rc = f(*args, torch.cuda.current_stream().cuda_stream)
+            rc = f(*args, torch._C._cuda_getCurrentRawStream(dev.index))
     int_ops._count()
     check(rc, what)
 
@@ -106,32 +120,31 @@ def attn_tree(q, Kc, Vc, pt, base, n_tree, mask, n_heads: int, n_kv: int, dh: in
     if t_lim < 1:
         raise ValueError(f"t_lim must be at least 1, got {t_lim}")
     B, d = lanes * nq, n_heads * dh
-    _need("q", q, I64, (B, d))
-    _need("Kc", Kc, I64, (None, n_kv, PAGE, dh))
-    _need("Vc", Vc, I64, tuple(Kc.shape))
-    ps = _rows("pt", pt, I32, lanes, 1)
-    _need("base", base, I32, (lanes,))
-    _need("n_tree", n_tree, I32, (lanes,))
-    _need("mask", mask, I64, (B,))
-    _need("err", err, I32, (1,))
+    dev = _device("Kc", Kc, 4)
+    pages = Kc.shape[0]
+    cache = (pages, n_kv, PAGE, dh)
+    _check(dev, ("q", q, I64, (B, d)), ("Kc", Kc, I64, cache), ("Vc", Vc, I64, cache), ("base", base, I32, (lanes,)),
+           ("n_tree", n_tree, I32, (lanes,)), ("mask", mask, I64, (B,)), ("err", err, I32, (1,)))
+    ps = _rows(dev, "pt", pt, I32, lanes, 1)
+    at = q.data_ptr() | Kc.data_ptr() | Vc.data_ptr()
     if X is None and o_out is None:
         raise ValueError("one of X and o_out must be given")
     if X is not None:
-        _need("X", X, I8, (None, d))
-        if X.shape[0] < 8 * int_ops.n_tiles(B) * int_ops.limb_slots(B):
-            raise ValueError(f"X has {X.shape[0]} rows, too few for {B} slots")
+        if _rows(dev, "X", X, I8, 8 * int_ops.n_tiles(B) * int_ops.limb_slots(B), d) != d or X.shape[1] != d:
+            raise ValueError(f"X must have {d} columns, got {tuple(X.shape)}")
+        at |= X.data_ptr()
     if lmax is not None:
-        _need("lmax", lmax, I32, (1,))
+        _check(dev, ("lmax", lmax, I32, (1,)))
     if o_out is not None:
-        _need("o_out", o_out, I64, (B, d))
-    dev = _place(q, Kc, Vc, pt, base, n_tree, mask, err, X, lmax, o_out)
-    if any(t is not None and t.data_ptr() % 16 for t in (q, Kc, Vc, X, o_out)):
+        _check(dev, ("o_out", o_out, I64, (B, d)))
+        at |= o_out.data_ptr()
+    if at % 16:
         raise ValueError("q, Kc, Vc, X and o_out must start on a 16-byte boundary")
     L = lib()
     ws = torch.empty(L.arcb_attn_tree_ws(lanes, nq, n_heads, n_kv, dh, t_lim), dtype=torch.uint8, device=dev)
-    _call(dev, L.arcb_attn_tree, "attn_tree", _p(q), _p(Kc), _p(Vc), Kc.shape[0], _p(pt), ps, pt.shape[1], _p(base),
-          _p(n_tree), _p(mask), nq, n_heads, n_kv, dh, int(attn_scale), t_lim, lanes, _p(ws), _p(X), _p(lmax),
-          _p(o_out), _p(err))
+    _call(dev, L.arcb_attn_tree, "attn_tree", q.data_ptr(), Kc.data_ptr(), Vc.data_ptr(), pages, pt.data_ptr(), ps,
+          pt.shape[1], base.data_ptr(), n_tree.data_ptr(), mask.data_ptr(), nq, n_heads, n_kv, dh, int(attn_scale),
+          t_lim, lanes, ws.data_ptr(), _p(X), _p(lmax), _p(o_out), err.data_ptr())
 
 
 def _vocab(V: int, lanes: int) -> None:
@@ -141,6 +154,7 @@ def _vocab(V: int, lanes: int) -> None:
         raise ValueError(f"lanes must be 1 to 65535, got {lanes}")
 
 
+@functools.lru_cache(maxsize=None)
 def lib_max_vocab() -> int:
     """Largest vocabulary of draw_tokens and verify_tree."""
     return lib().arcb_draw_max_vocab()
@@ -169,17 +183,14 @@ def draw_tokens(logits, V: int, lanes: int, nr: int, node0: int, m: int, inv_tem
         raise ValueError(f"rows stand for nodes {node0} to {node0 + nr - 1} of a {n}-node tree")
     if m < 1:
         raise ValueError(f"m must be at least 1, got {m}")
-    ldl = _rows("logits", logits, I64, lanes * nr, V)
-    _need("inv_temp", inv_temp, I64, (lanes,))
-    _need("u", u, I32, (lanes * nr, m))
-    _need("hist", hist, I32, (lanes, HIST))
-    _need("count", count, I32, (lanes,))
-    _need("tokens", tokens, I32, (lanes, n))
-    _need("parent", parent, I32, (lanes, n))
-    _need("out", out, I32, (lanes * nr, m))
-    dev = _place(logits, inv_temp, u, hist, count, tokens, parent, out)
-    _call(dev, lib().arcb_draw_tokens, "draw_tokens", _p(logits), ldl, V, lanes, nr, n, node0, m, _p(inv_temp), _p(u),
-          _p(hist), _p(count), _p(tokens), _p(parent), _p(out))
+    dev = _device("logits", logits, 2)
+    ldl = _rows(dev, "logits", logits, I64, lanes * nr, V)
+    _check(dev, ("inv_temp", inv_temp, I64, (lanes,)), ("u", u, I32, (lanes * nr, m)),
+           ("hist", hist, I32, (lanes, HIST)), ("count", count, I32, (lanes,)), ("tokens", tokens, I32, (lanes, n)),
+           ("parent", parent, I32, (lanes, n)), ("out", out, I32, (lanes * nr, m)))
+    _call(dev, lib().arcb_draw_tokens, "draw_tokens", logits.data_ptr(), ldl, V, lanes, nr, n, node0, m,
+          inv_temp.data_ptr(), u.data_ptr(), hist.data_ptr(), count.data_ptr(), tokens.data_ptr(), parent.data_ptr(),
+          out.data_ptr())
 
 
 def verify_tree(logits, dlogits, V: int, lanes: int, n: int, tokens, parent, n_tree, inv_temp, d_inv_temp, u, hist,
@@ -202,25 +213,19 @@ def verify_tree(logits, dlogits, V: int, lanes: int, n: int, tokens, parent, n_t
     _vocab(V, lanes)
     if n < 1 or n > MAX_NODES:
         raise ValueError(f"a tree has 1 to {MAX_NODES} nodes, got {n}")
-    ldl = _rows("logits", logits, I64, lanes * n, V)
-    ldd = _rows("dlogits", dlogits, I64, lanes * n, V)
-    _need("tokens", tokens, I32, (lanes, n))
-    _need("parent", parent, I32, (lanes, n))
-    _need("n_tree", n_tree, I32, (lanes,))
-    _need("inv_temp", inv_temp, I64, (lanes,))
-    _need("d_inv_temp", d_inv_temp, I64, (lanes,))
-    _need("u", u, I32, (lanes, n, 2))
-    _need("hist", hist, I32, (lanes, HIST))
-    _need("count", count, I32, (lanes,))
-    _need("path", path, I32, (lanes, n))
-    _need("n_path", n_path, I32, (lanes,))
-    _need("nxt", nxt, I32, (lanes,))
-    dev = _place(logits, dlogits, tokens, parent, n_tree, inv_temp, d_inv_temp, u, hist, count, path, n_path, nxt)
+    dev = _device("logits", logits, 2)
+    ldl = _rows(dev, "logits", logits, I64, lanes * n, V)
+    ldd = _rows(dev, "dlogits", dlogits, I64, lanes * n, V)
+    one, per = (lanes,), (lanes, n)
+    _check(dev, ("tokens", tokens, I32, per), ("parent", parent, I32, per), ("n_tree", n_tree, I32, one),
+           ("inv_temp", inv_temp, I64, one), ("d_inv_temp", d_inv_temp, I64, one), ("u", u, I32, (lanes, n, 2)),
+           ("hist", hist, I32, (lanes, HIST)), ("count", count, I32, one), ("path", path, I32, per),
+           ("n_path", n_path, I32, one), ("nxt", nxt, I32, one))
     scratch = torch.empty(2 * lanes * n, dtype=I32, device=dev)
-    _call(dev, lib().arcb_verify_tree, "verify_tree", _p(logits), ldl, _p(dlogits), ldd, V, lanes, n, _p(tokens),
-          _p(parent), _p(n_tree), _p(inv_temp), _p(d_inv_temp), _p(u), _p(hist), _p(count), _p(scratch), _p(path),
-          _p(n_path), _p(nxt))
-    int_ops._count()  # two kernels
+    _call(dev, lib().arcb_verify_tree, "verify_tree", logits.data_ptr(), ldl, dlogits.data_ptr(), ldd, V, lanes, n,
+          tokens.data_ptr(), parent.data_ptr(), n_tree.data_ptr(), inv_temp.data_ptr(), d_inv_temp.data_ptr(),
+          u.data_ptr(), hist.data_ptr(), count.data_ptr(), scratch.data_ptr(), path.data_ptr(), n_path.data_ptr(),
+          nxt.data_ptr())
 
 
 class KvPlanes:
@@ -235,10 +240,13 @@ class KvPlanes:
         first = self.tensors[0]
         if not isinstance(first, torch.Tensor) or first.dim() != 4 or first.shape[2] != PAGE or first.shape[3] % 2:
             raise ValueError("cache tensors are [pages, n_kv, 16, d_head] with an even d_head")
-        for t in self.tensors:
-            _need("cache tensor", t, I64, tuple(first.shape))
+        self.device = first.device
+        _check(self.device, *(("cache tensor", t, I64, first.shape) for t in self.tensors))
+        if self.device.type != "cuda":
+            raise ValueError(f"tensors must be on a CUDA device, got {self.device}")
+        if any(t.data_ptr() % 16 for t in self.tensors):
+            raise ValueError("cache tensors must start on a 16-byte boundary")
         self.n_pages, self.n_kv, _, self.dh = first.shape
-        self.device = _place(*self.tensors)
         self.table = torch.tensor([t.data_ptr() for t in self.tensors], dtype=I64, device=self.device)
 
 
@@ -256,11 +264,10 @@ def kv_keep_path(planes: KvPlanes, pt, base, path, n_path, lanes: int, n: int, e
         raise ValueError(f"a tree has 1 to {MAX_NODES} nodes, got {n}")
     if not isinstance(planes, KvPlanes):
         raise TypeError(f"planes must be KvPlanes, got {type(planes).__name__}")
-    ps = _rows("pt", pt, I32, lanes, 1)
-    _need("base", base, I32, (lanes,))
-    _need("path", path, I32, (lanes, n))
-    _need("n_path", n_path, I32, (lanes,))
-    _need("err", err, I32, (1,))
-    dev = _place(planes.table, pt, base, path, n_path, err)
-    _call(dev, lib().arcb_kv_keep_path, "kv_keep_path", _p(planes.table), len(planes.tensors), planes.n_pages,
-          planes.n_kv, planes.dh, _p(pt), ps, pt.shape[1], _p(base), _p(path), _p(n_path), lanes, n, _p(err))
+    dev = planes.device
+    ps = _rows(dev, "pt", pt, I32, lanes, 1)
+    _check(dev, ("base", base, I32, (lanes,)), ("path", path, I32, (lanes, n)), ("n_path", n_path, I32, (lanes,)),
+           ("err", err, I32, (1,)))
+    _call(dev, lib().arcb_kv_keep_path, "kv_keep_path", planes.table.data_ptr(), len(planes.tensors), planes.n_pages,
+          planes.n_kv, planes.dh, pt.data_ptr(), ps, pt.shape[1], base.data_ptr(), path.data_ptr(), n_path.data_ptr(),
+          lanes, n, err.data_ptr())

@@ -38,6 +38,8 @@
 //     Chunks with wider values take 64-bit terms.
 //     CTAs that share a lane add their sums with atomics (integers: any order
 //     gives the same), two int32 in one 64-bit word; the last to arrive writes.
+#include <atomic>
+
 #include "../common/tree.h"
 #include "common.cuh"
 #include "exp32.cuh"
@@ -58,6 +60,7 @@ constexpr int SMALL = 1 << 29;      // bound of scores stored as they are
 constexpr int FAR = -(1 << 30);     // a score whose exp is 0
 constexpr int64_t NONE = -(int64_t(1) << 62);  // max of no keys
 constexpr int VMAX = (1 << 22) - (1 << 17);    // values of the single-precision form
+constexpr int SMEM_V = 2 * (CK * (128 * 8 + MAX_RG * 4) + MAX_RG * 8);  // k_values shared memory, at most
 constexpr int MAX_RANGE = 1 << 16;             // keys per k_values CTA: VMAX + MAX_RANGE < 2^22
 
 struct Args {
@@ -883,8 +886,14 @@ static int run(Args A, const Plan& p, int lanes, cudaStream_t st) {
   constexpr int smem_s = 1024 + PLANES * (TILE + 2 * RQ) * 128;
   const int vals = 2 * (CK * (A.dh * 8 + p.RG * 4) + p.RG * 8), sums = p.RG * DHP * 4, smem_v = vals > sums ? vals : sums;
   const auto kv = k_values<DHP / 32, UR>;
-  cudaError_t e = cudaFuncSetAttribute(k_scores<DHP>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_s);
-  if (e == cudaSuccess) e = cudaFuncSetAttribute(kv, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_v);
+  static std::atomic<uint64_t> ready{0};  // the kernels' attributes are set, a bit per device
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess && !(ready.load() >> (dev & 63) & 1)) {
+    e = cudaFuncSetAttribute(k_scores<DHP>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_s);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(kv, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_V);
+    if (e == cudaSuccess && dev < 64) ready.fetch_or(uint64_t(1) << dev);
+  }
   if (e != cudaSuccess) return (int)e;
   for (int l0 = 0; l0 < lanes; l0 += p.lanes) {
     const int n = lanes - l0 < p.lanes ? lanes - l0 : p.lanes;

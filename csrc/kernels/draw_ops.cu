@@ -34,6 +34,7 @@
 // reaches it, and a second small kernel follows the decisions from the root:
 // one node's latency.  Larger trees and batches take one cluster per lane,
 // which walks from the root and reads only the rows that it meets.
+#include <atomic>
 #include <climits>
 
 #include "../common/tree.h"
@@ -599,10 +600,15 @@ static int64_t capacity(size_t smem, int most) {
 }
 
 template <typename... KArgs, typename... Args>
-static int launch_cluster(void (*k)(KArgs...), int cs, dim3 grid, size_t smem, cudaStream_t st,
-                          Args... args) {
-  cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM_MAX);
-  if (e == cudaSuccess && cs > 8) e = cudaFuncSetAttribute(k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+static int launch_cluster(void (*k)(KArgs...), std::atomic<uint64_t>& ready, int cs, dim3 grid, size_t smem,
+                          cudaStream_t st, Args... args) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess && !(ready.load() >> (dev & 63) & 1)) {  // the kernel's attributes, once per device
+    e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM_MAX);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e == cudaSuccess && dev < 64) ready.fetch_or(uint64_t(1) << dev);
+  }
   if (e != cudaSuccess) return (int)e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
@@ -645,7 +651,8 @@ int arcb_draw_tokens(const int64_t* logits, int64_t ldl, int V, int lanes, int n
     const size_t smem8 = dr::part_of(V, 8, 4, seg8);
     if (smem8 <= dr::SMEM_MAX) cs = 8, seg = seg8, smem = smem8;
   }
-  return dr::launch_cluster(dr::k_draw, cs, dim3(cs, nr, lanes), smem, (cudaStream_t)stream, logits, ldl, V, nr, n,
+  static std::atomic<uint64_t> ready{0};
+  return dr::launch_cluster(dr::k_draw, ready, cs, dim3(cs, nr, lanes), smem, (cudaStream_t)stream, logits, ldl, V, nr, n,
                             node0, m, inv_temp, u, hist, count, tokens, parent, seg, out);
 }
 
@@ -655,15 +662,16 @@ int arcb_verify_tree(const int64_t* logits, int64_t ldl, const int64_t* dlogits,
                      const int64_t* d_inv_temp, const int* u, const int* hist, const int* count, int* scratch,
                      int* path, int* n_path, int* next, void* stream) {
   if (V < 1 || V > arcb_draw_max_vocab() || lanes < 1 || n < 1 || n > tree::MAX_NODES || lanes > 65535) return -2;
+  static std::atomic<uint64_t> walk{0}, all{0};
   cudaStream_t st = (cudaStream_t)stream;
   int* drawn = scratch + (size_t)lanes * n;
   int seg = 0;
   size_t smem = dr::part_of(V, 16, 8, seg);
   if ((int64_t)lanes * n * 16 > dr::capacity(smem, 2))  // a cluster per node does not fit the GPU: one per lane
-    return dr::launch_cluster(dr::k_verify<true>, 16, dim3(16, 1, lanes), smem, st, logits, ldl, dlogits, ldd, V, n,
+    return dr::launch_cluster(dr::k_verify<true>, walk, 16, dim3(16, 1, lanes), smem, st, logits, ldl, dlogits, ldd, V, n,
                               tokens, parent, n_tree, inv_temp, d_inv_temp, u, hist, count, seg, scratch, drawn, path,
                               n_path, next);
-  const int rc = dr::launch_cluster(dr::k_verify<false>, 16, dim3(16, n, lanes), smem, st, logits, ldl, dlogits, ldd, V,
+  const int rc = dr::launch_cluster(dr::k_verify<false>, all, 16, dim3(16, n, lanes), smem, st, logits, ldl, dlogits, ldd, V,
                                     n, tokens, parent, n_tree, inv_temp, d_inv_temp, u, hist, count, seg, scratch,
                                     drawn, path, n_path, next);
   if (rc) return rc;
