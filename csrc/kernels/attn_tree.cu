@@ -305,15 +305,20 @@ __global__ void __launch_bounds__(NT_S, 2) k_scores(const Args A) {
     __syncthreads();
     const int lk_n = planes_of(or_k[0]);
     uint32_t products = 0;  // groups that took the tensor path
+    const uint64_t small_lim = (uint64_t(1) << 47) / A.dh;
+    const uint64_t kd = sw128_kmajor_desc(kbase), qd0 = sw128_kmajor_desc(qbase);  // start addresses count in 16 bytes
+    const uint4* qinfo = A.qinfo + lk * A.qgroups + r_lo / RQ;
+    uint4 q_next = __ldg(qinfo);
     for (int r0 = r_lo, n = 0; r0 < r_hi; r0 += RQ, ++n) {
       const int rows = min(RQ, r_hi - r0), b = n & 1;
-      const uint4 qi = __ldg(A.qinfo + lk * A.qgroups + r0 / RQ);
+      const uint4 qi = q_next;
+      if (r0 + RQ < r_hi) q_next = __ldg(qinfo + n + 1);
       const int lq_n = planes_of(qi.x);
       const bool wide = (or_k[1] | qi.y) != 0;
       // |q.k| <= dh * max|k| * max|q| < 2^47 and scale <= ONE / 4: 32 bits hold
       // every step below, and |score| <= 2^29
       const bool small = !wide && A.attn_scale >= 0 && A.attn_scale <= ONE / 4 &&
-                         ((uint64_t)or_k[2] + 1) * ((uint64_t)qi.z + 1) < (uint64_t(1) << 47) / A.dh;
+                         ((uint64_t)or_k[2] + 1) * ((uint64_t)qi.z + 1) < small_lim;
       if (!all_seen && tid < RQ)
         qmask[b][tid] = tid < rows ? (uint64_t)A.mask[(size_t)lane * A.nq + (r0 + tid) / A.G] : 0;
       if (tid == 0) {
@@ -323,17 +328,21 @@ __global__ void __launch_bounds__(NT_S, 2) k_scores(const Args A) {
         if (!wide) {
           // K_a times the stacked planes Q_0 | Q_1 | ..: plane b lands in accumulator a + b.
           // At k = 0 the accumulator that a reaches first is overwritten, by a product of its own.
-          const uint32_t qb = qbase + b * PLANES * QP;
-          for (int a = 0; a < lk_n; ++a)
-            for (int k = 0; k < kend; ++k) {
-              const uint64_t ka = sw128_kmajor_desc(kbase + a * KP + k * 32);
-              const bool split = a > 0 && k == 0;
-              const int nb = split ? lq_n - 1 : lq_n;
-              if (nb > 0)
-                mma_i8(tmem + a * RQ, ka, sw128_kmajor_desc(qb + k * 32), idesc_i8(TILE, nb * RQ), a > 0 || k > 0);
-              if (split)
-                mma_i8(tmem + (a + nb) * RQ, ka, sw128_kmajor_desc(qb + nb * QP + k * 32), idesc_i8(TILE, RQ), 0u);
+          const uint64_t qd = qd0 + b * (PLANES * QP / 16);
+          const uint32_t all = idesc_i8(TILE, lq_n * RQ), most = idesc_i8(TILE, (lq_n - 1) * RQ), one = idesc_i8(TILE, RQ);
+          for (int a = 0; a < lk_n; ++a) {
+            const uint64_t ka = kd + a * (KP / 16);
+            const uint32_t acc = tmem + a * RQ;
+            if (a == 0) {
+              mma_i8(acc, ka, qd, all, 0u);
+            } else {
+              if (lq_n > 1) mma_i8(acc, ka, qd, most, 1u);
+              mma_i8(acc + (lq_n - 1) * RQ, ka, qd + (lq_n - 1) * (QP / 16), one, 0u);
             }
+#pragma unroll
+            for (int k = 1; k < DHP / 32; ++k)  // 32 bytes along the planes' rows
+              if (k < kend) mma_i8(acc, ka + 2 * k, qd + 2 * k, all, 1u);
+          }
           mma_commit(smem_u32(&done));
         }
       }
