@@ -561,6 +561,8 @@ __global__ void __launch_bounds__(NT_V, 2) k_values(const Args A) {
   __shared__ int2 lut[EXP_LUT_N];
   __shared__ int64_t rmax[MAX_RG];
   __shared__ uint64_t rsum[MAX_RG];
+  __shared__ __align__(16) float rrcp[MAX_RG];     // ONE / sum
+  __shared__ __align__(16) uint32_t rden[MAX_RG];  // sum
   __shared__ __align__(8) uint64_t full[2];
   __shared__ int s_last, s_need, s_long;
   const int NT = blockDim.x, tid = threadIdx.x, ln = tid & 31, w = tid >> 5;
@@ -622,6 +624,8 @@ __global__ void __launch_bounds__(NT_V, 2) k_values(const Args A) {
       const uint64_t s = row ? A.sums[lk * A.Rp + r0 + tid] : 0;
       rmax[tid] = row ? A.gmax[lk * A.Rp + r0 + tid] : NONE;
       rsum[tid] = s ? s : 1;  // a row without keys: every exp is 0
+      rden[tid] = (uint32_t)rsum[tid];
+      rrcp[tid] = 65536.0f * __frcp_rn((float)(int64_t)rsum[tid]);
       if (s >> 30) s_long = 1;
     }
     float acc[DPL][UR];
@@ -633,15 +637,7 @@ __global__ void __launch_bounds__(NT_V, 2) k_values(const Args A) {
     bool any_wide = false;
     if (live) {
       const bool lng = s_long != 0;
-      float rcp[4];    // ONE / sum
-      uint32_t den[4];
-      int ro[4];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        den[c] = (uint32_t)rsum[rq + c];
-        rcp[c] = 65536.0f * __frcp_rn((float)(int64_t)rsum[rq + c]);
-        ro[c] = FAR;
-      }
+      int ro[4];       // what the tile's scores need added
       int pg[CK / PAGE];  // thread 0: page ids of the chunk to issue next
       auto fetch = [&](int c) {
 #pragma unroll
@@ -686,62 +682,76 @@ __global__ void __launch_bounds__(NT_V, 2) k_values(const Args A) {
         if (!mbar_wait(smem_u32(&full[used & 1]), (used >> 1) & 1)) set_error(A.err, ARCB_ERR_TIMEOUT_FULL);
         int64_t* vb = (int64_t*)(vbuf + (used & 1) * vbytes);
         float* wb = wbuf + (used & 1) * CK * RG;
+        if (c == a0 || c % (TILE / CK) == 0) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) ro[k] = rq + k < rows ? rebase(rbuf[(used & 1) * RG + rq + k], rmax[rq + k]) : FAR;
+          for (int k = 0; k < 4; ++k) ro[k] = rq + k < rows ? rebase(rbuf[(used & 1) * RG + rq + k], rmax[rq + k]) : FAR;
+        }
         ++used;
-        // values to single precision, v / 2^16 over each low word.  Where they fit, y = v + VMAX is in
-        // [0, 2 VMAX]: the low bits of the float 2^23 + y, then exact: (that - 2^23 - VMAX) / 2^16
+        // values to single precision, v / 2^16, into the first half of each row: a warp holds
+        // a whole row meanwhile.  Where they fit, y = v + VMAX is in [0, 2 VMAX]: the low bits
+        // of the float 2^23 + y, then exact: (that - 2^23 - VMAX) / 2^16
         uint32_t high = 0, most = 0;
-#pragma unroll 4
-        for (int i = tid; i < keys * A.dh / 2; i += NT) {
-          longlong2* cell = (longlong2*)(vb + 2 * i);
-          const longlong2 v = *cell;
-          const uint64_t y0 = (uint64_t)v.x + VMAX, y1 = (uint64_t)v.y + VMAX;
-          high |= (uint32_t)(y0 >> 32) | (uint32_t)(y1 >> 32);
-          most = max(most, max((uint32_t)y0, (uint32_t)y1));
-          const float c = -(float)(8388608 + VMAX) / 65536.0f;
-          *(float4*)cell = make_float4(__fmaf_rn(__uint_as_float(0x4B000000u + (uint32_t)y0), 1.0f / 65536.0f, c), 0.f,
-                                       __fmaf_rn(__uint_as_float(0x4B000000u + (uint32_t)y1), 1.0f / 65536.0f, c), 0.f);
+#pragma unroll 2
+        for (int k = w; k < keys; k += NT / 32) {
+          int64_t* row = vb + k * A.dh;
+          float2 f[DPL / 2];
+#pragma unroll
+          for (int h = 0; h < DPL / 2; ++h) {
+            const int e = 2 * ln + 64 * h;
+            const longlong2 v = e < A.dh ? *(const longlong2*)(row + e) : make_longlong2(0, 0);
+            const uint64_t y0 = (uint64_t)v.x + VMAX, y1 = (uint64_t)v.y + VMAX;
+            high |= (uint32_t)(y0 >> 32) | (uint32_t)(y1 >> 32);
+            most = max(most, max((uint32_t)y0, (uint32_t)y1));
+            const float c = -(float)(8388608 + VMAX) / 65536.0f;
+            f[h] = make_float2(__fmaf_rn(__uint_as_float(0x4B000000u + (uint32_t)y0), 1.0f / 65536.0f, c),
+                               __fmaf_rn(__uint_as_float(0x4B000000u + (uint32_t)y1), 1.0f / 65536.0f, c));
+          }
+          __syncwarp();
+#pragma unroll
+          for (int h = 0; h < DPL / 2; ++h)
+            if (2 * ln + 64 * h < A.dh) *(float2*)((float*)row + 2 * ln + 64 * h) = f[h];
         }
         // weights floor(e * ONE / sum), at most ONE, in place: the estimate e * (ONE / sum)
         // in single precision is within 1, the remainder decides (in 32 bits for sums below 2^30)
-#pragma unroll 4
-        for (int k = kq; k < CK; k += kq_step) {
-          float4* cell = (float4*)(wb + k * RG + rq);
-          const int4 sc = *(const int4*)cell;
-          const int xs[4] = {sc.x, sc.y, sc.z, sc.w};
-          float o[4];
+        float* wq = wb + rq;
+        if (!lng) {
+#pragma unroll 2
+          for (int k = kq; k < CK; k += kq_step) {
+            const int4 sc = *(const int4*)(wq + k * RG);
+            const float4 rc = *(const float4*)(rrcp + rq);
+            const uint4 de = *(const uint4*)(rden + rq);
+            const int xs[4] = {sc.x, sc.y, sc.z, sc.w};
+            const float rcp[4] = {rc.x, rc.y, rc.z, rc.w};
+            const uint32_t den[4] = {de.x, de.y, de.z, de.w};
+            float o[4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint32_t e = (uint32_t)exp32(xs[i] + ro[i], lut);
-            const float ef = __uint_as_float(0x4B000000u + e) - 8388608.0f;
-            const float qf = __fmaf_rd(ef, rcp[i], 8388608.0f);
-            const uint32_t q = __float_as_uint(qf) - 0x4B000000u;
-            int rem = (int)((e << 16) - q * den[i]);
-            bool up = rem >= (int)den[i];
-            if (lng) {
-              const int64_t r64 = (int64_t)(((uint64_t)e << 16) - (uint64_t)q * rsum[rq + i]);
-              rem = r64 < 0 ? -1 : 0;
-              up = r64 >= (int64_t)rsum[rq + i];
+            for (int i = 0; i < 4; ++i) {
+              const uint32_t e = (uint32_t)exp32(xs[i] + ro[i], lut);
+              const float qf = __fmaf_rd(__uint_as_float(0x4B000000u + e) - 8388608.0f, rcp[i], 8388608.0f);
+              const int rem = (int)((e << 16) - (__float_as_uint(qf) - 0x4B000000u) * den[i]);
+              o[i] = qf - (rem < 0 ? 8388609.0f : (rem >= (int)den[i] ? 8388607.0f : 8388608.0f));
             }
-            o[i] = qf - (rem < 0 ? 8388609.0f : (up ? 8388607.0f : 8388608.0f));
+            *(float4*)(wq + k * RG) = make_float4(o[0], o[1], o[2], o[3]);
           }
-          *cell = make_float4(o[0], o[1], o[2], o[3]);
+        } else {
+          for (int k = kq; k < CK; k += kq_step)
+            for (int i = 0; i < 4; ++i) {
+              const int64_t e = exp32(__float_as_int(wq[k * RG + i]) + ro[i], lut);
+              wq[k * RG + i] = (float)(int)(e * ONE / (int64_t)rsum[rq + i]);
+            }
         }
         const bool fit = __syncthreads_and(high == 0 && most <= 2 * VMAX);
         if (fit) {
-          const int64_t* vrow = vb + min(2 * ln, A.dh - 2);
-          const int second = min(64, A.dh - 2 - min(2 * ln, A.dh - 2));  // dims of the second pair, inside the row
-#pragma unroll 2
+          const float* vrow = (const float*)vb + min(ln * DPL, A.dh - DPL);
+          const float* wrow = wb + unit * UR;
+#pragma unroll 1
           for (int k = kpart; k < keys; k += kparts) {  // rows behind may hold anything
-            float wt[UR], v[DPL];
+            float wt[UR];
+            float v[DPL];
 #pragma unroll
-            for (int i = 0; i < UR; i += 4) *(float4*)(wt + i) = *(const float4*)(wb + k * RG + unit * UR + i);
-#pragma unroll
-            for (int d = 0; d < DPL; d += 2) {
-              const float4 p = *(const float4*)(vrow + k * A.dh + (d ? second : 0));
-              v[d] = p.x, v[d + 1] = p.z;
-            }
+            for (int i = 0; i < UR; i += 4) *(float4*)(wt + i) = *(const float4*)(wrow + k * RG + i);
+            if constexpr (DPL == 4) *(float4*)v = *(const float4*)(vrow + k * 2 * A.dh);
+            else *(float2*)v = *(const float2*)(vrow + k * 2 * A.dh);
 #pragma unroll
             for (int d = 0; d < DPL; ++d)
 #pragma unroll
@@ -769,7 +779,7 @@ __global__ void __launch_bounds__(NT_V, 2) k_values(const Args A) {
       for (int d = 0; d < DPL; ++d)
 #pragma unroll
         for (int i = 0; i < UR; ++i) {
-          int* o = osum + (unit * UR + i) * DHP + 2 * ln + (d & 1) + (d >> 1) * 64;
+          int* o = osum + (unit * UR + i) * DHP + ln * DPL + d;
           const int a = __float_as_int(acc[d][i]) - 0x4B400000;
           if (kparts == 1) *o = a;
           else atomicAdd(o, a);
