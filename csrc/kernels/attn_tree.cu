@@ -54,13 +54,12 @@ constexpr int RQ = 32;              // query rows per MMA group
 constexpr int PLANES = 4;           // digits that take the tensor path
 constexpr int NT_S = 256;           // k_scores threads
 constexpr int NT_V = 256;           // k_sums and k_values threads, at most
-constexpr int CK = 32;              // keys per k_values chunk: two pages
 constexpr int MAX_RG = 128;         // rows per k_values CTA
 constexpr int SMALL = 1 << 29;      // bound of scores stored as they are
 constexpr int FAR = -(1 << 30);     // a score whose exp is 0
 constexpr int64_t NONE = -(int64_t(1) << 62);  // max of no keys
 constexpr int VMAX = (1 << 22) - (1 << 17);    // values of the single-precision form
-constexpr int SMEM_V = 2 * (CK * (128 * 8 + MAX_RG * 4) + MAX_RG * 8);  // k_values shared memory, at most
+constexpr int SMEM_V = 2 * (32 * (128 * 8 + MAX_RG * 4) + MAX_RG * 8);  // k_values shared memory, at most
 constexpr int MAX_RANGE = 1 << 16;             // keys per k_values CTA: VMAX + MAX_RANGE < 2^22
 
 struct Args {
@@ -554,7 +553,7 @@ __device__ __forceinline__ int store_limbs4(int8_t* X, int slot, int B, size_t l
 // copies, one chunk ahead.  A warp takes UR rows (unit) x all dims, a lane
 // the dims 2 ln, 2 ln + 1 (and 64 + those); kparts warps per unit take every
 // kparts-th key.
-template <int DPL, int UR>
+template <int DPL, int UR, int CK>
 __global__ void __launch_bounds__(NT_V, 2) k_values(const Args A) {
   extern __shared__ __align__(1024) uint8_t dsm[];
   constexpr int DHP = 32 * DPL;
@@ -844,7 +843,7 @@ __global__ void __launch_bounds__(NT_V, 2) k_values(const Args A) {
 
 // Sizes that follow from the shapes; `lanes` of them per launch.
 struct Plan {
-  int lanes, R, Rp, G, tiles, chunks, groups, RG, splits, threads, unit, rows_s, qgroups;
+  int lanes, R, Rp, G, tiles, chunks, groups, RG, splits, threads, unit, rows_s, qgroups, per_sm;
   size_t oS, oQ, oI, oR, oG, oSum, oW, oAcc, oA, oB, oF, bytes;
 };
 
@@ -863,16 +862,20 @@ static Plan plan(int lanes, int nq, int n_heads, int n_kv, int dh, int t_lim) {
   p.lanes = (int)(WS_TARGET / per_s);
   p.lanes = p.lanes < 1 ? 1 : (p.lanes > lanes ? lanes : p.lanes);
   const int have = p.lanes * n_kv * p.groups;
-  // the lanes' keys are divided evenly over two CTAs per SM in all; a CTA's
-  // part of a lane stays below MAX_RANGE keys
-  p.splits = 2 * 148 / (n_kv * p.groups);
-  if (p.splits < 1) p.splits = 1;
-  const int64_t least = ((int64_t)p.lanes * p.tiles * TILE + MAX_RANGE - 1) / (MAX_RANGE - CK);
-  if (p.splits < least) p.splits = (int)least;
-  p.chunks = (4 * 148 + have - 1) / have;
-  if (p.chunks > p.tiles) p.chunks = p.tiles;
   const int units = p.RG / p.unit;
   p.threads = 32 * units * (units >= 5 ? 1 : (units >= 3 ? 2 : (units == 2 ? 4 : 8)));
+  // five-warp value CTAs run three to an SM with chunks of one page (9 nodes, 8 query
+  // heads per KV head, 30 thousand keys: 281 us against 322 with two and two pages); the
+  // others two, with two pages (64 nodes: 207 us, 240 with one page)
+  p.per_sm = p.threads == 160 ? 3 : 2;
+  // the lanes' keys are divided evenly over the CTAs that run at once; a CTA's
+  // part of a lane stays below MAX_RANGE keys
+  p.splits = p.per_sm * 148 / (n_kv * p.groups);
+  if (p.splits < 1) p.splits = 1;
+  const int64_t least = ((int64_t)p.lanes * p.tiles * TILE + MAX_RANGE - 1) / (MAX_RANGE - 32);
+  if (p.splits < least) p.splits = (int)least;
+  p.chunks = (12 * 148 + have - 1) / have;  // of the sums: short ones, many loads in flight
+  if (p.chunks > p.tiles) p.chunks = p.tiles;
   // score CTAs take all rows of their tile unless that leaves SMs idle (two CTAs each)
   const int blocks = p.tiles * n_kv * p.lanes, want = (4 * 148 + blocks - 1) / blocks, most = (p.R + 63) / 64;
   p.rows_s = ((p.R + (want < most ? want : most) - 1) / (want < most ? want : most) + RQ - 1) / RQ * RQ;
@@ -900,11 +903,11 @@ static Plan plan(int lanes, int nq, int n_heads, int n_kv, int dh, int t_lim) {
   return p;
 }
 
-template <int DHP, int UR>
+template <int DHP, int UR, int CK>
 static int run(Args A, const Plan& p, int lanes, cudaStream_t st) {
   constexpr int smem_s = 1024 + PLANES * (TILE + 2 * RQ) * 128;
   const int vals = 2 * (CK * (A.dh * 8 + p.RG * 4) + p.RG * 8), sums = p.RG * DHP * 4, smem_v = vals > sums ? vals : sums;
-  const auto kv = k_values<DHP / 32, UR>;
+  const auto kv = k_values<DHP / 32, UR, CK>;
   static std::atomic<uint64_t> ready{0};  // the kernels' attributes are set, a bit per device
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
@@ -960,8 +963,9 @@ int arcb_attn_tree(const int64_t* q, const int64_t* Kc, const int64_t* Vc, int n
   A.arrived = (int*)(b + p.oA), A.bad = (int*)(b + p.oB), A.is_wide = (int*)(b + p.oF);
   A.X = X, A.lmax = lmax, A.o_out = o_out, A.err = err;
   cudaStream_t st = (cudaStream_t)stream;
-  if (p.unit == 8) return dh <= 64 ? at::run<64, 8>(A, p, lanes, st) : at::run<128, 8>(A, p, lanes, st);
-  return dh <= 64 ? at::run<64, 16>(A, p, lanes, st) : at::run<128, 16>(A, p, lanes, st);
+  if (p.unit == 8) return dh <= 64 ? at::run<64, 8, 32>(A, p, lanes, st) : at::run<128, 8, 32>(A, p, lanes, st);
+  if (p.per_sm == 3) return dh <= 64 ? at::run<64, 16, 16>(A, p, lanes, st) : at::run<128, 16, 16>(A, p, lanes, st);
+  return dh <= 64 ? at::run<64, 16, 32>(A, p, lanes, st) : at::run<128, 16, 32>(A, p, lanes, st);
 }
 
 }  // extern "C"
