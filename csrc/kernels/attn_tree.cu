@@ -14,7 +14,8 @@
 //
 // The queries of a KV head (nq nodes x G query heads: R rows) share its K and
 // V.  Exact weights need the global max and sum before the first value, so
-// there are four kernels:
+// there are four kernels (for few rows and keys, two: k_scores makes the query
+// digits itself, and each value CTA the maxima and sums of its lane's rows):
 //
 //  0. k_queries: the query rows' digits (see 1) in groups of 32 rows.
 //  1. k_scores, one CTA per 128 keys.  K's int64 elements become signed
@@ -60,6 +61,11 @@ constexpr int FAR = -(1 << 30);     // a score whose exp is 0
 constexpr int64_t NONE = -(int64_t(1) << 62);  // max of no keys
 constexpr int VMAX = (1 << 22) - (1 << 17);    // values of the single-precision form
 constexpr int SMEM_V = 2 * (32 * (128 * 8 + MAX_RG * 4) + MAX_RG * 8);  // k_values shared memory, at most
+// Lanes * rows * keys up to which two kernels do the work of four (FEW).  Measured, two against
+// four: 32 heads of 128, one lane, 16 rows, 250 keys 40 / 43 us, 506 keys 47 / 52, 1018 keys
+// 64 / 63; 31 rows of 506 keys 55 / 55; 4 lanes, 16 rows, 250 keys 68 / 67; 8 lanes, 31 rows, 500
+// keys 142 / 131; 64 heads over 8, one lane, 4 nodes, 250 keys 41 / 42, 506 keys 47 / 43.
+constexpr int FEW_MOST = 1 << 13;
 constexpr int MAX_RANGE = 1 << 16;             // keys per k_values CTA: VMAX + MAX_RANGE < 2^22
 
 struct Args {
@@ -76,6 +82,7 @@ struct Args {
   // workspace
   int* S;              // [lanes][n_kv][tiles][groups][TILE][RG] scores less ref
   int64_t* ref;        // [lanes][n_kv][tiles][Rp]: 0, or the tile's max where scores are not small
+  int64_t* M;          // [lanes][n_kv][tiles][Rp]: the tile's max (FEW)
   uint8_t* planes;     // [lanes][n_kv][qgroups][PLANES][RQ][128] query digits, swizzled
   uint4* qinfo;        // [lanes][n_kv][qgroups] ors of low and high digit words, largest magnitude
   int64_t* wide;       // [n_kv][groups][splits + lanes][RG][dh]: 64-bit terms of a segment
@@ -134,45 +141,22 @@ __device__ __forceinline__ void load4(int64_t* x, const int64_t* src) {
 }
 
 // ----------------------------------------------------------------- 0. queries
-// grid (qgroups, n_kv, lanes): the digit planes of RQ query rows in the layout
-// that k_scores copies, and the start values of what the next kernels add to.
+// Digit planes of query rows r0 .. r0 + RQ - 1 into out, and into info (zero
+// before) the ors of their low and high digit words and the largest magnitude.
+// All NT_S threads call it.
 template <int DHP>
-__global__ void __launch_bounds__(NT_S) k_queries(const Args A) {
+__device__ __forceinline__ void query_planes(const Args& A, int lane, int kvh, int r0, uint8_t* out, uint32_t* info) {
   constexpr int TPR = DHP / 4, QN = RQ * TPR / NT_S;
-  __shared__ uint32_t info[3];
-  const int tid = threadIdx.x, ln = tid & 31;
-  const int g = blockIdx.x, kvh = blockIdx.y, lane = A.lane0 + blockIdx.z;
-  const size_t lk = (size_t)blockIdx.z * A.n_kv + kvh;
-  if (tid < 3) info[tid] = 0;
-  __syncthreads();
-  pdl_wait_dep();
-  pdl_allow_next();
-  const int col = (tid % TPR) * 4;
+  const int tid = threadIdx.x, col = (tid % TPR) * 4;
   int64_t x[QN][4];
 #pragma unroll
   for (int i = 0; i < QN; ++i) {
-    const int rr = g * RQ + tid / TPR + i * (NT_S / TPR);
+    const int rr = r0 + tid / TPR + i * (NT_S / TPR);
     if (rr < A.R && col < A.dh)
       load4(x[i], A.q + ((size_t)(lane * A.nq + rr / A.G) * A.n_heads + kvh * A.G + rr % A.G) * A.dh + col);
     else
       x[i][0] = x[i][1] = x[i][2] = x[i][3] = 0;
   }
-  {
-    ulonglong2* z = (ulonglong2*)(A.acc + lk * A.groups * A.RG * (A.dh / 2));
-    for (int i = g * NT_S + tid; i < A.groups * A.RG * (A.dh / 4); i += A.qgroups * NT_S) z[i] = make_ulonglong2(0, 0);
-    for (int i = g * NT_S + tid; i < A.Rp; i += A.qgroups * NT_S) {
-      A.sums[lk * A.Rp + i] = 0;
-      A.gmax[lk * A.Rp + i] = NONE;
-    }
-    if (g == 0) {
-      for (int i = tid; i < A.groups; i += NT_S) A.arrived[lk * A.groups + i] = 0;
-      if (kvh == 0 && tid == 0) A.bad[blockIdx.z] = 0;
-      if (blockIdx.z == 0)
-        for (int i = tid; i < A.groups * (A.splits + A.lanes); i += NT_S)
-          A.is_wide[(size_t)kvh * A.groups * (A.splits + A.lanes) + i] = 0;
-    }
-  }
-  uint8_t* out = A.planes + (lk * A.qgroups + g) * (PLANES * RQ * 128);
   uint32_t lo = 0, hi = 0, mag = 0;
 #pragma unroll
   for (int i = 0; i < QN; ++i) {
@@ -187,13 +171,48 @@ __global__ void __launch_bounds__(NT_S) k_queries(const Args A) {
   lo = __reduce_or_sync(0xffffffffu, lo);
   hi = __reduce_or_sync(0xffffffffu, hi);
   mag = __reduce_max_sync(0xffffffffu, mag);
-  if (ln == 0) {
+  if ((tid & 31) == 0) {
     atomicOr(&info[0], lo);
     atomicOr(&info[1], hi);
     atomicMax(&info[2], mag);
   }
+}
+
+// Start values of what the later kernels add to, for lane z of the launch and
+// KV head kvh; CTA i of n writes its part.
+__device__ __forceinline__ void start_values(const Args& A, int z, int kvh, int i, int n) {
+  const int tid = threadIdx.x;
+  const size_t lk = (size_t)z * A.n_kv + kvh;
+  ulonglong2* acc = (ulonglong2*)(A.acc + lk * A.groups * A.RG * (A.dh / 2));
+  for (int k = i * NT_S + tid; k < A.groups * A.RG * (A.dh / 4); k += n * NT_S) acc[k] = make_ulonglong2(0, 0);
+  for (int k = i * NT_S + tid; k < A.Rp; k += n * NT_S) {
+    A.sums[lk * A.Rp + k] = 0;
+    A.gmax[lk * A.Rp + k] = NONE;
+  }
+  if (i == 0) {
+    for (int k = tid; k < A.groups; k += NT_S) A.arrived[lk * A.groups + k] = 0;
+    if (kvh == 0 && tid == 0) A.bad[z] = 0;
+    if (z == 0)
+      for (int k = tid; k < A.groups * (A.splits + A.lanes); k += NT_S)
+        A.is_wide[(size_t)kvh * A.groups * (A.splits + A.lanes) + k] = 0;
+  }
+}
+
+// grid (qgroups, n_kv, lanes): query digits in the layout that k_scores
+// copies, and the start values.
+template <int DHP>
+__global__ void __launch_bounds__(NT_S) k_queries(const __grid_constant__ Args A) {
+  __shared__ uint32_t info[3];
+  const int tid = threadIdx.x, g = blockIdx.x, kvh = blockIdx.y;
+  const size_t at = ((size_t)blockIdx.z * A.n_kv + kvh) * A.qgroups + g;
+  if (tid < 3) info[tid] = 0;
   __syncthreads();
-  if (tid == 0) A.qinfo[lk * A.qgroups + g] = make_uint4(info[0], info[1], info[2], 0);
+  pdl_wait_dep();
+  pdl_allow_next();
+  start_values(A, blockIdx.z, kvh, g, A.qgroups);
+  query_planes<DHP>(A, A.lane0 + blockIdx.z, kvh, g * RQ, A.planes + at * (PLANES * RQ * 128), info);
+  __syncthreads();
+  if (tid == 0) A.qinfo[at] = make_uint4(info[0], info[1], info[2], 0);
 }
 
 // ------------------------------------------------------------------ 1. scores
@@ -205,8 +224,10 @@ __device__ __forceinline__ void bulk_g2s(uint32_t dst, const void* src, uint32_t
 
 // grid (tiles, n_kv * row blocks of rows_s, lanes).
 // DHP: row pitch class of the planes (64 or 128 >= dh).
-template <int DHP>
-__global__ void __launch_bounds__(NT_S, 2) k_scores(const Args A) {
+// FEW: at most RQ rows, whose digits each CTA makes itself; the tiles' maxima
+// are stored for k_values, which does k_sums' work too: two launches.
+template <int DHP, bool FEW>
+__global__ void __launch_bounds__(NT_S, 2) k_scores(const __grid_constant__ Args A) {
   constexpr int KP = TILE * 128, QP = RQ * 128;  // bytes per plane
   constexpr int TPR = DHP / 4;                   // threads per row
   constexpr int TMEM_COLS = 256;                 // (2 * PLANES - 1) * RQ = 224 used
@@ -214,7 +235,7 @@ __global__ void __launch_bounds__(NT_S, 2) k_scores(const Args A) {
   __shared__ int64_t wmax[2][4][RQ];
   __shared__ uint64_t qmask[2][RQ];
   __shared__ int pages[TILE / PAGE];
-  __shared__ uint32_t or_k[3];  // ors of the keys' low and high digit words, largest magnitude
+  __shared__ uint32_t or_k[3], or_q[3];  // ors of the keys' (queries') low and high digit words, largest magnitude
   __shared__ uint32_t tslot;
   __shared__ __align__(8) uint64_t done, qfull[2];
   __shared__ int s_abort;
@@ -236,7 +257,7 @@ __global__ void __launch_bounds__(NT_S, 2) k_scores(const Args A) {
     fence_barrier_init();
     s_abort = 0;
   }
-  if (tid < 3) or_k[tid] = 0;
+  if (tid < 3) or_k[tid] = or_q[tid] = 0;
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -258,9 +279,11 @@ __global__ void __launch_bounds__(NT_S, 2) k_scores(const Args A) {
     mbar_arrive_expect_tx(bar, PLANES * QP);
     bulk_g2s(qbase + b * PLANES * QP, A.planes + (lk * A.qgroups + r0 / RQ) * (PLANES * QP), PLANES * QP, bar);
   };
-  if (live && tid == 0) load_q(r_lo, 0);
+  if constexpr (FEW) start_values(A, blockIdx.z, kvh, tile, gridDim.x);
+  if (!FEW && live && tid == 0) load_q(r_lo, 0);
   __syncthreads();
   if (live) {
+    if constexpr (FEW) query_planes<DHP>(A, lane, kvh, 0, kp + PLANES * KP, or_q);
     const int col = (ln % TPR) * 4;
     // ---- K digit planes: a warp reads 32 / TPR whole rows at a time
     constexpr int RPW = 32 / TPR, STEPS = TILE / (8 * RPW), UN = STEPS < 8 ? STEPS : 8;
@@ -307,7 +330,7 @@ __global__ void __launch_bounds__(NT_S, 2) k_scores(const Args A) {
     const uint64_t small_lim = (uint64_t(1) << 47) / A.dh;
     const uint64_t kd = sw128_kmajor_desc(kbase), qd0 = sw128_kmajor_desc(qbase);  // start addresses count in 16 bytes
     const uint4* qinfo = A.qinfo + lk * A.qgroups + r_lo / RQ;
-    uint4 q_next = __ldg(qinfo);
+    uint4 q_next = FEW ? make_uint4(or_q[0], or_q[1], or_q[2], 0) : __ldg(qinfo);
     for (int r0 = r_lo, n = 0; r0 < r_hi; r0 += RQ, ++n) {
       const int rows = min(RQ, r_hi - r0), b = n & 1;
       const uint4 qi = q_next;
@@ -323,7 +346,7 @@ __global__ void __launch_bounds__(NT_S, 2) k_scores(const Args A) {
       if (tid == 0) {
         // the other buffer's products are done (waited for by all before the last barrier)
         if (r0 + RQ < r_hi) load_q(r0 + RQ, b ^ 1);
-        if (!mbar_wait(smem_u32(&qfull[b]), (n >> 1) & 1)) s_abort = 1;
+        if (!FEW && !mbar_wait(smem_u32(&qfull[b]), (n >> 1) & 1)) s_abort = 1;
         if (!wide) {
           // K_a times the stacked planes Q_0 | Q_1 | ..: plane b lands in accumulator a + b.
           // At k = 0 the accumulator that a reaches first is overwritten, by a product of its own.
@@ -463,7 +486,8 @@ __global__ void __launch_bounds__(NT_S, 2) k_scores(const Args A) {
 #pragma unroll
         for (int k = 1; k < 4; ++k) m = wmax[b][k][tid] > m ? wmax[b][k][tid] : m;
         A.ref[(lk * A.tiles + tile) * A.Rp + r0 + tid] = small ? 0 : m;
-        if (m != NONE) atomicMax((long long*)A.gmax + lk * A.Rp + r0 + tid, (long long)m);
+        if (FEW) A.M[(lk * A.tiles + tile) * A.Rp + r0 + tid] = m;
+        else if (m != NONE) atomicMax((long long*)A.gmax + lk * A.Rp + r0 + tid, (long long)m);
       }
     }
   }
@@ -479,7 +503,7 @@ __global__ void __launch_bounds__(NT_S, 2) k_scores(const Args A) {
 // -------------------------------------------------------------------- 2. sums
 // grid (chunks, n_kv * groups, lanes): a thread takes four rows of every
 // (threads / (RG / 4))-th key.
-__global__ void __launch_bounds__(NT_V) k_sums(const Args A) {
+__global__ void __launch_bounds__(NT_V) k_sums(const __grid_constant__ Args A) {
   __shared__ int2 lut[EXP_LUT_N];
   __shared__ int64_t rmax[MAX_RG];
   __shared__ unsigned long long rsum[MAX_RG];
@@ -553,8 +577,10 @@ __device__ __forceinline__ int store_limbs4(int8_t* X, int slot, int B, size_t l
 // copies, one chunk ahead.  A warp takes UR rows (unit) x all dims, a lane
 // the dims 2 ln, 2 ln + 1 (and 64 + those); kparts warps per unit take every
 // kparts-th key.
-template <int DPL, int UR, int CK>
-__global__ void __launch_bounds__(NT_V, 2) k_values(const Args A) {
+// FEW: at most RQ rows (one group) of few keys; each segment finds its rows'
+// maxima and sums from all scores of the lane.
+template <int DPL, int UR, int CK, bool FEW>
+__global__ void __launch_bounds__(NT_V, 2) k_values(const __grid_constant__ Args A) {
   extern __shared__ __align__(1024) uint8_t dsm[];
   constexpr int DHP = 32 * DPL;
   __shared__ int2 lut[EXP_LUT_N];
@@ -618,10 +644,43 @@ __global__ void __launch_bounds__(NT_V, 2) k_values(const Args A) {
       atomicOr(A.bad + bz, 1);
     }
     const bool live = T > 0 && !bad;
+    if (FEW && live) {
+      const int nt = (T + TILE - 1) / TILE;
+      if (tid < RG) {
+        int64_t m = NONE;
+        if (tid < rows)
+#pragma unroll 4
+          for (int t = 0; t < nt; ++t) m = max(m, A.M[(lk * A.tiles + t) * A.Rp + tid]);
+        rmax[tid] = m;
+        rsum[tid] = 0;
+      }
+      __syncthreads();
+      uint64_t s[4] = {0, 0, 0, 0};
+      for (int t = 0; t < nt; ++t) {
+        const int64_t* ref = A.ref + (lk * A.tiles + t) * A.Rp + rq;
+        const int* S = A.S + (lk * A.tiles + t) * (size_t)TILE * RG + rq;
+        int off4[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) off4[c] = rq + c < rows ? rebase(ref[c], rmax[rq + c]) : FAR;
+        const int k1 = min(TILE, T - t * TILE);  // keys behind are as far as unseen ones
+#pragma unroll 4
+        for (int k = kq; k < k1; k += kq_step) {
+          const int4 v = *(const int4*)(S + k * RG);
+          s[0] += exp32(v.x + off4[0], lut);
+          s[1] += exp32(v.y + off4[1], lut);
+          s[2] += exp32(v.z + off4[2], lut);
+          s[3] += exp32(v.w + off4[3], lut);
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        if (rq + c < rows) atomicAdd((unsigned long long*)&rsum[rq + c], (unsigned long long)s[c]);
+      __syncthreads();
+    }
     if (live && tid < RG) {
       const bool row = tid < rows;
-      const uint64_t s = row ? A.sums[lk * A.Rp + r0 + tid] : 0;
-      rmax[tid] = row ? A.gmax[lk * A.Rp + r0 + tid] : NONE;
+      const uint64_t s = FEW ? rsum[tid] : (row ? A.sums[lk * A.Rp + r0 + tid] : 0);
+      if (!FEW) rmax[tid] = row ? A.gmax[lk * A.Rp + r0 + tid] : NONE;
       rsum[tid] = s ? s : 1;  // a row without keys: every exp is 0
       rden[tid] = (uint32_t)rsum[tid];
       rrcp[tid] = 65536.0f * __frcp_rn((float)(int64_t)rsum[tid]);
@@ -844,7 +903,8 @@ __global__ void __launch_bounds__(NT_V, 2) k_values(const Args A) {
 // Sizes that follow from the shapes; `lanes` of them per launch.
 struct Plan {
   int lanes, R, Rp, G, tiles, chunks, groups, RG, splits, threads, unit, rows_s, qgroups, per_sm;
-  size_t oS, oQ, oI, oR, oG, oSum, oW, oAcc, oA, oB, oF, bytes;
+  bool few;
+  size_t oS, oQ, oI, oR, oM, oG, oSum, oW, oAcc, oA, oB, oF, bytes;
 };
 
 constexpr size_t WS_TARGET = size_t(1) << 30;  // lanes are batched to about this much workspace
@@ -891,6 +951,8 @@ static Plan plan(int lanes, int nq, int n_heads, int n_kv, int dh, int t_lim) {
   p.oQ = take(lk * p.qgroups * PLANES * RQ * 128);
   p.oI = take(lk * p.qgroups * sizeof(uint4));
   p.oR = take(lk * p.tiles * p.Rp * 8);
+  p.few = p.R <= RQ && (int64_t)lanes * p.RG * t_lim <= FEW_MOST;
+  p.oM = take(p.few ? lk * p.tiles * p.Rp * 8 : 0);
   p.oG = take(lk * p.Rp * 8);
   p.oSum = take(lk * p.Rp * 8);
   const size_t slots = (size_t)n_kv * p.groups * (p.splits + p.lanes);
@@ -903,16 +965,17 @@ static Plan plan(int lanes, int nq, int n_heads, int n_kv, int dh, int t_lim) {
   return p;
 }
 
-template <int DHP, int UR, int CK>
+template <int DHP, int UR, int CK, bool FEW>
 static int run(Args A, const Plan& p, int lanes, cudaStream_t st) {
   constexpr int smem_s = 1024 + PLANES * (TILE + 2 * RQ) * 128;
   const int vals = 2 * (CK * (A.dh * 8 + p.RG * 4) + p.RG * 8), sums = p.RG * DHP * 4, smem_v = vals > sums ? vals : sums;
-  const auto kv = k_values<DHP / 32, UR, CK>;
+  const auto ks = k_scores<DHP, FEW>;
+  const auto kv = k_values<DHP / 32, UR, CK, FEW>;
   static std::atomic<uint64_t> ready{0};  // the kernels' attributes are set, a bit per device
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e == cudaSuccess && !(ready.load() >> (dev & 63) & 1)) {
-    e = cudaFuncSetAttribute(k_scores<DHP>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_s);
+    e = cudaFuncSetAttribute(ks, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_s);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(kv, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_V);
     if (e == cudaSuccess && dev < 64) ready.fetch_or(uint64_t(1) << dev);
   }
@@ -920,15 +983,20 @@ static int run(Args A, const Plan& p, int lanes, cudaStream_t st) {
   for (int l0 = 0; l0 < lanes; l0 += p.lanes) {
     const int n = lanes - l0 < p.lanes ? lanes - l0 : p.lanes;
     A.lane0 = l0, A.lanes = n;
-    int rc = launch_k(k_queries<DHP>, dim3(p.qgroups, A.n_kv, n), dim3(NT_S), 0, st, A);
-    if (!rc)
-      rc = launch_k(k_scores<DHP>, dim3(p.tiles, A.n_kv * ((p.R + p.rows_s - 1) / p.rows_s), n), dim3(NT_S), smem_s,
-                      st, A);
-    if (!rc) rc = launch_k(k_sums, dim3(p.chunks, A.n_kv * p.groups, n), dim3(p.threads), 0, st, A);
+    int rc = FEW ? 0 : launch_k(k_queries<DHP>, dim3(p.qgroups, A.n_kv, n), dim3(NT_S), 0, st, A);
+    if (!rc) rc = launch_k(ks, dim3(p.tiles, A.n_kv * ((p.R + p.rows_s - 1) / p.rows_s), n), dim3(NT_S), smem_s, st, A);
+    if (!rc && !FEW) rc = launch_k(k_sums, dim3(p.chunks, A.n_kv * p.groups, n), dim3(p.threads), 0, st, A);
     if (!rc) rc = launch_k(kv, dim3(p.splits, A.n_kv * p.groups), dim3(p.threads), smem_v, st, A);
     if (rc) return rc;
   }
   return 0;
+}
+
+template <int DHP>
+static int run_dh(const Args& A, const Plan& p, int lanes, cudaStream_t st) {
+  if (p.unit == 8) return p.few ? run<DHP, 8, 32, true>(A, p, lanes, st) : run<DHP, 8, 32, false>(A, p, lanes, st);
+  if (p.few) return run<DHP, 16, 32, true>(A, p, lanes, st);
+  return p.per_sm == 3 ? run<DHP, 16, 16, false>(A, p, lanes, st) : run<DHP, 16, 32, false>(A, p, lanes, st);
 }
 
 }  // namespace at
@@ -958,14 +1026,14 @@ int arcb_attn_tree(const int64_t* q, const int64_t* Kc, const int64_t* Vc, int n
   A.B = lanes * nq;
   A.R = p.R, A.Rp = p.Rp, A.G = p.G, A.tiles = p.tiles, A.chunks = p.chunks, A.groups = p.groups, A.RG = p.RG;
   A.splits = p.splits, A.rows_s = p.rows_s, A.qgroups = p.qgroups;
-  A.S = (int*)(b + p.oS), A.planes = b + p.oQ, A.qinfo = (uint4*)(b + p.oI), A.ref = (int64_t*)(b + p.oR), A.gmax = (int64_t*)(b + p.oG);
+  A.S = (int*)(b + p.oS), A.planes = b + p.oQ, A.qinfo = (uint4*)(b + p.oI), A.ref = (int64_t*)(b + p.oR);
+  A.M = (int64_t*)(b + p.oM), A.gmax = (int64_t*)(b + p.oG);
   A.sums = (uint64_t*)(b + p.oSum), A.wide = (int64_t*)(b + p.oW), A.acc = (uint64_t*)(b + p.oAcc);
   A.arrived = (int*)(b + p.oA), A.bad = (int*)(b + p.oB), A.is_wide = (int*)(b + p.oF);
   A.X = X, A.lmax = lmax, A.o_out = o_out, A.err = err;
   cudaStream_t st = (cudaStream_t)stream;
-  if (p.unit == 8) return dh <= 64 ? at::run<64, 8, 32>(A, p, lanes, st) : at::run<128, 8, 32>(A, p, lanes, st);
-  if (p.per_sm == 3) return dh <= 64 ? at::run<64, 16, 16>(A, p, lanes, st) : at::run<128, 16, 16>(A, p, lanes, st);
-  return dh <= 64 ? at::run<64, 16, 32>(A, p, lanes, st) : at::run<128, 16, 32>(A, p, lanes, st);
+  if (dh <= 64) return at::run_dh<64>(A, p, lanes, st);
+  return at::run_dh<128>(A, p, lanes, st);
 }
 
 }  // extern "C"
