@@ -229,6 +229,72 @@ def test_attn_tree_calls_on_two_streams_at_once():
         np.testing.assert_array_equal(o.cpu().numpy(), x.want())
 
 
+@pytest.mark.parametrize("dh,heads,kv,lens,nodes,nq", [
+    (64, 2, 1, [40], [4], 4),            # 8 rows
+    (128, 8, 1, [250], [4], 4),          # 32 rows of 254 keys: 8128, the most that two kernels take
+    (128, 8, 1, [252], [5], 4),          # 32 rows of 257 keys
+    (128, 11, 1, [40], [3], 3),          # 33 rows
+    (128, 8, 2, [60, 3], [8, 8], 8),     # 32 rows, two lanes
+    (128, 5, 1, [300], [13], 13),        # 65 rows: value CTAs of five warps
+    (128, 8, 1, [300], [10], 10),        # 80 rows
+    (64, 8, 1, [90, 500, 1], [9, 9, 9], 9),
+    (128, 3, 1, [131], [27], 27),        # 81 rows
+    (128, 8, 1, [131], [17], 17),        # 136 rows: two groups
+], ids=str)
+def test_attn_tree_row_counts(dh, heads, kv, lens, nodes, nq):
+    """Row counts around the variants' borders; the keys' limit decides one of
+    them and must not change a result."""
+    a = Attn(dh, heads, kv, lens, nodes, nq, 2, M18, M18)
+    want = a.want()
+    a.pt = np.concatenate([a.pt, np.full((a.lanes, 700), -1, np.int32)], 1)  # pages behind the last key are not read
+    for t_lim in (a.t_lim, 2100, 9000):
+        got, err = a.run(t_lim=t_lim)
+        assert err == 0
+        np.testing.assert_array_equal(got.cpu().numpy(), want)
+
+
+@pytest.mark.parametrize("kind", ["wide values", "wide keys", "empty", "bad"])
+def test_attn_tree_few_keys(kind):
+    """Two lanes of few rows and keys: the other kinds of values, keys and lanes."""
+    a = Attn(64, 4, 2, [100, 17], [9, 5], 5, 2, (1 << 63) - 1 if kind == "wide keys" else M18,
+             1 << 62 if kind == "wide values" else M18, seed=3)
+    if kind == "empty":
+        a.base[1] = a.nodes[1] = 0
+        a.mask[2] = 0
+        a.base[0] = 0
+    want = a.want()
+    if kind == "bad":
+        a.pt[1, 0] = -2
+        want[5:] = 0
+    for _ in range(2):
+        got, err = a.run()
+        assert err == (ERR_BOUNDS if kind == "bad" else 0)
+        np.testing.assert_array_equal(got.cpu().numpy(), want)
+
+
+def test_attn_tree_sums_beyond_32_bits():
+    """Equal scores: every exp is ONE, and from 2^14 keys a row's sum passes
+    2^30, from 2^16 keys 2^32; the weights of the longer one are all 0."""
+    for n, vmag in ((16500, M18), (40000, 1 << 30), (65600, M18)):
+        a = Attn(64, 3, 1, [n], [3], 3, 2, M18, vmag)
+        a.q[:] = 0
+        want = a.want()
+        got, err = a.run()
+        assert err == 0 and (n > 65536) == (not want.any())
+        np.testing.assert_array_equal(got.cpu().numpy(), want)
+
+
+def test_attn_tree_lanes_in_several_launches():
+    """Scores of more keys and rows than one launch's workspace holds: the
+    lanes go in batches."""
+    a = Attn(8, 64, 8, [50, 0, 17, 130, 16, 3, 64], [64, 2, 64, 40, 1, 64, 0], 64, 3, M18, M18)
+    want = a.want()
+    a.pt = np.concatenate([a.pt, np.zeros((a.lanes, 1300), np.int32)], 1)
+    got, err = a.run(t_lim=20000)
+    assert err == 0
+    np.testing.assert_array_equal(got.cpu().numpy(), want)
+
+
 def test_attn_tree_equals_decode_attention():
     """Chain queries equal the decode kernel at consecutive positions."""
     from arc_chain_b200.ops import int_ops
@@ -308,7 +374,7 @@ class Rows:
     (3, 9, 2, dict(fan=8)),
     (1, 3, 102400, dict(fan=2)),
     (1, 2, 152064, dict(fan=1)),                                           # 16 CTAs per row
-    (1, 2, 272896, dict(fan=1)),                                           # the largest vocabulary
+    (1, 2, 272896, dict(fan=1)),                                           # more shared memory per CTA
 ])
 def test_verify_tree(lanes, n, V, kw):
     for seed in range(3 if V < 50000 else 1):
@@ -332,6 +398,73 @@ def test_verify_tree_ragged_strange_and_masked():
     r.count[:] = [64, 64, 14, 64, 64, 64]
     n_path = r.check()
     assert n_path[0] == 0 and n_path[5] == 0
+
+
+def test_verify_tree_one_lane_equals_its_place_in_a_batch():
+    """A small call gives every node its cluster, a larger one every lane: the
+    same drafts are kept either way."""
+    from arc_chain_b200.ops import tree_ops as ops
+
+    for V, near, inv in ((901, 0.4, 65536), (5000, 1.0, 90000), (64, 0.5, 0)):
+        r = Rows(8, 13, V, fan=3, seed=11, near=near, inv=(inv,), dinv=(inv,))
+        r.n_tree[:] = [13, 12, 1, 2, 13, 0, 40, 13]
+        r.parent[4] = [-1, 0, 0, 7, 1, 4, 4, 3, 0, 8, 8, -2, 13]
+        r.logits[13 * 7:, 1::2] = np.iinfo(np.int64).min
+        r.check()
+        path, n_path, nxt = r.verify()
+        for b in range(8):
+            z = lambda *s: torch.full(s, 9, dtype=I32, device="cuda")
+            p, k, t = z(1, 13), z(1), z(1)
+            ops.verify_tree(dev(r.logits[13 * b:][:13]), dev(r.dlogits[13 * b:][:13]), V, 1, 13, dev(r.tokens[b:b + 1]),
+                            dev(r.parent[b:b + 1]), dev(r.n_tree[b:b + 1]), dev(r.inv[b:b + 1]), dev(r.dinv[b:b + 1]),
+                            dev(r.u[b:b + 1]), dev(r.hist[b:b + 1]), dev(r.count[b:b + 1]), p, k, t)
+            assert p[0].tolist() == list(path[b]) and int(k) == n_path[b] and int(t) == nxt[b], (V, b)
+
+
+def test_verify_and_draw_in_a_graph_and_on_two_streams():
+    from arc_chain_b200.ops import tree_ops as ops
+
+    rs = [Rows(1, 5, 2000, fan=2, seed=s) for s in range(2)] + [Rows(6, 9, 700, fan=2, seed=9)]
+    want = [r.verify() for r in rs]
+    ins = [[dev(x) for x in (r.logits, r.dlogits, r.tokens, r.parent, r.n_tree, r.inv, r.dinv, r.u, r.hist, r.count)]
+           for r in rs]
+    outs = [[torch.zeros(s, dtype=I32, device="cuda") for s in ((r.lanes, r.n), (r.lanes,), (r.lanes,))] for r in rs]
+
+    def call(r, i, o):
+        ops.verify_tree(i[0], i[1], r.V, r.lanes, r.n, *i[2:], *o)
+
+    streams = [torch.cuda.Stream() for _ in rs]
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for r, i, o, s in zip(rs, ins, outs, streams):
+            with torch.cuda.stream(s):
+                call(r, i, o)
+    torch.cuda.synchronize()
+    for w, o in zip(want, outs):
+        for x, y in zip(w, o):
+            np.testing.assert_array_equal(x, y.cpu().numpy())
+    for o in outs:
+        for y in o:
+            y.fill_(-9)
+    g = torch.cuda.CUDAGraph()
+    draws = torch.zeros(2, 3, dtype=I32, device="cuda")
+    u = torch.randint(0, (1 << 31) - 1, (2, 3), dtype=I32, device="cuda")
+    row = ins[0][0][:2].contiguous()
+    args = (row, 2000, 1, 2, 0, 3, ins[0][5], u, ins[0][8], ins[0][9], ins[0][2], ins[0][3])
+    ops.draw_tokens(*args, draws)
+    plain = draws.clone()
+    with torch.cuda.graph(g):
+        for r, i, o in zip(rs, ins, outs):
+            call(r, i, o)
+        ops.draw_tokens(*args, draws)
+    draws.zero_()
+    for _ in range(3):
+        g.replay()
+    torch.cuda.synchronize()
+    for w, o in zip(want, outs):
+        for x, y in zip(w, o):
+            np.testing.assert_array_equal(x, y.cpu().numpy())
+    assert torch.equal(draws, plain)
 
 
 def test_verify_tree_strided_rows():
