@@ -82,11 +82,9 @@ __device__ __forceinline__ int64_t clamp40(int64_t x) { return x > CLAMP ? CLAMP
 // floor(num / den) for num <= 2^62 and a quotient of at most 2^31: the double
 // estimate is within 1 (three roundings of 2^-53 each), the remainder decides.
 __device__ __forceinline__ uint32_t div31(uint64_t num, uint64_t den, double rcp) {
-  uint64_t q = (uint64_t)((double)num * rcp);
+  const uint64_t q = (uint64_t)((double)num * rcp);
   const int64_t r = (int64_t)(num - q * den);
-  if (r < 0) --q;
-  else if ((uint64_t)r >= den) ++q;
-  return (uint32_t)q;
+  return (uint32_t)q + (r < 0 ? -1 : (uint64_t)r >= den ? 1 : 0);
 }
 
 // Scratch, and what the CTAs of a cluster exchange: every CTA stores its value
@@ -95,8 +93,8 @@ __device__ __forceinline__ uint32_t div31(uint64_t num, uint64_t den, double rcp
 // in two phases, so that the next exchange may start while a peer still reads.
 struct Shared {
   int2 lut[EXP_LUT_N];
-  int64_t redv[2][NW];
-  int redi[2][NW];
+  int64_t redv[NW];  // the first row's warps, then the second's
+  int redi[NW];
   uint64_t wsum[2][NW];
   int64_t xmax[2][MAX_CS];      // largest values (target, draft) and their first indexes
   int xidx[2][MAX_CS];
@@ -105,6 +103,7 @@ struct Shared {
   int ids[HIST];                // newest first
   int met[HIST];                // times that an id is penalised; 0: not its first entry, or not an id
   int parent[tree::MAX_NODES], token[tree::MAX_NODES], hist[HIST];
+  int wide[2];                  // the part of the target's, the draft's row has a logit beyond 32 bits
   int count, n_ids, n_path;
 };
 
@@ -128,6 +127,7 @@ __device__ __forceinline__ void load_lane(Shared& sh, const int* tokens, const i
 __device__ void gather_ids(Shared& sh, uint32_t* skip, int node, int V, int v0, int len) {
   const int tid = threadIdx.x;
   for (int i = tid; i < (len + 31) / 32; i += NT) skip[i] = 0;
+  if (tid < 2) sh.wide[tid] = 0;
   if (tid == 0) {
     int k = 0;
     for (int i = node; i > 0 && k < HIST; i = sh.parent[i]) sh.ids[k++] = sh.token[i];
@@ -138,45 +138,52 @@ __device__ void gather_ids(Shared& sh, uint32_t* skip, int node, int V, int v0, 
   if (tid >= np && tid < n) sh.ids[tid] = sh.hist[(unsigned)(c - 1 - (tid - np)) & (HIST - 1)];
   if (tid == 0) sh.n_ids = n;
   __syncthreads();
-  if (tid < n) {
-    const int t = sh.ids[tid];
-    int m = 0;
-    bool first = t >= 0 && t < V;
-#pragma unroll 8
-    for (int j = 0; j < n; ++j) {
-      const bool same = sh.ids[j] == t;
+  {  // eight threads an id
+    const int i = tid >> 3, t = i < n ? sh.ids[i] : -1;
+    int m = 0, before = 0;
+#pragma unroll
+    for (int j = tid & 7; j < HIST; j += 8) {
+      const int same = j < n && sh.ids[j] == t;
       m += same;
-      first &= !(same && j < tid);
+      before += j < i ? same : 0;
     }
-    sh.met[tid] = first ? m : 0;
-    if (first && t >= v0 && t < v0 + len) atomicOr(&skip[(t - v0) >> 5], 1u << ((t - v0) & 31));
+    m |= before << 16;
+#pragma unroll
+    for (int k = 4; k >= 1; k >>= 1) m += __shfl_xor_sync(0xffffffffu, m, k);
+    const bool first = t >= 0 && t < V && m >> 16 == 0;
+    if ((tid & 7) == 0 && i < n) {
+      sh.met[i] = first ? m : 0;
+      if (first && t >= v0 && t < v0 + len) atomicOr(&skip[(t - v0) >> 5], 1u << ((t - v0) & 31));
+    }
   }
   __syncthreads();
 }
 
-// f(i, x) for this thread's elements i of the part, x the logit; the skipped
-// ones too.  16-byte loads, several in flight, where the row allows them.
+// The threads that share a row: all of the CTA, or half of them a row.
+struct Team {
+  int k, t, n;  // which row, this thread's place, threads
+};
+
+// f(i, x, y) for this thread's pairs of elements i, i + 1 of the part (i even),
+// f(i, x) for single ones; x and y are the logits, the skipped ones too.
+// 16-byte loads, several in flight, where the row allows them.
 template <class F>
-__device__ __forceinline__ void each(const int64_t* __restrict__ part, int len, F f) {
+__device__ __forceinline__ void each(const int64_t* __restrict__ part, int len, const Team& tm, F f) {
   if (((uintptr_t)part & 15) == 0) {
     const longlong2* p = (const longlong2*)part;
     const int n2 = len / 2;
-    int i = threadIdx.x;
-    for (; i < n2; i += 4 * NT) {
+    for (int i = tm.t; i < n2; i += 4 * tm.n) {
       longlong2 x[4];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) x[k] = i + k * NT < n2 ? __ldg(p + i + k * NT) : make_longlong2(0, 0);
+      for (int k = 0; k < 4; ++k) x[k] = i + k * tm.n < n2 ? __ldg(p + i + k * tm.n) : make_longlong2(0, 0);
 #pragma unroll
       for (int k = 0; k < 4; ++k)
-        if (i + k * NT < n2) {
-          f(2 * (i + k * NT), (int64_t)x[k].x);
-          f(2 * (i + k * NT) + 1, (int64_t)x[k].y);
-        }
+        if (i + k * tm.n < n2) f(2 * (i + k * tm.n), (int64_t)x[k].x, (int64_t)x[k].y);
     }
-    if ((len & 1) && threadIdx.x == 0) f(len - 1, (int64_t)__ldg((const long long*)part + len - 1));
+    if ((len & 1) && tm.t == 0) f(len - 1, (int64_t)__ldg((const long long*)part + len - 1));
   } else {
-#pragma unroll 4
-    for (int i = threadIdx.x; i < len; i += NT) f(i, (int64_t)__ldg((const long long*)part + i));
+#pragma unroll 1
+    for (int i = tm.t; i < len; i += tm.n) f(i, (int64_t)__ldg((const long long*)part + i));
   }
 }
 
@@ -194,10 +201,7 @@ struct Row {
   __device__ Row(const int64_t* row, int v0, int64_t inv_temp)
       : part(row + v0), inv(inv_temp > MAX_INV_T ? MAX_INV_T : inv_temp) {}
   __device__ bool greedy() const { return inv <= 0; }
-  // the weighted value of a logit; 32-bit logits need no clamp and one product
-  __device__ int64_t value(int64_t x) const {
-    return x == (int64_t)(int)x ? ((int64_t)(int)x * (int)inv) >> FRAC_BITS : (clamp40(x) * inv) >> FRAC_BITS;
-  }
+  __device__ int64_t value(int64_t x) const { return (clamp40(x) * inv) >> FRAC_BITS; }
   __device__ int64_t penalised(int64_t x, int times) const {  // not scaled
     x = clamp40(x);
     for (int r = 0; r < times; ++r) x = clamp40(penalize(x));
@@ -205,10 +209,10 @@ struct Row {
   }
 };
 
-// Which of this thread's ids lies in the part: its index there, or -1.
-__device__ __forceinline__ int own_id(const Shared& sh, int v0, int len) {
-  if (threadIdx.x >= sh.n_ids || !sh.met[threadIdx.x]) return -1;
-  const int t = sh.ids[threadIdx.x] - v0;
+// Where in the part this thread's id of the row's team stands, or -1.
+__device__ __forceinline__ int own_id(const Shared& sh, int v0, int len, const Team& tm) {
+  if (tm.t >= sh.n_ids || !sh.met[tm.t]) return -1;
+  const int t = sh.ids[tm.t] - v0;
   return t >= 0 && t < len ? t : -1;
 }
 
@@ -216,30 +220,82 @@ __device__ __forceinline__ void better(int64_t& v, int& i, int64_t ov, int oi) {
   if (ov > v || (ov == v && oi < i)) v = ov, i = oi;
 }
 
-// Largest clamped logit and its first index over the CTA's part of row r, into
-// the cell k of redv / redi (per warp).  The index matters to greedy rows only.
-__device__ void warp_max(Shared& sh, const uint32_t* skip, const Row& r, int v0, int len, int k) {
-  int64_t bv = INT64_MIN;
-  int bi = INT_MAX;
-  each(r.part, len, [&](int i, int64_t x) {
-    x = r.greedy() ? clamp40(x) : x;
-    if (x > bv && !(skip[i >> 5] >> (i & 31) & 1)) bv = x, bi = v0 + i;  // a thread meets rising indexes
-  });
-  if (bi != INT_MAX) bv = clamp40(bv);
-  const int t = own_id(sh, v0, len);
-  if (t >= 0) better(bv, bi, r.penalised(r.part[t], sh.met[threadIdx.x]), v0 + t);
+constexpr int WIDE = INT_MIN;  // stands for a logit that 32 bits do not hold
+
+struct MaxOf {  // the largest logit that is not skipped; the logits in 32 bits for weights()
+  const uint32_t* skip;
+  int* low;
+  int64_t v = INT64_MIN;
+  bool some = false, wide = false;
+  static __device__ int pack(int64_t x) { return (int)(x >> 32) == (int)x >> 31 ? (int)x : WIDE; }
+  __device__ void operator()(int i, int64_t x) {
+    low[i] = pack(x);
+    wide |= low[i] == WIDE;
+    if (skip[i >> 5] >> (i & 31) & 1) return;
+    v = max(v, x);
+    some = true;
+  }
+  __device__ void operator()(int i, int64_t x, int64_t y) {
+    const int2 l = make_int2(pack(x), pack(y));
+    *(int2*)(low + i) = l;
+    wide |= l.x == WIDE | l.y == WIDE;
+    const uint32_t s = skip[i >> 5] >> (i & 31);
+    v = max(v, s & 1 ? INT64_MIN : x);
+    v = max(v, s & 2 ? INT64_MIN : y);
+    some |= (s & 3) != 3;
+  }
+};
+
+struct FirstMaxOf {  // a greedy row: the largest clamped one and where it stands first
+  const uint32_t* skip;
+  int64_t v = INT64_MIN;
+  int at = INT_MAX;
+  __device__ void operator()(int i, int64_t x) {
+    x = clamp40(x);
+    if (x > v && !(skip[i >> 5] >> (i & 31) & 1)) v = x, at = i;  // a thread meets rising indexes
+  }
+  __device__ void operator()(int i, int64_t x, int64_t y) {
+    (*this)(i, x);
+    (*this)(i + 1, y);
+  }
+};
+
+// Largest clamped logit and (of a greedy row) its first index over the CTA's
+// part of row r, by warps into redv / redi, and the part's logits in 32 bits
+// into e (not of a greedy row).  Returns what the logit of this thread's id
+// (own_id) becomes.
+__device__ int64_t warp_max(Shared& sh, const uint32_t* skip, const Row& r, int v0, int len, const Team& tm,
+                            uint32_t* e) {
+  int64_t bv;
+  int bi;
+  const int t = own_id(sh, v0, len, tm);
+  const int64_t raw = t >= 0 ? __ldg((const long long*)r.part + t) : 0;
+  if (r.greedy()) {
+    FirstMaxOf m{skip};
+    each(r.part, len, tm, [&](auto... a) { m(a...); });
+    bv = m.v, bi = m.at == INT_MAX ? m.at : v0 + m.at;
+  } else {
+    MaxOf m{skip, (int*)e};
+    each(r.part, len, tm, [&](auto... a) { m(a...); });
+    if (m.wide) sh.wide[tm.k] = 1;
+    bv = m.some ? clamp40(m.v) : INT64_MIN, bi = 0;
+  }
+  const int64_t pen = r.penalised(raw, t >= 0 ? sh.met[tm.t] : 0);
+  if (t >= 0) better(bv, bi, pen, v0 + t);
 #pragma unroll
   for (int m = 16; m >= 1; m >>= 1) better(bv, bi, shfl_xor_i64(bv, m), __shfl_xor_sync(0xffffffffu, bi, m));
-  if ((threadIdx.x & 31) == 0) sh.redv[k][threadIdx.x >> 5] = bv, sh.redi[k][threadIdx.x >> 5] = bi;
+  if ((threadIdx.x & 31) == 0) sh.redv[threadIdx.x >> 5] = bv, sh.redi[threadIdx.x >> 5] = bi;
+  return pen;
 }
 
-// The cluster's largest value and first index of cells 0 .. n - 1 (n <= 2).
+// The cluster's largest value and first index of n <= 2 rows.
 __device__ void cluster_max(Shared& sh, int n, uint32_t rank, uint32_t cs, int64_t* v, int* i) {
   __syncthreads();
   const int k = threadIdx.x >> 5, l = threadIdx.x & 31;
-  if (k < n) {  // warp k: cell k
-    int64_t bv = l < NW ? sh.redv[k][l] : INT64_MIN;
-    int bi = l < NW ? sh.redi[k][l] : INT_MAX;
+  if (k < n) {  // warp k: row k
+    const int nw = NW / n;
+    int64_t bv = l < nw ? sh.redv[k * nw + l] : INT64_MIN;
+    int bi = l < nw ? sh.redi[k * nw + l] : INT_MAX;
 #pragma unroll
     for (int m = 16; m >= 1; m >>= 1) better(bv, bi, shfl_xor_i64(bv, m), __shfl_xor_sync(0xffffffffu, bi, m));
     if (l < (int)cs) {
@@ -248,36 +304,58 @@ __device__ void cluster_max(Shared& sh, int n, uint32_t rank, uint32_t cs, int64
     }
   }
   cluster_sync();
+#pragma unroll 1
   for (int c = 0; c < n; ++c) {
-    v[c] = sh.xmax[c][0];
-    i[c] = sh.xidx[c][0];
-#pragma unroll 4
-    for (uint32_t r = 1; r < cs; ++r) better(v[c], i[c], sh.xmax[c][r], sh.xidx[c][r]);
+    int64_t bv = l < (int)cs ? sh.xmax[c][l] : INT64_MIN;
+    int bi = l < (int)cs ? sh.xidx[c][l] : INT_MAX;
+#pragma unroll
+    for (int m = MAX_CS / 2; m >= 1; m >>= 1) better(bv, bi, shfl_xor_i64(bv, m), __shfl_xor_sync(0xffffffffu, bi, m));
+    // lanes 16 and up hold nothing: from the lower half
+    bv = __shfl_sync(0xffffffffu, bv, 0), bi = __shfl_sync(0xffffffffu, bi, 0);
+    if (c == 0) v[0] = bv, i[0] = bi;
+    else v[1] = bv, i[1] = bi;
   }
 }
 
-// Weights of the CTA's part into e; this thread's part of their sum.  `top` is
-// the row's largest clamped logit.
-__device__ uint64_t weights(Shared& sh, const Row& r, int v0, int len, int64_t top, int first, uint32_t* e) {
-  const int64_t zt = (clamp40(top) * r.inv) >> FRAC_BITS;  // a row of the type's lowest value has no larger one
-  uint64_t s = 0;
-  auto weight = [&](int i, int64_t z) -> uint32_t {  // z the scaled value
-    if (r.greedy()) return v0 + i == first ? (uint32_t)ONE : 0u;
+// Weights of the CTA's part into e, from what warp_max left there; this
+// thread's part of their sum.  `top` is the row's largest clamped logit, `first`
+// its index, pen what warp_max returned.  The whole CTA calls it.
+__device__ uint64_t weights(Shared& sh, const Row& r, int v0, int len, int64_t top, int first, int64_t pen,
+                            const Team& tm, uint32_t* e) {
+  const int64_t zt = r.value(top);  // a row of the type's lowest value has no larger one
+  const int inv = (int)r.inv;
+  auto weight = [&](int64_t z) {  // z: scaled
     const int64_t d = z - zt;
     return (uint32_t)exp32(d < -(1 << 30) ? -(1 << 30) : (int)d, sh.lut);
   };
-  each(r.part, len, [&](int i, int64_t x) {
-    const uint32_t w = weight(i, r.value(x));
-    e[i] = w;
-    s += w;
-  });
+  uint32_t sum = 0;  // a thread has fewer than 2^15 elements of at most 2^16
+  if (r.greedy()) {
+    for (int i = tm.t; i < len; i += tm.n) e[i] = v0 + i == first ? (uint32_t)ONE : 0u;
+    if (tm.t == 0 && first >= v0 && first < v0 + len) sum = (uint32_t)ONE;
+  } else if (!sh.wide[tm.k]) {
+#pragma unroll 4
+    for (int i = tm.t * 2; i < len; i += 2 * tm.n) {  // e has an even number of elements
+      const int2 x = *(const int2*)(e + i);
+      const uint32_t wx = weight(((int64_t)x.x * inv) >> FRAC_BITS), wy = weight(((int64_t)x.y * inv) >> FRAC_BITS);
+      const uint2 w = make_uint2(wx, i + 1 < len ? wy : 0);
+      *(uint2*)(e + i) = w;
+      sum += w.x + w.y;
+    }
+  } else {
+#pragma unroll 1
+    for (int i = tm.t; i < len; i += tm.n) {
+      const int x = (int)e[i];
+      e[i] = weight(r.value(x != WIDE ? x : (int64_t)__ldg((const long long*)r.part + i)));
+      sum += e[i];
+    }
+  }
+  uint64_t s = sum;
   __syncthreads();
-  const int t = own_id(sh, v0, len);
-  if (t >= 0) {
+  const int t = own_id(sh, v0, len, tm);
+  if (t >= 0 && !r.greedy()) {
     s -= e[t];  // what the logit would have weighed, and what it does
-    const uint32_t w = weight(t, (r.penalised(r.part[t], sh.met[threadIdx.x]) * r.inv) >> FRAC_BITS);
-    e[t] = w;
-    s += w;
+    e[t] = weight((pen * r.inv) >> FRAC_BITS);
+    s += e[t];
   }
   return s;
 }
@@ -378,11 +456,12 @@ __global__ void __launch_bounds__(NT, 3) k_draw(const int64_t* __restrict__ logi
   fetch(r.part, len);
   load_lane(sh, tokens + (size_t)lane * n, parent + (size_t)lane * n, n, hist + lane * HIST, count + lane);
   gather_ids(sh, skip, node0 + blockIdx.y, V, v0, len);
-  int64_t top;
-  int first;
-  warp_max(sh, skip, r, v0, len, 0);
-  cluster_max(sh, 1, rank, cs, &top, &first);
-  uint64_t mine = weights(sh, r, v0, len, top, first, e);
+  int64_t top[2];
+  int first[2];
+  const Team tm{0, (int)threadIdx.x, NT};
+  const int64_t pen = warp_max(sh, skip, r, v0, len, tm, e);
+  cluster_max(sh, 1, rank, cs, top, first);
+  uint64_t mine = weights(sh, r, v0, len, top[0], first[0], pen, tm, e);
   block_sum<1>(sh, &mine);
   for (int k = 0; k < m; ++k) {
     uint64_t total;
@@ -442,13 +521,21 @@ __global__ void __launch_bounds__(NT, 2) k_verify(const int64_t* __restrict__ lo
   load_lane(sh, tokens + lane0, parent + lane0, n, hist + lane * HIST, count + lane);
   u += lane0 * 2;
   int ph = 0, length = 0;
-  auto next_child = [&](int c) {  // of the node, from c on, whose token is one
-    while (c < live && !(sh.parent[c] == node && sh.token[c] >= 0 && sh.token[c] < V)) ++c;
+  uint64_t kids = 0;  // the node's children whose token is one, not asked yet
+  auto next_child = [&]() {
+    const int c = kids ? __ffsll((long long)kids) - 1 : live;
+    kids &= kids - 1;
     return c;
   };
   for (;;) {
     const size_t row = lane0 + node;
-    int c = next_child(node + 1);
+    kids = 0;
+    for (int h = 0; h < 2; ++h) {
+      const int i = 32 * h + (tid & 31);
+      const bool kid = i < live && sh.parent[i] == node && sh.token[i] >= 0 && sh.token[i] < V;
+      kids |= (uint64_t)__ballot_sync(0xffffffffu, kid) << 32 * h;
+    }
+    int c = next_child();
     const bool inner = c < live;
     const Row rt(logits + row * ldl, v0, inv_temp[lane]), rd(dlogits + row * ldd, v0, d_inv_temp[lane]);
     fetch(rt.part, len);
@@ -456,9 +543,14 @@ __global__ void __launch_bounds__(NT, 2) k_verify(const int64_t* __restrict__ lo
     gather_ids(sh, skip, node, V, v0, len);
     int64_t top[2];
     int first[2];
-    warp_max(sh, skip, rt, v0, len, 0);
-    if (inner) warp_max(sh, skip, rd, v0, len, 1);
-    cluster_max(sh, inner ? 2 : 1, rank, cs, top, first);
+    // half of the warps for each of the two rows: one latency, and one copy of
+    // the code (instructions come from DRAM too)
+    const int n_rows = inner ? 2 : 1, tn = NT / n_rows;
+    const Team tm{tid / tn, tid % tn, tn};
+    const Row& r = tm.k ? rd : rt;
+    uint32_t* e = tm.k ? eq : P;
+    const int64_t pen = warp_max(sh, skip, r, v0, len, tm, e);
+    cluster_max(sh, n_rows, rank, cs, top, first);
     // one CTA stores what child c's test needs into all of them, with the sums of phase ph
     auto push_child = [&](uint32_t a, uint32_t b, uint32_t e) {
       if (tid < cs) {
@@ -468,8 +560,8 @@ __global__ void __launch_bounds__(NT, 2) k_verify(const int64_t* __restrict__ lo
       }
     };
     uint64_t mine[2], S[2], before;
-    mine[0] = weights(sh, rt, v0, len, top[0], first[0], P);
-    mine[1] = inner ? weights(sh, rd, v0, len, top[1], first[1], eq) : 0;
+    const uint64_t sum = weights(sh, r, v0, len, top[tm.k], first[tm.k], pen, tm, e);
+    mine[0] = tm.k ? 0 : sum, mine[1] = tm.k ? sum : 0;
     block_sum<2>(sh, mine);
     ph ^= 1;
     if (inner && sh.token[c] / seg == (int)rank) push_child(P[sh.token[c] - v0], 0, eq[sh.token[c] - v0]);
@@ -477,10 +569,8 @@ __global__ void __launch_bounds__(NT, 2) k_verify(const int64_t* __restrict__ lo
     // P = floor(e * 2^31 / S), made of the weights in place once it is needed as a whole
     const double rp = 1.0 / (double)S[0];
     auto normalise = [&]() {
-      for (int i = tid; i < len; i += NT) {
-        const uint32_t e = P[i];
-        P[i] = e ? div31((uint64_t)e << 31, S[0], rp) : 0;
-      }
+#pragma unroll 4
+      for (int i = tid; i < len; i += NT) P[i] = div31((uint64_t)P[i] << 31, S[0], rp);
     };
     int taken = -1;
     bool whole = false;
@@ -499,23 +589,21 @@ __global__ void __launch_bounds__(NT, 2) k_verify(const int64_t* __restrict__ lo
         whole = true;
       }
       auto rest = [&](int i) -> uint32_t {
-        const uint32_t p = P[i], e = eq[i];
-        const uint32_t q = e ? div31((uint64_t)e << 31, sq, rq) : 0;
+        const uint32_t p = P[i], q = div31((uint64_t)eq[i] << 31, sq, rq);
         return p > q ? p - q : 0;
       };
       uint64_t s = 0, left;
+#pragma unroll 4
       for (int i = tid; i < len; i += NT) s += rest(i);
       block_sum<1>(sh, &s);
-      const int c2 = next_child(c + 1), d2 = c2 < live ? sh.token[c2] : 0;
+      const int c2 = next_child(), d2 = c2 < live ? sh.token[c2] : 0;
       ph ^= 1;
       if (c2 < live && d2 / seg == (int)rank) push_child(P[d2 - v0], rest(d2 - v0), d2 == d ? 0 : eq[d2 - v0]);
       cluster_sum<1>(sh, &s, ph, rank, cs, &left);
       if (left > 0) {
         const double rl = 1.0 / (double)left;
-        for (int i = tid; i < len; i += NT) {
-          const uint32_t r = rest(i);
-          P[i] = r ? div31((uint64_t)r << 31, left, rl) : 0;
-        }
+#pragma unroll 4
+        for (int i = tid; i < len; i += NT) P[i] = div31((uint64_t)rest(i) << 31, left, rl);
         pd = div31((uint64_t)sh.xchild[ph][1] << 31, left, rl);
       } else {
         pd = sh.xchild[ph][0];
@@ -593,10 +681,38 @@ static size_t part_of(int V, int cs, int per, int& seg) {
   return (size_t)seg * per + seg / 8;
 }
 
-// CTAs that the GPU holds at once, `most` per SM by their registers.
-static int64_t capacity(size_t smem, int most) {
+// CTAs per SM: `most` by their registers.
+static int per_sm(size_t smem, int most) {
   const int by_smem = (int)((224 * 1024) / (smem + sizeof(Shared) + 1024));
-  return 148 * (int64_t)(by_smem < most ? by_smem : most);
+  return by_smem < most ? by_smem : most;
+}
+
+// How `rows` rows are divided over clusters.
+struct Split {
+  int cs, seg;
+  size_t smem;
+  int64_t cost;
+};
+
+// The cluster size whose clusters finish first: the number that run one after
+// another times what one takes: a fixed part (exchanges and loads: as long as
+// FIXED elements) and its elements, `per` / 4 words of each, the longer the more
+// CTAs share an SM.
+static Split split_of(int64_t rows, int V, int per, int most) {
+  constexpr int FIXED = 16000;
+  constexpr int AT_ONCE[4] = {7, 16, 35, 74};  // clusters of 16, 8, 4, 2 CTAs that the GPU's SM groups hold, one CTA per SM
+  Split best = {};
+  for (int i = 0; i < 4; ++i) {
+    Split x = {};
+    x.cs = 16 >> i;
+    x.smem = part_of(V, x.cs, per, x.seg);
+    if (i > 0 && x.smem > SMEM_MAX) break;
+    const int64_t held = per_sm(x.smem, most), at_once = AT_ONCE[i] * held, share = (rows * x.cs + 147) / 148;
+    const int64_t waves = (rows + at_once - 1) / at_once;
+    x.cost = waves * (FIXED + x.seg * (per / 4) * (share < held ? share : held));
+    if (i == 0 || x.cost < best.cost) best = x;
+  }
+  return best;
 }
 
 template <typename... KArgs, typename... Args>
@@ -643,17 +759,10 @@ int arcb_draw_tokens(const int64_t* logits, int64_t ldl, int V, int lanes, int n
   if (V < 1 || V > arcb_draw_max_vocab() || lanes < 1 || nr < 1 || m < 1 || node0 < 0 || node0 + nr > n ||
       n > tree::MAX_NODES || lanes > 65535)
     return -2;
-  // 16 CTAs a row while they all run at once, else 8
-  int seg = 0, cs = 16;
-  size_t smem = dr::part_of(V, cs, 4, seg);
-  if ((int64_t)lanes * nr * cs > dr::capacity(smem, 3)) {
-    int seg8 = 0;
-    const size_t smem8 = dr::part_of(V, 8, 4, seg8);
-    if (smem8 <= dr::SMEM_MAX) cs = 8, seg = seg8, smem = smem8;
-  }
+  const dr::Split x = dr::split_of((int64_t)lanes * nr, V, 4, 3);
   static std::atomic<uint64_t> ready{0};
-  return dr::launch_cluster(dr::k_draw, ready, cs, dim3(cs, nr, lanes), smem, (cudaStream_t)stream, logits, ldl, V, nr, n,
-                            node0, m, inv_temp, u, hist, count, tokens, parent, seg, out);
+  return dr::launch_cluster(dr::k_draw, ready, x.cs, dim3(x.cs, nr, lanes), x.smem, (cudaStream_t)stream, logits, ldl, V,
+                            nr, n, node0, m, inv_temp, u, hist, count, tokens, parent, x.seg, out);
 }
 
 // scratch: 2 * lanes * n ints.
@@ -665,15 +774,14 @@ int arcb_verify_tree(const int64_t* logits, int64_t ldl, const int64_t* dlogits,
   static std::atomic<uint64_t> walk{0}, all{0};
   cudaStream_t st = (cudaStream_t)stream;
   int* drawn = scratch + (size_t)lanes * n;
-  int seg = 0;
-  size_t smem = dr::part_of(V, 16, 8, seg);
-  if ((int64_t)lanes * n * 16 > dr::capacity(smem, 2))  // a cluster per node does not fit the GPU: one per lane
-    return dr::launch_cluster(dr::k_verify<true>, walk, 16, dim3(16, 1, lanes), smem, st, logits, ldl, dlogits, ldd, V, n,
-                              tokens, parent, n_tree, inv_temp, d_inv_temp, u, hist, count, seg, scratch, drawn, path,
-                              n_path, next);
-  const int rc = dr::launch_cluster(dr::k_verify<false>, all, 16, dim3(16, n, lanes), smem, st, logits, ldl, dlogits, ldd, V,
-                                    n, tokens, parent, n_tree, inv_temp, d_inv_temp, u, hist, count, seg, scratch,
-                                    drawn, path, n_path, next);
+  const dr::Split each = dr::split_of((int64_t)lanes * n, V, 8, 2), walk_of = dr::split_of(lanes, V, 8, 2);
+  if (each.cost * 5 > walk_of.cost * 11)  // a path is a few nodes long: all at once for up to the time of 2.2
+    return dr::launch_cluster(dr::k_verify<true>, walk, walk_of.cs, dim3(walk_of.cs, 1, lanes), walk_of.smem, st, logits,
+                              ldl, dlogits, ldd, V, n, tokens, parent, n_tree, inv_temp, d_inv_temp, u, hist, count,
+                              walk_of.seg, scratch, drawn, path, n_path, next);
+  const int rc = dr::launch_cluster(dr::k_verify<false>, all, each.cs, dim3(each.cs, n, lanes), each.smem, st, logits,
+                                    ldl, dlogits, ldd, V, n, tokens, parent, n_tree, inv_temp, d_inv_temp, u, hist,
+                                    count, each.seg, scratch, drawn, path, n_path, next);
   if (rc) return rc;
   return launch_k(dr::k_verify_path, dim3((lanes + 63) / 64), dim3(64), 0, st, lanes, n, n_tree, scratch, drawn, path,
                   n_path, next);

@@ -372,6 +372,9 @@ class Rows:
     (2, 1, 33, dict()),                                                    # a root alone: a plain draw
     (3, 9, 1, dict(fan=8)),                                                # one token: drafts run out
     (3, 9, 2, dict(fan=8)),
+    (12, 40, 300, dict(fan=3, near=0.4)),                                  # more nodes than the GPU decides at once
+    (10, 64, 65, dict(fan=2, near=0.2, inv=(40000, 65536))),
+    (9, 31, 2001, dict(fan=2, near=0.5)),
     (1, 3, 102400, dict(fan=2)),
     (1, 2, 152064, dict(fan=1)),                                           # 16 CTAs per row
     (1, 2, 272896, dict(fan=1)),                                           # more shared memory per CTA
@@ -406,13 +409,13 @@ def test_verify_tree_one_lane_equals_its_place_in_a_batch():
     from arc_chain_b200.ops import tree_ops as ops
 
     for V, near, inv in ((901, 0.4, 65536), (5000, 1.0, 90000), (64, 0.5, 0)):
-        r = Rows(8, 13, V, fan=3, seed=11, near=near, inv=(inv,), dinv=(inv,))
-        r.n_tree[:] = [13, 12, 1, 2, 13, 0, 40, 13]
+        r = Rows(45, 13, V, fan=3, seed=11, near=near, inv=(inv,), dinv=(inv,))
+        r.n_tree[:8] = [13, 12, 1, 2, 13, 0, 40, 13]
         r.parent[4] = [-1, 0, 0, 7, 1, 4, 4, 3, 0, 8, 8, -2, 13]
-        r.logits[13 * 7:, 1::2] = np.iinfo(np.int64).min
-        r.check()
+        r.logits[13 * 7:13 * 20, 1::2] = np.iinfo(np.int64).min
+        assert r.check().max() > 2
         path, n_path, nxt = r.verify()
-        for b in range(8):
+        for b in range(45):
             z = lambda *s: torch.full(s, 9, dtype=I32, device="cuda")
             p, k, t = z(1, 13), z(1), z(1)
             ops.verify_tree(dev(r.logits[13 * b:][:13]), dev(r.dlogits[13 * b:][:13]), V, 1, 13, dev(r.tokens[b:b + 1]),
