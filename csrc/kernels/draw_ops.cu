@@ -25,8 +25,9 @@
 //
 // A cluster serves one row (draw) or one node at a time (verify): each CTA
 // holds the weights of a contiguous part of the vocabulary in shared memory
-// (4 bytes an element; P and Q: 8), reads its logits twice (for the maximum,
-// then from the caches for the weights), and the sums and the single elements
+// (4 bytes an element; P and Q: 8).  The logits are read once, where 32 bits
+// hold the part's (else again for each pass): their low words stand in shared
+// memory until they become weights there.  The sums and the single elements
 // that all of them need cross through distributed shared memory.
 //
 // Verification has two schedules.  Where a cluster per node fills no more than
@@ -39,7 +40,7 @@
 
 #include "../common/tree.h"
 #include "common.cuh"
-#include "exp32.cuh"
+#include "lut.cuh"
 
 using namespace q16;
 
@@ -65,6 +66,8 @@ __device__ __forceinline__ uint32_t cluster_size() {
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 __device__ __forceinline__ uint32_t peer_addr(const void* local, uint32_t rank) {
   uint32_t ra;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(ra) : "r"(smem_u32(local)), "r"(rank));
@@ -95,7 +98,7 @@ struct Shared {
   int2 lut[EXP_LUT_N];
   int64_t redv[NW];  // the first row's warps, then the second's
   int redi[NW];
-  uint64_t wsum[2][NW];
+  uint64_t wsum[NW];
   int64_t xmax[2][MAX_CS];      // largest values (target, draft) and their first indexes
   int xidx[2][MAX_CS];
   uint64_t xsum[2][2][MAX_CS];  // [phase][target, draft]
@@ -108,16 +111,20 @@ struct Shared {
 };
 
 // The lane's tree (each node's token and parent, -1 where that is no earlier
-// node) and ring.
+// node), its ring, and the table of exps (entries times 2^11,
+// see weights): all loads at once.
 __device__ __forceinline__ void load_lane(Shared& sh, const int* tokens, const int* parent, int n, const int* hist,
                                           const int* count) {
-  const int tid = threadIdx.x;
-  if (tid < n) {
-    sh.token[tid] = tokens[tid];
-    sh.parent[tid] = tree::parent_of(parent, tid);
+  static_assert(EXP_LUT_N <= NT && tree::MAX_NODES + HIST < NT, "one element a thread");
+  const int tid = threadIdx.x, i = min(tid, n - 1), h = tid & (HIST - 1);
+  const int token = __ldg(tokens + i), up = tree::parent_of(parent, i), id = __ldg(hist + h), c = __ldg(count);
+  if (tid < EXP_LUT_N) {
+    const int lo = (int)g_exp_lut.v[tid];
+    sh.lut[tid] = make_int2(lo << 11, tid < EXP_LUT_N - 1 ? (int)g_exp_lut.v[tid + 1] - lo : 0);
   }
-  if (tid >= 64 && tid < 64 + HIST) sh.hist[tid - 64] = hist[tid - 64];
-  if (tid == 128) sh.count = max(*count, 0);
+  if (tid < n) sh.token[tid] = token, sh.parent[tid] = up;
+  if (tid < HIST) sh.hist[tid] = id;
+  if (tid == 0) sh.count = max(c, 0);
   __syncthreads();
 }
 
@@ -187,12 +194,6 @@ __device__ __forceinline__ void each(const int64_t* __restrict__ part, int len, 
   }
 }
 
-// The part into the cache, ahead of its first use.
-__device__ __forceinline__ void fetch(const int64_t* part, int len) {
-  for (int i = threadIdx.x * 16; i < len; i += NT * 16)
-    asm volatile("prefetch.global.L2 [%0];" ::"l"(part + i));
-}
-
 // A row's part as it is used.  Clamping and scaling keep the order, so the
 // maximum is found before them.
 struct Row {
@@ -220,72 +221,74 @@ __device__ __forceinline__ void better(int64_t& v, int& i, int64_t ov, int oi) {
   if (ov > v || (ov == v && oi < i)) v = ov, i = oi;
 }
 
-constexpr int WIDE = INT_MIN;  // stands for a logit that 32 bits do not hold
+// What row r's logit i of the part becomes, not scaled: the long way.
+__device__ int64_t exact(const Shared& sh, const uint32_t* skip, const Row& r, int v0, int i) {
+  int times = 0;
+  if (skip[i >> 5] >> (i & 31) & 1)
+    for (int j = 0; j < sh.n_ids; ++j)
+      if (sh.ids[j] == v0 + i) times |= sh.met[j];  // 0 but for the first entry
+  return r.penalised(__ldg((const long long*)r.part + i), times);
+}
 
-struct MaxOf {  // the largest logit that is not skipped; the logits in 32 bits for weights()
-  const uint32_t* skip;
-  int* low;
-  int64_t v = INT64_MIN;
-  bool some = false, wide = false;
-  static __device__ int pack(int64_t x) { return (int)(x >> 32) == (int)x >> 31 ? (int)x : WIDE; }
+struct Low {  // low words of the logits, and whether those are all
+  int* e;
+  int high = 0;
   __device__ void operator()(int i, int64_t x) {
-    low[i] = pack(x);
-    wide |= low[i] == WIDE;
-    if (skip[i >> 5] >> (i & 31) & 1) return;
-    v = max(v, x);
-    some = true;
+    e[i] = (int)x;
+    high |= (int)(x >> 32) ^ (int)x >> 31;
   }
   __device__ void operator()(int i, int64_t x, int64_t y) {
-    const int2 l = make_int2(pack(x), pack(y));
-    *(int2*)(low + i) = l;
-    wide |= l.x == WIDE | l.y == WIDE;
-    const uint32_t s = skip[i >> 5] >> (i & 31);
-    v = max(v, s & 1 ? INT64_MIN : x);
-    v = max(v, s & 2 ? INT64_MIN : y);
-    some |= (s & 3) != 3;
+    *(int2*)(e + i) = make_int2((int)x, (int)y);
+    high |= (int)(x >> 32) ^ (int)x >> 31;
+    high |= (int)(y >> 32) ^ (int)y >> 31;
   }
 };
 
-struct FirstMaxOf {  // a greedy row: the largest clamped one and where it stands first
-  const uint32_t* skip;
-  int64_t v = INT64_MIN;
-  int at = INT_MAX;
-  __device__ void operator()(int i, int64_t x) {
-    x = clamp40(x);
-    if (x > v && !(skip[i >> 5] >> (i & 31) & 1)) v = x, at = i;  // a thread meets rising indexes
-  }
-  __device__ void operator()(int i, int64_t x, int64_t y) {
-    (*this)(i, x);
-    (*this)(i + 1, y);
-  }
-};
-
-// Largest clamped logit and (of a greedy row) its first index over the CTA's
-// part of row r, by warps into redv / redi, and the part's logits in 32 bits
-// into e (not of a greedy row).  Returns what the logit of this thread's id
-// (own_id) becomes.
-__device__ int64_t warp_max(Shared& sh, const uint32_t* skip, const Row& r, int v0, int len, const Team& tm,
-                            uint32_t* e) {
-  int64_t bv;
-  int bi;
+// The part's logits, penalised, in 32 bits into e (sh.wide: some do not fit, e
+// is void), and the largest clamped one and (of a greedy row) its first index
+// by warps into redv / redi.  The whole CTA calls it.
+__device__ void warp_max(Shared& sh, const uint32_t* skip, const Row& r, int v0, int len, const Team& tm, uint32_t* e) {
+  Low low{(int*)e};
+  each(r.part, len, tm, [&](auto... a) { low(a...); });
+  if (low.high) sh.wide[tm.k] = 1;
+  __syncthreads();
   const int t = own_id(sh, v0, len, tm);
-  const int64_t raw = t >= 0 ? __ldg((const long long*)r.part + t) : 0;
-  if (r.greedy()) {
-    FirstMaxOf m{skip};
-    each(r.part, len, tm, [&](auto... a) { m(a...); });
-    bv = m.v, bi = m.at == INT_MAX ? m.at : v0 + m.at;
-  } else {
-    MaxOf m{skip, (int*)e};
-    each(r.part, len, tm, [&](auto... a) { m(a...); });
-    if (m.wide) sh.wide[tm.k] = 1;
-    bv = m.some ? clamp40(m.v) : INT64_MIN, bi = 0;
+  if (t >= 0) {
+    const int64_t x = r.penalised((int)e[t], sh.met[tm.t]);
+    e[t] = (uint32_t)x;
+    if (x != (int)x) sh.wide[tm.k] = 1;
   }
-  const int64_t pen = r.penalised(raw, t >= 0 ? sh.met[tm.t] : 0);
-  if (t >= 0) better(bv, bi, pen, v0 + t);
-#pragma unroll
-  for (int m = 16; m >= 1; m >>= 1) better(bv, bi, shfl_xor_i64(bv, m), __shfl_xor_sync(0xffffffffu, bi, m));
+  __syncthreads();
+  int64_t bv = INT64_MIN;
+  int bi = INT_MAX;
+  if (sh.wide[tm.k]) {
+#pragma unroll 1
+    for (int i = tm.t; i < len; i += tm.n) {
+      const int64_t x = exact(sh, skip, r, v0, i);
+      if (x > bv) bv = x, bi = v0 + i;  // a thread meets rising indexes
+    }
+  } else if (r.greedy()) {
+    int m = INT_MIN;
+#pragma unroll 2
+    for (int i = tm.t; i < len; i += tm.n) {
+      const int x = (int)e[i];
+      if (x > m || bi == INT_MAX) m = x, bi = v0 + i;
+    }
+    if (bi != INT_MAX) bv = m;
+  } else {
+    int m = INT_MIN;
+#pragma unroll 4
+    for (int i = tm.t * 2; i < len; i += 2 * tm.n) {  // e has an even number of elements
+      const int2 x = *(const int2*)(e + i);
+      m = max(m, i + 1 < len ? max(x.x, x.y) : x.x);
+    }
+    m = __reduce_max_sync(0xffffffffu, m);
+    if (len > 0) bv = m, bi = 0;
+  }
+  if (sh.wide[tm.k] || r.greedy())
+#pragma unroll 1
+    for (int m = 16; m >= 1; m >>= 1) better(bv, bi, shfl_xor_i64(bv, m), __shfl_xor_sync(0xffffffffu, bi, m));
   if ((threadIdx.x & 31) == 0) sh.redv[threadIdx.x >> 5] = bv, sh.redi[threadIdx.x >> 5] = bi;
-  return pen;
 }
 
 // The cluster's largest value and first index of n <= 2 rows.
@@ -318,17 +321,24 @@ __device__ void cluster_max(Shared& sh, int n, uint32_t rank, uint32_t cs, int64
 }
 
 // Weights of the CTA's part into e, from what warp_max left there; this
-// thread's part of their sum.  `top` is the row's largest clamped logit, `first`
-// its index, pen what warp_max returned.  The whole CTA calls it.
-__device__ uint64_t weights(Shared& sh, const Row& r, int v0, int len, int64_t top, int first, int64_t pen,
+// thread's part of their sum, in 32 bits: fewer than 2^10 elements of at most
+// 2^16 (and 2^15 in a warp).  `top` is the row's largest clamped logit, `first`
+// its index.
+//
+// With zt the scaled top, the place in the table off = max(z - zt + EXP_RANGE, 0)
+// comes of one product and sum: x * inv - ((zt - EXP_RANGE) << 16), shifted; no
+// x is above the top.  The table holds (entry << 11, step): one more product and
+// shift, ((entry << 11) + step * (off mod 2^11)) >> 11.
+__device__ uint32_t weights(Shared& sh, const uint32_t* skip, const Row& r, int v0, int len, int64_t top, int first,
                             const Team& tm, uint32_t* e) {
-  const int64_t zt = r.value(top);  // a row of the type's lowest value has no larger one
+  const int64_t zt = r.value(top), c = -((zt - EXP_RANGE) << FRAC_BITS);
   const int inv = (int)r.inv;
-  auto weight = [&](int64_t z) {  // z: scaled
-    const int64_t d = z - zt;
-    return (uint32_t)exp32(d < -(1 << 30) ? -(1 << 30) : (int)d, sh.lut);
+  auto weight = [&](int64_t y) {  // y = x * inv + c
+    const int off = max((int)__funnelshift_r((uint32_t)y, (uint32_t)max((int)(y >> 32), -32768), FRAC_BITS), 0);
+    const int2 t = *(const int2*)((const uint8_t*)sh.lut + (off >> 8 & 0xff8));
+    return off > 0 ? (uint32_t)(t.x + t.y * (off & 2047)) >> 11 : 0u;
   };
-  uint32_t sum = 0;  // a thread has fewer than 2^15 elements of at most 2^16
+  uint32_t sum = 0;
   if (r.greedy()) {
     for (int i = tm.t; i < len; i += tm.n) e[i] = v0 + i == first ? (uint32_t)ONE : 0u;
     if (tm.t == 0 && first >= v0 && first < v0 + len) sum = (uint32_t)ONE;
@@ -336,7 +346,7 @@ __device__ uint64_t weights(Shared& sh, const Row& r, int v0, int len, int64_t t
 #pragma unroll 4
     for (int i = tm.t * 2; i < len; i += 2 * tm.n) {  // e has an even number of elements
       const int2 x = *(const int2*)(e + i);
-      const uint32_t wx = weight(((int64_t)x.x * inv) >> FRAC_BITS), wy = weight(((int64_t)x.y * inv) >> FRAC_BITS);
+      const uint32_t wx = weight((int64_t)x.x * inv + c), wy = weight((int64_t)x.y * inv + c);
       const uint2 w = make_uint2(wx, i + 1 < len ? wy : 0);
       *(uint2*)(e + i) = w;
       sum += w.x + w.y;
@@ -344,40 +354,37 @@ __device__ uint64_t weights(Shared& sh, const Row& r, int v0, int len, int64_t t
   } else {
 #pragma unroll 1
     for (int i = tm.t; i < len; i += tm.n) {
-      const int x = (int)e[i];
-      e[i] = weight(r.value(x != WIDE ? x : (int64_t)__ldg((const long long*)r.part + i)));
+      e[i] = weight(exact(sh, skip, r, v0, i) * inv + c);
       sum += e[i];
     }
   }
-  uint64_t s = sum;
-  __syncthreads();
-  const int t = own_id(sh, v0, len, tm);
-  if (t >= 0 && !r.greedy()) {
-    s -= e[t];  // what the logit would have weighed, and what it does
-    e[t] = weight((pen * r.inv) >> FRAC_BITS);
-    s += e[t];
-  }
-  return s;
+  return sum;
 }
 
-// Sums over the CTA; every thread gets them.
+// Sums over the CTA's teams of what weights returned; every thread gets them.
 template <int N>
-__device__ __forceinline__ void block_sum(Shared& sh, uint64_t* s) {
-#pragma unroll
-  for (int k = 0; k < N; ++k)
-#pragma unroll
-    for (int m = 16; m >= 1; m >>= 1) s[k] += (uint64_t)shfl_xor_i64((int64_t)s[k], m);
+__device__ __forceinline__ void team_sums(Shared& sh, int n, uint32_t s, uint64_t* out) {
+  s = __reduce_add_sync(0xffffffffu, s);
   __syncthreads();
-  if ((threadIdx.x & 31) == 0)
-#pragma unroll
-    for (int k = 0; k < N; ++k) sh.wsum[k][threadIdx.x >> 5] = s[k];
+  if ((threadIdx.x & 31) == 0) sh.wsum[threadIdx.x >> 5] = s;
   __syncthreads();
+  uint64_t a = 0, b = 0;
 #pragma unroll
-  for (int k = 0; k < N; ++k) {
-    s[k] = 0;
+  for (int w = 0; w < NW / 2; ++w) a += sh.wsum[w], b += sh.wsum[w + NW / 2];
+  out[0] = N == 1 || n == 1 ? a + b : a;
+  if (N == 2) out[1] = n == 1 ? 0 : b;
+}
+
+// The sum over the CTA; every thread gets it.
+__device__ __forceinline__ void block_sum(Shared& sh, uint64_t& s) {
 #pragma unroll
-    for (int w = 0; w < NW; ++w) s[k] += sh.wsum[k][w];
-  }
+  for (int m = 16; m >= 1; m >>= 1) s += (uint64_t)shfl_xor_i64((int64_t)s, m);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) sh.wsum[threadIdx.x >> 5] = s;
+  __syncthreads();
+  s = 0;
+#pragma unroll
+  for (int w = 0; w < NW; ++w) s += sh.wsum[w];
 }
 
 // Exchange of the CTAs' sums mine[0 .. N); total over the cluster, and the
@@ -419,10 +426,10 @@ __device__ int find(Shared& sh, int len, uint64_t t, F val) {
     if (lane >= m) incl += y;
   }
   __syncthreads();
-  if (lane == 31) sh.wsum[0][w] = incl;
+  if (lane == 31) sh.wsum[w] = incl;
   __syncthreads();
   uint64_t before = incl - s;
-  for (int k = 0; k < w; ++k) before += sh.wsum[0][k];
+  for (int k = 0; k < w; ++k) before += sh.wsum[k];
   if (before <= t && t < before + s) {
     int i = a;
     for (before += val(i); before <= t; before += val(i)) ++i;
@@ -448,21 +455,20 @@ __global__ void __launch_bounds__(NT, 3) k_draw(const int64_t* __restrict__ logi
   const int v0 = min(V, (int)rank * seg), len = min(V - v0, seg);
   uint32_t* e = (uint32_t*)dsm;
   uint32_t* skip = e + seg;
-  load_lut(sh.lut, NT);
-  cluster_sync();  // every peer runs: its shared memory may be stored to
+  cluster_arrive();  // waited for before the first store to a peer: it runs by then
   pdl_wait_dep();
   pdl_allow_next();
   const Row r(logits + (size_t)row * ldl, v0, inv_temp[lane]);
-  fetch(r.part, len);
   load_lane(sh, tokens + (size_t)lane * n, parent + (size_t)lane * n, n, hist + lane * HIST, count + lane);
   gather_ids(sh, skip, node0 + blockIdx.y, V, v0, len);
   int64_t top[2];
   int first[2];
   const Team tm{0, (int)threadIdx.x, NT};
-  const int64_t pen = warp_max(sh, skip, r, v0, len, tm, e);
+  warp_max(sh, skip, r, v0, len, tm, e);
+  cluster_wait();
   cluster_max(sh, 1, rank, cs, top, first);
-  uint64_t mine = weights(sh, r, v0, len, top[0], first[0], pen, tm, e);
-  block_sum<1>(sh, &mine);
+  uint64_t mine;
+  team_sums<1>(sh, 1, weights(sh, skip, r, v0, len, top[0], first[0], tm, e), &mine);
   for (int k = 0; k < m; ++k) {
     uint64_t total;
     const uint64_t before = cluster_sum<1>(sh, &mine, k & 1, rank, cs, &total);
@@ -504,14 +510,14 @@ __global__ void __launch_bounds__(NT, 2) k_verify(const int64_t* __restrict__ lo
   uint32_t* P = (uint32_t*)dsm;
   uint32_t* eq = P + seg;
   uint32_t* skip = eq + seg;
-  load_lut(sh.lut, NT);
-  cluster_sync();  // every peer runs: its shared memory may be stored to
+  cluster_arrive();  // waited for before the first store to a peer: it runs by then
   pdl_wait_dep();
   pdl_allow_next();
   const int live = min(n_tree[lane], n);
   int node = WALK ? 0 : blockIdx.y;
   const size_t lane0 = (size_t)lane * n;
   if (node >= live) {  // the whole cluster
+    cluster_wait();
     if (WALK && rank == 0) {
       for (int i = tid; i < n; i += NT) path[lane0 + i] = -1;
       if (tid == 0) n_path[lane] = 0, next[lane] = -1;
@@ -521,6 +527,7 @@ __global__ void __launch_bounds__(NT, 2) k_verify(const int64_t* __restrict__ lo
   load_lane(sh, tokens + lane0, parent + lane0, n, hist + lane * HIST, count + lane);
   u += lane0 * 2;
   int ph = 0, length = 0;
+  bool first_node = true;
   uint64_t kids = 0;  // the node's children whose token is one, not asked yet
   auto next_child = [&]() {
     const int c = kids ? __ffsll((long long)kids) - 1 : live;
@@ -530,6 +537,7 @@ __global__ void __launch_bounds__(NT, 2) k_verify(const int64_t* __restrict__ lo
   for (;;) {
     const size_t row = lane0 + node;
     kids = 0;
+#pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int i = 32 * h + (tid & 31);
       const bool kid = i < live && sh.parent[i] == node && sh.token[i] >= 0 && sh.token[i] < V;
@@ -537,19 +545,18 @@ __global__ void __launch_bounds__(NT, 2) k_verify(const int64_t* __restrict__ lo
     }
     int c = next_child();
     const bool inner = c < live;
-    const Row rt(logits + row * ldl, v0, inv_temp[lane]), rd(dlogits + row * ldd, v0, d_inv_temp[lane]);
-    fetch(rt.part, len);
-    if (inner) fetch(rd.part, len);
     gather_ids(sh, skip, node, V, v0, len);
-    int64_t top[2];
-    int first[2];
     // half of the warps for each of the two rows: one latency, and one copy of
     // the code (instructions come from DRAM too)
     const int n_rows = inner ? 2 : 1, tn = NT / n_rows;
     const Team tm{tid / tn, tid % tn, tn};
-    const Row& r = tm.k ? rd : rt;
+    const Row r(tm.k ? dlogits + row * ldd : logits + row * ldl, v0, (tm.k ? d_inv_temp : inv_temp)[lane]);
     uint32_t* e = tm.k ? eq : P;
-    const int64_t pen = warp_max(sh, skip, r, v0, len, tm, e);
+    warp_max(sh, skip, r, v0, len, tm, e);
+    if (first_node) cluster_wait();
+    first_node = false;
+    int64_t top[2];
+    int first[2];
     cluster_max(sh, n_rows, rank, cs, top, first);
     // one CTA stores what child c's test needs into all of them, with the sums of phase ph
     auto push_child = [&](uint32_t a, uint32_t b, uint32_t e) {
@@ -560,9 +567,9 @@ __global__ void __launch_bounds__(NT, 2) k_verify(const int64_t* __restrict__ lo
       }
     };
     uint64_t mine[2], S[2], before;
-    const uint64_t sum = weights(sh, r, v0, len, top[tm.k], first[tm.k], pen, tm, e);
-    mine[0] = tm.k ? 0 : sum, mine[1] = tm.k ? sum : 0;
-    block_sum<2>(sh, mine);
+    const uint32_t sum =
+        weights(sh, skip, r, v0, len, tm.k ? top[1] : top[0], tm.k ? first[1] : first[0], tm, e);
+    team_sums<2>(sh, n_rows, sum, mine);
     ph ^= 1;
     if (inner && sh.token[c] / seg == (int)rank) push_child(P[sh.token[c] - v0], 0, eq[sh.token[c] - v0]);
     before = cluster_sum<2>(sh, mine, ph, rank, cs, S);
@@ -595,7 +602,7 @@ __global__ void __launch_bounds__(NT, 2) k_verify(const int64_t* __restrict__ lo
       uint64_t s = 0, left;
 #pragma unroll 4
       for (int i = tid; i < len; i += NT) s += rest(i);
-      block_sum<1>(sh, &s);
+      block_sum(sh, s);
       const int c2 = next_child(), d2 = c2 < live ? sh.token[c2] : 0;
       ph ^= 1;
       if (c2 < live && d2 / seg == (int)rank) push_child(P[d2 - v0], rest(d2 - v0), d2 == d ? 0 : eq[d2 - v0]);
@@ -622,7 +629,7 @@ __global__ void __launch_bounds__(NT, 2) k_verify(const int64_t* __restrict__ lo
       }
       uint64_t s = 0, all;
       for (int i = tid; i < len; i += NT) s += P[i];
-      block_sum<1>(sh, &s);
+      block_sum(sh, s);
       ph ^= 1;
       before = cluster_sum<1>(sh, &s, ph, rank, cs, &all);
       const uint64_t t = scale31((uint32_t)u[2 * node + 1], all);
