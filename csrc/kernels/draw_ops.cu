@@ -30,11 +30,18 @@
 // memory until they become weights there.  The sums and the single elements
 // that all of them need cross through distributed shared memory.
 //
-// Verification has two schedules.  Where a cluster per node fills no more than
-// the GPU, every node is decided at once, whether or not the accepted path
-// reaches it, and a second small kernel follows the decisions from the root:
-// one node's latency.  Larger trees and batches take one cluster per lane,
-// which walks from the root and reads only the rows that it meets.
+// Verification has two schedules.  Where clusters for all nodes cost little more
+// than one for the root, every node is decided at once, whether or not the
+// accepted path reaches it, and a second small kernel follows the decisions from
+// the root: one node's latency.  Larger trees and batches take one cluster per
+// lane, which walks from the root and reads only the rows that it meets.
+//
+// What bounds it is latency: a cluster barrier takes half a microsecond, a first
+// touch of DRAM one to two, and a decision needs some eight of them in turn.
+// One row of 32000 takes 9.4 us in the kernel (12.3 us a call), a drafted chain
+// of 5 of them 20 us a call, 8 trees of 31 nodes 45 us, 4 trees of 64 nodes of
+// 102400 59 us.  72 rows of 102400, three tokens of each, take 57 us: 59 MB, two
+// waves of clusters, 1 TB/s.
 #include <atomic>
 #include <climits>
 
@@ -703,10 +710,14 @@ struct Split {
 
 // The cluster size whose clusters finish first: the number that run one after
 // another times what one takes: a fixed part (exchanges and loads: as long as
-// FIXED elements) and its elements, `per` / 4 words of each, the longer the more
-// CTAs share an SM.
+// FIXED elements, and EACH for every CTA) and its elements, `per` / 4 words of
+// each, the longer the more CTAs share an SM.  Measured for three draws of each
+// row, with clusters of 16 / 8 / 4 / 2 CTAs: V = 32000, one row 16.4 / 16.4 /
+// 20.5 / 24.6 us, 24 rows 31 / 21 / 21 / 27, 128 rows 100 / 53 / 43 / 35;
+// V = 102400, one row 21 / 25 / 31 / (no room), 32 rows 43 / 31 / 35, 128 rows
+// 133 / 86 / 82.
 static Split split_of(int64_t rows, int V, int per, int most) {
-  constexpr int FIXED = 16000;
+  constexpr int FIXED = 28000, EACH = 60;
   constexpr int AT_ONCE[4] = {7, 16, 35, 74};  // clusters of 16, 8, 4, 2 CTAs that the GPU's SM groups hold, one CTA per SM
   Split best = {};
   for (int i = 0; i < 4; ++i) {
@@ -716,7 +727,7 @@ static Split split_of(int64_t rows, int V, int per, int most) {
     if (i > 0 && x.smem > SMEM_MAX) break;
     const int64_t held = per_sm(x.smem, most), at_once = AT_ONCE[i] * held, share = (rows * x.cs + 147) / 148;
     const int64_t waves = (rows + at_once - 1) / at_once;
-    x.cost = waves * (FIXED + x.seg * (per / 4) * (share < held ? share : held));
+    x.cost = waves * (FIXED + EACH * x.cs + x.seg * (per / 4) * (share < held ? share : held));
     if (i == 0 || x.cost < best.cost) best = x;
   }
   return best;
@@ -782,7 +793,10 @@ int arcb_verify_tree(const int64_t* logits, int64_t ldl, const int64_t* dlogits,
   cudaStream_t st = (cudaStream_t)stream;
   int* drawn = scratch + (size_t)lanes * n;
   const dr::Split each = dr::split_of((int64_t)lanes * n, V, 8, 2), walk_of = dr::split_of(lanes, V, 8, 2);
-  if (each.cost * 5 > walk_of.cost * 11)  // a path is a few nodes long: all at once for up to the time of 2.2
+  // A path is a few nodes long, so all nodes at once may take the time of 1.7.  Measured, at
+  // once / along the path, V = 32000: 16 nodes of a lane 25 / 38 us, 31 nodes 28 / 38, 64 nodes
+  // 47 / 37, 8 lanes of 31 nodes 90 / 45; V = 102400: 13 nodes 37 / 44, 31 nodes 49 / 39.
+  if (each.cost * 10 > walk_of.cost * 17)
     return dr::launch_cluster(dr::k_verify<true>, walk, walk_of.cs, dim3(walk_of.cs, 1, lanes), walk_of.smem, st, logits,
                               ldl, dlogits, ldd, V, n, tokens, parent, n_tree, inv_temp, d_inv_temp, u, hist, count,
                               walk_of.seg, scratch, drawn, path, n_path, next);
