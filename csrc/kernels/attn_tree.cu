@@ -101,10 +101,10 @@ struct Args {
 
 // What a tile's stored scores need added to be relative to the row's max.  A
 // score that is not seen is stored as FAR; both clamps leave its exp 0 and
-// the sum within int32.
+// the sum within int32.  EXP_AT more: exp32's second argument.
 __device__ __forceinline__ int rebase(int64_t ref, int64_t row_max) {
   const int64_t d = ref - row_max;
-  return d < FAR ? FAR : (d > SMALL ? SMALL : (int)d);
+  return (d < FAR ? FAR : (d > SMALL ? SMALL : (int)d)) + EXP_AT;
 }
 
 // Four int64 -> digit words: plane l's word in p[l]; the low and high digit
@@ -504,11 +504,11 @@ __global__ void __launch_bounds__(NT_S, 2) k_scores(const __grid_constant__ Args
 // grid (chunks, n_kv * groups, lanes): a thread takes four rows of every
 // (threads / (RG / 4))-th key.
 __global__ void __launch_bounds__(NT_V) k_sums(const __grid_constant__ Args A) {
-  __shared__ int2 lut[EXP_LUT_N];
+  __shared__ int2 lut[EXP_TABLE_N];
   __shared__ int64_t rmax[MAX_RG];
-  __shared__ unsigned long long rsum[MAX_RG];
+  __shared__ uint32_t rlow[MAX_RG], rhigh[MAX_RG];  // sums of 24-bit words: 64-bit shared atomics are loops
   const int NT = blockDim.x, tid = threadIdx.x, RG = A.RG;
-  load_lut(lut, NT);
+  load_exp(lut, NT);
   pdl_wait_dep();
   pdl_allow_next();
   const int kvh = blockIdx.y / A.groups, grp = blockIdx.y % A.groups, r0 = grp * RG, rows = min(RG, A.R - r0);
@@ -519,7 +519,7 @@ __global__ void __launch_bounds__(NT_V) k_sums(const __grid_constant__ Args A) {
   if ((int)blockIdx.x >= X) return;
   const int t0 = (int)((int64_t)blockIdx.x * nt / X), t1 = (int)((int64_t)(blockIdx.x + 1) * nt / X);
   const int64_t* ref = A.ref + lk * A.tiles * A.Rp + r0;
-  if (tid < RG) rmax[tid] = tid < rows ? A.gmax[lk * A.Rp + r0 + tid] : NONE, rsum[tid] = 0;
+  if (tid < RG) rmax[tid] = tid < rows ? A.gmax[lk * A.Rp + r0 + tid] : NONE, rlow[tid] = rhigh[tid] = 0;
   __syncthreads();
   const int q = tid % (RG / 4) * 4, k0 = tid / (RG / 4), kl = NT / (RG / 4);
   uint64_t s[4] = {0, 0, 0, 0};
@@ -532,19 +532,23 @@ __global__ void __launch_bounds__(NT_V) k_sums(const __grid_constant__ Args A) {
 #pragma unroll 8
     for (int k = k0; k < TILE; k += kl) {
       const int4 x = *(const int4*)(S + k * RG);
-      p[0] += exp32(x.x + off[0], lut);
-      p[1] += exp32(x.y + off[1], lut);
-      p[2] += exp32(x.z + off[2], lut);
-      p[3] += exp32(x.w + off[3], lut);
+      p[0] += exp32(x.x, off[0], lut);
+      p[1] += exp32(x.y, off[1], lut);
+      p[2] += exp32(x.z, off[2], lut);
+      p[3] += exp32(x.w, off[3], lut);
     }
 #pragma unroll
     for (int c = 0; c < 4; ++c) s[c] += p[c];
   }
 #pragma unroll
   for (int c = 0; c < 4; ++c)
-    if (q + c < rows) atomicAdd(&rsum[q + c], (unsigned long long)s[c]);
+    if (q + c < rows) {
+      atomicAdd(&rlow[q + c], (uint32_t)s[c] & 0xffffff);
+      if (s[c] >> 24) atomicAdd(&rhigh[q + c], (uint32_t)(s[c] >> 24));
+    }
   __syncthreads();
-  if (tid < rows) atomicAdd((unsigned long long*)A.sums + lk * A.Rp + r0 + tid, rsum[tid]);
+  if (tid < rows)
+    atomicAdd((unsigned long long*)A.sums + lk * A.Rp + r0 + tid, rlow[tid] + ((unsigned long long)rhigh[tid] << 24));
 }
 
 // ------------------------------------------------------------------ 3. values
@@ -583,7 +587,7 @@ template <int DPL, int UR, int CK, bool FEW>
 __global__ void __launch_bounds__(NT_V, 2) k_values(const __grid_constant__ Args A) {
   extern __shared__ __align__(1024) uint8_t dsm[];
   constexpr int DHP = 32 * DPL;
-  __shared__ int2 lut[EXP_LUT_N];
+  __shared__ int2 lut[EXP_TABLE_N];
   __shared__ int64_t rmax[MAX_RG];
   __shared__ uint64_t rsum[MAX_RG];
   __shared__ __align__(16) float rrcp[MAX_RG];     // ONE / sum
@@ -597,7 +601,7 @@ __global__ void __launch_bounds__(NT_V, 2) k_values(const __grid_constant__ Args
   float* wbuf = (float*)(dsm + 2 * vbytes);            // 2 x [CK][RG] scores, then weights in place
   int64_t* rbuf = (int64_t*)(dsm + 2 * (vbytes + sbytes));  // 2 x [RG] what the scores are relative to
   int* osum = (int*)dsm;                               // [RG][DHP] at a segment's end
-  load_lut(lut, NT);
+  load_exp(lut, NT);
   if (tid == 0) {
     s_need = 0;
     mbar_init(smem_u32(&full[0]), 1);
@@ -666,10 +670,10 @@ __global__ void __launch_bounds__(NT_V, 2) k_values(const __grid_constant__ Args
 #pragma unroll 4
         for (int k = kq; k < k1; k += kq_step) {
           const int4 v = *(const int4*)(S + k * RG);
-          s[0] += exp32(v.x + off4[0], lut);
-          s[1] += exp32(v.y + off4[1], lut);
-          s[2] += exp32(v.z + off4[2], lut);
-          s[3] += exp32(v.w + off4[3], lut);
+          s[0] += exp32(v.x, off4[0], lut);
+          s[1] += exp32(v.y, off4[1], lut);
+          s[2] += exp32(v.z, off4[2], lut);
+          s[3] += exp32(v.w, off4[3], lut);
         }
       }
 #pragma unroll
@@ -784,7 +788,7 @@ __global__ void __launch_bounds__(NT_V, 2) k_values(const __grid_constant__ Args
             float o[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              const uint32_t e = (uint32_t)exp32(xs[i] + ro[i], lut);
+              const uint32_t e = exp32(xs[i], ro[i], lut);
               const float qf = __fmaf_rd(__uint_as_float(0x4B000000u + e) - 8388608.0f, rcp[i], 8388608.0f);
               const int rem = (int)((e << 16) - (__float_as_uint(qf) - 0x4B000000u) * den[i]);
               o[i] = qf - (rem < 0 ? 8388609.0f : (rem >= (int)den[i] ? 8388607.0f : 8388608.0f));
@@ -794,7 +798,7 @@ __global__ void __launch_bounds__(NT_V, 2) k_values(const __grid_constant__ Args
         } else {
           for (int k = kq; k < CK; k += kq_step)
             for (int i = 0; i < 4; ++i) {
-              const int64_t e = exp32(__float_as_int(wq[k * RG + i]) + ro[i], lut);
+              const int64_t e = exp32(__float_as_int(wq[k * RG + i]), ro[i], lut);
               wq[k * RG + i] = (float)(int)(e * ONE / (int64_t)rsum[rq + i]);
             }
         }

@@ -47,7 +47,7 @@
 
 #include "../common/tree.h"
 #include "common.cuh"
-#include "lut.cuh"
+#include "exp32.cuh"
 
 using namespace q16;
 
@@ -102,7 +102,7 @@ __device__ __forceinline__ uint32_t div31(uint64_t num, uint64_t den, double rcp
 // (reading sixteen peers one after another cost 2 us an exchange).  Sums come
 // in two phases, so that the next exchange may start while a peer still reads.
 struct Shared {
-  int2 lut[EXP_LUT_N];
+  int2 lut[EXP_TABLE_N];
   int64_t redv[NW];  // the first row's warps, then the second's
   int redi[NW];
   uint64_t wsum[NW];
@@ -118,17 +118,13 @@ struct Shared {
 };
 
 // The lane's tree (each node's token and parent, -1 where that is no earlier
-// node), its ring, and the table of exps (entries times 2^11,
-// see weights): all loads at once.
+// node), its ring, and the table of exps: all loads at once.
 __device__ __forceinline__ void load_lane(Shared& sh, const int* tokens, const int* parent, int n, const int* hist,
                                           const int* count) {
   static_assert(EXP_LUT_N <= NT && tree::MAX_NODES + HIST < NT, "one element a thread");
   const int tid = threadIdx.x, i = min(tid, n - 1), h = tid & (HIST - 1);
   const int token = __ldg(tokens + i), up = tree::parent_of(parent, i), id = __ldg(hist + h), c = __ldg(count);
-  if (tid < EXP_LUT_N) {
-    const int lo = (int)g_exp_lut.v[tid];
-    sh.lut[tid] = make_int2(lo << 11, tid < EXP_LUT_N - 1 ? (int)g_exp_lut.v[tid + 1] - lo : 0);
-  }
+  if (tid < EXP_LUT_N) sh.lut[tid] = exp_entry(tid);
   if (tid < n) sh.token[tid] = token, sh.parent[tid] = up;
   if (tid < HIST) sh.hist[tid] = id;
   if (tid == 0) sh.count = max(c, 0);
@@ -332,18 +328,15 @@ __device__ void cluster_max(Shared& sh, int n, uint32_t rank, uint32_t cs, int64
 // 2^16 (and 2^15 in a warp).  `top` is the row's largest clamped logit, `first`
 // its index.
 //
-// With zt the scaled top, the place in the table off = max(z - zt + EXP_RANGE, 0)
-// comes of one product and sum: x * inv - ((zt - EXP_RANGE) << 16), shifted; no
-// x is above the top.  The table holds (entry << 11, step): one more product and
-// shift, ((entry << 11) + step * (off mod 2^11)) >> 11.
+// With zt the scaled top, z - zt + EXP_AT comes of one product and sum,
+// x * inv - ((zt - EXP_AT) << 16), shifted; no x is above the top.
 __device__ uint32_t weights(Shared& sh, const uint32_t* skip, const Row& r, int v0, int len, int64_t top, int first,
                             const Team& tm, uint32_t* e) {
-  const int64_t zt = r.value(top), c = -((zt - EXP_RANGE) << FRAC_BITS);
+  const int64_t zt = r.value(top), c = -((zt - EXP_AT) << FRAC_BITS);
   const int inv = (int)r.inv;
   auto weight = [&](int64_t y) {  // y = x * inv + c
-    const int off = max((int)__funnelshift_r((uint32_t)y, (uint32_t)max((int)(y >> 32), -32768), FRAC_BITS), 0);
-    const int2 t = *(const int2*)((const uint8_t*)sh.lut + (off >> 8 & 0xff8));
-    return off > 0 ? (uint32_t)(t.x + t.y * (off & 2047)) >> 11 : 0u;
+    const int at = (int)__funnelshift_r((uint32_t)y, (uint32_t)max((int)(y >> 32), -32768), FRAC_BITS);
+    return exp_at(max(at, 2047), sh.lut);
   };
   uint32_t sum = 0;
   if (r.greedy()) {
