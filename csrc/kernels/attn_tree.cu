@@ -656,10 +656,10 @@ __global__ void __launch_bounds__(NT_V, 2) k_values(const __grid_constant__ Args
 #pragma unroll 4
           for (int t = 0; t < nt; ++t) m = max(m, A.M[(lk * A.tiles + t) * A.Rp + tid]);
         rmax[tid] = m;
-        rsum[tid] = 0;
+        rden[tid] = 0;
       }
       __syncthreads();
-      uint64_t s[4] = {0, 0, 0, 0};
+      uint32_t s[4] = {0, 0, 0, 0};  // FEW_MOST exps at most
       for (int t = 0; t < nt; ++t) {
         const int64_t* ref = A.ref + (lk * A.tiles + t) * A.Rp + rq;
         const int* S = A.S + (lk * A.tiles + t) * (size_t)TILE * RG + rq;
@@ -678,12 +678,12 @@ __global__ void __launch_bounds__(NT_V, 2) k_values(const __grid_constant__ Args
       }
 #pragma unroll
       for (int c = 0; c < 4; ++c)
-        if (rq + c < rows) atomicAdd((unsigned long long*)&rsum[rq + c], (unsigned long long)s[c]);
+        if (rq + c < rows) atomicAdd(&rden[rq + c], s[c]);
       __syncthreads();
     }
     if (live && tid < RG) {
       const bool row = tid < rows;
-      const uint64_t s = FEW ? rsum[tid] : (row ? A.sums[lk * A.Rp + r0 + tid] : 0);
+      const uint64_t s = FEW ? rden[tid] : (row ? A.sums[lk * A.Rp + r0 + tid] : 0);
       if (!FEW) rmax[tid] = row ? A.gmax[lk * A.Rp + r0 + tid] : NONE;
       rsum[tid] = s ? s : 1;  // a row without keys: every exp is 0
       rden[tid] = (uint32_t)rsum[tid];
