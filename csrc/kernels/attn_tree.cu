@@ -61,10 +61,10 @@ constexpr int FAR = -(1 << 30);     // a score whose exp is 0
 constexpr int64_t NONE = -(int64_t(1) << 62);  // max of no keys
 constexpr int VMAX = (1 << 22) - (1 << 17);    // values of the single-precision form
 constexpr int SMEM_V = 2 * (32 * (128 * 8 + MAX_RG * 4) + MAX_RG * 8);  // k_values shared memory, at most
-// Lanes * rows * keys up to which two kernels do the work of four (FEW).  Measured, two against
-// four: 32 heads of 128, one lane, 16 rows, 250 keys 40 / 43 us, 506 keys 47 / 52, 1018 keys
-// 64 / 63; 31 rows of 506 keys 55 / 55; 4 lanes, 16 rows, 250 keys 68 / 67; 8 lanes, 31 rows, 500
-// keys 142 / 131; 64 heads over 8, one lane, 4 nodes, 250 keys 41 / 42, 506 keys 47 / 43.
+// Rows * keys of a lane and KV head up to which two kernels do the work of four (FEW).
+// Measured, two against four: 32 heads of 128, one lane, 16 rows, 250 keys 34 / 37 us, 506 keys
+// 40 / 44, 1018 keys 54 / 51; 31 rows of 250 keys 40 / 42; 4 lanes of 31 rows 65 / 64; 16 lanes
+// of 8 rows, 250 keys 116 / 119; 64 heads over 8, 4 nodes, 250 keys 38 / 39, 506 keys 42 / 41.
 constexpr int FEW_MOST = 1 << 13;
 constexpr int MAX_RANGE = 1 << 16;             // keys per k_values CTA: VMAX + MAX_RANGE < 2^22
 
@@ -955,7 +955,7 @@ static Plan plan(int lanes, int nq, int n_heads, int n_kv, int dh, int t_lim) {
   p.oQ = take(lk * p.qgroups * PLANES * RQ * 128);
   p.oI = take(lk * p.qgroups * sizeof(uint4));
   p.oR = take(lk * p.tiles * p.Rp * 8);
-  p.few = p.R <= RQ && (int64_t)lanes * p.RG * t_lim <= FEW_MOST;
+  p.few = p.R <= RQ && (int64_t)p.RG * t_lim <= FEW_MOST;
   p.oM = take(p.few ? lk * p.tiles * p.Rp * 8 : 0);
   p.oG = take(lk * p.Rp * 8);
   p.oSum = take(lk * p.Rp * 8);
