@@ -320,7 +320,7 @@ __global__ void __launch_bounds__(NT_S, 2) k_scores(const __grid_constant__ Args
     }
     const int j = j0 + (w & 3) * 32 + ln;  // this thread's key in the epilogue
     const size_t group_elems = (size_t)TILE * A.RG;
-    int* Srow = A.S + (lk * A.tiles + tile) * A.groups * group_elems + (size_t)((w & 3) * 32 + ln) * A.RG;
+    int* S0 = A.S + (lk * A.tiles + tile) * A.groups * group_elems;
     const int kend = (A.dh + 31) / 32;
     const bool all_seen = j0 + TILE <= base;  // every key of the tile is below the tree
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -386,7 +386,6 @@ __global__ void __launch_bounds__(NT_S, 2) k_scores(const __grid_constant__ Args
             if (tree::visible(j, base, nt, qmask[b][c0 + i])) seen |= 1u << i;
         }
         int out[16];
-        int64_t m64 = NONE;  // lane i: max of row c0 + i over the warp's keys
         if (small) {
           // dot >> 16 = D_2 + (D_3 << 8) + (D_4 << 16) + .. + ((D_0 + (D_1 << 8)) >> 16): modulo 2^32
           uint32_t r[16], t[16];
@@ -410,17 +409,13 @@ __global__ void __launch_bounds__(NT_S, 2) k_scores(const __grid_constant__ Args
               for (int i = 0; i < 16; ++i) t[i] += r[i] << (8 * s - 16);
             }
           const int sc = (int)A.attn_scale << 16;  // (x * scale) >> 16 = the high word of x * (scale << 16)
-          int m32 = FAR;
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             out[i] = __mulhi((int)t[i], sc);
             if (!all_seen && !(seen >> i & 1)) out[i] = FAR;
-            const int m = __reduce_max_sync(0xffffffffu, out[i]);
-            if (ln == i) m32 = m;
           }
-          m64 = m32 == FAR ? NONE : m32;
         } else {
-          int64_t sc[16];
+          int64_t sc[16], m64 = NONE;  // lane i: max of row c0 + i over the warp's keys
 #pragma unroll
           for (int i = 0; i < 16; ++i) sc[i] = 0;
           if (!wide) {
@@ -471,12 +466,38 @@ __global__ void __launch_bounds__(NT_S, 2) k_scores(const __grid_constant__ Args
             out[i] = (seen >> i & 1) && d > FAR ? (int)d : FAR;
           }
         }
-        if (ln < 16) wmax[b][w & 3][c0 + ln] = m64;
-        // 16 rows lie in one group: RG is a multiple of 16, or the only group's 8
-        int* dst = Srow + (r0 + c0) / A.RG * group_elems + (r0 + c0) % A.RG;
+        // Four lanes' scores of 16 rows become each lane's of four rows of the four keys, so that
+        // a store writes whole 64-byte pieces of a key's rows.
 #pragma unroll
-        for (int i = 0; i < 16; i += 4)
-          if (c0 + i < rows) *(int4*)(dst + i) = make_int4(out[i], out[i + 1], out[i + 2], out[i + 3]);
+        for (int x = 1; x <= 2; x <<= 1) {
+          const bool up = ln & x;
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            if (!(q & x))
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                int &lo_ = out[4 * q + i], &hi_ = out[4 * (q + x) + i];
+                const int got = __shfl_xor_sync(0xffffffffu, up ? lo_ : hi_, x);
+                (up ? lo_ : hi_) = got;
+              }
+        }
+        // 16 rows lie in one group: RG is a multiple of 16, or the only group's 8
+        const int c4 = c0 + 4 * (ln & 3);
+        int* dst = S0 + (size_t)((r0 + c0) / A.RG) * group_elems + (r0 + c4) % A.RG;
+        if (c4 < rows)
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            *(int4*)(dst + ((w & 3) * 32 + (ln & ~3) + k) * A.RG) =
+                make_int4(out[4 * k], out[4 * k + 1], out[4 * k + 2], out[4 * k + 3]);
+        if (small) {  // the rows' maxima over the warp's keys
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            int m = max(max(out[i], out[4 + i]), max(out[8 + i], out[12 + i]));
+#pragma unroll
+            for (int x = 4; x <= 16; x <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, x));
+            if (ln < 4) wmax[b][w & 3][c4 + i] = m == FAR ? NONE : m;
+          }
+        }
       }
       tc_fence_before();
       __syncthreads();  // wmax; this group's accumulators and query planes are read
