@@ -110,7 +110,11 @@ def attn_tree(q, Kc, Vc, pt, base, n_tree, mask, n_heads: int, n_kv: int, dh: in
     Outputs: the limb planes X of the W_o operand with their count lmax
     (int_ops.limb_row layout of lanes * nq slots), and / or o_out [lanes * nq,
     n_heads * dh] int64.  A lane whose lengths or pages are out of range gets
-    zeros and sets a bit of err."""
+    zeros and sets a bit of err.
+
+    A call takes a workspace of 4 bytes per query row, query head and key up to
+    t_lim for as many lanes as about 1 GB holds (one at least); the others
+    follow in further launches."""
     if lanes < 1 or nq < 1 or lanes * nq > 65535:
         raise ValueError(f"lanes and nq must be at least 1 and lanes * nq at most 65535, got {lanes} and {nq}")
     if n_kv < 1 or n_heads < 1 or n_heads % n_kv:
@@ -119,6 +123,8 @@ def attn_tree(q, Kc, Vc, pt, base, n_tree, mask, n_heads: int, n_kv: int, dh: in
         raise ValueError(f"dh must be a multiple of 8 up to 128, got {dh}")
     if t_lim < 1:
         raise ValueError(f"t_lim must be at least 1, got {t_lim}")
+    if not -1 << 63 <= attn_scale < 1 << 63:
+        raise ValueError(f"attn_scale must be a 64-bit integer, got {attn_scale}")
     B, d = lanes * nq, n_heads * dh
     dev = _device("Kc", Kc, 4)
     pages = Kc.shape[0]
@@ -126,6 +132,7 @@ def attn_tree(q, Kc, Vc, pt, base, n_tree, mask, n_heads: int, n_kv: int, dh: in
     _check(dev, ("q", q, I64, (B, d)), ("Kc", Kc, I64, cache), ("Vc", Vc, I64, cache), ("base", base, I32, (lanes,)),
            ("n_tree", n_tree, I32, (lanes,)), ("mask", mask, I64, (B,)), ("err", err, I32, (1,)))
     ps = _rows(dev, "pt", pt, I32, lanes, 1)
+    t_lim = min(t_lim, pt.shape[1] * PAGE)  # no lane has more keys than its pages hold
     at = q.data_ptr() | Kc.data_ptr() | Vc.data_ptr()
     if X is None and o_out is None:
         raise ValueError("one of X and o_out must be given")

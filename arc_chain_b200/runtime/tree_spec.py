@@ -278,9 +278,15 @@ class TreeSpecDecoder:
     def generate(self, prompts: Sequence[Sequence[int]], max_tokens: int, eos: Sequence[int] = ()) \
             -> List[Tuple[List[int], bytes]]:
         """Tokens and output hash of each prompt.  Request i of a call uses
-        random stream i of the decoder's seed."""
+        random stream i of the decoder's seed.  A request takes positions for
+        its prompt, max_tokens and one tree, up to the engines' max_seq."""
         if len(prompts) != self.n_lanes:
             raise ValueError(f"one prompt per lane: {self.n_lanes} lanes, {len(prompts)} prompts")
+        most = min(e.max_seq for e in (self.t, self.d) if e is not None)
+        for p in prompts:
+            if 1 + len(p) + max_tokens + self.n > most:
+                raise ValueError(f"a prompt of {len(p)} tokens, {max_tokens} new ones and a tree of {self.n} nodes "
+                                 f"exceed max_seq {most}")
         ends = set(int(e) for e in eos)
         lanes: List[_Lane] = []
         try:

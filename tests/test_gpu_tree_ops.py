@@ -295,6 +295,21 @@ def test_attn_tree_lanes_in_several_launches():
     np.testing.assert_array_equal(got.cpu().numpy(), want)
 
 
+def test_attn_tree_key_limit_beyond_the_table():
+    """t_lim bounds lengths only as far as the table's pages reach."""
+    a = Attn(64, 4, 2, [40, 70], [5, 6], 5, 2, M18, M18)
+    want = a.want()
+    for t_lim in (a.width * PAGE + 1, 1 << 30, 1 << 40):
+        got, err = a.run(t_lim=t_lim)
+        assert err == 0
+        np.testing.assert_array_equal(got.cpu().numpy(), want)
+    a.base[0] = a.width * PAGE - 4  # 5 nodes: one beyond the table
+    want[:5] = 0
+    got, err = a.run(t_lim=1 << 30)
+    assert err == ERR_SEQ
+    np.testing.assert_array_equal(got.cpu().numpy(), want)
+
+
 def test_attn_tree_equals_decode_attention():
     """Chain queries equal the decode kernel at consecutive positions."""
     from arc_chain_b200.ops import int_ops
@@ -401,6 +416,22 @@ def test_verify_tree_ragged_strange_and_masked():
     r.count[:] = [64, 64, 14, 64, 64, 64]
     n_path = r.check()
     assert n_path[0] == 0 and n_path[5] == 0
+
+
+def test_largest_vocabulary():
+    from arc_chain_b200.ops import tree_ops as ops
+
+    V = ops.lib_max_vocab()
+    r = Rows(1, 3, V, fan=2, seed=8)
+    r.tokens[0, 1] = V - 1
+    r.check()
+    out = torch.full((3, 2), 9, dtype=I32, device="cuda")
+    u = np.array([[0, 1 << 30], [(1 << 31) - 1, 5], [77, 1 << 29]], np.int32)
+    ops.draw_tokens(dev(r.logits), V, 1, 3, 0, 2, dev(r.inv), dev(u), dev(r.hist), dev(r.count), dev(r.tokens),
+                    dev(r.parent), out)
+    for i in range(3):
+        ids = spec.tree_history(r.tokens[0], r.parent[0], r.hist[0], max(int(r.count[0]), 0), i)
+        assert out[i].tolist() == spec.draw_tokens(r.logits[i], ids, int(r.inv[0]), u[i]), i
 
 
 def test_verify_tree_one_lane_equals_its_place_in_a_batch():

@@ -122,6 +122,24 @@ def test_sampled_equals_the_simulation(branches, temp, dtemp):
     assert target.kv.pool.used <= 1
 
 
+def test_the_longest_request_and_one_beyond():
+    """The last positions of max_seq, which is no multiple of a page here."""
+    from arc_chain_b200.models import dense
+    from arc_chain_b200.runtime.engine import Engine
+    from arc_chain_b200.runtime.tree_spec import TreeSpecDecoder
+
+    cfg = preset("micro_gqa")
+    host = gen.random_model(cfg, 0)
+    target, draft = (Engine(dense.from_host(host, "cuda"), max_seq=m) for m in (77, 73))
+    p = gen.seeded_prompt(40, cfg.vocab, 5)
+    sd = TreeSpecDecoder(target, draft, (2, 2), 1, draft_temperature=0.0)
+    toks, _ = sd.generate([p], 73 - 41 - 7)[0]
+    assert toks == arcref.Model(host).generate(p, 73 - 41 - 7)[0]
+    with pytest.raises(ValueError, match="max_seq 73"):
+        sd.generate([p], 73 - 41 - 6)
+    assert target.check_errors() == 0 and draft.check_errors() == 0 and target.kv.pool.used <= 1
+
+
 def test_command_line_samples(capsys):
     import json
 

@@ -80,6 +80,20 @@ def test_attn_tree_refuses(bad, exc):
         ops.attn_tree(**_attn_args(**bad))
 
 
+def test_attn_tree_refuses_unaligned_tensors_and_wide_scales():
+    from arc_chain_b200.ops import tree_ops as ops
+
+    good = _attn_args()
+    for name in ("q", "Kc", "Vc", "o_out"):
+        t = good[name]
+        moved = torch.zeros(t.numel() + 1, dtype=t.dtype)[1:].view(t.shape)
+        with pytest.raises(ValueError, match="16-byte"):
+            ops.attn_tree(**{**good, name: moved})
+    for scale in (1 << 63, -(1 << 63) - 1):
+        with pytest.raises(ValueError, match="64-bit"):
+            ops.attn_tree(**{**good, "attn_scale": scale})
+
+
 def _verify_args(**kw):
     lanes, n, V = 2, 4, 10
     z = dict(logits=torch.zeros(lanes * n, V, dtype=I64), dlogits=torch.zeros(lanes * n, V, dtype=I64), V=V,
