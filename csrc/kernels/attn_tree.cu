@@ -21,8 +21,8 @@
 //  1. k_scores, one CTA per 128 keys.  K's int64 elements become signed
 //     radix-256 digits (byte l of (x + 0x80..80) ^ 0x80..80, int8), one
 //     128-byte-swizzled plane of 128 keys x dh per digit, read once from DRAM;
-//     the query rows' planes come by bulk copies, 32 rows at a time.  q.k = sum over digit pairs (a, b) of
-//     D_{a+b} << 8(a+b) with D_s = sum_{a+b=s} K_a.Q_b^T: tcgen05 kind::i8
+//     the query rows' planes come by bulk copies, 32 rows at a time.  q.k =
+//     sum_s D_s << 8s with D_s = sum_{a+b=s} K_a.Q_b^T: tcgen05 kind::i8
 //     products of M = 128 keys, N = 32 rows into one TMEM accumulator per s
 //     (exact in int32: at most 4 * 128 * 2^14).  3 digits (|x| < 2^23) are
 //     usual; up to 4 (|x| < 2^31) run this way, wider tiles take 64-bit
@@ -39,6 +39,12 @@
 //     Chunks with wider values take 64-bit terms.
 //     CTAs that share a lane add their sums with atomics (integers: any order
 //     gives the same), two int32 in one 64-bit word; the last to arrive writes.
+//
+// Measured, a call and its kernels 0 to 3 by themselves: 4 lanes of 64 nodes, 64
+// heads over 8 KV heads, up to 1552 keys 314 us (9, 88, 31, 198); 9 nodes, 30
+// thousand keys 362 us (5, 118, 38, 210: K and V, 493 MB, at 1.4 TB/s); 8 lanes
+// of 31 nodes, 32 heads, up to 528 keys 122 us (6, 41, 13, 64); 16 nodes, 402
+// keys 37 us; 5 nodes, 42 keys, 4 heads 24 us.
 #include <atomic>
 
 #include "../common/tree.h"
@@ -223,6 +229,11 @@ __device__ __forceinline__ void bulk_g2s(uint32_t dst, const void* src, uint32_t
 }
 
 // grid (tiles, n_kv * row blocks of rows_s, lanes).
+// Two CTAs an SM take turns at the tensor cores, the loads of K (two rounds of
+// 64 KB a CTA) and the epilogues, of which each group of 32 rows costs about 2300
+// cycles, its products 1300 and the steps between them 1500; a ninth warp that
+// issues the products a group ahead took the same time (wide trees 84 us against
+// 88, long ones 122 against 119), and so did K's second round fetched ahead.
 // DHP: row pitch class of the planes (64 or 128 >= dh).
 // FEW: at most RQ rows, whose digits each CTA makes itself; the tiles' maxima
 // are stored for k_values, which does k_sums' work too: two launches.
@@ -523,7 +534,8 @@ __global__ void __launch_bounds__(NT_S, 2) k_scores(const __grid_constant__ Args
 
 // -------------------------------------------------------------------- 2. sums
 // grid (chunks, n_kv * groups, lanes): a thread takes four rows of every
-// (threads / (RG / 4))-th key.
+// (threads / (RG / 4))-th key.  About 20 instructions an exp and a table lookup:
+// 19 million exps of 77 MB in 31 us.
 __global__ void __launch_bounds__(NT_V) k_sums(const __grid_constant__ Args A) {
   __shared__ int2 lut[EXP_TABLE_N];
   __shared__ int64_t rmax[MAX_RG];
@@ -602,6 +614,11 @@ __device__ __forceinline__ int store_limbs4(int8_t* X, int slot, int B, size_t l
 // copies, one chunk ahead.  A warp takes UR rows (unit) x all dims, a lane
 // the dims 2 ln, 2 ln + 1 (and 64 + those); kparts warps per unit take every
 // kparts-th key.
+// Bound by the FMAs and what feeds them: of 130 million warp instructions for 4 x
+// 64 nodes, 58 % are FMAs (their pipe 51 % busy, issue slots 65 %), the rest the
+// weights, the conversion of V and the loads from shared memory.  FMAs of two
+// terms run at the same rate and cost moves; warps that only convert and weigh
+// while others add were no faster.
 // FEW: at most RQ rows (one group) of few keys; each segment finds its rows'
 // maxima and sums from all scores of the lane.
 template <int DPL, int UR, int CK, bool FEW>
@@ -939,6 +956,8 @@ static Plan plan(int lanes, int nq, int n_heads, int n_kv, int dh, int t_lim) {
   p.G = n_heads / n_kv;
   p.R = nq * p.G;
   p.groups = (p.R + MAX_RG - 1) / MAX_RG;
+  // rows a warp holds: 16, or the only 8 (8 query heads of one node a lane, 32 lanes of 2000
+  // keys: 307 us, padded to 16 358; 4 nodes of 8 lanes, 500 keys: 110 and 128)
   p.unit = p.R <= 8 ? 8 : 16;
   p.RG = ((p.R + p.groups - 1) / p.groups + p.unit - 1) / p.unit * p.unit;
   p.Rp = p.groups * p.RG;
@@ -950,8 +969,8 @@ static Plan plan(int lanes, int nq, int n_heads, int n_kv, int dh, int t_lim) {
   const int units = p.RG / p.unit;
   p.threads = 32 * units * (units >= 5 ? 1 : (units >= 3 ? 2 : (units == 2 ? 4 : 8)));
   // five-warp value CTAs run three to an SM with chunks of one page (9 nodes, 8 query
-  // heads per KV head, 30 thousand keys: 281 us against 322 with two and two pages); the
-  // others two, with two pages (64 nodes: 207 us, 240 with one page)
+  // heads per KV head, 30 thousand keys: a call 362 us against 393 with two and two pages);
+  // the others two, with two pages (64 nodes: 315 us, 325 with one page)
   p.per_sm = p.threads == 160 ? 3 : 2;
   // the lanes' keys are divided evenly over the CTAs that run at once; a CTA's
   // part of a lane stays below MAX_RANGE keys
@@ -961,7 +980,8 @@ static Plan plan(int lanes, int nq, int n_heads, int n_kv, int dh, int t_lim) {
   if (p.splits < least) p.splits = (int)least;
   p.chunks = (12 * 148 + have - 1) / have;  // of the sums: short ones, many loads in flight
   if (p.chunks > p.tiles) p.chunks = p.tiles;
-  // score CTAs take all rows of their tile unless that leaves SMs idle (two CTAs each)
+  // score CTAs take all rows of their tile unless that leaves SMs idle (two CTAs each, and
+  // tiles without keys): 4 lanes of 64 nodes in two blocks of rows 88 us, in one 103
   const int blocks = p.tiles * n_kv * p.lanes, want = (4 * 148 + blocks - 1) / blocks, most = (p.R + 63) / 64;
   p.rows_s = ((p.R + (want < most ? want : most) - 1) / (want < most ? want : most) + RQ - 1) / RQ * RQ;
   size_t o = 0;
