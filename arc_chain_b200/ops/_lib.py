@@ -55,7 +55,7 @@ _SIGS = {
                              vp, vp]),
     "arcb_draw_max_vocab": (i32, []),
     "arcb_draw_tokens": (i32, [vp, i64, i32, i32, i32, i32, i32, i32, vp, vp, vp, vp, vp, vp, vp, vp]),
-    "arcb_verify_tree": (i32, [vp, i64, vp, i64, i32, i32, i32, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp]),
+    "arcb_verify_tree": (i32, [vp, i64, vp, i64, i32, i32, i32, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp]),
     "arcb_kv_keep_path": (i32, [vp, i32, i32, i32, i32, vp, i64, i32, vp, vp, vp, i32, i32, vp, vp]),
     "arcb_set_pdl": (None, [i32]),
     "arcb_set_attn_paged": (None, [i32]),

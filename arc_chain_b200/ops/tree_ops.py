@@ -47,11 +47,16 @@ def _refuse(what: str, t, dtype, shape, dev) -> None:
 
 
 def _check(dev, *specs) -> None:
-    """Every (name, tensor, type, shape) is a contiguous tensor on dev."""
-    for what, t, dtype, shape in specs:
-        if not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.shape != shape or not t.is_contiguous() \
-                or t.device != dev:
-            _refuse(what, t, dtype, shape, dev)
+    """Every (name, tensor, type, shape) is a contiguous tensor on dev.  On the
+    path of calls of some 10 us: only what costs least is asked of a good one."""
+    at = -1 if dev.index is None else dev.index
+    try:
+        for what, t, dtype, shape in specs:
+            if t.dtype is not dtype or t.shape != shape or not t.is_contiguous() or t.get_device() != at:
+                _refuse(what, t, dtype, shape, dev)
+    except AttributeError:
+        _refuse(what, t, dtype, shape, dev)
+        raise
 
 
 def _rows(dev, what: str, t, dtype, rows: int, cols: int) -> int:
@@ -83,7 +88,7 @@ def _call(dev: torch.device, f, what: str, *args) -> None:
     """Launches on dev's current stream."""
     if dev.type != "cuda":
         raise ValueError(f"tensors must be on a CUDA device, got {dev}")
-    if dev.index == torch.cuda.current_device():
+    if dev.index == torch._C._cuda_getDevice():  # tensors on the device: CUDA is initialised
         rc = f(*args, torch._C._cuda_getCurrentRawStream(dev.index))
     else:
         with torch.cuda.device(dev):
@@ -94,6 +99,12 @@ def _call(dev: torch.device, f, what: str, *args) -> None:
 
 def _p(t: Optional[torch.Tensor]):
     return None if t is None else t.data_ptr()
+
+
+@functools.lru_cache(maxsize=256)
+def _attn_ws(lanes: int, nq: int, n_heads: int, n_kv: int, dh: int, t_lim: int) -> int:
+    """Bytes of attn_tree's workspace."""
+    return lib().arcb_attn_tree_ws(lanes, nq, n_heads, n_kv, dh, t_lim)
 
 
 def attn_tree(q, Kc, Vc, pt, base, n_tree, mask, n_heads: int, n_kv: int, dh: int, attn_scale: int, lanes: int,
@@ -147,9 +158,8 @@ def attn_tree(q, Kc, Vc, pt, base, n_tree, mask, n_heads: int, n_kv: int, dh: in
         at |= o_out.data_ptr()
     if at % 16:
         raise ValueError("q, Kc, Vc, X and o_out must start on a 16-byte boundary")
-    L = lib()
-    ws = torch.empty(L.arcb_attn_tree_ws(lanes, nq, n_heads, n_kv, dh, t_lim), dtype=torch.uint8, device=dev)
-    _call(dev, L.arcb_attn_tree, "attn_tree", q.data_ptr(), Kc.data_ptr(), Vc.data_ptr(), pages, pt.data_ptr(), ps,
+    ws = torch.empty(_attn_ws(lanes, nq, n_heads, n_kv, dh, t_lim), dtype=torch.uint8, device=dev)
+    _call(dev, lib().arcb_attn_tree, "attn_tree", q.data_ptr(), Kc.data_ptr(), Vc.data_ptr(), pages, pt.data_ptr(), ps,
           pt.shape[1], base.data_ptr(), n_tree.data_ptr(), mask.data_ptr(), nq, n_heads, n_kv, dh, int(attn_scale),
           t_lim, lanes, ws.data_ptr(), _p(X), _p(lmax), _p(o_out), err.data_ptr())
 
@@ -228,11 +238,9 @@ def verify_tree(logits, dlogits, V: int, lanes: int, n: int, tokens, parent, n_t
            ("inv_temp", inv_temp, I64, one), ("d_inv_temp", d_inv_temp, I64, one), ("u", u, I32, (lanes, n, 2)),
            ("hist", hist, I32, (lanes, HIST)), ("count", count, I32, one), ("path", path, I32, per),
            ("n_path", n_path, I32, one), ("nxt", nxt, I32, one))
-    scratch = torch.empty(2 * lanes * n, dtype=I32, device=dev)
     _call(dev, lib().arcb_verify_tree, "verify_tree", logits.data_ptr(), ldl, dlogits.data_ptr(), ldd, V, lanes, n,
           tokens.data_ptr(), parent.data_ptr(), n_tree.data_ptr(), inv_temp.data_ptr(), d_inv_temp.data_ptr(),
-          u.data_ptr(), hist.data_ptr(), count.data_ptr(), scratch.data_ptr(), path.data_ptr(), n_path.data_ptr(),
-          nxt.data_ptr())
+          u.data_ptr(), hist.data_ptr(), count.data_ptr(), path.data_ptr(), n_path.data_ptr(), nxt.data_ptr())
 
 
 class KvPlanes:

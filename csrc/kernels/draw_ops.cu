@@ -489,9 +489,9 @@ __global__ void __launch_bounds__(NT, 3) k_draw(const int64_t* __restrict__ logi
   cluster_sync();  // no CTA may exit while a peer still reads its shared memory
 }
 
-// grid (cluster, nodes, lanes): every node's decision into choice (the
-// accepted child or -1) and drawn (the token that follows the node when no
-// child is accepted).  WALK, grid (cluster, 1, lanes): the lane's path.
+// grid (cluster, nodes, lanes): every node's decision into path: the accepted
+// child c, or -1 - t for the token t that follows the node when none is.  WALK,
+// grid (cluster, 1, lanes): the lane's path.
 template <bool WALK>
 __global__ void __launch_bounds__(NT, 2) k_verify(const int64_t* __restrict__ logits, int64_t ldl,
                                                const int64_t* __restrict__ dlogits, int64_t ldd, int V, int n,
@@ -499,7 +499,6 @@ __global__ void __launch_bounds__(NT, 2) k_verify(const int64_t* __restrict__ lo
                                                const int* __restrict__ n_tree, const int64_t* __restrict__ inv_temp,
                                                const int64_t* __restrict__ d_inv_temp, const int* __restrict__ u,
                                                const int* __restrict__ hist, const int* __restrict__ count, int seg,
-                                               int* __restrict__ choice, int* __restrict__ drawn,
                                                int* __restrict__ path, int* __restrict__ n_path,
                                                int* __restrict__ next) {
   extern __shared__ __align__(16) uint8_t dsm[];
@@ -635,11 +634,14 @@ __global__ void __launch_bounds__(NT, 2) k_verify(const int64_t* __restrict__ lo
       const uint64_t t = scale31((uint32_t)u[2 * node + 1], all);
       if (before <= t && t < before + s) {
         const int i = find(sh, len, t - before, [&](int j) { return (uint64_t)P[j]; });
-        if (tid == 0) (WALK ? next[lane] : drawn[row]) = v0 + i;
+        if (tid == 0) {
+          if (WALK) next[lane] = v0 + i;
+          else path[row] = -1 - (v0 + i);
+        }
       }
     }
     if (!WALK) {
-      if (rank == 0 && tid == 0) choice[row] = taken;
+      if (rank == 0 && tid == 0 && taken >= 0) path[row] = taken;
       break;
     }
     if (rank == 0 && tid == 0) path[lane0 + length] = node;
@@ -656,29 +658,30 @@ __global__ void __launch_bounds__(NT, 2) k_verify(const int64_t* __restrict__ lo
   cluster_sync();  // no CTA may exit while a peer still reads its shared memory
 }
 
-// Follows the decisions from each lane's root.  One thread per lane.
-__global__ void k_verify_path(int lanes, int n, const int* __restrict__ n_tree, const int* __restrict__ choice,
-                              const int* __restrict__ drawn, int* __restrict__ path, int* __restrict__ n_path,
+// Follows the decisions, in place, from each lane's root: the k-th node of a
+// path is k or a later one, whose decision is read before entry k is written.
+// One thread per lane.
+__global__ void k_verify_path(int lanes, int n, const int* __restrict__ n_tree, int* path, int* __restrict__ n_path,
                               int* __restrict__ next) {
   pdl_wait_dep();
   pdl_allow_next();
   const int lane = blockIdx.x * blockDim.x + threadIdx.x;
   if (lane >= lanes) return;
-  const size_t r0 = (size_t)lane * n;
+  path += (size_t)lane * n;
   int k = 0, node = 0, tok = -1;
   if (min(n_tree[lane], n) > 0)
     for (;;) {  // children come after their parent, so this ends
-      path[r0 + k++] = node;
-      const int c = choice[r0 + node];
+      const int c = path[node];
+      path[k++] = node;
       if (c <= node || c >= n) {
-        tok = drawn[r0 + node];
+        tok = -1 - c;
         break;
       }
       node = c;
     }
   n_path[lane] = k;
   next[lane] = tok;
-  for (; k < n; ++k) path[r0 + k] = -1;
+  for (; k < n; ++k) path[k] = -1;
 }
 
 // Part of the vocabulary per CTA of a cluster of cs, and its shared memory
@@ -776,15 +779,13 @@ int arcb_draw_tokens(const int64_t* logits, int64_t ldl, int V, int lanes, int n
                             nr, n, node0, m, inv_temp, u, hist, count, tokens, parent, x.seg, out);
 }
 
-// scratch: 2 * lanes * n ints.
 int arcb_verify_tree(const int64_t* logits, int64_t ldl, const int64_t* dlogits, int64_t ldd, int V, int lanes, int n,
                      const int* tokens, const int* parent, const int* n_tree, const int64_t* inv_temp,
-                     const int64_t* d_inv_temp, const int* u, const int* hist, const int* count, int* scratch,
-                     int* path, int* n_path, int* next, void* stream) {
+                     const int64_t* d_inv_temp, const int* u, const int* hist, const int* count, int* path,
+                     int* n_path, int* next, void* stream) {
   if (V < 1 || V > arcb_draw_max_vocab() || lanes < 1 || n < 1 || n > tree::MAX_NODES || lanes > 65535) return -2;
   static std::atomic<uint64_t> walk{0}, all{0};
   cudaStream_t st = (cudaStream_t)stream;
-  int* drawn = scratch + (size_t)lanes * n;
   const dr::Split each = dr::split_of((int64_t)lanes * n, V, 8, 2), walk_of = dr::split_of(lanes, V, 8, 2);
   // A path is a few nodes long, so all nodes at once may take the time of 1.7.  Measured, at
   // once / along the path, V = 32000: 16 nodes of a lane 25 / 38 us, 31 nodes 28 / 38, 64 nodes
@@ -792,13 +793,12 @@ int arcb_verify_tree(const int64_t* logits, int64_t ldl, const int64_t* dlogits,
   if (each.cost * 10 > walk_of.cost * 17)
     return dr::launch_cluster(dr::k_verify<true>, walk, walk_of.cs, dim3(walk_of.cs, 1, lanes), walk_of.smem, st, logits,
                               ldl, dlogits, ldd, V, n, tokens, parent, n_tree, inv_temp, d_inv_temp, u, hist, count,
-                              walk_of.seg, scratch, drawn, path, n_path, next);
+                              walk_of.seg, path, n_path, next);
   const int rc = dr::launch_cluster(dr::k_verify<false>, all, each.cs, dim3(each.cs, n, lanes), each.smem, st, logits,
                                     ldl, dlogits, ldd, V, n, tokens, parent, n_tree, inv_temp, d_inv_temp, u, hist,
-                                    count, each.seg, scratch, drawn, path, n_path, next);
+                                    count, each.seg, path, n_path, next);
   if (rc) return rc;
-  return launch_k(dr::k_verify_path, dim3((lanes + 63) / 64), dim3(64), 0, st, lanes, n, n_tree, scratch, drawn, path,
-                  n_path, next);
+  return launch_k(dr::k_verify_path, dim3((lanes + 63) / 64), dim3(64), 0, st, lanes, n, n_tree, path, n_path, next);
 }
 
 }  // extern "C"
