@@ -38,9 +38,9 @@
 //
 // What bounds it is latency: a cluster barrier takes half a microsecond, a first
 // touch of DRAM one to two, and a decision needs some eight of them in turn.
-// One row of 32000 takes 9.4 us in the kernel (12.3 us a call), a drafted chain
-// of 5 of them 20 us a call, 8 trees of 31 nodes 45 us, 4 trees of 64 nodes of
-// 102400 59 us.  72 rows of 102400, three tokens of each, take 57 us: 59 MB, two
+// One row of 32000 takes 9.0 us in the kernel (12.3 us a call), a drafted chain
+// of 5 of them 20 us a call, 8 trees of 31 nodes 44 us, 4 trees of 64 nodes of
+// 102400 59 us.  72 rows of 102400, three tokens of each, take 55 us: 59 MB, two
 // waves of clusters, 1 TB/s.
 #include <atomic>
 #include <climits>
@@ -101,6 +101,9 @@ __device__ __forceinline__ uint32_t div31(uint64_t num, uint64_t den, double rcp
 // into all of them before a cluster barrier and reads its own copies after
 // (reading sixteen peers one after another cost 2 us an exchange).  Sums come
 // in two phases, so that the next exchange may start while a peer still reads.
+// No CTA stores to a peer after its last barrier: any may exit then.  (Stores
+// that count their bytes at a barrier of the receiver in place of the cluster
+// barriers: one row 8.3 us in the kernel against 9.0, wide trees 57 against 56.)
 struct Shared {
   int2 lut[EXP_TABLE_N];
   int64_t redv[NW];  // the first row's warps, then the second's
@@ -486,7 +489,6 @@ __global__ void __launch_bounds__(NT, 3) k_draw(const int64_t* __restrict__ logi
       __syncthreads();
     }
   }
-  cluster_sync();  // no CTA may exit while a peer still reads its shared memory
 }
 
 // grid (cluster, nodes, lanes): every node's decision into path: the accepted
@@ -655,7 +657,6 @@ __global__ void __launch_bounds__(NT, 2) k_verify(const int64_t* __restrict__ lo
     }
     node = taken;  // a later node: the walk ends
   }
-  cluster_sync();  // no CTA may exit while a peer still reads its shared memory
 }
 
 // Follows the decisions, in place, from each lane's root: the k-th node of a
