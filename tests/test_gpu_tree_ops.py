@@ -295,6 +295,20 @@ def test_attn_tree_lanes_in_several_launches():
     np.testing.assert_array_equal(got.cpu().numpy(), want)
 
 
+def test_attn_tree_many_lanes():
+    """More lanes than the GPU has value CTAs, idle ones among them."""
+    rng = np.random.default_rng(12)
+    lens, nodes = rng.integers(0, 40, 2500).tolist(), rng.integers(0, 3, 2500).tolist()
+    a = Attn(8, 2, 1, lens, nodes, 1, 1, M18, M18)
+    want = a.want()
+    a.pt[7, 0] = -1
+    want[7] = 0
+    for t_lim in (a.t_lim, 1000):
+        got, err = a.run(t_lim=t_lim)
+        assert err == (ERR_BOUNDS if lens[7] + nodes[7] else 0)
+        np.testing.assert_array_equal(got.cpu().numpy(), want)
+
+
 def test_attn_tree_key_limit_beyond_the_table():
     """t_lim bounds lengths only as far as the table's pages reach."""
     a = Attn(64, 4, 2, [40, 70], [5, 6], 5, 2, M18, M18)
