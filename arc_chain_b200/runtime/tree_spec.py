@@ -213,6 +213,20 @@ class TreeSpecDecoder:
         self._graph.replay()
 
     # ------------------------------------------------------------ host side
+    def _error_words(self) -> List[torch.Tensor]:
+        """The error words of every buffer of the engines: a round's, and the prompts'."""
+        engines = [self.t] + ([self.d] if self.d is not None and self.d is not self.t else [])
+        return [bb.err for e in engines for bb in e._bufs.values()]
+
+    def _check_errors(self) -> None:
+        """Raises where a kernel reported that it could not do its work (a page or a length
+        out of range, a wait that ran out): the tokens behind that are not the model's."""
+        bits = 0
+        for w in torch.cat(self._error_words()).tolist():
+            bits |= w
+        if bits:
+            raise RuntimeError(f"a kernel reported an error (error bits {bits:#x})")
+
     def _numbers(self, ln: _Lane, k: int) -> np.ndarray:
         r = gen.rng_u64(self.seed, ln.stream, k, start=ln.drawn)
         ln.drawn += k
@@ -254,13 +268,12 @@ class TreeSpecDecoder:
         self._run()
         path, n_path, nxt = self.path.cpu().numpy(), self.n_path.cpu().numpy(), self.nxt.cpu().numpy()
         tokens = self.tokens.cpu().numpy()
+        self._check_errors()
         self.rounds += 1
         for i, ln in enumerate(lanes):
             if ln.done:
                 continue
             k = int(n_path[i])
-            if k < 1:
-                raise RuntimeError("the verification kernel returned no path (a kernel error bit is set)")
             new = [int(tokens[i, j]) for j in path[i, 1:k]] + [int(nxt[i])]
             self.proposed += len(self.branches)
             self.accepted += k - 1
@@ -279,7 +292,9 @@ class TreeSpecDecoder:
             -> List[Tuple[List[int], bytes]]:
         """Tokens and output hash of each prompt.  Request i of a call uses
         random stream i of the decoder's seed.  A request takes positions for
-        its prompt, max_tokens and one tree, up to the engines' max_seq."""
+        its prompt, max_tokens and one tree, up to the engines' max_seq.
+        Raises RuntimeError, with no tokens of any prompt, where a kernel
+        reports an error."""
         if len(prompts) != self.n_lanes:
             raise ValueError(f"one prompt per lane: {self.n_lanes} lanes, {len(prompts)} prompts")
         most = min(e.max_seq for e in (self.t, self.d) if e is not None)
@@ -289,6 +304,9 @@ class TreeSpecDecoder:
                                  f"exceed max_seq {most}")
         ends = set(int(e) for e in eos)
         lanes: List[_Lane] = []
+        before = [(w, w.clone()) for w in self._error_words()]  # other calls' errors stay readable
+        for w, _ in before:
+            w.zero_()
         try:
             for i, p in enumerate(prompts):
                 p = [int(x) for x in p]
@@ -300,6 +318,7 @@ class TreeSpecDecoder:
                 if self.db:
                     ln.rid_d = self.d.new_request(need)
                     self.d.prefill(ln.rid_d, [1] + p)
+            self._check_errors()
             while not all(ln.done for ln in lanes):
                 self._step(lanes, ends)
         finally:
@@ -307,6 +326,8 @@ class TreeSpecDecoder:
                 self.t.kv.release(ln.rid_t)
                 if ln.rid_d >= 0:
                     self.d.kv.release(ln.rid_d)
+            for w, b in before:
+                w.bitwise_or_(b)
         return [(ln.gen, blake3(np.asarray(ln.gen, dtype="<u4").tobytes())) for ln in lanes]
 
     @property
