@@ -24,10 +24,15 @@ A round, per lane (request), with branches (b_1, ..., b_L):
 With branches () there is no draft: plain sampled decoding.  The draft never
 runs the deepest level; where the path ends there, it is fed that token before
 the next round.  With tensor parallelism the draft, the drawing and the
-decision run on rank 0 and are broadcast; every rank runs the target's forward.
+decision run on rank 0 of the target's communicator and are broadcast over its
+group; every rank runs the target's forward.  Every rank builds the decoder and
+calls generate with the same arguments (only rank 0 needs the draft); where one
+rank refuses or fails outside the target's forward, all of them raise before the
+next collective.
 """
 from __future__ import annotations
 
+from contextlib import contextmanager
 from dataclasses import dataclass, field
 from typing import List, Optional, Sequence, Tuple
 
@@ -77,6 +82,7 @@ class _Lane:
     rid_d: int
     max_tokens: int
     stream: int
+    prompt: List[int]                                 # with BOS
     gen: List[int] = field(default_factory=list)
     last: int = 0
     pos: int = 0
@@ -89,22 +95,35 @@ class TreeSpecDecoder:
     def __init__(self, target: Engine, draft: Optional[Engine] = None, branches: Sequence[int] = (3, 2, 1),
                  lanes: int = 1, temperature: float = 0.0, draft_temperature: float = 1.0, seed: int = 0,
                  use_graph: bool = True):
-        for e in (target, draft):
-            if e is not None and not hasattr(e, "tree_buffers"):
-                raise TypeError(f"tree speculation runs dense engines, got {type(e).__name__}")
+        self._dense(target)
+        self.cm = target.comm
+        self.leads = self.cm.rank == 0
+        self.dev = target.m.emb.device
+        with self._together():
+            self._build(target, draft, branches, lanes, temperature, draft_temperature, seed, use_graph)
+
+    @staticmethod
+    def _dense(e) -> None:
+        if not hasattr(e, "tree_buffers"):
+            raise TypeError(f"tree speculation runs dense engines, got {type(e).__name__}")
+
+    def _build(self, target, draft, branches, lanes, temperature, draft_temperature, seed, use_graph) -> None:
+        if draft is not None:
+            self._dense(draft)
         if lanes < 1:
             raise ValueError(f"lanes must be at least 1, got {lanes}")
         self.branches = tuple(int(b) for b in branches)
-        self.t, self.d, self.n_lanes, self.seed, self.use_graph = target, draft, lanes, seed, use_graph
-        self.cm = target.comm
-        self.leads = self.cm.rank == 0
+        self.t, self.n_lanes, self.seed, self.use_graph = target, lanes, seed, use_graph
         if self.branches and self.leads and draft is None:
             raise ValueError("a tree of drafted tokens needs a draft engine")
         if draft is not None and draft.m.cfg.vocab != target.m.cfg.vocab:
             raise ValueError("target and draft must share a vocabulary")
+        self.d = draft if self.branches and self.leads else None
+        if self.d is not None and self.d.comm.size > 1:
+            raise ValueError("the draft runs on one rank: its engine takes no communicator")
         self.levels = tree_levels(self.branches)
         self.n = n = self.levels[-1][1]
-        dev = target.m.emb.device
+        dev = self.dev
         par = tree_parents(self.branches)
         depth, mask = [], []
         for i, p in enumerate(par):
@@ -117,7 +136,7 @@ class TreeSpecDecoder:
         self.mask = torch.tensor(signed, dtype=I64, device=dev)
         V = target.m.cfg.vocab
         self.tb = target.tree_buffers(lanes, n)
-        self.db = [draft.tree_buffers(lanes, b - a) for a, b in self.levels[:-1]] if draft is not None else []
+        self.db = [self.d.tree_buffers(lanes, b - a) for a, b in self.levels[:-1]] if self.d is not None else []
         z = lambda *s, dt=I32: torch.zeros(*s, dtype=dt, device=dev)
         self.pos, self.live, self.root = z(lanes), z(lanes), z(lanes)
         self.tokens = z(lanes, n)
@@ -131,6 +150,38 @@ class TreeSpecDecoder:
         self.path, self.n_path, self.nxt = z(lanes, n), z(lanes), z(lanes)
         self._graph = None
         self.rounds = self.proposed = self.accepted = 0
+
+    # ------------------------------------------------------------ ranks
+    def _agree(self, x: int, least: bool) -> int:
+        """The least or the largest of the ranks' numbers."""
+        if self.cm.size == 1:
+            return x
+        import torch.distributed as dist
+
+        t = torch.tensor([x], dtype=I64, device=self.dev)
+        dist.all_reduce(t, dist.ReduceOp.MIN if least else dist.ReduceOp.MAX, group=self.cm.group)
+        return int(t.item())
+
+    @contextmanager
+    def _together(self):
+        """A part that every rank enters and that holds no collective: where it
+        raises on one rank, it raises on all."""
+        err: Optional[Exception] = None
+        try:
+            yield
+        except Exception as e:
+            err = e
+        if self._agree(int(err is not None), False) and err is None:
+            err = RuntimeError("tree speculation failed on another rank")
+        if err is not None:
+            raise err
+
+    def _broadcast(self, *tensors: torch.Tensor) -> None:
+        if self.cm.size > 1:
+            import torch.distributed as dist
+
+            for x in tensors:
+                dist.broadcast(x, group=self.cm.group, group_src=0)
 
     # ------------------------------------------------------------ device side
     def _set(self, bb, a: int, b: int) -> None:
@@ -164,29 +215,33 @@ class TreeSpecDecoder:
     def _keep(self, eng: Engine, bb) -> None:
         eng.kv.keep_path(bb.pt[::bb.tree.nq], bb.tree.base, self.path, self.n_path, self.n_lanes, self.n, bb.err)
 
-    def _round(self) -> None:
-        if self.cm.size > 1:
-            import torch.distributed as dist
-
+    def _propose(self) -> None:
         self.tokens[:, 0].copy_(self.root)
-        if self.branches and self.leads:
+        if self.db:
             self._draft()
-        if self.cm.size > 1:
-            dist.broadcast(self.tokens, src=0)
+
+    def _judge(self) -> None:
+        self._broadcast(self.tokens)
         self._set(self.tb, 0, self.n)
         self.t.forward(self.tb, self.tb.B, True)
-        if self.leads:
-            self._decide()
-        if self.cm.size > 1:
-            for x in (self.path, self.n_path, self.nxt):
-                dist.broadcast(x, src=0)
+        with self._together():
+            if self.leads:
+                self._decide()
+        self._broadcast(self.path, self.n_path, self.nxt)
+
+    def _settle(self) -> None:
         if self.branches:
             self._keep(self.t, self.tb)
-            if self.leads:
+            if self.db:
                 self._keep(self.d, self.db[0])
 
+    def _round(self) -> None:
+        self._propose()
+        self._judge()
+        self._settle()
+
     def _run(self) -> None:
-        if not self.use_graph or self.cm.size > 1:
+        if not self.use_graph:
             self._round()
             return
         if self._graph is None:
@@ -215,7 +270,7 @@ class TreeSpecDecoder:
     # ------------------------------------------------------------ host side
     def _error_words(self) -> List[torch.Tensor]:
         """The error words of every buffer of the engines: a round's, and the prompts'."""
-        engines = [self.t] + ([self.d] if self.d is not None and self.d is not self.t else [])
+        engines = [self.t] if self.d is None or self.d is self.t else [self.t, self.d]
         return [bb.err for e in engines for bb in e._bufs.values()]
 
     def _check_errors(self) -> None:
@@ -259,16 +314,26 @@ class TreeSpecDecoder:
             bb.pt.copy_(I(np.repeat(rows, bb.tree.nq, 0)))
 
     def _step(self, lanes: List[_Lane], eos: set) -> None:
-        if self.db:
-            for ln in lanes:
-                if not ln.done and ln.pending:
-                    self.d.prefill(ln.rid_d, ln.pending, start_pos=ln.pos - len(ln.pending))
-                    ln.pending = []
-        self._upload(lanes)
-        self._run()
-        path, n_path, nxt = self.path.cpu().numpy(), self.n_path.cpu().numpy(), self.nxt.cpu().numpy()
-        tokens = self.tokens.cpu().numpy()
-        self._check_errors()
+        one = self.cm.size == 1
+        with self._together():
+            if self.db:
+                for ln in lanes:
+                    if not ln.done and ln.pending:
+                        self.d.prefill(ln.rid_d, ln.pending, start_pos=ln.pos - len(ln.pending))
+                        ln.pending = []
+            self._upload(lanes)
+            if one:
+                self._run()
+            else:
+                self._propose()
+        if not one:
+            self._judge()
+        with self._together():
+            if not one:
+                self._settle()
+            path, n_path, nxt = self.path.cpu().numpy(), self.n_path.cpu().numpy(), self.nxt.cpu().numpy()
+            tokens = self.tokens.cpu().numpy()
+            self._check_errors()
         self.rounds += 1
         for i, ln in enumerate(lanes):
             if ln.done:
@@ -295,30 +360,34 @@ class TreeSpecDecoder:
         its prompt, max_tokens and one tree, up to the engines' max_seq.
         Raises RuntimeError, with no tokens of any prompt, where a kernel
         reports an error."""
-        if len(prompts) != self.n_lanes:
-            raise ValueError(f"one prompt per lane: {self.n_lanes} lanes, {len(prompts)} prompts")
-        most = min(e.max_seq for e in (self.t, self.d) if e is not None)
-        for p in prompts:
-            if 1 + len(p) + max_tokens + self.n > most:
-                raise ValueError(f"a prompt of {len(p)} tokens, {max_tokens} new ones and a tree of {self.n} nodes "
-                                 f"exceed max_seq {most}")
-        ends = set(int(e) for e in eos)
+        most = self._agree(min(e.max_seq for e in (self.t, self.d) if e is not None), True)
         lanes: List[_Lane] = []
-        before = [(w, w.clone()) for w in self._error_words()]  # other calls' errors stay readable
-        for w, _ in before:
-            w.zero_()
+        before: List[Tuple[torch.Tensor, torch.Tensor]] = []
         try:
-            for i, p in enumerate(prompts):
-                p = [int(x) for x in p]
-                need = 1 + len(p) + max_tokens + self.n
-                ln = _Lane(self.t.new_request(need), -1, max_tokens, STREAM + i, last=p[-1] if p else 0,
-                           pos=len(p) + 1, done=max_tokens <= 0)
-                lanes.append(ln)
-                self.t.prefill(ln.rid_t, [1] + p)
-                if self.db:
-                    ln.rid_d = self.d.new_request(need)
-                    self.d.prefill(ln.rid_d, [1] + p)
-            self._check_errors()
+            with self._together():
+                if len(prompts) != self.n_lanes:
+                    raise ValueError(f"one prompt per lane: {self.n_lanes} lanes, {len(prompts)} prompts")
+                for p in prompts:
+                    if 1 + len(p) + max_tokens + self.n > most:
+                        raise ValueError(f"a prompt of {len(p)} tokens, {max_tokens} new ones and a tree of {self.n} "
+                                         f"nodes exceed max_seq {most}")
+                ends = set(int(e) for e in eos)
+                before = [(w, w.clone()) for w in self._error_words()]  # other calls' errors stay readable
+                for w, _ in before:
+                    w.zero_()
+                for i, p in enumerate(prompts):
+                    p = [int(x) for x in p]
+                    need = 1 + len(p) + max_tokens + self.n
+                    ln = _Lane(self.t.new_request(need), -1, max_tokens, STREAM + i, [1] + p, last=p[-1] if p else 0,
+                               pos=len(p) + 1, done=max_tokens <= 0)
+                    lanes.append(ln)
+                    if self.db:
+                        ln.rid_d = self.d.new_request(need)
+                        self.d.prefill(ln.rid_d, ln.prompt)
+            for ln in lanes:
+                self.t.prefill(ln.rid_t, ln.prompt)
+            with self._together():
+                self._check_errors()
             while not all(ln.done for ln in lanes):
                 self._step(lanes, ends)
         finally:

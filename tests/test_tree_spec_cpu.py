@@ -1,5 +1,10 @@
 """Host logic of TreeSpecDecoder on the CPU: a toy engine, the operators by
-their definitions."""
+their definitions, tensor parallelism as gloo ranks."""
+import datetime
+import os
+import socket
+import time
+
 import pytest
 
 torch = pytest.importorskip("torch")
@@ -64,3 +69,108 @@ def test_an_error_word_of_the_prompt_ends_the_call(toy_ops):
     with pytest.raises(RuntimeError, match="0x20"):
         sd.generate(PROMPTS, 20)
     assert sd.rounds == 0 and sd.t.kv.pool.used <= 1
+
+
+# ------------------------------------------------------------ ranks
+def _fail(*a, **kw):
+    raise MemoryError("planted")
+
+
+def _worker(rank, world, port, group_ranks, fault, q):
+    import torch.distributed as dist
+
+    from arc_chain_b200.parallel.tp import NcclComm
+
+    os.environ["MASTER_ADDR"], os.environ["MASTER_PORT"] = "127.0.0.1", str(port)
+    dist.init_process_group("gloo", rank=rank, world_size=world, timeout=datetime.timedelta(seconds=15))
+    ts.ops.draw_tokens, ts.ops.verify_tree = stub.draw_tokens, stub.verify_tree
+    try:
+        group = dist.new_group(group_ranks) if group_ranks else None
+        if group_ranks and rank not in group_ranks:
+            q.put((rank, None))
+            return
+        comm = NcclComm(group)
+        leads = comm.rank == 0
+        target, draft = stub.ToyEngine(0, comm=comm), stub.ToyEngine(3, max_seq=48 if fault == "limit" else 128)
+        if fault == "request" and leads:
+            draft.new_request = _fail
+        if fault == "prompt" and leads:
+            draft.prefill = _fail
+        if fault == "level" and leads:
+            draft.forward = _fail
+        if fault == "decision" and leads:
+            ts.ops.verify_tree = _fail
+        if fault == "kept rows" and leads:
+            draft.kv.keep_path = _fail
+        if fault == "pages" and not leads:
+            target.kv.pool.free = target.kv.pool.free[:2]
+        used = target.kv.pool.used
+        out = []
+        try:
+            sd = ts.TreeSpecDecoder(target, draft if leads and fault != "no draft" else None, (2, 2), 2, 0.9, seed=4)
+            if fault == "word" and not leads:
+                forward = target.forward
+                target.forward = lambda *a: (forward(*a), sd.tb.err.fill_(8))
+            out = [t for t, _ in sd.generate(PROMPTS, 20 if fault != "limit" else 40)]
+        except (ValueError, MemoryError, RuntimeError) as e:
+            out = f"{type(e).__name__}: {e}"
+        q.put((rank, (out, target.kv.pool.used <= used + 1 and draft.kv.pool.used <= 1)))
+        # every rank is still in step with the others
+        t = torch.ones(1)
+        dist.all_reduce(t, group=group)
+        assert int(t) == comm.size
+    finally:
+        dist.destroy_process_group()
+
+
+def _ranks(fault="", group_ranks=()):
+    import multiprocessing as mp
+
+    s = socket.socket()
+    s.bind(("127.0.0.1", 0))
+    port = s.getsockname()[1]
+    s.close()
+    ctx, world = mp.get_context("spawn"), 3 if group_ranks else 2
+    q = ctx.Queue()
+    ps = [ctx.Process(target=_worker, args=(r, world, port, list(group_ranks), fault, q)) for r in range(world)]
+    for p in ps:
+        p.start()
+    res, t0 = {}, time.time()
+    while len(res) < world and time.time() - t0 < 90:
+        try:
+            r, v = q.get(timeout=1)
+            res[r] = v
+        except Exception:
+            pass
+    for p in ps:
+        p.join(timeout=30)
+        if p.is_alive():
+            p.kill()
+    return [res.get(r) for r in range(world)], [p.exitcode for p in ps]
+
+
+@pytest.mark.parametrize("group_ranks", [(), (1, 2)])
+def test_ranks_equal_one_process(toy_ops, group_ranks):
+    """Also over a communicator of some of the ranks, whose first is not the world's."""
+    want = [t for t, _ in decoder((2, 2), 0.9, 3, seed=4).generate(PROMPTS, 20)]
+    res, codes = _ranks("", group_ranks)
+    assert codes == [0] * len(codes)
+    assert [r for r in res if r is not None] == [(want, True)] * 2
+
+
+@pytest.mark.parametrize("fault,first,second", [
+    ("limit", "ValueError: a prompt of 3 tokens, 40 new ones and a tree of 7 nodes exceed max_seq 48", None),
+    ("no draft", "ValueError: a tree of drafted tokens needs a draft engine", "RuntimeError: tree spec"),
+    ("request", "MemoryError: planted", "RuntimeError: tree spec"),
+    ("prompt", "MemoryError: planted", "RuntimeError: tree spec"),
+    ("level", "MemoryError: planted", "RuntimeError: tree spec"),
+    ("decision", "MemoryError: planted", "RuntimeError: tree spec"),
+    ("kept rows", "MemoryError: planted", "RuntimeError: tree spec"),
+    ("pages", "RuntimeError: tree spec", "MemoryError: KV cache out of pages"),
+    ("word", "RuntimeError: tree spec", "RuntimeError: a kernel reported an error (error bits 0x8)")])
+def test_ranks_fail_together(fault, first, second):
+    """What one rank refuses or fails at ends the call on both, and both stay in step."""
+    res, codes = _ranks(fault)
+    assert codes == [0, 0], (codes, res)
+    for (out, released), want in zip(res, (first, second or first)):
+        assert isinstance(out, str) and out.startswith(want) and released
