@@ -224,6 +224,8 @@ class MlaMoeEngine(Engine):
     """Engine for the MLA + MoE model (single GPU); reuses the dense engine's
     request, prefill, generate and CUDA-graph machinery."""
 
+    runs_trees = False
+
     def __init__(self, model: MlaMoeModel, n_pages: Optional[int] = None, max_seq: Optional[int] = None,
                  comm: Optional[Comm] = None):
         self.m = model

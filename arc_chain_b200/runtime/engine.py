@@ -121,6 +121,8 @@ class TreeStep:
 
 
 class Engine:
+    runs_trees = True  # forwards over drafted-tree nodes (tree_buffers)
+
     def __init__(self, model: DenseModel, n_pages: Optional[int] = None, max_seq: Optional[int] = None,
                  comm: Optional[Comm] = None, kv_bytes: Optional[int] = None):
         self.m = model
@@ -158,6 +160,8 @@ class Engine:
         """Buffers of a forward over nq drafted-tree nodes of each of `lanes`
         requests (slot = lane * nq + node): besides tokens, pos (RoPE) and pt,
         the caller sets kv_pos (cache rows) and the fields of `tree`."""
+        if not self.runs_trees:
+            raise TypeError(f"drafted trees run on dense engines, not on {type(self).__name__}")
         key = ("tree", lanes, nq)
         if key not in self._bufs:
             bb = StepBuffers(self.m, lanes * nq, self.max_pages)

@@ -104,7 +104,7 @@ class TreeSpecDecoder:
 
     @staticmethod
     def _dense(e) -> None:
-        if not hasattr(e, "tree_buffers"):
+        if not getattr(e, "runs_trees", False):
             raise TypeError(f"tree speculation runs dense engines, got {type(e).__name__}")
 
     def _build(self, target, draft, branches, lanes, temperature, draft_temperature, seed, use_graph) -> None:

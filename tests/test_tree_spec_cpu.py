@@ -174,3 +174,18 @@ def test_ranks_fail_together(fault, first, second):
     assert codes == [0, 0], (codes, res)
     for (out, released), want in zip(res, (first, second or first)):
         assert isinstance(out, str) and out.startswith(want) and released
+
+
+# ------------------------------------------------------------ refusals
+def test_latent_attention_engines_are_refused(toy_ops):
+    """They share the dense engine's class, but neither its cache rows nor its buffers."""
+    from arc_chain_b200.models.mla_moe_engine import MlaMoeEngine
+
+    mla = object.__new__(MlaMoeEngine)
+    mla.m = stub.ToyEngine().m
+    mla.comm, mla.max_pages, mla._bufs = stub.Comm(), 8, {}
+    for target, draft in ((mla, None), (stub.ToyEngine(), mla)):
+        with pytest.raises(TypeError, match="MlaMoeEngine"):
+            ts.TreeSpecDecoder(target, draft, (2, 2) if draft else (), 1)
+    with pytest.raises(TypeError, match="MlaMoeEngine"):
+        mla.tree_buffers(1, 4)
