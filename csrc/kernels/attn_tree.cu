@@ -949,7 +949,7 @@ struct Plan {
   size_t oS, oQ, oI, oR, oM, oG, oSum, oW, oAcc, oA, oB, oF, bytes;
 };
 
-constexpr size_t WS_TARGET = size_t(1) << 30;  // lanes are batched to about this much workspace
+constexpr size_t WS_TARGET = size_t(1) << 30;  // lanes are batched to at most this much workspace, but one at least
 
 static Plan plan(int lanes, int nq, int n_heads, int n_kv, int dh, int t_lim) {
   Plan p;
@@ -962,20 +962,30 @@ static Plan plan(int lanes, int nq, int n_heads, int n_kv, int dh, int t_lim) {
   p.RG = ((p.R + p.groups - 1) / p.groups + p.unit - 1) / p.unit * p.unit;
   p.Rp = p.groups * p.RG;
   p.tiles = (t_lim + TILE - 1) / TILE;
-  const size_t per_s = (size_t)n_kv * p.tiles * TILE * p.Rp * 4;
-  p.lanes = (int)(WS_TARGET / per_s);
-  p.lanes = p.lanes < 1 ? 1 : (p.lanes > lanes ? lanes : p.lanes);
-  const int have = p.lanes * n_kv * p.groups;
   const int units = p.RG / p.unit;
   p.threads = 32 * units * (units >= 5 ? 1 : (units >= 3 ? 2 : (units == 2 ? 4 : 8)));
   // five-warp value CTAs run three to an SM with chunks of one page (9 nodes, 8 query
   // heads per KV head, 30 thousand keys: a call 362 us against 393 with two and two pages);
   // the others two, with two pages (64 nodes: 315 us, 325 with one page)
   p.per_sm = p.threads == 160 ? 3 : 2;
+  p.qgroups = (p.R + RQ - 1) / RQ;
+  p.few = p.R <= RQ && (int64_t)p.RG * t_lim <= FEW_MOST;
   // the lanes' keys are divided evenly over the CTAs that run at once; a CTA's
   // part of a lane stays below MAX_RANGE keys
   p.splits = p.per_sm * 148 / (n_kv * p.groups);
   if (p.splits < 1) p.splits = 1;
+  // workspace of a lane: scores, query digits, maxima and sums, output sums, and the slots of
+  // 64-bit terms that it adds (its own, and its share of `least` below); and of any number of lanes
+  const size_t per_s = (size_t)n_kv * p.tiles * TILE * p.Rp * 4;
+  const size_t slot = (size_t)n_kv * p.groups * ((size_t)p.RG * dh * 8 + 4);
+  const size_t per_lane = per_s + (size_t)n_kv * (p.qgroups * (PLANES * RQ * 128 + sizeof(uint4)) +
+                                                  (size_t)p.tiles * p.Rp * (p.few ? 16 : 8) + p.Rp * 16 +
+                                                  (size_t)p.groups * (p.RG * dh * 4 + 4)) +
+                          4 + slot + (size_t)p.tiles * TILE * slot / (MAX_RANGE - 32) + 1;
+  const size_t fixed = (p.splits + 1) * slot + 16 * 256;
+  const size_t fit = fixed < WS_TARGET ? (WS_TARGET - fixed) / per_lane : 0;
+  p.lanes = fit < 1 ? 1 : (fit < (size_t)lanes ? (int)fit : lanes);
+  const int have = p.lanes * n_kv * p.groups;
   const int64_t least = ((int64_t)p.lanes * p.tiles * TILE + MAX_RANGE - 1) / (MAX_RANGE - 32);
   if (p.splits < least) p.splits = (int)least;
   p.chunks = (12 * 148 + have - 1) / have;  // of the sums: short ones, many loads in flight
@@ -992,11 +1002,9 @@ static Plan plan(int lanes, int nq, int n_heads, int n_kv, int dh, int t_lim) {
   };
   const size_t lk = (size_t)p.lanes * n_kv;
   p.oS = take((size_t)p.lanes * per_s);
-  p.qgroups = (p.R + RQ - 1) / RQ;
   p.oQ = take(lk * p.qgroups * PLANES * RQ * 128);
   p.oI = take(lk * p.qgroups * sizeof(uint4));
   p.oR = take(lk * p.tiles * p.Rp * 8);
-  p.few = p.R <= RQ && (int64_t)p.RG * t_lim <= FEW_MOST;
   p.oM = take(p.few ? lk * p.tiles * p.Rp * 8 : 0);
   p.oG = take(lk * p.Rp * 8);
   p.oSum = take(lk * p.Rp * 8);

@@ -51,3 +51,49 @@ def test_an_error_word_ends_the_call(where, use_graph):
     if where == "prompt":
         target.prefill = prefill
     assert sd.generate([prompt], 20) == [want]
+
+
+@pytest.mark.parametrize("nq,heads,kv,dh,lanes,few", [(4, 64, 64, 8, 900, True), (64, 64, 8, 8, 700, False)])
+def test_attn_tree_batches_of_short_lanes(nq, heads, kv, dh, lanes, few):
+    """Lanes of few keys whose digits and sums fill a launch's workspace: the
+    result is that of calls of fewer lanes, and a lane's is the definition's."""
+    import numpy as np
+
+    from arc_chain_b200 import spec
+    from arc_chain_b200.ops import tree_ops as ops
+    from arc_chain_b200.ops._lib import lib
+
+    t_lim = 100 if few else 128
+    # all of the lanes in one launch would pass 1 GB: they go in several
+    per = (lib().arcb_attn_tree_ws(2, nq, heads, kv, dh, t_lim) - lib().arcb_attn_tree_ws(1, nq, heads, kv, dh, t_lim))
+    assert lanes * per > 1 << 30
+    g = torch.Generator("cuda").manual_seed(nq)
+    I32, I64 = torch.int32, torch.int64
+    i = lambda lo, hi, s, t=I64: torch.randint(lo, hi, s, generator=g, device="cuda", dtype=t)
+    q = i(-1 << 18, 1 << 18, (lanes * nq, heads * dh))
+    pages = 500
+    K, V = (i(-1 << 18, 1 << 18, (pages, kv, 16, dh)) for _ in range(2))
+    pt = i(0, pages, (lanes, t_lim // 16 + 1), I32)
+    base, n_tree = i(0, t_lim - nq - 1, (lanes,), I32), i(0, nq + 1, (lanes,), I32)
+    mask = i(0, 1 << 62, (lanes * nq,)) | 1
+    err = torch.zeros(1, dtype=I32, device="cuda")
+
+    def run(a, b):
+        out = torch.full(((b - a) * nq, heads * dh), 77, dtype=I64, device="cuda")
+        ops.attn_tree(q[a * nq:b * nq], K, V, pt[a:b], base[a:b], n_tree[a:b], mask[a * nq:b * nq], heads, kv, dh,
+                      9000, b - a, nq, None, None, t_lim, err, o_out=out)
+        return out
+
+    got = run(0, lanes)
+    assert torch.equal(got, torch.cat([run(a, min(lanes, a + 50)) for a in range(0, lanes, 50)]))
+    assert int(err.item()) == 0
+    for b in (0, lanes // 2, lanes - 1):
+        t = int(base[b] + n_tree[b])
+        rows = pt[b, :(t + 15) // 16].long()
+        for h in (0, heads - 1):
+            k, v = (c[rows, h * kv // heads].reshape(-1, dh)[:t].cpu().numpy() for c in (K, V))
+            for j in (0, nq - 1):
+                s = b * nq + j
+                want = spec.tree_attention(q[s, h * dh:(h + 1) * dh].cpu().numpy(), k, v, int(base[b]), int(n_tree[b]),
+                                           int(mask[s]), 9000)
+                np.testing.assert_array_equal(got[s, h * dh:(h + 1) * dh].cpu().numpy(), want)
