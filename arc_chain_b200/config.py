@@ -17,6 +17,8 @@ import os
 from dataclasses import dataclass, field
 from typing import List, Optional, Sequence
 
+from arc_chain_b200.spec import check_temperature
+
 QUANTS = ("int8", "q4-row", "q4-group")
 
 
@@ -36,9 +38,10 @@ class RunConfig:
     draft: str = ""              # speculative decoding draft (preset or path); "" = off
     spec_k: int = 4
     spec_tree: List[int] = field(default_factory=list)  # children per node of each drafted level; [] = no tree
-    temperature: float = 0.0     # 0: greedy (the reference's step); else sampled from the target's distribution
+    # 0: greedy (the reference's step); 1/16 to 65536: sampled from the target's distribution
+    temperature: float = 0.0
     draft_temperature: float = 1.0
-    sample_seed: int = 0         # random streams of sampled decoding
+    sample_seed: int = 0         # random streams of sampled decoding (low 32 bits)
     eos: List[int] = field(default_factory=list)
     use_graph: bool = True       # CUDA-graph the decode step
     pdl: bool = True             # programmatic dependent launch between kernels
@@ -53,8 +56,8 @@ class RunConfig:
             raise ValueError("comm must be 'fused' or 'nccl'")
         if self.tp < 1 or self.ep < 1 or (self.tp > 1 and self.ep > 1):
             raise ValueError("tp and ep are >= 1, and at most one of them is > 1")
-        if not self.temperature >= 0 or not self.draft_temperature >= 0:
-            raise ValueError("temperatures are >= 0")
+        check_temperature(self.temperature)
+        check_temperature(self.draft_temperature)
         if self.spec_tree:
             from arc_chain_b200.runtime.tree_spec import tree_levels
 

@@ -5,10 +5,11 @@ greedy step's (crates/arc-inference/src/cached_integer_model.rs:1518-1557) token
 for token, like ``runtime.spec_decode``.  With a temperature the tokens follow
 the target's own distribution (softmax of its penalised logits over the
 temperature, in the exact integers of csrc/kernels/draw_ops.cu), whatever the
-draft proposes.  Random numbers come from the seeded SplitMix64 streams of
+draft proposes, to within the 2^-31 that probabilities and random numbers are
+held to.  Random numbers come from the seeded SplitMix64 streams of
 ``formats.gen``, one stream per request, so a run is a function of the
-model, the prompts and the seed: neither the other requests of the batch nor
-CUDA graphs change it.
+model, the prompts and the seed (its low 32 bits): neither the other requests
+of the batch nor CUDA graphs change it.
 
 A round, per lane (request), with branches (b_1, ..., b_L):
 
@@ -42,6 +43,7 @@ import torch
 from arc_chain_b200.formats import gen
 from arc_chain_b200.ops import tree_ops as ops
 from arc_chain_b200.runtime.engine import Engine, I32, I64
+from arc_chain_b200.spec import check_temperature
 from arc_chain_b200.utils.hashing import blake3
 
 ONE = 1 << 16
@@ -70,10 +72,10 @@ def tree_parents(branches: Sequence[int]) -> List[int]:
 
 
 def inverse_temperature(t: float) -> int:
-    """Q16 inverse temperature; 0 is greedy."""
+    """Q16 inverse temperature, the nearest that the operators use; 0 is greedy."""
     if not t >= 0:
         raise ValueError(f"a temperature is at least 0, got {t}")
-    return 0 if t == 0 else max(1, min(ops.MAX_INV_TEMP, int(round(ONE / t))))
+    return 0 if t == 0 else max(1, round(min(ops.MAX_INV_TEMP, ONE / t)))
 
 
 @dataclass
@@ -110,6 +112,8 @@ class TreeSpecDecoder:
     def _build(self, target, draft, branches, lanes, temperature, draft_temperature, seed, use_graph) -> None:
         if draft is not None:
             self._dense(draft)
+        check_temperature(temperature)
+        check_temperature(draft_temperature)
         if lanes < 1:
             raise ValueError(f"lanes must be at least 1, got {lanes}")
         self.branches = tuple(int(b) for b in branches)

@@ -346,6 +346,12 @@ LOGIT_CLAMP = 1 << 40
 MAX_INV_TEMP = 1 << 20
 
 
+def check_temperature(t: float) -> None:
+    """Refuses a temperature whose Q16 inverse would be cut off at MAX_INV_TEMP or at 1."""
+    if t != 0 and not ONE / MAX_INV_TEMP <= t <= ONE:
+        raise ValueError(f"a temperature is 0 (greedy) or from {ONE / MAX_INV_TEMP:g} to {ONE}, got {t}")
+
+
 def tree_attention(q: np.ndarray, K: np.ndarray, V: np.ndarray, base: int, n_tree: int, mask: int,
                    attn_scale: int) -> np.ndarray:
     """One query [dh] over the rows K, V [base + n_tree, dh]: the keys below

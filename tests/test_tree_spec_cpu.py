@@ -189,3 +189,24 @@ def test_latent_attention_engines_are_refused(toy_ops):
             ts.TreeSpecDecoder(target, draft, (2, 2) if draft else (), 1)
     with pytest.raises(TypeError, match="MlaMoeEngine"):
         mla.tree_buffers(1, 4)
+
+
+@pytest.mark.parametrize("t", [1e-9, 1e-310, 0.01, 0.0624, 65537.0, 1e9, float("inf"), float("nan"), -1.0])
+def test_temperatures_that_would_be_another(toy_ops, t):
+    """Inverse temperatures are Q16 up to 16: 0.01 would be sampled as 1/16, 1e9 as 65536."""
+    from arc_chain_b200.config import RunConfig
+
+    for kw in (dict(temperature=t), dict(draft_temperature=t)):
+        with pytest.raises(ValueError, match="temperature"):
+            decoder((2, 2), **kw)
+        with pytest.raises(ValueError, match="temperature"):
+            RunConfig(**kw)
+
+
+@pytest.mark.parametrize("t", [0.0, 1 / 16, 0.7, 1, 65536.0])
+def test_temperatures_that_are_taken(toy_ops, t):
+    from arc_chain_b200.config import RunConfig
+
+    sd = decoder((2,), temperature=t, draft_temperature=t)
+    assert sd.inv.tolist() == sd.dinv.tolist() == [0 if t == 0 else round(65536 / t)] * 2
+    assert RunConfig(temperature=t, draft_temperature=t).temperature == t
