@@ -249,21 +249,33 @@ class KvPlanes:
     their addresses, for kernels that touch every layer in one launch."""
 
     def __init__(self, Ks: Sequence[torch.Tensor], Vs: Sequence[torch.Tensor]):
-        ts = {id(t): t for t in [*Ks, *Vs]}  # a latent cache's V is its K
-        self.tensors = list(ts.values())
-        if not self.tensors:
+        ts = [*Ks, *Vs]
+        if not ts:
             raise ValueError("a cache has at least one layer")
-        first = self.tensors[0]
+        first = ts[0]
         if not isinstance(first, torch.Tensor) or first.dim() != 4 or first.shape[2] != PAGE or first.shape[3] % 2:
             raise ValueError("cache tensors are [pages, n_kv, 16, d_head] with an even d_head")
         self.device = first.device
-        _check(self.device, *(("cache tensor", t, I64, first.shape) for t in self.tensors))
+        _check(self.device, *(("cache tensor", t, I64, first.shape) for t in ts))
+        self.tensors = self.distinct(ts)
         if self.device.type != "cuda":
             raise ValueError(f"tensors must be on a CUDA device, got {self.device}")
         if any(t.data_ptr() % 16 for t in self.tensors):
             raise ValueError("cache tensors must start on a 16-byte boundary")
         self.n_pages, self.n_kv, _, self.dh = first.shape
         self.table = torch.tensor([t.data_ptr() for t in self.tensors], dtype=I64, device=self.device)
+
+    @staticmethod
+    def distinct(ts: Sequence[torch.Tensor]) -> list:
+        """Tensors of one shape, each piece of memory once (a latent cache's V
+        is its K): every plane's rows are moved at the same time."""
+        at = {}
+        for t in ts:
+            at.setdefault(t.data_ptr(), t)
+        starts = sorted(at)
+        if any(b - a < t.numel() * t.element_size() for a, b in zip(starts, starts[1:])):
+            raise ValueError("cache tensors overlap")
+        return list(at.values())
 
 
 def kv_keep_path(planes: KvPlanes, pt, base, path, n_path, lanes: int, n: int, err) -> None:
