@@ -159,7 +159,11 @@ def attn_tree(q, Kc, Vc, pt, base, n_tree, mask, n_heads: int, n_kv: int, dh: in
         at |= o_out.data_ptr()
     if at % 16:
         raise ValueError("q, Kc, Vc, X and o_out must start on a 16-byte boundary")
-    ws = torch.empty(_attn_ws(lanes, nq, n_heads, n_kv, dh, t_lim), dtype=torch.uint8, device=dev)
+    size = _attn_ws(lanes, nq, n_heads, n_kv, dh, t_lim)
+    if size < 0:
+        raise ValueError(f"attn_tree takes up to {65535 * 32 // n_kv} queries times query heads per KV head and "
+                         f"{65535 * 16 * 128} keys a lane, got {nq * (n_heads // n_kv)} and {t_lim}")
+    ws = torch.empty(size, dtype=torch.uint8, device=dev)
     _call(dev, lib().arcb_attn_tree, "attn_tree", q.data_ptr(), Kc.data_ptr(), Vc.data_ptr(), pages, pt.data_ptr(), ps,
           pt.shape[1], base.data_ptr(), n_tree.data_ptr(), mask.data_ptr(), nq, n_heads, n_kv, dh, int(attn_scale),
           t_lim, lanes, ws.data_ptr(), _p(X), _p(lmax), _p(o_out), err.data_ptr())

@@ -951,6 +951,15 @@ struct Plan {
 
 constexpr size_t WS_TARGET = size_t(1) << 30;  // lanes are batched to at most this much workspace, but one at least
 
+// Whether no call takes these sizes (plan() divides by some of them, and the grids and
+// 32-bit products below hold the others).
+static bool refused(int lanes, int nq, int n_heads, int n_kv, int dh, int t_lim) {
+  if (lanes < 1 || nq < 1 || n_kv < 1 || n_heads < 1 || n_heads % n_kv || dh < 8 || dh > 128 || dh % 8 || t_lim < 1)
+    return true;
+  const int64_t R = (int64_t)nq * (n_heads / n_kv);
+  return (int64_t)lanes * nq > 65535 || t_lim > 65535 * 16 * TILE || n_kv * ((R + RQ - 1) / RQ) > 65535;
+}
+
 static Plan plan(int lanes, int nq, int n_heads, int n_kv, int dh, int t_lim) {
   Plan p;
   p.G = n_heads / n_kv;
@@ -1056,8 +1065,9 @@ static int run_dh(const Args& A, const Plan& p, int lanes, cudaStream_t st) {
 
 extern "C" {
 
-// Workspace bytes of arcb_attn_tree.
+// Workspace bytes of arcb_attn_tree; -1 for sizes that it refuses.
 int64_t arcb_attn_tree_ws(int lanes, int nq, int n_heads, int n_kv, int dh, int t_lim) {
+  if (at::refused(lanes, nq, n_heads, n_kv, dh, t_lim)) return -1;
   return (int64_t)at::plan(lanes, nq, n_heads, n_kv, dh, t_lim).bytes;
 }
 
@@ -1065,12 +1075,8 @@ int arcb_attn_tree(const int64_t* q, const int64_t* Kc, const int64_t* Vc, int n
                    int64_t pt_stride, int width, const int* base, const int* n_tree, const int64_t* mask, int nq,
                    int n_heads, int n_kv, int dh, int64_t attn_scale, int t_lim, int lanes, void* ws, int8_t* X,
                    int* lmax, int64_t* o_out, int* err, void* stream) {
-  if (lanes < 1 || nq < 1 || n_kv < 1 || n_heads < 1 || n_heads % n_kv || dh < 8 || dh > 128 || dh % 8 || t_lim < 1)
-    return -2;
+  if (at::refused(lanes, nq, n_heads, n_kv, dh, t_lim) || width < 1) return -2;
   const at::Plan p = at::plan(lanes, nq, n_heads, n_kv, dh, t_lim);
-  if (p.tiles > 65535 * 16 || (int64_t)n_kv * p.groups > 65535 || (int64_t)n_kv * ((p.R + at::RQ - 1) / at::RQ) > 65535 ||
-      p.lanes > 65535)
-    return -2;
   uint8_t* b = (uint8_t*)ws;
   at::Args A = {};
   A.q = q, A.Kc = Kc, A.Vc = Vc, A.pt = pt, A.base = base, A.n_tree = n_tree, A.mask = mask;

@@ -15,3 +15,18 @@ GB = 1 << 30
 def test_workspace_stays_within_its_bound(lanes, nq, heads, kv, dh, t_lim):
     ws = lib().arcb_attn_tree_ws(lanes, nq, heads, kv, dh, t_lim)
     assert 0 < ws <= max(GB, lib().arcb_attn_tree_ws(1, nq, heads, kv, dh, t_lim))
+
+
+@pytest.mark.parametrize("bad", [dict(kv=0), dict(kv=-1), dict(t_lim=0), dict(t_lim=-5), dict(lanes=0), dict(nq=0),
+                                 dict(heads=0), dict(dh=0), dict(heads=7), dict(dh=136), dict(dh=12), dict(t_lim=(1 << 31) - 1),
+                                 dict(lanes=1 << 20), dict(nq=1 << 30)], ids=str)
+def test_sizes_that_no_call_takes(bad):
+    """Asked in a process of its own: a division by zero would end it."""
+    import subprocess
+    import sys
+
+    a = {**dict(lanes=2, nq=4, heads=8, kv=2, dh=64, t_lim=100), **bad}
+    code = (f"from arc_chain_b200.ops._lib import lib; print(lib().arcb_attn_tree_ws({a['lanes']}, {a['nq']}, "
+            f"{a['heads']}, {a['kv']}, {a['dh']}, {a['t_lim']}))")
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0 and int(r.stdout.strip()) < 0, (r.returncode, r.stdout, r.stderr)
