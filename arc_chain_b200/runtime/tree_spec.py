@@ -123,6 +123,8 @@ class TreeSpecDecoder:
         if draft is not None and draft.m.cfg.vocab != target.m.cfg.vocab:
             raise ValueError("target and draft must share a vocabulary")
         self.d = draft if self.branches and self.leads else None
+        if self.d is not None and self.d.m.emb.device != self.dev:
+            raise ValueError(f"target and draft share a device, got {self.dev} and {self.d.m.emb.device}")
         if self.d is not None and self.d.comm.size > 1:
             raise ValueError("the draft runs on one rank: its engine takes no communicator")
         self.levels = tree_levels(self.branches)

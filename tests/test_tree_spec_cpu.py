@@ -210,3 +210,10 @@ def test_temperatures_that_are_taken(toy_ops, t):
     sd = decoder((2,), temperature=t, draft_temperature=t)
     assert sd.inv.tolist() == sd.dinv.tolist() == [0 if t == 0 else round(65536 / t)] * 2
     assert RunConfig(temperature=t, draft_temperature=t).temperature == t
+
+
+def test_engines_on_two_devices_are_refused(toy_ops):
+    target, draft = stub.ToyEngine(), stub.ToyEngine()
+    draft.m.emb = torch.zeros(1, device="meta")
+    with pytest.raises(ValueError, match="device"):
+        ts.TreeSpecDecoder(target, draft, (2,), 1)
