@@ -123,10 +123,10 @@ def attn_tree(q, Kc, Vc, pt, base, n_tree, mask, n_heads: int, n_kv: int, dh: in
     n_heads * dh] int64.  A lane whose lengths or pages are out of range gets
     zeros and sets a bit of err.
 
-    A call takes a workspace for as many lanes as 1 GB holds (one at least); the
-    others follow in further launches.  A lane takes some 4 bytes for each key
-    up to t_lim, and 2 to 4 KB, for every query and query head (those of a KV
-    head counted as 8, or as a multiple of 16)."""
+    A call takes a workspace of some 4 bytes for each key up to t_lim, and 2 to
+    4 KB, for every query and query head (those of a KV head counted as 8, or
+    as a multiple of 16): of as many lanes as 1 GB of scores and 6 GB in all
+    hold (one at least); the others follow in further launches."""
     if lanes < 1 or nq < 1 or lanes * nq > 65535:
         raise ValueError(f"lanes and nq must be at least 1 and lanes * nq at most 65535, got {lanes} and {nq}")
     if n_kv < 1 or n_heads < 1 or n_heads % n_kv:

@@ -949,7 +949,10 @@ struct Plan {
   size_t oS, oQ, oI, oR, oM, oG, oSum, oW, oAcc, oA, oB, oF, bytes;
 };
 
-constexpr size_t WS_TARGET = size_t(1) << 30;  // lanes are batched to at most this much workspace, but one at least
+// Lanes are batched to this many bytes of scores and of workspace in all, but one at least.
+// 512 lanes of 64 nodes and 64 keys, 64 heads over 8, take 5.5 GB and 4.68 ms in one batch,
+// 5.04 ms in the five that 1.25 GB hold; inputs and outputs are 4 GB and more there.
+constexpr size_t WS_SCORES = size_t(1) << 30, WS_MOST = 6 * WS_SCORES;
 
 // Whether no call takes these sizes (plan() divides by some of them, and the grids and
 // 32-bit products below hold the others).
@@ -992,7 +995,8 @@ static Plan plan(int lanes, int nq, int n_heads, int n_kv, int dh, int t_lim) {
                                                   (size_t)p.groups * (p.RG * dh * 4 + 4)) +
                           4 + slot + (size_t)p.tiles * TILE * slot / (MAX_RANGE - 32) + 1;
   const size_t fixed = (p.splits + 1) * slot + 16 * 256;
-  const size_t fit = fixed < WS_TARGET ? (WS_TARGET - fixed) / per_lane : 0;
+  const size_t all = fixed < WS_MOST ? (WS_MOST - fixed) / per_lane : 0, scores = WS_SCORES / per_s;
+  const size_t fit = all < scores ? all : scores;
   p.lanes = fit < 1 ? 1 : (fit < (size_t)lanes ? (int)fit : lanes);
   const int have = p.lanes * n_kv * p.groups;
   const int64_t least = ((int64_t)p.lanes * p.tiles * TILE + MAX_RANGE - 1) / (MAX_RANGE - 32);
