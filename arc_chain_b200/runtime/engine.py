@@ -23,8 +23,10 @@ so the LM head is skipped there).  Decode steps replay one CUDA graph.
 """
 from __future__ import annotations
 
+import gc
 import os
 import time
+from contextlib import contextmanager
 from typing import Dict, List, Optional, Sequence, Tuple
 
 import torch
@@ -106,6 +108,25 @@ class StepBuffers:
         # drafted trees (Engine.tree_buffers): cache rows of the slots, and what attn_tree reads
         self.tree: Optional[TreeStep] = None
         self.kv_pos: Optional[torch.Tensor] = None
+
+
+@contextmanager
+def capturing(g: torch.cuda.CUDAGraph):
+    """Captures the body into `g`, on a stream of its own.  Python's collector
+    rests meanwhile: another graph that it freed (of a decoder that some cycle
+    held) would end the capture."""
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    collects = gc.isenabled()
+    gc.disable()
+    try:
+        with torch.cuda.stream(s):
+            with torch.cuda.graph(g, stream=s):
+                yield
+    finally:
+        if collects:
+            gc.enable()
+    torch.cuda.current_stream().wait_stream(s)
 
 
 class TreeStep:
@@ -295,12 +316,8 @@ class Engine:
         """Capture one decode step of `bb` into a CUDA graph (after a warm-up
         step has run eagerly, so kernel attributes are already set)."""
         g = torch.cuda.CUDAGraph()
-        s = torch.cuda.Stream()
-        s.wait_stream(torch.cuda.current_stream())
-        with torch.cuda.stream(s):
-            with torch.cuda.graph(g, stream=s):
-                self.decode_step(bb)
-        torch.cuda.current_stream().wait_stream(s)
+        with capturing(g):
+            self.decode_step(bb)
         return g
 
     # ------------------------------------------------------------------ requests

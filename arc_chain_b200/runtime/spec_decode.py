@@ -32,7 +32,7 @@ import numpy as np
 import torch
 
 from arc_chain_b200.ops import int_ops as ops
-from arc_chain_b200.runtime.engine import Engine, I32
+from arc_chain_b200.runtime.engine import Engine, I32, capturing
 from arc_chain_b200.utils.hashing import blake3
 
 
@@ -86,12 +86,8 @@ class SpecDecoder:
             self._verify()  # warm-up (sets kernel attributes); its KV writes are rewritten later
             torch.cuda.synchronize()
             g = torch.cuda.CUDAGraph()
-            s = torch.cuda.Stream()
-            s.wait_stream(torch.cuda.current_stream())
-            with torch.cuda.stream(s):
-                with torch.cuda.graph(g, stream=s):
-                    self._verify()
-            torch.cuda.current_stream().wait_stream(s)
+            with capturing(g):
+                self._verify()
             self._vgraph = g
         return self._vgraph
 

@@ -42,7 +42,7 @@ import torch
 
 from arc_chain_b200.formats import gen
 from arc_chain_b200.ops import tree_ops as ops
-from arc_chain_b200.runtime.engine import Engine, I32, I64
+from arc_chain_b200.runtime.engine import Engine, I32, I64, capturing
 from arc_chain_b200.spec import check_temperature
 from arc_chain_b200.utils.hashing import blake3
 
@@ -264,12 +264,8 @@ class TreeSpecDecoder:
                 bb.pt.copy_(s)
             self.live.copy_(live)
             g = torch.cuda.CUDAGraph()
-            s = torch.cuda.Stream()
-            s.wait_stream(torch.cuda.current_stream())
-            with torch.cuda.stream(s):
-                with torch.cuda.graph(g, stream=s):
-                    self._round()
-            torch.cuda.current_stream().wait_stream(s)
+            with capturing(g):
+                self._round()
             self._graph = g
         self._graph.replay()
 

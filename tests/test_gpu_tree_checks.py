@@ -97,3 +97,45 @@ def test_attn_tree_batches_of_short_lanes(nq, heads, kv, dh, lanes, few):
                 want = spec.tree_attention(q[s, h * dh:(h + 1) * dh].cpu().numpy(), k, v, int(base[b]), int(n_tree[b]),
                                            int(mask[s]), 9000)
                 np.testing.assert_array_equal(got[s, h * dh:(h + 1) * dh].cpu().numpy(), want)
+
+
+@pytest.mark.parametrize("kind", ["tree", "chain", "plain"])
+def test_a_graph_left_in_a_cycle_does_not_end_a_capture(kind):
+    """A decoder that an exception's traceback held is freed by Python's
+    collector, at any allocation: not while another one is captured."""
+    import gc
+
+    from arc_chain_b200.runtime.spec_decode import SpecDecoder
+    from arc_chain_b200.runtime.tree_spec import TreeSpecDecoder
+
+    class Holder:
+        pass
+
+    host = gen.random_model(preset("micro_gqa"), 0)
+    target, draft = engine(host), engine(host)
+    prompt = gen.seeded_prompt(12, preset("micro_gqa").vocab, 21)
+    old, x = torch.cuda.CUDAGraph(), torch.zeros(4, device="cuda")
+    x.add_(1)
+    torch.cuda.synchronize()
+    with torch.cuda.graph(old):
+        x.add_(1)
+    box, forward = [old], target.forward
+    del old
+
+    def littering(*a, **kw):
+        if box and torch.cuda.is_current_stream_capturing():
+            h = Holder()
+            h.self, h.graph = h, box.pop()
+            del h
+            [[] for _ in range(20000)]  # the collector's allocation count passes its limit
+        return forward(*a, **kw)
+
+    target.forward = littering
+    if kind == "tree":
+        got = TreeSpecDecoder(target, draft, (2, 1), draft_temperature=0.0).generate([prompt], 20)[0]
+    elif kind == "chain":
+        got = SpecDecoder(target, draft, k=2).generate([prompt], 20)[0]
+    else:
+        got = target.generate(prompt, 20)
+    assert not box and gc.isenabled()
+    assert got == arcref.Model(host).generate(prompt, 20)
