@@ -275,14 +275,17 @@ class TreeSpecDecoder:
         engines = [self.t] if self.d is None or self.d is self.t else [self.t, self.d]
         return [bb.err for e in engines for bb in e._bufs.values()]
 
-    def _check_errors(self) -> None:
-        """Raises where a kernel reported that it could not do its work (a page or a length
-        out of range, a wait that ran out): the tokens behind that are not the model's."""
-        bits = 0
-        for w in torch.cat(self._error_words()).tolist():
-            bits |= w
+    def _read(self, *tensors: torch.Tensor) -> List[np.ndarray]:
+        """Copies of int32 tensors on the host, in one transfer with the error words.  Raises
+        where a kernel reported that it could not do its work (a page or a length out of
+        range, a wait that ran out): the tokens behind that are not the model's."""
+        parts = [t.reshape(-1) for t in (*tensors, *self._error_words())]
+        flat = torch.cat(parts).cpu().numpy()
+        ends = np.cumsum([len(p) for p in parts[:len(tensors)]], dtype=np.int64)
+        bits = int(np.bitwise_or.reduce(flat[ends[-1] if len(ends) else 0:]))
         if bits:
             raise RuntimeError(f"a kernel reported an error (error bits {bits:#x})")
+        return [x.reshape(t.shape) for x, t in zip(np.split(flat, ends), tensors)]
 
     def _numbers(self, ln: _Lane, k: int) -> np.ndarray:
         r = gen.rng_u64(self.seed, ln.stream, k, start=ln.drawn)
@@ -333,9 +336,7 @@ class TreeSpecDecoder:
         with self._together():
             if not one:
                 self._settle()
-            path, n_path, nxt = self.path.cpu().numpy(), self.n_path.cpu().numpy(), self.nxt.cpu().numpy()
-            tokens = self.tokens.cpu().numpy()
-            self._check_errors()
+            path, n_path, nxt, tokens = self._read(self.path, self.n_path, self.nxt, self.tokens)
         self.rounds += 1
         for i, ln in enumerate(lanes):
             if ln.done:
@@ -389,7 +390,7 @@ class TreeSpecDecoder:
             for ln in lanes:
                 self.t.prefill(ln.rid_t, ln.prompt)
             with self._together():
-                self._check_errors()
+                self._read()
             while not all(ln.done for ln in lanes):
                 self._step(lanes, ends)
         finally:
