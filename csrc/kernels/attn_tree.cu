@@ -40,11 +40,18 @@
 //     CTAs that share a lane add their sums with atomics (integers: any order
 //     gives the same), two int32 in one 64-bit word; the last to arrive writes.
 //
-// Measured, a call and its kernels 0 to 3 by themselves: 4 lanes of 64 nodes, 64
-// heads over 8 KV heads, up to 1552 keys 314 us (9, 88, 31, 198); 9 nodes, 30
-// thousand keys 362 us (5, 118, 38, 210: K and V, 493 MB, at 1.4 TB/s); 8 lanes
-// of 31 nodes, 32 heads, up to 528 keys 122 us (6, 41, 13, 64); 16 nodes, 402
-// keys 37 us; 5 nodes, 42 keys, 4 heads 24 us.
+// Measured with nothing left in L2 and t_lim at the longest lane's keys, a call
+// (in brackets: one of a row of calls) and its kernels 0 to 3 by themselves: 4
+// lanes of 64 nodes, 64 heads over 8 KV heads, up to 1552 keys 314 us [309] (9,
+// 88, 31, 198); 9 nodes, 30 thousand keys 362 us [354] (5, 118, 38, 210: K and V,
+// 493 MB, at 1.4 TB/s); 8 lanes of 31 nodes, 32 heads, up to 528 keys 122 us [116]
+// (6, 41, 13, 64); 16 nodes, 402 keys 37 us [32]; 5 nodes, 42 keys, 4 heads 24 us
+// [17].  A larger t_lim costs score CTAs that find no keys, workspace, and the
+// form of two kernels: at 2048, in a row of calls, 312, 135, 39 and 21 us.
+// Values of 62.0 and more, or keys and queries of more than 32 bits, take 64-bit
+// products: 31 nodes a lane 1390 or 1580 us, 30 thousand keys 5.6 or 8.7 ms; rows
+// whose exps sum to 2^30 (flat scores over 16 thousand keys) 64-bit divisions:
+// 30 thousand keys 489 us.
 #include <atomic>
 
 #include "../common/tree.h"
@@ -615,7 +622,7 @@ __device__ __forceinline__ int store_limbs4(int8_t* X, int slot, int B, size_t l
 // the dims 2 ln, 2 ln + 1 (and 64 + those); kparts warps per unit take every
 // kparts-th key.
 // Bound by the FMAs and what feeds them: of 130 million warp instructions for 4 x
-// 64 nodes, 58 % are FMAs (their pipe 51 % busy, issue slots 65 %), the rest the
+// 64 nodes, 58 % are FMAs (their pipe 49 % busy, issue slots 65 %), the rest the
 // weights, the conversion of V and the loads from shared memory.  FMAs of two
 // terms run at the same rate and cost moves; warps that only convert and weigh
 // while others add were no faster.
@@ -976,9 +983,11 @@ static Plan plan(int lanes, int nq, int n_heads, int n_kv, int dh, int t_lim) {
   p.tiles = (t_lim + TILE - 1) / TILE;
   const int units = p.RG / p.unit;
   p.threads = 32 * units * (units >= 5 ? 1 : (units >= 3 ? 2 : (units == 2 ? 4 : 8)));
-  // five-warp value CTAs run three to an SM with chunks of one page (9 nodes, 8 query
-  // heads per KV head, 30 thousand keys: a call 362 us against 393 with two and two pages);
-  // the others two, with two pages (64 nodes: 315 us, 325 with one page)
+  // five-warp value CTAs run three to an SM with chunks of one page; the others two, with
+  // two pages (64 nodes: 315 us, 325 with one page).  9 nodes, 8 query heads per KV head, three
+  // against two, a lane of 100 / 500 / 2000 / 8000 / 30000 keys: 59 / 61 / 78 / 145 / 361 us and
+  // 59 / 64 / 80 / 153 / 392; 8 lanes of 100 / 500 / 2000 / 8000 keys: 82 / 121 / 229 / 708 and
+  // 70 / 123 / 244 / 762
   p.per_sm = p.threads == 160 ? 3 : 2;
   p.qgroups = (p.R + RQ - 1) / RQ;
   p.few = p.R <= RQ && (int64_t)p.RG * t_lim <= FEW_MOST;

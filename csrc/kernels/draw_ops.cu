@@ -36,12 +36,15 @@
 // the root: one node's latency.  Larger trees and batches take one cluster per
 // lane, which walks from the root and reads only the rows that it meets.
 //
-// What bounds it is latency: a cluster barrier takes half a microsecond, a first
-// touch of DRAM one to two, and a decision needs some eight of them in turn.
-// One row of 32000 takes 9.0 us in the kernel (12.3 us a call), a drafted chain
-// of 5 of them 20 us a call, 8 trees of 31 nodes 44 us, 4 trees of 64 nodes of
-// 102400 59 us.  72 rows of 102400, three tokens of each, take 55 us: 59 MB, two
-// waves of clusters, 1 TB/s.
+// What bounds it is latency: a first touch of DRAM takes one to three
+// microseconds (the lane's tree and ring, then the logits, which wait for it), an
+// exchange between the CTAs one to one and a half, and a decision needs some
+// eight of them in turn.  With nothing left in L2 one row of 32000 takes 9.0 us in
+// the kernel (12 to 14 us a call), a drafted chain of 5 of them 20 us a call, 8
+// trees of 31 nodes 44 us, 4 trees of 64 nodes of 102400 59 us.  72 rows of
+// 102400, three tokens of each, take 55 us: 59 MB, 1 TB/s, in two waves of
+// clusters of 8, since half of a row's weights pass SMEM_MAX.  In a row of calls:
+// 13, 21, 41, 50 to 57 and 48 us.
 #include <atomic>
 #include <climits>
 
