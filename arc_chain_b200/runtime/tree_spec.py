@@ -99,7 +99,7 @@ class TreeSpecDecoder:
                  use_graph: bool = True):
         self._dense(target)
         self.cm = target.comm
-        self.leads = self.cm.rank == 0
+        self.leads, self.group = self.cm.rank == 0, getattr(self.cm, "group", None)
         self.dev = target.m.emb.device
         with self._together():
             self._build(target, draft, branches, lanes, temperature, draft_temperature, seed, use_graph)
@@ -165,7 +165,7 @@ class TreeSpecDecoder:
         import torch.distributed as dist
 
         t = torch.tensor([x], dtype=I64, device=self.dev)
-        dist.all_reduce(t, dist.ReduceOp.MIN if least else dist.ReduceOp.MAX, group=self.cm.group)
+        dist.all_reduce(t, dist.ReduceOp.MIN if least else dist.ReduceOp.MAX, group=self.group)
         return int(t.item())
 
     @contextmanager
@@ -177,8 +177,11 @@ class TreeSpecDecoder:
             yield
         except Exception as e:
             err = e
-        if self._agree(int(err is not None), False) and err is None:
-            err = RuntimeError("tree speculation failed on another rank")
+        try:
+            if self._agree(int(err is not None), False) and err is None:
+                err = RuntimeError("tree speculation failed on another rank")
+        except Exception as e:
+            raise e if err is None else err
         if err is not None:
             raise err
 
@@ -187,7 +190,7 @@ class TreeSpecDecoder:
             import torch.distributed as dist
 
             for x in tensors:
-                dist.broadcast(x, group=self.cm.group, group_src=0)
+                dist.broadcast(x, group=self.group, group_src=0)
 
     # ------------------------------------------------------------ device side
     def _set(self, bb, a: int, b: int) -> None:

@@ -76,54 +76,53 @@ def _fail(*a, **kw):
     raise MemoryError("planted")
 
 
-def _worker(rank, world, port, group_ranks, fault, q):
+def _call(comm, fault):
+    """A call on this rank, with a fault planted in it: its tokens or its
+    error, and whether the pages are free again."""
+    leads, verify = comm.rank == 0, stub.verify_tree
+    target, draft = stub.ToyEngine(0, comm=comm), stub.ToyEngine(3, max_seq=48 if fault == "limit" else 128)
+    if fault == "request" and leads:
+        draft.new_request = _fail
+    if fault == "prompt" and leads:
+        draft.prefill = _fail
+    if fault == "level" and leads:
+        draft.forward = _fail
+    if fault == "kept rows" and leads:
+        draft.kv.keep_path = _fail
+    if fault == "pages" and not leads:
+        target.kv.pool.free = target.kv.pool.free[:2]
+    ts.ops.draw_tokens, ts.ops.verify_tree = stub.draw_tokens, _fail if fault == "decision" and leads else verify
+    used = target.kv.pool.used
+    try:
+        sd = ts.TreeSpecDecoder(target, draft if leads and fault != "no draft" else None, (2, 2), 2, 0.9, seed=4)
+        if fault == "word" and not leads:
+            forward = target.forward
+            target.forward = lambda *a: (forward(*a), sd.tb.err.fill_(8))
+        out = [t for t, _ in sd.generate(PROMPTS, 20 if fault != "limit" else 40)]
+    except (ValueError, MemoryError, RuntimeError) as e:
+        out = f"{type(e).__name__}: {e}"
+    return out, target.kv.pool.used <= used + 1 and draft.kv.pool.used <= 1
+
+
+def _worker(rank, world, port, group_ranks, faults, q):
     import torch.distributed as dist
 
     from arc_chain_b200.parallel.tp import NcclComm
 
     os.environ["MASTER_ADDR"], os.environ["MASTER_PORT"] = "127.0.0.1", str(port)
     dist.init_process_group("gloo", rank=rank, world_size=world, timeout=datetime.timedelta(seconds=15))
-    ts.ops.draw_tokens, ts.ops.verify_tree = stub.draw_tokens, stub.verify_tree
     try:
         group = dist.new_group(group_ranks) if group_ranks else None
         if group_ranks and rank not in group_ranks:
             q.put((rank, None))
             return
         comm = NcclComm(group)
-        leads = comm.rank == 0
-        target, draft = stub.ToyEngine(0, comm=comm), stub.ToyEngine(3, max_seq=48 if fault == "limit" else 128)
-        if fault == "request" and leads:
-            draft.new_request = _fail
-        if fault == "prompt" and leads:
-            draft.prefill = _fail
-        if fault == "level" and leads:
-            draft.forward = _fail
-        if fault == "decision" and leads:
-            ts.ops.verify_tree = _fail
-        if fault == "kept rows" and leads:
-            draft.kv.keep_path = _fail
-        if fault == "pages" and not leads:
-            target.kv.pool.free = target.kv.pool.free[:2]
-        used = target.kv.pool.used
-        out = []
-        try:
-            sd = ts.TreeSpecDecoder(target, draft if leads and fault != "no draft" else None, (2, 2), 2, 0.9, seed=4)
-            if fault == "word" and not leads:
-                forward = target.forward
-                target.forward = lambda *a: (forward(*a), sd.tb.err.fill_(8))
-            out = [t for t, _ in sd.generate(PROMPTS, 20 if fault != "limit" else 40)]
-        except (ValueError, MemoryError, RuntimeError) as e:
-            out = f"{type(e).__name__}: {e}"
-        q.put((rank, (out, target.kv.pool.used <= used + 1 and draft.kv.pool.used <= 1)))
-        # every rank is still in step with the others
-        t = torch.ones(1)
-        dist.all_reduce(t, group=group)
-        assert int(t) == comm.size
+        q.put((rank, {f: _call(comm, f) for f in faults}))  # each on the same group: in step all along
     finally:
         dist.destroy_process_group()
 
 
-def _ranks(fault="", group_ranks=()):
+def _ranks(faults, group_ranks=()):
     import multiprocessing as mp
 
     s = socket.socket()
@@ -132,11 +131,11 @@ def _ranks(fault="", group_ranks=()):
     s.close()
     ctx, world = mp.get_context("spawn"), 3 if group_ranks else 2
     q = ctx.Queue()
-    ps = [ctx.Process(target=_worker, args=(r, world, port, list(group_ranks), fault, q)) for r in range(world)]
+    ps = [ctx.Process(target=_worker, args=(r, world, port, list(group_ranks), faults, q)) for r in range(world)]
     for p in ps:
         p.start()
     res, t0 = {}, time.time()
-    while len(res) < world and time.time() - t0 < 90:
+    while len(res) < world and time.time() - t0 < 120:
         try:
             r, v = q.get(timeout=1)
             res[r] = v
@@ -146,34 +145,58 @@ def _ranks(fault="", group_ranks=()):
         p.join(timeout=30)
         if p.is_alive():
             p.kill()
-    return [res.get(r) for r in range(world)], [p.exitcode for p in ps]
+    assert [p.exitcode for p in ps] == [0] * world and len(res) == world
+    return [res[r] for r in range(world)]
 
 
-@pytest.mark.parametrize("group_ranks", [(), (1, 2)])
-def test_ranks_equal_one_process(toy_ops, group_ranks):
-    """Also over a communicator of some of the ranks, whose first is not the world's."""
+FAULTS = {
+    "limit": ("ValueError: a prompt of 3 tokens, 40 new ones and a tree of 7 nodes exceed max_seq 48",) * 2,
+    "no draft": ("ValueError: a tree of drafted tokens needs a draft engine", "RuntimeError: tree spec"),
+    "request": ("MemoryError: planted", "RuntimeError: tree spec"),
+    "prompt": ("MemoryError: planted", "RuntimeError: tree spec"),
+    "level": ("MemoryError: planted", "RuntimeError: tree spec"),
+    "decision": ("MemoryError: planted", "RuntimeError: tree spec"),
+    "kept rows": ("MemoryError: planted", "RuntimeError: tree spec"),
+    "pages": ("RuntimeError: tree spec", "MemoryError: KV cache out of pages"),
+    "word": ("RuntimeError: tree spec", "RuntimeError: a kernel reported an error (error bits 0x8)"),
+}
+
+
+@pytest.fixture(scope="module")
+def two_ranks():
+    return _ranks([*FAULTS, "none"])
+
+
+def test_ranks_equal_one_process(toy_ops, two_ranks):
+    """Also behind failed calls, and over a communicator of some of the ranks,
+    whose first is not the world's."""
     want = [t for t, _ in decoder((2, 2), 0.9, 3, seed=4).generate(PROMPTS, 20)]
-    res, codes = _ranks("", group_ranks)
-    assert codes == [0] * len(codes)
-    assert [r for r in res if r is not None] == [(want, True)] * 2
+    assert [r["none"] for r in two_ranks] == [(want, True)] * 2
+    some = _ranks(["none"], (1, 2))
+    assert some == [None, {"none": (want, True)}, {"none": (want, True)}]
 
 
-@pytest.mark.parametrize("fault,first,second", [
-    ("limit", "ValueError: a prompt of 3 tokens, 40 new ones and a tree of 7 nodes exceed max_seq 48", None),
-    ("no draft", "ValueError: a tree of drafted tokens needs a draft engine", "RuntimeError: tree spec"),
-    ("request", "MemoryError: planted", "RuntimeError: tree spec"),
-    ("prompt", "MemoryError: planted", "RuntimeError: tree spec"),
-    ("level", "MemoryError: planted", "RuntimeError: tree spec"),
-    ("decision", "MemoryError: planted", "RuntimeError: tree spec"),
-    ("kept rows", "MemoryError: planted", "RuntimeError: tree spec"),
-    ("pages", "RuntimeError: tree spec", "MemoryError: KV cache out of pages"),
-    ("word", "RuntimeError: tree spec", "RuntimeError: a kernel reported an error (error bits 0x8)")])
-def test_ranks_fail_together(fault, first, second):
-    """What one rank refuses or fails at ends the call on both, and both stay in step."""
-    res, codes = _ranks(fault)
-    assert codes == [0, 0], (codes, res)
-    for (out, released), want in zip(res, (first, second or first)):
+@pytest.mark.parametrize("fault", FAULTS)
+def test_ranks_fail_together(two_ranks, fault):
+    """What one rank refuses or fails at ends the call on both."""
+    for r, want in zip(two_ranks, FAULTS[fault]):
+        out, released = r[fault]
         assert isinstance(out, str) and out.startswith(want) and released
+
+
+def test_a_rank_that_cannot_ask_the_others_raises_its_own_error(toy_ops):
+    sd = decoder((2,))
+
+    def lost(*a):
+        raise RuntimeError("connection closed")
+
+    sd._agree = lost
+    with pytest.raises(RuntimeError, match="connection closed"):
+        with sd._together():
+            pass
+    with pytest.raises(MemoryError, match="planted"):
+        with sd._together():
+            _fail()
 
 
 # ------------------------------------------------------------ refusals
