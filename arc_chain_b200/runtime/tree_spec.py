@@ -229,7 +229,7 @@ class TreeSpecDecoder:
         if self.db:
             self._draft()
 
-    def _judge(self) -> None:
+    def _verify(self) -> None:
         self._broadcast(self.tokens)
         self._set(self.tb, 0, self.n)
         self.t.forward(self.tb, self.tb.B, True)
@@ -246,7 +246,7 @@ class TreeSpecDecoder:
 
     def _round(self) -> None:
         self._propose()
-        self._judge()
+        self._verify()
         self._settle()
 
     def _run(self) -> None:
@@ -335,7 +335,7 @@ class TreeSpecDecoder:
             else:
                 self._propose()
         if not one:
-            self._judge()
+            self._verify()
         with self._together():
             if not one:
                 self._settle()

@@ -44,7 +44,7 @@
 // trees of 31 nodes 44 us, 4 trees of 64 nodes of 102400 59 us.  72 rows of
 // 102400, three tokens of each, take 55 us: 59 MB, 1 TB/s, in two waves of
 // clusters of 8, since half of a row's weights pass SMEM_MAX.  In a row of calls:
-// 13, 21, 41, 50 to 57 and 48 us.
+// 13, 21, 37 to 45, 50 to 57 and 48 us.
 #include <atomic>
 #include <climits>
 
